@@ -255,6 +255,87 @@ int dfl_test_queue_timeout(dfl_ctx* ctx, int32_t on);
  * results are invalid); reading clears. */
 int dfl_device_errors(dfl_ctx* ctx, int32_t* flags, void* stream);
 
+/* ---- Paged key/value cache in 4 bits (no counterpart in the reference) ----
+ *
+ * For callers that hold many or long sequences: the cached rows of every sequence lie in pages
+ * of one pool, in 68 bytes a row, head and half (K or V) instead of 256.  No context is needed;
+ * every buffer is the caller's device memory, and no call allocates.
+ *
+ * A row of one head (128 values) is four groups of 32: an exponent byte b and 32 four-bit codes,
+ * standing for code * 2^(b - 127), the code a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6.  b is
+ * the smallest exponent >= 0 with the group's largest magnitude <= 7 * 2^(b - 127); codes round
+ * to nearest, ties to the even code.  A group with an infinity or NaN has b = 255 and is NaN.
+ *
+ * A layer's pool is n_pages * n_kv * (page / 32) blocks of DFL_KV4_BLOCK_BYTES, 16-byte
+ * aligned; `page` rows of a page are 32, 64, 128 or 256.  Slot p * page + r is row r of page p.
+ * table [n_seq][width] holds each sequence's pages in order (sequence s's row n is in page
+ * table[s][n / page]), lens [n_seq] its rows.  dtype: 0 fp32, 1 fp16, 2 bf16.
+ * err_flags is a device word that error bits are OR'ed into (the caller clears it): bit 3 a
+ * length out of range (dfl_kv4_step), bit 4 too few free pages, bit 5 more new rows than
+ * max_rows, bit 6 a slot outside the pool, bit 7 pages, lengths or row ranges that do not fit
+ * each other (a page id outside the pool, lens beyond the table, starts out of order). */
+#define DFL_KV4_BLOCK_BYTES 4352
+
+/* One step of every sequence: sequence s keeps its first keep[s] rows (NULL: all lens[s]) and
+ * grows by grow[s] (NULL: none).  Pages past the kept rows go back to the free pages, then pages
+ * for the new rows are taken from them; lens, table, free_pages [n_pages] (a stack, its top at
+ * *n_free - 1) and *n_free are updated in place.  Pages put back lie on the stack with the first
+ * sequence's first page on top, and pages are taken from the top, first sequence first.  Table
+ * places past a sequence's pages and free places past *n_free that the step gives up become -1.
+ * Out: starts [n_seq + 1] (the new rows of sequence s are starts[s] .. starts[s+1] - 1), and for
+ * each new row its slot and its position (the row's number in its sequence), max_rows of each;
+ * those past starts[n_seq] are -1.  A step that cannot be done (bits 3, 4, 5, 7) changes nothing,
+ * and gives no rows.  scratch: dfl_kv4_step_scratch(n_seq) int32, any content, not shared with a
+ * step that may run at the same time. */
+int dfl_kv4_step(int32_t n_seq, int32_t page, int32_t width, int32_t n_pages, const int32_t* keep,
+                 const int32_t* grow, int32_t* lens, int32_t* table, int32_t* free_pages,
+                 int32_t* n_free, int32_t max_rows, int32_t* starts, int32_t* slots,
+                 int32_t* positions, int32_t* scratch, int32_t* err_flags, void* stream);
+int64_t dfl_kv4_step_scratch(int32_t n_seq);
+
+/* Quantise rows of keys and values into their slots: row i, head h of k is at
+ * k + i * k_row + h * k_head elements (strides multiples of 8, 16-byte aligned), v alike.  Slots
+ * are int32; -1 skips the row, any other slot outside the pool skips it and sets bit 6.  The
+ * slots of a call must differ from each other (a slot given twice holds a mix of its rows). */
+int dfl_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                   int64_t v_head, int32_t dtype, int32_t rows, int32_t n_kv, int32_t page,
+                   int32_t n_pages, const int32_t* slots, uint8_t* pool, int32_t* err_flags,
+                   void* stream);
+/* The values of the rows at slots, into k and v [rows][n_kv][128] of the dtype (a value outside
+ * fp16's range becomes an infinity); zeros for slots outside the pool (-1 sets no error bit). */
+int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page, int32_t n_pages,
+                 const uint8_t* pool, int32_t dtype, void* k, void* v, int32_t* err_flags,
+                 void* stream);
+
+/* Attention over the cached rows.  The query rows of sequence s are starts[s] .. starts[s+1] - 1
+ * of q (row i, head h at q + i * q_row + h * q_head elements, strides multiples of 8, 16-byte
+ * aligned; fp16 or bf16); query head h reads kv head h / (n_heads / n_kv).  Every row sees all
+ * lens[s] cached rows of its sequence, or with causal != 0 row t of the sequence's m rows the
+ * first lens[s] - m + t + 1.  out [n_rows][n_heads][128] (dtype of q) = softmax(scale * q.k) v;
+ * lse [n_rows][n_heads] fp32 (or NULL) = log sum exp(scale * q.k).  A row that sees no key gives
+ * zeros and -infinity; rows of no sequence are left as they were.  What a row does not see does
+ * not reach it, whatever it holds.  Keys in a page outside the pool count as absent (bit 7).
+ * Weights are rounded to q's dtype, all else is held in fp32.  With fp16 queries, cached values
+ * beyond +-65504 read as infinities.  ws: dfl_kv4_attend_ws(...) bytes for the same arguments,
+ * 16-byte aligned, any content, not shared with a call that may run at the same time. */
+typedef struct dfl_kv4_attn {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_row, q_head;
+  int32_t dtype;
+  int32_t n_rows, n_heads, n_kv, n_seq, causal;
+  float scale;
+  const int32_t *starts, *lens, *table;
+  int32_t width, page, n_pages;
+  const uint8_t* pool;
+  void* ws;
+  int64_t ws_bytes;
+  int32_t* err_flags;
+} dfl_kv4_attn;
+int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream);
+int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq);
+
 #ifdef __cplusplus
 }
 #endif

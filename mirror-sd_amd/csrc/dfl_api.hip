@@ -13,6 +13,7 @@
 #include "dflash_hip.h"
 #include "dfl_kernels.h"
 #include "dfl_check.h"
+#include "dfl_kv4.h"
 #include "dfl_sk_plan.h"
 #include "dfl_tile_plan.h"
 
@@ -1647,6 +1648,127 @@ int dfl_device_errors(dfl_ctx* ctx, int32_t* flags, void* stream) {
   DFL_HIP(hipMemsetAsync(ctx->err, 0, sizeof(int), st));
   *flags = v;
   return DFL_OK;
+}
+
+// ---- paged 4-bit cache: context-free entry points over dfl_kv4.hip ----
+
+static int page_shift_of(int32_t page) {   // -1: not a power of two
+  return page > 0 && (page & (page - 1)) == 0 ? __builtin_ctz((unsigned)page) : -1;
+}
+
+int64_t dfl_kv4_step_scratch(int32_t n_seq) {
+  return n_seq < 1 || n_seq > KV4_MAX_SEQS ? 0 : kv4_step_scratch(n_seq);
+}
+
+int dfl_kv4_step(int32_t n_seq, int32_t page, int32_t width, int32_t n_pages, const int32_t* keep,
+                 const int32_t* grow, int32_t* lens, int32_t* table, int32_t* free_pages,
+                 int32_t* n_free, int32_t max_rows, int32_t* starts, int32_t* slots,
+                 int32_t* positions, int32_t* scratch, int32_t* err_flags, void* stream) {
+  Kv4StepArgs a{};
+  a.n_seq = n_seq;
+  a.page_shift = page_shift_of(page);
+  a.width = width;
+  a.n_pages = n_pages;
+  a.max_rows = max_rows;
+  a.keep = keep;
+  a.grow = grow;
+  a.lens = lens;
+  a.table = table;
+  a.free_pages = free_pages;
+  a.n_free = n_free;
+  a.starts = starts;
+  a.slots = slots;
+  a.positions = positions;
+  a.scratch = scratch;
+  a.err = err_flags;
+  if (const char* e = check_kv4_step(a)) return fail(DFL_EINVAL, std::string("dfl_kv4_step: ") + e);
+  launch_kv4_step(a, (hipStream_t)stream);
+  return check_launch("dfl_kv4_step");
+}
+
+int dfl_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
+                   int64_t v_head, int32_t dtype, int32_t rows, int32_t n_kv, int32_t page,
+                   int32_t n_pages, const int32_t* slots, uint8_t* pool, int32_t* err_flags,
+                   void* stream) {
+  Kv4RowsArgs a{};
+  a.k = k;
+  a.v = v;
+  a.k_row = k_row;
+  a.k_head = k_head;
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n_kv = n_kv;
+  a.page_shift = page_shift_of(page);
+  a.n_pages = n_pages;
+  a.slots = slots;
+  a.pool = pool;
+  a.err = err_flags;
+  if (rows == 0) return DFL_OK;
+  if (const char* e = check_kv4_rows(a, true)) return fail(DFL_EINVAL, std::string("dfl_kv4_append: ") + e);
+  launch_kv4_append(a, (hipStream_t)stream);
+  return check_launch("dfl_kv4_append");
+}
+
+int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page, int32_t n_pages,
+                 const uint8_t* pool, int32_t dtype, void* k, void* v, int32_t* err_flags,
+                 void* stream) {
+  Kv4RowsArgs a{};
+  a.ok = k;
+  a.ov = v;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.n_kv = n_kv;
+  a.page_shift = page_shift_of(page);
+  a.n_pages = n_pages;
+  a.slots = slots;
+  a.pool = const_cast<uint8_t*>(pool);   // (read only)
+  a.err = err_flags;
+  if (rows == 0) return DFL_OK;
+  if (const char* e = check_kv4_rows(a, false)) return fail(DFL_EINVAL, std::string("dfl_kv4_read: ") + e);
+  launch_kv4_read(a, (hipStream_t)stream);
+  return check_launch("dfl_kv4_read");
+}
+
+int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq) {
+  if (n_rows < 1 || n_heads < 1 || n_kv < 1 || n_seq < 1 || n_heads % n_kv) return 0;
+  return 2ll * kv4_workers(n_rows, n_heads, n_kv, n_seq) *
+         kv4_piece_floats(kv4_tile_rows(n_rows, n_heads, n_kv, n_seq)) * (long long)sizeof(float);
+}
+
+int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
+  if (!args) return fail(DFL_EINVAL, "dfl_kv4_attend: null argument");
+  Kv4AttnArgs a{};
+  a.q = args->q;
+  a.out = args->out;
+  a.lse = args->lse;
+  a.q_row = args->q_row;
+  a.q_head = args->q_head;
+  a.dtype = args->dtype;
+  a.n_rows = args->n_rows;
+  a.n_heads = args->n_heads;
+  a.n_kv = args->n_kv;
+  a.n_seq = args->n_seq;
+  a.causal = args->causal;
+  a.scale_log2 = args->scale * 1.44269504088896340736f;
+  a.starts = args->starts;
+  a.lens = args->lens;
+  a.table = args->table;
+  a.width = args->width;
+  a.page_shift = page_shift_of(args->page);
+  a.n_pages = args->n_pages;
+  a.pool = args->pool;
+  a.ws = static_cast<float*>(args->ws);
+  a.err = args->err_flags;
+  if (a.n_rows == 0) return DFL_OK;
+  if (const char* e = check_kv4_attn(a)) return fail(DFL_EINVAL, std::string("dfl_kv4_attend: ") + e);
+  a.workers = kv4_workers(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
+  const int64_t need = dfl_kv4_attend_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
+  if (need > 0 && (!a.ws || args->ws_bytes < need))
+    return fail(DFL_EINVAL, "dfl_kv4_attend: workspace of " + std::to_string(need) + " bytes needed");
+  launch_kv4_attend(a, (hipStream_t)stream);
+  return check_launch("dfl_kv4_attend");
 }
 
 }  // extern "C"

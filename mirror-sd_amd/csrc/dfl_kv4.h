@@ -1,0 +1,207 @@
+// Paged key/value cache in 4 bits: layout, launch interface and host checks.
+//
+// Format.  A row of one head (128 values) is four groups of 32.  A group is a shared exponent
+// byte b and 32 four-bit codes, standing for code * 2^(b - 127) with the code a sign and one of
+// 0, 0.5, 1, 1.5, 2, 3, 4, 6 (the 4-bit floats of gfx950's conversions; the OCP microscaling
+// layout of 32 elements to an e8m0 scale).  b is the smallest exponent >= 0 for which the group's
+// largest magnitude is at most 7 * 2^(b - 127): what lies in (6, 7] rounds to 6, nothing is
+// clipped further than half a step.  b = 255 marks a group that held an infinity or a NaN and
+// stands for NaN.
+//
+// Layout.  The pool is [layer][page][kv head][page / 32] blocks of 4352 bytes, a block being 32
+// consecutive rows (keys) of one head:
+//   bytes    0 .. 2047   K codes, 64 bytes a row, in the row order kv4_row
+//   bytes 2048 .. 4095   V codes, the same
+//   bytes 4096 .. 4351   exponent bytes, 4 a word: word i + 16 g holds group g of the keys
+//                        kv4_key(i, 0) and kv4_key(i, 1): bytes K0, K1, V0, V1
+// In a row the byte e holds values 2e (low nibble) and 2e + 1.  So a wave reads a block as four
+// 1 KiB loads and one of 256 bytes, every lane getting the operand of its own matrix row: lane
+// l = i + 16 g takes, of K and of V, 16 bytes of row i and of row 16 + i (values 32 g .. 32 g + 31,
+// one group) and the four exponent bytes that go with them.
+//
+// Everything here but the launchers is plain host code too, so that it can be tested on a CPU.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace dfl {
+
+#define DFL_HD __host__ __device__ inline
+
+constexpr int KV4_D = 128;                 // head dimension
+constexpr int KV4_KEYS = 32;               // rows of a block
+constexpr int KV4_V = 2048, KV4_SC = 4096; // V codes and exponent bytes of a block
+constexpr int KV4_BLOCK = 4352;            // bytes of a block
+constexpr int KV4_CUS = 256;               // compute units of an MI355X
+constexpr int KV4_MAX_SEQS = 65536;
+
+// error bits (they follow the library's bits 0 .. 2)
+constexpr int KV4_ERR_LEN = 8;       // step: a length out of range
+constexpr int KV4_ERR_POOL = 16;     // step: not enough free pages
+constexpr int KV4_ERR_ROWS = 32;     // step: more new rows than the slot map holds
+constexpr int KV4_ERR_SLOT = 64;     // append, read: a slot outside the pool
+constexpr int KV4_ERR_PAGE = 128;    // attend, step: a page, length or row range out of bounds
+
+// Row of a block that holds key k (k in [0, 32)) and back.  The matrix product S^T = K Q^T gives
+// lane (q, g) rows 4g .. 4g+3 of each 16-row tile; with tile 0 holding keys 8g + 0..3 and tile 1
+// keys 8g + 4..7 these are the 8 consecutive keys that the product with V takes from that lane.
+DFL_HD int kv4_row(int k) { return ((k >> 3) << 2) + (k & 3) + ((k & 4) << 2); }
+DFL_HD int kv4_key(int i, int tile) { return ((i >> 2) << 3) + (i & 3) + 4 * tile; }
+// Offset in a block of the exponent byte of group g of K (v = 0) or V (v = 1), row r of the block.
+DFL_HD int kv4_scale_at(int r, int g, int v) {
+  return KV4_SC + 4 * ((r & 15) + 16 * g) + 2 * v + (r >> 4);
+}
+// Byte offset of block `sub` of a page's head.
+DFL_HD long long kv4_block_at(long long page_idx, int n_kv, int head, int subs, int sub) {
+  return ((page_idx * n_kv + head) * subs + sub) * (long long)KV4_BLOCK;
+}
+
+DFL_HD int kv4_pages(int n, int page_shift) { return (int)(((long long)n + (1 << page_shift) - 1) >> page_shift); }
+
+// ---- step (block tables and slot maps) ----
+struct Kv4StepArgs {
+  int n_seq, page_shift, width, n_pages, max_rows;
+  const int *keep, *grow;      // [n_seq], either may be null (keep everything, grow by nothing)
+  int *lens, *table, *free_pages, *n_free;
+  int *starts, *slots, *positions;
+  int* scratch;                // kv4_step_scratch(n_seq) ints
+  int* err;
+};
+// scratch: status, freed and taken totals, free pages before; then [n_seq] kept lengths, freed
+// and taken pages before each sequence
+DFL_HD long long kv4_step_scratch(int n_seq) { return 4 + 3ll * n_seq; }
+
+// What one sequence asks of a step; false if a length is out of range.
+struct Kv4Ask { int keep, grow, freed, taken; };
+DFL_HD bool kv4_ask(int len, int keep, int grow, int width, int page_shift, Kv4Ask& a) {
+  const bool ok = len >= 0 && (long long)len <= ((long long)width << page_shift) && keep >= 0 &&
+                  keep <= len && grow >= 0 &&
+                  (long long)keep + grow <= ((long long)width << page_shift);
+  a = Kv4Ask{ok ? keep : 0, ok ? grow : 0, 0, 0};
+  if (!ok) return false;
+  const int pk = kv4_pages(keep, page_shift);
+  a.freed = kv4_pages(len, page_shift) - pk;
+  a.taken = kv4_pages(keep + grow, page_shift) - pk;
+  return true;
+}
+
+// ---- append / read ----
+struct Kv4RowsArgs {
+  const void *k, *v;           // append: rows in; read: unused
+  void *ok, *ov;               // read: rows out
+  long long k_row, k_head, v_row, v_head;   // strides in elements
+  int dtype;                   // 0 fp32, 1 fp16, 2 bf16
+  int rows, n_kv, page_shift, n_pages;
+  const int* slots;
+  unsigned char* pool;         // one layer's pages
+  int* err;
+};
+
+// ---- attention ----
+struct Kv4AttnArgs {
+  const void* q;
+  void* out;
+  float* lse;                  // [n_rows][n_heads] or null
+  long long q_row, q_head;     // strides in elements (out is contiguous)
+  int dtype;                   // 1 fp16, 2 bf16
+  int n_rows, n_heads, n_kv, n_seq, causal;
+  float scale_log2;
+  const int *starts, *lens, *table;
+  int width, page_shift, n_pages;
+  const unsigned char* pool;   // one layer's pages
+  float* ws;
+  int workers;                 // workgroups that share the key blocks
+  int* err;
+};
+
+// The work of a launch in key blocks: sequence s contributes, for each of its query tiles and kv
+// heads, one unit of nblk blocks; units are numbered sequence by sequence, head by head.  Worker w
+// takes blocks [w * per, (w + 1) * per) of all units in a row; a unit that several workers share
+// leaves one partial result with each (slot kv4_piece), which the merge joins.
+struct Kv4Seq { int q0, qlen, len, tiles, nblk; bool bad; };
+DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_shift, int ratio,
+                      int tile_rows) {
+  Kv4Seq s;
+  const long long cap = (long long)width << page_shift;
+  s.bad = q0 < 0 || q1 < q0 || q1 > n_rows || len < 0 || (long long)len > cap;
+  s.q0 = s.bad ? 0 : q0;
+  s.qlen = s.bad ? 0 : q1 - q0;
+  s.len = s.bad ? 0 : len;
+  s.tiles = (int)(((long long)s.qlen * ratio + tile_rows - 1) / tile_rows);
+  // a sequence without keys still has its rows written: one block, all of it masked
+  s.nblk = s.qlen ? (s.len > 0 ? (s.len + KV4_KEYS - 1) / KV4_KEYS : 1) : 0;
+  return s;
+}
+DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return (long long)s.tiles * n_kv * s.nblk; }
+constexpr int KV4_MIN_BLOCKS = 16;   // fewest blocks of a worker (four for each of its waves)
+DFL_HD long long kv4_per(long long total, int workers) {
+  const long long per = (total + workers - 1) / workers;
+  return per < KV4_MIN_BLOCKS ? KV4_MIN_BLOCKS : per;
+}
+// Partial slot of worker w for a unit that begins at block u0 (of all) and is shared: the unit a
+// worker begins with, and the one it ends with.
+DFL_HD long long kv4_piece(long long w, long long per, long long u0) {
+  return 2 * w + (u0 < w * per ? 0 : 1);
+}
+// Floats of one partial: O [tile rows][128], then (max, sum) a row.
+DFL_HD long long kv4_piece_floats(int tile_rows) { return (long long)tile_rows * (KV4_D + 2); }
+
+// Query rows of a tile, and workgroups, of a launch.
+int kv4_tile_rows(int n_rows, int n_heads, int n_kv, int n_seq);
+int kv4_workers(int n_rows, int n_heads, int n_kv, int n_seq);
+
+inline const char* check_kv4_pool(int n_kv, int page_shift, int n_pages) {
+  if (n_kv < 1 || n_kv > 1024) return "kv heads outside [1, 1024]";
+  if (page_shift < 5 || page_shift > 8) return "page rows must be 32, 64, 128 or 256";
+  if (n_pages < 1 || ((long long)n_pages << page_shift) > 0x7fffffffll)
+    return "pool pages out of range (at least one, slots below 2^31)";
+  return nullptr;
+}
+inline const char* check_kv4_step(const Kv4StepArgs& a) {
+  if (const char* e = check_kv4_pool(1, a.page_shift, a.n_pages)) return e;
+  if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
+  if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll)
+    return "table width out of range";
+  if (a.max_rows < 0) return "negative row capacity";
+  if (!a.lens || !a.table || !a.free_pages || !a.n_free || !a.starts || !a.scratch || !a.err)
+    return "null pointer";
+  if (a.max_rows > 0 && (!a.slots || !a.positions)) return "null slot map";
+  return nullptr;
+}
+inline const char* check_kv4_rows(const Kv4RowsArgs& a, bool append) {
+  if (const char* e = check_kv4_pool(a.n_kv, a.page_shift, a.n_pages)) return e;
+  if (a.rows < 0) return "negative row count";
+  if (a.dtype < 0 || a.dtype > 2) return "dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)";
+  if (!a.slots || !a.pool || !a.err) return "null pointer";
+  if (append ? (!a.k || !a.v) : (!a.ok || !a.ov)) return "null rows";
+  auto mis = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  if (mis(a.k) || mis(a.v) || mis(a.ok) || mis(a.ov) || mis(a.pool))
+    return "rows and pool must be 16-byte aligned";
+  if ((a.k_row | a.k_head | a.v_row | a.v_head) & 7) return "row and head strides must be multiples of 8";
+  return nullptr;
+}
+inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
+  if (const char* e = check_kv4_pool(a.n_kv, a.page_shift, a.n_pages)) return e;
+  if (a.n_rows < 0) return "negative row count";
+  if (a.n_heads < 1 || a.n_heads % a.n_kv) return "query heads must be a multiple of the kv heads";
+  if (a.n_heads / a.n_kv > 1024) return "more than 1024 query heads to a kv head";
+  if ((long long)a.n_rows * a.n_heads > 0x7fffffffll) return "too many query rows";
+  if (a.dtype != 1 && a.dtype != 2) return "dtype must be 1 (fp16) or 2 (bf16)";
+  if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
+  if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll)
+    return "table width out of range";
+  if (!(a.scale_log2 > 0.f) || a.scale_log2 > 1e30f) return "scale must be positive and finite";
+  if (!a.q || !a.out || !a.starts || !a.lens || !a.table || !a.pool || !a.err) return "null pointer";
+  auto mis = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  if (mis(a.q) || mis(a.out) || mis(a.pool) || mis(a.ws)) return "rows, pool and workspace must be 16-byte aligned";
+  if ((a.q_row | a.q_head) & 7) return "row and head strides must be multiples of 8";
+  return nullptr;
+}
+
+void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st);
+void launch_kv4_append(const Kv4RowsArgs& a, hipStream_t st);
+void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st);
+void launch_kv4_attend(const Kv4AttnArgs& a, hipStream_t st);
+
+}  // namespace dfl

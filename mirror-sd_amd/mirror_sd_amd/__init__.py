@@ -7,7 +7,7 @@ include/dflash_hip.h).
 
 from .config import DFlashConfig, Workload, build_target_layer_ids, extract_context_feature, workload
 
-__all__ = ["DFlashConfig", "DFlashDraftModel", "DFlashKVCache", "Workload",
+__all__ = ["DFlashConfig", "DFlashDraftModel", "DFlashKVCache", "KV4Cache", "Workload",
            "build_target_layer_ids", "extract_context_feature", "workload", "sample"]
 
 
@@ -16,4 +16,7 @@ def __getattr__(name):
     if name in ("DFlashDraftModel", "DFlashKVCache", "sample"):
         from . import dflash
         return getattr(dflash, name)
+    if name == "KV4Cache":
+        from .kv4 import KV4Cache
+        return KV4Cache
     raise AttributeError(name)

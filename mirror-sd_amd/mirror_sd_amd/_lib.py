@@ -34,6 +34,17 @@ class DflConfig(ctypes.Structure):
     ]
 
 
+class DflKv4Attn(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("q_row", c_int64),
+        ("q_head", c_int64), ("dtype", c_int32), ("n_rows", c_int32), ("n_heads", c_int32),
+        ("n_kv", c_int32), ("n_seq", c_int32), ("causal", c_int32), ("scale", ctypes.c_float),
+        ("starts", c_void_p), ("lens", c_void_p), ("table", c_void_p), ("width", c_int32),
+        ("page", c_int32), ("n_pages", c_int32), ("pool", c_void_p), ("ws", c_void_p),
+        ("ws_bytes", c_int64), ("err_flags", c_void_p),
+    ]
+
+
 PtrArray7 = c_void_p * 7
 
 # name -> (restype, argtypes); every symbol declared in include/dflash_hip.h
@@ -84,6 +95,17 @@ SIGNATURES = {
     "dfl_cache_assign": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
     "dfl_set_rope_scaling": (c_int32, [c_void_p, c_int32, ctypes.c_double, ctypes.c_double,
                                        ctypes.c_double, c_int32]),
+    "dfl_kv4_step": (c_int32, [c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_void_p]),
+    "dfl_kv4_step_scratch": (c_int64, [c_int32]),
+    "dfl_kv4_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                                 c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                                 c_void_p]),
+    "dfl_kv4_read": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int32,
+                               c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dfl_kv4_attend": (c_int32, [ctypes.POINTER(DflKv4Attn), c_void_p]),
+    "dfl_kv4_attend_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
 }
 
 _lib = None
