@@ -70,8 +70,10 @@ class KV4Cache:
         self.n_kv_heads, self.n_pages, self.page = int(n_kv_heads), int(n_pages), int(page)
         self.max_seqs, self.n_layers = int(max_seqs), int(n_layers)
         self.width = -(-int(max_len) // self.page)
-        self._L = _lib.load()
         dev = torch.device(device if device is not None else "cuda")
+        if dev.type != "cuda":
+            raise ValueError(f"the cache lives on a GPU, not on {dev}")
+        self._L = _lib.load()
         if dev.index is None:
             dev = torch.device(dev.type, torch.cuda.current_device())
         self.device = dev

@@ -241,7 +241,7 @@ def check(c, q, starts, held, lens, causal, out, lse=None, scale=128 ** -0.5):
             got = lse[a:b].double().cpu().numpy()
             empty = np.isneginf(l)
             assert (np.isneginf(got) == empty).all()
-            assert (np.abs(got - l)[~empty] <= ltol[~empty]).all(), s
+            assert (np.abs(got[~empty] - l[~empty]) <= ltol[~empty]).all(), s
 
 
 CASES = [  # heads, kv, q rows, lens, page
@@ -269,3 +269,309 @@ def test_attend(heads, kv, q_lens, lens, page, causal, dtype):
     check(c, q, starts, held, lens, causal, out, lse)
     # the same call again gives the same bits (no order of sums is left to chance)
     assert torch.equal(c.attend(q, starts, causal=causal), out)
+
+
+def test_long_caches():
+    """Tens of thousands of keys, one of them far above the rest (fp16 weights of the others lie
+    far below 1), and a short sequence beside."""
+    for dtype in ("fp16", "bf16"):
+        lens = [40007, 65]
+        c = make(n_kv_heads=1, max_seqs=2, max_len=40960, page=256, n_pages=170)
+        c.free.copy_(torch.arange(170, dtype=torch.int32))
+        step = c.step(grow=lens)
+        x = rows(sum(lens), 1, 3, DT[dtype])
+        q = queries(3, 4, 0, DT[dtype])
+        x[12345, 0, 0] = (q[0, 1] * 3).to(x.dtype)          # q.k about 3 * 128 * 2.25 * 128^-0.5 = 76
+        x[12345, 1, 0] = 0.0
+        c.append(x[:, 0], x[:, 1], step.slots)
+        held = R.values(x.double().cpu().numpy())
+        out, lse = c.attend(q, [0, 2, 3], return_lse=True, scale=0.02)
+        check(c, q, [0, 2, 3], held, lens, False, out, lse, scale=0.02)
+
+
+@pytest.mark.parametrize("q_rows", [1, 24])
+def test_pool_past_32_bits(q_rows):
+    """Pages whose bytes lie past 2^32 from the pool's start, in the second layer too."""
+    c = make(n_kv_heads=8, n_pages=17000, max_seqs=2, max_len=1024, page=256, n_layers=2)
+    assert c.pool[0].numel() > 2**32 and int(c.n_free) == 17000
+    c.free.copy_(torch.arange(17000, dtype=torch.int32))    # page 16999 first
+    lens = [300, 700]
+    _, held, step = fill(c, lens, 9, torch.float16, layer=1, shuffle=False)
+    assert int(step.slots[0]) == 16999 * 256
+    q = queries(2 * q_rows, 16, 1, torch.float16)
+    out = c.attend(q, [0, q_rows, 2 * q_rows], layer=1, causal=True)
+    check(c, q, [0, q_rows, 2 * q_rows], held, lens, True, out)
+    assert int(c.pool[0].max()) == 0
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("q_rows,heads", [(1, 4), (6, 4), (40, 6)])
+def test_what_a_row_does_not_see(dtype, q_rows, heads):
+    """Pool bytes that nobody wrote (all ones: NaN groups), NaN and infinite keys and values past a
+    row's last key: none of it reaches the row, all of it reaches the rows that see it."""
+    lens = [77, 130, 0, 33]
+    c = make(max_seqs=4, n_pages=14, page=64)
+    c.pool.fill_(255)
+    x, held, step = fill(c, lens, 21, DT[dtype])
+    starts = np.concatenate(([0], np.cumsum([min(q_rows, max(n, 1)) for n in lens]))).tolist()
+    q = queries(starts[-1], heads, 2, DT[dtype])
+    for causal in (False, True):
+        out, lse = c.attend(q, starts, causal=causal, return_lse=True)
+        check(c, q, starts, held, lens, causal, out, lse)
+    if q_rows == 1:
+        return
+    # sequence 1: its last key but two is NaN, a group of values two before it infinite
+    k_at, v_at = 77 + 127, 77 + 125
+    x[k_at, 0, :, 3] = float("nan")
+    x[v_at, 1, 1, 70] = float("inf")
+    c.append(x[:, 0], x[:, 1], step.slots)
+    out, lse = c.attend(q, starts, causal=True, return_lse=True)
+    want = R.values(x.double().cpu().numpy())
+    clean = np.nan_to_num(want, nan=0.0)
+    m = starts[2] - starts[1]
+    got = out[starts[1]:starts[2]].double().cpu().numpy()
+    for t in range(m):
+        see = 130 - m + t + 1
+        if see > 127:                                       # the NaN key: everything
+            assert np.isnan(got[t]).all(), t
+            assert np.isnan(lse[starts[1] + t].cpu().numpy()).all()
+        elif see > 125:                                     # the values' group 64 .. 95 of kv head 1
+            nan = np.zeros((heads, 128), bool)
+            nan[heads // 2:, 64:96] = True
+            assert (np.isnan(got[t]) == nan).all(), t
+        else:
+            assert np.isfinite(got[t]).all(), t
+    # the other sequences, and the rows before, are what they are without them
+    o, l, mass, size = R.attend(q[starts[1]:starts[2]].double().cpu().numpy(), clean[77:207, 0],
+                                clean[77:207, 1], True, 128 ** -0.5)
+    tol, _ = R.attend_tolerance(o, l, mass, size, 130, torch.finfo(q.dtype).eps / 2)
+    before = max(0, m - 5)
+    assert (np.abs(got - o)[:before] <= tol[:before]).all()
+    got0 = out[:starts[1]].double().cpu().numpy()
+    assert np.isfinite(got0).all()
+
+
+def test_largest_fp16_values():
+    """65504 in keys and values: a group's 65504 is held as 65536, past fp16's range, and still
+    weighs as such."""
+    c = make(n_kv_heads=1, max_seqs=1)
+    x = rows(40, 1, 4)
+    x[7, 1, 0, 9] = 65504.0
+    x[9, 1, 0, 100] = -61500.0
+    x[30, 0, 0, 64] = 65504.0
+    step = c.step(grow=[40, ])
+    c.append(x[:, 0], x[:, 1], step.slots)
+    held = R.values(x.double().cpu().numpy())
+    assert held.max() == 65536
+    q = queries(2, 2, 0, torch.float16) * 0.01
+    q[:, :, 64] = 0.0
+    out, lse = c.attend(q, [0, 2], return_lse=True)
+    check(c, q, [0, 2], held, [40], False, out, lse)
+
+
+def test_pages_and_ranges_that_do_not_fit():
+    from mirror_sd_amd import kv4
+    lens = [100, 90, 64]
+    c = make(max_seqs=3, n_pages=12, page=32)
+    _, held, _ = fill(c, lens, 1, torch.float16)
+    q = queries(6, 4, 0, torch.float16)
+    starts = [0, 2, 4, 6]
+    good = c.attend(q, starts)
+    table = c.table.clone()
+    for page in (-1, 12, -2**31, 2**31 - 1):
+        c.table[1, 1] = page                                # keys 32 .. 63 of sequence 1
+        out = c.attend(q, starts)
+        assert c.errors() == kv4.ERR_PAGE
+        assert torch.equal(out[:2], good[:2]) and torch.equal(out[4:], good[4:])
+        kv = np.concatenate((held[100:132], held[164:190]))
+        o, l, mass, size = R.attend(q[2:4].double().cpu().numpy(), kv[:, 0], kv[:, 1], False, 128 ** -0.5)
+        tol, _ = R.attend_tolerance(o, l, mass, size, 90, 2.0 ** -11)
+        assert (np.abs(out[2:4].double().cpu().numpy() - o) <= tol).all()
+        c.table.copy_(table)
+    # lengths beyond the table, rows beyond q or out of order: those sequences have no rows, and
+    # their rows of out stay as they were
+    for field, value, bad in [("lens", 1025, 1), ("lens", -1, 1), ("starts", [0, 2, 1, 3], 1),
+                              ("starts", [0, 2, 4, 7], 2), ("starts", [-1, 2, 4, 6], 0),
+                              ("lens", 2**31 - 1, 1)]:
+        st, keep = starts, c.lens.clone()
+        if field == "lens":
+            c.lens[1] = value
+        else:
+            st = value
+        out = torch.full_like(q, 7.0)
+        c.attend(q, st, out=out)
+        assert c.errors() == kv4.ERR_PAGE, (field, value)
+        assert (out[starts[bad]:starts[bad + 1]][-1] == 7.0).all(), (field, value)
+        c.lens.copy_(keep)
+    assert torch.equal(c.attend(q, starts), good) and c.errors() == 0
+
+
+def test_rows_of_no_sequence_stay():
+    c = make(max_seqs=3, n_pages=12)
+    _, held, _ = fill(c, [40, 0, 50], 1, torch.float16)
+    q = queries(9, 4, 0, torch.float16)
+    out = torch.full_like(q, 3.0)
+    got, lse = c.attend(q, [2, 3, 3, 6], causal=True, out=out, return_lse=True)
+    assert got is out and (out[:2] == 3.0).all() and (out[6:] == 3.0).all()
+    check(c, q[2:6], [0, 1, 1, 4], held, [40, 0, 50], True, out[2:6], lse[2:6])
+    none = c.attend(q, [4, 4, 4, 4], out=torch.full_like(q, 3.0))
+    assert (none == 3.0).all() and c.errors() == 0
+    assert c.attend(q[:0], [0, 0, 0, 0]).shape == (0, 4, 128)
+
+
+def test_queries_in_place_of_a_projection():
+    c = make(max_seqs=2, n_pages=12, n_kv_heads=2)
+    _, held, _ = fill(c, [70, 33], 5, torch.bfloat16)
+    wide = torch.randn((5, 6 * 128 + 40), device="cuda").bfloat16()
+    q = wide[:, 8:8 + 6 * 128].unflatten(1, (6, 128))
+    out = c.attend(q, [0, 3, 5], causal=True)
+    assert torch.equal(out, c.attend(q.contiguous(), [0, 3, 5], causal=True))
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(out, c.attend(heads_first, [0, 3, 5], causal=True))
+    check(c, q, [0, 3, 5], held, [70, 33], True, out)
+
+
+# ------------------------------------------------------------------ together
+
+
+def reference_step(hist, q, k, v, starts, causal):
+    """Plain caches (lists of held rows a sequence) after appending, and attention over them."""
+    out = np.zeros(q.shape)
+    bounds = []
+    for s in range(len(hist)):
+        a, b = starts[s], starts[s + 1]
+        hist[s] = np.concatenate((hist[s], np.stack((k[a:b], v[a:b]), 1)))
+        if a == b:
+            continue
+        o, l, mass, size = R.attend(q[a:b], hist[s][:, 0], hist[s][:, 1], causal, 128 ** -0.5)
+        out[a:b] = o
+        bounds.append((a, b, R.attend_tolerance(o, l, mass, size, len(hist[s]), 2.0 ** -11)[0]))
+    return out, bounds
+
+
+def test_drafting_loop():
+    """Prompts, then blocks whose rejected rows the next step drops, requests that end and others
+    that take their place, over two layers: as a drafting program runs it."""
+    rng = np.random.default_rng(2)
+    n_seq, layers, kv, heads = 5, 2, 2, 6
+    c = make(n_kv_heads=kv, max_seqs=n_seq, n_pages=40, max_len=320, page=32, n_layers=layers)
+    hist = [[np.zeros((0, 2, kv, 128)) for _ in range(n_seq)] for _ in range(layers)]
+    lens = np.zeros(n_seq, int)
+    for turn in range(12):
+        if turn % 4 == 0:                                   # a sequence or two begin anew
+            keep = np.where(rng.random(n_seq) < 0.4, 0, lens) if turn else lens
+            grow = np.where(keep == 0, rng.integers(1, 120, n_seq), 0)
+            causal = True
+        else:                                               # 8-row blocks, some of the last kept
+            keep = np.maximum(lens - rng.integers(0, 8, n_seq) * (turn % 4 > 1), 1)
+            grow = np.where(rng.random(n_seq) < 0.2, 0, 8)
+            causal = False
+        step = c.step(grow=grow.tolist(), keep=keep.tolist(), max_rows=int(grow.sum()) + 3)
+        starts = step.starts.tolist()
+        n = starts[-1]
+        assert n == grow.sum() and step.positions[:n].tolist() == [
+            p for s in range(n_seq) for p in range(keep[s], keep[s] + grow[s])]
+        lens = keep + grow
+        for layer in range(layers):
+            hist[layer] = [h[:keep[s]] for s, h in enumerate(hist[layer])]
+            x = rows(n + 3, kv, 100 * turn + layer)         # rows past the step's: slot -1
+            q = queries(n + 3, heads, turn + layer, torch.float16)
+            c.append(x[:, 0], x[:, 1], step.slots, layer)
+            out = c.attend(q, step.starts, layer, causal=causal)
+            held = R.values(x.double().cpu().numpy())
+            want, bounds = reference_step(hist[layer], q.double().cpu().numpy(), held[:, 0], held[:, 1],
+                                          starts, causal)
+            for a, b, tol in bounds:
+                assert (np.abs(out[a:b].double().cpu().numpy() - want[a:b]) <= tol).all(), (turn, layer)
+    assert c.errors() == 0 and c.lens.tolist() == lens.tolist()
+
+
+def test_results_join_over_keys():
+    """Attention over two caches joined by their sums equals attention over one with all rows."""
+    x = rows(200, 2, 8)
+    q = queries(3, 4, 8, torch.float16)
+    parts = []
+    for a, b in ((0, 200), (0, 77), (77, 200)):
+        c = make(max_seqs=1)
+        c.append(x[a:b, 0], x[a:b, 1], c.step(grow=[b - a]).slots)
+        parts.append(c.attend(q, [0, 3], return_lse=True))
+    (o, l), (o1, l1), (o2, l2) = [(a.double(), b.double()) for a, b in parts]
+    both = torch.logaddexp(l1, l2)
+    joined = o1 * torch.exp(l1 - both)[..., None] + o2 * torch.exp(l2 - both)[..., None]
+    # each side is off by its weights' and its result's rounding, 3 half steps of values below 10
+    assert float((joined - o).abs().max()) <= 2 * 3 * 2.0 ** -11 * 10 and float((both - l).abs().max()) <= 2.0 ** -9
+
+
+def test_captured_steps():
+    """A step, its rows and its attention in a graph, replayed with other lengths and rows between
+    eager work; a second graph beside it."""
+    caches = [make(max_seqs=3, n_pages=30, page=32) for _ in range(2)]
+    n = 12
+    grow, keep = (torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2))
+    x = rows(n, 2, 0)
+    q = queries(n, 4, 0, torch.float16)
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                           # first use outside of a capture
+        s = caches[0].step(grow=grow, keep=keep, max_rows=n)
+        caches[0].append(x[:, 0], x[:, 1], s.slots)
+        caches[0].attend(q, s.starts)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for causal in (False, True):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s = caches[0].step(grow=grow, keep=keep, max_rows=n)
+            caches[0].append(x[:, 0], x[:, 1], s.slots)
+            out = torch.zeros_like(q)
+            caches[0].attend(q, s.starts, causal=causal, out=out)
+        graphs.append(g)
+        outs.append((s, out))
+    rng = np.random.default_rng(0)
+    lens = np.zeros(3, int)
+    for turn in range(8):
+        k = np.maximum(lens - rng.integers(0, 4, 3), 0)
+        gr = rng.integers(0, 5, 3)
+        lens = k + gr
+        grow.copy_(torch.tensor(gr, dtype=torch.int32))
+        keep.copy_(torch.tensor(k, dtype=torch.int32))
+        x.copy_(rows(n, 2, turn))
+        q.copy_(queries(n, 4, turn, torch.float16))
+        graphs[turn % 2].replay()
+        got, out = outs[turn % 2]
+        e = caches[1].step(grow=grow, keep=keep, max_rows=n)
+        caches[1].append(x[:, 0], x[:, 1], e.slots)
+        want = caches[1].attend(q, e.starts, causal=bool(turn % 2), out=torch.zeros_like(q))
+        for a, b in zip(got, e):
+            assert torch.equal(a, b), turn
+        assert torch.equal(out, want), turn
+        torch.cuda.synchronize()
+    assert caches[0].errors() == caches[1].errors() == 0 and caches[0].lens.tolist() == lens.tolist()
+
+
+def test_another_stream():
+    c, d = make(max_seqs=2), make(max_seqs=2)
+    x, q = rows(90, 2, 0), queries(4, 4, 0, torch.float16)
+    d.append(x[:, 0], x[:, 1], d.step(grow=[60, 30]).slots)
+    want = d.attend(q, [0, 2, 4])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        s = c.step(grow=[60, 30])
+        c.append(x[:, 0], x[:, 1], s.slots)
+        got = c.attend(q, [0, 2, 4])
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_refusals_on_the_device():
+    c = make()
+    with pytest.raises(ValueError, match="max_rows"):
+        c.step(grow=torch.zeros(4, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError, match="cpu"):
+        c.attend(torch.zeros((1, 4, 128), dtype=torch.float16), [0, 1, 1, 1, 1])
+    with pytest.raises(ValueError, match="layer"):
+        c.read([0], layer=1)
+    assert c.read([], dtype=torch.float32)[0].shape == (0, 2, 128)
+    assert c.errors() == 0
