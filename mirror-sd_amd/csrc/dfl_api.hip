@@ -1733,8 +1733,8 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
 
 int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq) {
   if (n_rows < 1 || n_heads < 1 || n_kv < 1 || n_seq < 1 || n_heads % n_kv) return 0;
-  return 2ll * kv4_workers(n_rows, n_heads, n_kv, n_seq) *
-         kv4_piece_floats(kv4_tile_rows(n_rows, n_heads, n_kv, n_seq)) * (long long)sizeof(float);
+  const Kv4Cut c = kv4_cut(n_rows, n_heads, n_kv, n_seq);
+  return c.whole ? 0 : 2ll * c.workers * kv4_piece_floats(c.tile_rows) * (long long)sizeof(float);
 }
 
 int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
@@ -1763,7 +1763,6 @@ int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
   a.err = args->err_flags;
   if (a.n_rows == 0) return DFL_OK;
   if (const char* e = check_kv4_attn(a)) return fail(DFL_EINVAL, std::string("dfl_kv4_attend: ") + e);
-  a.workers = kv4_workers(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
   const int64_t need = dfl_kv4_attend_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
   if (need > 0 && (!a.ws || args->ws_bytes < need))
     return fail(DFL_EINVAL, "dfl_kv4_attend: workspace of " + std::to_string(need) + " bytes needed");

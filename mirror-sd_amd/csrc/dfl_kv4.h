@@ -10,14 +10,13 @@
 //
 // Layout.  The pool is [layer][page][kv head][page / 32] blocks of 4352 bytes, a block being 32
 // consecutive rows (keys) of one head:
-//   bytes    0 .. 2047   K codes, 64 bytes a row, in the row order kv4_row
+//   bytes    0 .. 2047   K codes: 16 bytes of each row's group 0, then of group 1, 2, 3
 //   bytes 2048 .. 4095   V codes, the same
-//   bytes 4096 .. 4351   exponent bytes, 4 a word: word i + 16 g holds group g of the keys
-//                        kv4_key(i, 0) and kv4_key(i, 1): bytes K0, K1, V0, V1
-// In a row the byte e holds values 2e (low nibble) and 2e + 1.  So a wave reads a block as four
-// 1 KiB loads and one of 256 bytes, every lane getting the operand of its own matrix row: lane
-// l = i + 16 g takes, of K and of V, 16 bytes of row i and of row 16 + i (values 32 g .. 32 g + 31,
-// one group) and the four exponent bytes that go with them.
+//   bytes 4096 .. 4351   exponent bytes, 4 a word: word i + 16 g holds group g of the rows i and
+//                        16 + i: bytes K0, K1, V0, V1
+// In a group's 16 bytes the byte e holds values 2e (low nibble) and 2e + 1.  A lane's operand of a
+// matrix product is a row's group, so a wave reads a block in pieces of 1 KiB in which lane after
+// lane takes 16 bytes, from memory as from LDS.
 //
 // Everything here but the launchers is plain host code too, so that it can be tested on a CPU.
 #pragma once
@@ -43,19 +42,18 @@ constexpr int KV4_ERR_ROWS = 32;     // step: more new rows than the slot map ho
 constexpr int KV4_ERR_SLOT = 64;     // append, read: a slot outside the pool
 constexpr int KV4_ERR_PAGE = 128;    // attend, step: a page, length or row range out of bounds
 
-// Row of a block that holds key k (k in [0, 32)) and back.  The matrix product S^T = K Q^T gives
-// lane (q, g) rows 4g .. 4g+3 of each 16-row tile; with tile 0 holding keys 8g + 0..3 and tile 1
-// keys 8g + 4..7 these are the 8 consecutive keys that the product with V takes from that lane.
-DFL_HD int kv4_row(int k) { return ((k >> 3) << 2) + (k & 3) + ((k & 4) << 2); }
-DFL_HD int kv4_key(int i, int tile) { return ((i >> 2) << 3) + (i & 3) + 4 * tile; }
-// Offset in a block of the exponent byte of group g of K (v = 0) or V (v = 1), row r of the block.
+// Offsets in a block, of K (v = 0) or V (v = 1): the 16 code bytes of group g of row r, and its
+// exponent byte.
+DFL_HD int kv4_code_at(int r, int g, int v) { return v * KV4_V + g * 512 + r * 16; }
 DFL_HD int kv4_scale_at(int r, int g, int v) {
   return KV4_SC + 4 * ((r & 15) + 16 * g) + 2 * v + (r >> 4);
 }
-// Byte offset of block `sub` of a page's head.
-DFL_HD long long kv4_block_at(long long page_idx, int n_kv, int head, int subs, int sub) {
-  return ((page_idx * n_kv + head) * subs + sub) * (long long)KV4_BLOCK;
+// Number and byte offset in a layer's pool of block `sub` of a page's head (check_kv4_pool keeps
+// the number within 32 bits).
+DFL_HD uint32_t kv4_block_no(uint32_t page, int n_kv, int head, int sub_shift, int sub) {
+  return ((page * (uint32_t)n_kv + (uint32_t)head) << sub_shift) + (uint32_t)sub;
 }
+DFL_HD unsigned long long kv4_block_at(uint32_t no) { return (unsigned long long)no * KV4_BLOCK; }
 
 DFL_HD int kv4_pages(int n, int page_shift) { return (int)(((long long)n + (1 << page_shift) - 1) >> page_shift); }
 
@@ -111,14 +109,18 @@ struct Kv4AttnArgs {
   int width, page_shift, n_pages;
   const unsigned char* pool;   // one layer's pages
   float* ws;
-  int workers;                 // workgroups that share the key blocks
+  int workers;                 // workgroups that share the places (Kv4Cut)
   int* err;
 };
 
-// The work of a launch in key blocks: sequence s contributes, for each of its query tiles and kv
-// heads, one unit of nblk blocks; units are numbered sequence by sequence, head by head.  Worker w
-// takes blocks [w * per, (w + 1) * per) of all units in a row; a unit that several workers share
-// leaves one partial result with each (slot kv4_piece), which the merge joins.
+// The work of a launch.  Sequence s contributes, for each of its query tiles and kv heads, one
+// unit of nblk key blocks; units are numbered sequence by sequence, head by head.  A unit spans
+// KV4_PAD + nblk places: the first KV4_PAD stand for what a unit costs besides its blocks (finding
+// it, its queries, the first loads' latency, its result), so that a worker with many short units
+// has no more to do than one with a part of a long one.  Worker w takes the places
+// [w * per, (w + 1) * per); a unit whose blocks several workers share leaves one partial result
+// with each (slot kv4_piece), which the merge joins.
+constexpr int KV4_PAD = 8;
 struct Kv4Seq { int q0, qlen, len, tiles, nblk; bool bad; };
 DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_shift, int ratio,
                       int tile_rows) {
@@ -133,29 +135,37 @@ DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_s
   s.nblk = s.qlen ? (s.len > 0 ? (s.len + KV4_KEYS - 1) / KV4_KEYS : 1) : 0;
   return s;
 }
-DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return (long long)s.tiles * n_kv * s.nblk; }
-constexpr int KV4_MIN_BLOCKS = 16;   // fewest blocks of a worker (four for each of its waves)
+DFL_HD int kv4_span(const Kv4Seq& s) { return KV4_PAD + s.nblk; }
+DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return (long long)s.tiles * n_kv * kv4_span(s); }
+constexpr int KV4_MIN_PLACES = 24;   // fewest places of a worker
 DFL_HD long long kv4_per(long long total, int workers) {
   const long long per = (total + workers - 1) / workers;
-  return per < KV4_MIN_BLOCKS ? KV4_MIN_BLOCKS : per;
+  return per < KV4_MIN_PLACES ? KV4_MIN_PLACES : per;
 }
-// Partial slot of worker w for a unit that begins at block u0 (of all) and is shared: the unit a
-// worker begins with, and the one it ends with.
-DFL_HD long long kv4_piece(long long w, long long per, long long u0) {
-  return 2 * w + (u0 < w * per ? 0 : 1);
+// Partial slot of worker w for a shared unit whose first block is at place r0: a worker has at
+// most one unit that it goes on with, and one that it begins and leaves.
+DFL_HD long long kv4_piece(long long w, long long per, long long r0) {
+  return 2 * w + (r0 < w * per ? 0 : 1);
 }
-// Floats of one partial: O [tile rows][128], then (max, sum) a row.
+// Floats of one partial: O [tile rows][128] in the order of the kernel's registers, then (max,
+// sum) a row.
 DFL_HD long long kv4_piece_floats(int tile_rows) { return (long long)tile_rows * (KV4_D + 2); }
 
-// Query rows of a tile, and workgroups, of a launch.
-int kv4_tile_rows(int n_rows, int n_heads, int n_kv, int n_seq);
-int kv4_workers(int n_rows, int n_heads, int n_kv, int n_seq);
+// How a launch is cut (what its workspace holds follows from it).
+struct Kv4Cut {
+  int tile_rows;   // query rows of a unit: 16 or 32 (each wave has them all and a fourth of the
+                   // keys) or 64, 128 (each wave has 32 of them and all keys)
+  int workers;     // workgroups, or
+  bool whole;      // each unit whole to a workgroup of its own, no workspace
+};
+Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq);
 
 inline const char* check_kv4_pool(int n_kv, int page_shift, int n_pages) {
   if (n_kv < 1 || n_kv > 1024) return "kv heads outside [1, 1024]";
   if (page_shift < 5 || page_shift > 8) return "page rows must be 32, 64, 128 or 256";
-  if (n_pages < 1 || ((long long)n_pages << page_shift) > 0x7fffffffll)
-    return "pool pages out of range (at least one, slots below 2^31)";
+  if (n_pages < 1 || ((long long)n_pages << page_shift) > 0x7fffffffll ||
+      (((long long)n_pages * n_kv) << (page_shift - 5)) > 0xffffffffll)
+    return "pool pages out of range (at least one, slots below 2^31, blocks below 2^32)";
   return nullptr;
 }
 inline const char* check_kv4_step(const Kv4StepArgs& a) {

@@ -213,8 +213,8 @@ DFL_DEV bool slot_at(const Kv4RowsArgs& a, int slot, int head, unsigned char*& b
     return false;
   }
   const int in = slot & ((1 << a.page_shift) - 1);
-  blk = a.pool + kv4_block_at(slot >> a.page_shift, a.n_kv, head, 1 << (a.page_shift - 5), in >> 5);
-  r = kv4_row(in & 31);
+  blk = a.pool + kv4_block_at(kv4_block_no(slot >> a.page_shift, a.n_kv, head, a.page_shift - 5, in >> 5));
+  r = in & 31;
   return true;
 }
 
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4RowsArgs a) {
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-    *reinterpret_cast<uint32_t*>(blk + v * KV4_V + r * 64 + part * 4) = bad ? 0u : w;
+    *reinterpret_cast<uint32_t*>(blk + kv4_code_at(r, part >> 2, v) + 4 * (part & 3)) = bad ? 0u : w;
     if ((part & 3) == 0) blk[kv4_scale_at(r, part >> 2, v)] = (unsigned char)b;
   }
 }
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsArgs a) {
     uint32_t w = 0;
     float s = 1.f;
     if (slot_at(a, a.slots[row], head, blk, r)) {
-      w = *reinterpret_cast<const uint32_t*>(blk + v * KV4_V + r * 64 + part * 4);
+      w = *reinterpret_cast<const uint32_t*>(blk + kv4_code_at(r, part >> 2, v) + 4 * (part & 3));
       s = __uint_as_float((uint32_t)blk[kv4_scale_at(r, part >> 2, v)] << 23);
     }
     typedef typename RowT<DT>::t E;
@@ -304,26 +304,23 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsArgs a) {
 //
 // O = softmax(scale * Q K^T) V over each sequence's cached rows, K and V in 4 bits.
 //
-// A unit is a tile of 16 NT query rows (row = token * ratio + head in group) of one sequence and
-// kv head.  A workgroup takes a run of key blocks of a unit, its four waves every fourth block
-// each, with a wave's whole work on a block in its own registers and its own 9 KiB of LDS (no
-// barrier in the loop):
-//   S^T = K Q^T   v_mfma 16x16x32, keys on the M axis, K converted from codes in registers (two
-//                 values an instruction, their power of two applied by it: exact);
-//   softmax       fp32, log2 domain, reference maximum raised only when a block exceeds it by
+// A unit is a tile of query rows (row = token * ratio + head in group) of one sequence and kv
+// head; a workgroup takes a run of key blocks of a unit (32 keys each).  Of a block:
+//   S^T = K Q^T   matrix instructions with keys on the M axis, K converted from codes in registers
+//                 (two values an instruction, which applies their power of two: exact);
+//   softmax       fp32, log2 domain, the reference maximum raised only when a block exceeds it by
 //                 more than KV4_SLACK; weights rounded to the type of Q, and summed as rounded;
 //   O^T += V^T P  V converted in registers, written to LDS as rows, read back transposed
-//                 (ds_read_b64_tr_b16); P from the S^T accumulators as they lie (kv4_row).
-// The next block's codes load while this one computes.
+//                 (ds_read_b64_tr_b16); P from the S^T accumulators as they lie: the rows of V that
+//                 a lane's weights stand for are those whose keys its accumulators hold.
+// Two kernels: kv4_attn_kernel for up to 32 rows (single tokens, small blocks), where HBM and
+// latency count, and kv4_tile_kernel for more.
 
 constexpr float KV4_SLACK = 6.f;
 // Weights are 2^(s - m + KV4_LIFT) <= 2^15 for a reference m: fp16 then keeps 2^-23 of the
 // largest weight as a normal number and 2^-34 as the rounding of the smallest, so that a million
 // keys far below one large one still add up.
 constexpr float KV4_LIFT = 9.f;
-constexpr int VROW = 288;                 // bytes of a V row in LDS: 8 banks apart, so that the 8
-                                          // rows of a half wave's transposing read do not collide
-constexpr int VWAVE = 32 * VROW;
 
 template <typename T> struct Mat;
 template <> struct Mat<half_t> {
@@ -334,6 +331,9 @@ template <> struct Mat<half_t> {
   typedef half2_t v2;
   static DFL_DEV floatx4 mfma(v8 a, v8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static DFL_DEV floatx16 mfma(v8 a, v8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   static DFL_DEV v8 dequant(uint32_t w, float s) {
     const v2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0);
@@ -353,6 +353,9 @@ template <> struct Mat<bf16_t> {
   static DFL_DEV floatx4 mfma(v8 a, v8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
+  static DFL_DEV floatx16 mfma(v8 a, v8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
   static DFL_DEV v8 dequant(uint32_t w, float s) {
     const v2 p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0);
     const v2 p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
@@ -360,20 +363,47 @@ template <> struct Mat<bf16_t> {
     const v2 p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
     return (v8){p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
   }
-  static DFL_DEV float sum2(v2 p, float c) { return c + ((float)p.x + (float)p.y); }
+  static DFL_DEV float sum2(v2 p, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, (v2){(bf16_t)1.f, (bf16_t)1.f}, c, false);
+  }
 };
+// Two 4-key halves of a V operand, read transposed: the lanes' addresses are those of rows, what
+// they get is 4 keys of one value.
+template <typename T>
+DFL_DEV typename Mat<T>::v8 read_vt(const unsigned char* lo, const unsigned char* hi) {
+  typedef __attribute__((address_space(3))) short4_t* lp;
+  typedef short short8_t __attribute__((ext_vector_type(8)));
+  const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)lo);
+  const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)hi);
+  return __builtin_bit_cast(typename Mat<T>::v8, (short8_t){a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
+}
+DFL_DEV float exponent(uint32_t b) { return __uint_as_float(b << 23); }
 
-// Sequence s of the launch, and (lane 0 of the caller's choice) its error bit.
+// An int that no kernel writes while this one runs, at a uniform address: a scalar load.
+DFL_DEV int load_const(const int* p) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
+}
+// A value that is the same in all lanes, as the compiler cannot know: into scalar registers.
+DFL_DEV long long uniform(long long v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((unsigned long long)v >> 32));
+  return (long long)((unsigned long long)hi << 32 | lo);
+}
 DFL_DEV Kv4Seq attn_seq(const Kv4AttnArgs& a, int s, int tile_rows) {
   return kv4_seq(a.starts[s], a.starts[s + 1], a.lens[s], a.n_rows, a.width, a.page_shift,
                  a.n_heads / a.n_kv, tile_rows);
+}
+// The same for an s that is uniform.
+DFL_DEV Kv4Seq attn_seq_uniform(const Kv4AttnArgs& a, int s, int tile_rows) {
+  return kv4_seq(load_const(a.starts + s), load_const(a.starts + s + 1), load_const(a.lens + s),
+                 a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, tile_rows);
 }
 DFL_DEV long long wave_sum_ll(long long v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// Key blocks of all units; every lane gets the sum.
+// Places of all units; every lane gets the sum.
 DFL_DEV long long attn_total(const Kv4AttnArgs& a, int tile_rows) {
   const int lane = threadIdx.x & 63;
   long long t = 0;
@@ -384,8 +414,8 @@ DFL_DEV long long attn_total(const Kv4AttnArgs& a, int tile_rows) {
   }
   return wave_sum_ll(t);
 }
-// The sequence that holds position pos of a cumulative count (blocks: its blocks; else its units),
-// and the count before it.  pos must lie below the total.
+// The sequence that holds place (UNITS: unit) pos, and the places (units) before it; n_seq if pos
+// is past the last.
 template <bool UNITS>
 DFL_DEV int attn_find(const Kv4AttnArgs& a, int tile_rows, long long pos, long long& before) {
   const int lane = threadIdx.x & 63;
@@ -413,11 +443,94 @@ DFL_DEV int attn_find(const Kv4AttnArgs& a, int tile_rows, long long pos, long l
   before = acc;
   return a.n_seq;
 }
+// n / d for 0 <= n, 0 < d, in 32 bits where it fits (the wide division is a hundred instructions).
+DFL_DEV long long div_ll(long long n, int d) {
+  return n <= 0xffffffffll ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+}
 
-// Visible keys of row `row` (token * ratio + head) of a sequence.
+// Visible keys of a token of a sequence (they grow with the token).
 DFL_DEV int attn_visible(const Kv4AttnArgs& a, const Kv4Seq& q, int token) {
   return a.causal ? max(0, min(q.len, q.len - q.qlen + token + 1)) : q.len;
 }
+
+// A worker's walk over its places: run after run of blocks [b0, b1) of a unit.
+struct Run {
+  Kv4Seq sq;
+  int s, head, tile, b0, b1;
+  bool whole;          // all of the unit's blocks
+  long long r0;        // place of the unit's first block
+};
+struct Walk { long long pos, end, per, w; };
+template <bool WHOLE>
+DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k) {
+  k.w = blockIdx.x;
+  if constexpr (WHOLE) {
+    if (k.w == 0) attn_total(a, tile_rows);   // (for its error bit)
+    k.pos = k.w;
+    k.end = k.w + 1;
+    k.per = 1;
+  } else {
+    const long long total = uniform(attn_total(a, tile_rows));
+    k.per = kv4_per(total, a.workers);
+    k.pos = k.w * k.per;
+    k.end = min(total, k.pos + k.per);
+  }
+  return k.pos < k.end;
+}
+// The next run; false at the end.  (Everything here is uniform over the workgroup.)
+template <bool WHOLE>
+DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
+  while (k.pos < k.end) {
+    long long at;
+    r.s = __builtin_amdgcn_readfirstlane(attn_find<WHOLE>(a, tile_rows, k.pos, at));
+    if (r.s >= a.n_seq) return false;
+    at = uniform(at);
+    r.sq = attn_seq_uniform(a, r.s, tile_rows);
+    const int span = WHOLE ? 1 : kv4_span(r.sq);
+    const long long unit = div_ll(k.pos - at, span);
+    r.head = (int)div_ll(unit, r.sq.tiles);
+    r.tile = (int)(unit - (long long)r.head * r.sq.tiles);
+    r.whole = true;
+    if constexpr (WHOLE) {
+      // the last tiles of a prompt see the most keys: they go first
+      r.tile = r.sq.tiles - 1 - r.tile;
+      r.b0 = 0;
+      r.b1 = r.sq.nblk;
+      r.r0 = 0;
+      k.pos = k.end;
+    } else {
+      r.r0 = at + unit * span + KV4_PAD;
+      r.b0 = (int)max(0ll, k.pos - r.r0);
+      r.b1 = (int)min((long long)r.sq.nblk, k.end - r.r0);
+      r.whole = r.b0 == 0 && r.b1 == r.sq.nblk;
+      k.pos = r.r0 + r.sq.nblk;
+      if (r.b1 <= 0) continue;   // only places before the first block
+    }
+    return true;
+  }
+  return false;
+}
+
+// The page of block b of a run's keys; -1: there is no such page (its keys are absent).
+DFL_DEV int page_of(const Kv4AttnArgs& a, const Run& r, int b) {
+  const int page = load_const(a.table + (long long)r.s * a.width + (b >> (a.page_shift - 5)));
+  return page >= a.n_pages || page < 0 ? -1 : page;
+}
+// Address of block b in a page (for page -1 some address in the pool).
+DFL_DEV const unsigned char* block_in(const Kv4AttnArgs& a, const Run& r, int b, int page) {
+  const int sh = a.page_shift - 5;
+  return a.pool + kv4_block_at(kv4_block_no(max(page, 0), a.n_kv, r.head, sh, b & ((1 << sh) - 1)));
+}
+
+// ---- up to 32 query rows
+//
+// The four waves of a workgroup take every fourth block of a run each, a wave's whole work on a
+// block in its own registers and its own 9 KiB of LDS (no barrier in the loop); their states are
+// joined at the run's end.  The next block's codes load while this one computes.
+
+constexpr int VROW = 288;                 // bytes of a V row in LDS: 8 banks apart, so that the 8
+                                          // rows of a half wave's transposing read do not collide
+constexpr int VWAVE = 32 * VROW;
 
 template <typename T, int NT>
 __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnArgs a) {
@@ -433,51 +546,29 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
   unsigned char* vbuf = lds + wv * VWAVE;
   const unsigned char* vread = vbuf + (4 * g + (i >> 2)) * VROW + 8 * (i & 3);
   unsigned char* vwrite = vbuf + i * VROW + 64 * g;
-
   const float scale = a.scale_log2 * (1.f / M::kUnit);
-  const long long total = attn_total(a, ROWS);
-  const long long per = kv4_per(total, a.workers);
-  const long long w = blockIdx.x;
-  long long pos = w * per;
-  const long long end = min(total, pos + per);
-  while (pos < end) {
-    // the unit at pos, and the run [b0, b1) of its blocks
-    long long s_at;
-    const int s = __builtin_amdgcn_readfirstlane(attn_find<false>(a, ROWS, pos, s_at));
-    if (s >= a.n_seq) break;   // (cannot be: pos < total)
-    const Kv4Seq sq = attn_seq(a, s, ROWS);
-    const long long unit = (pos - s_at) / sq.nblk;
-    const long long u0 = s_at + unit * sq.nblk;
-    const int b0 = (int)(pos - u0), b1 = (int)min((long long)sq.nblk, b0 + (end - pos));
-    const int head = (int)(unit / sq.tiles), tile = (int)(unit - (long long)head * sq.tiles);
-    pos += b1 - b0;
-    const bool whole = b0 == 0 && b1 == sq.nblk;
 
+  Walk walk;
+  Run run;
+  if (!walk_begin<false>(a, ROWS, walk)) return;
+  while (walk_next<false>(a, ROWS, walk, run)) {
+    const Kv4Seq& sq = run.sq;
     // query fragments: step st covers values 32 g + 8 st ..; visible keys of this lane's rows
     v8 qf[NT][4];
     int vis[NT];
-    int vmin = 0x7fffffff, vmax = 0;
     const int n_row = sq.qlen * ratio;   // rows of the sequence and kv head
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = (tile * NT + n) * 16 + i;
-      const int rr = min(r, n_row - 1);
-      const int tok = rr / ratio;
+      const int r = min((run.tile * NT + n) * 16 + i, n_row - 1);
+      const int tok = r / ratio;
       const T* qp = reinterpret_cast<const T*>(a.q) + (long long)(sq.q0 + tok) * a.q_row +
-                    (long long)(head * ratio + rr - tok * ratio) * a.q_head + 32 * g;
+                    (long long)(run.head * ratio + r - tok * ratio) * a.q_head + 32 * g;
 #pragma unroll
       for (int st = 0; st < 4; ++st) qf[n][st] = *reinterpret_cast<const v8*>(qp + 8 * st);
       vis[n] = attn_visible(a, sq, tok);
-      vmin = min(vmin, vis[n]);
-      vmax = max(vmax, vis[n]);
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-      vmin = min(vmin, __shfl_xor(vmin, o, 64));
-      vmax = max(vmax, __shfl_xor(vmax, o, 64));
-    }
-    vmin = __builtin_amdgcn_readfirstlane(vmin);
-    vmax = __builtin_amdgcn_readfirstlane(vmax);
+    const int vmin = attn_visible(a, sq, run.tile * ROWS / ratio);
+    const int vmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
 
     floatx4 o[NT][8];
     float mrun[NT], lrun[NT];
@@ -488,30 +579,21 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 #pragma unroll
       for (int d = 0; d < 8; ++d) o[n][d] = (floatx4){0.f, 0.f, 0.f, 0.f};
     }
-
-    const int subs_shift = a.page_shift - 5;
-    const int* trow = a.table + (long long)s * a.width;
-    // block b's address; pg < 0: no such page (its keys are absent)
-    auto block_ptr = [&](int b, int& pg) {
-      pg = trow[b >> subs_shift];
-      if (pg >= a.n_pages) pg = -1;
-      return a.pool + kv4_block_at(max(pg, 0), a.n_kv, head, 1 << subs_shift,
-                                   b & ((1 << subs_shift) - 1));
-    };
     u32x4 kc[2], vc[2];
     uint32_t sc = 0;
     int pg = 0;
     auto load_block = [&](int b) {
-      const unsigned char* p = block_ptr(b, pg);
-      kc[0] = load_vec(p + 16 * (4 * i + g));
-      kc[1] = load_vec(p + 1024 + 16 * (4 * i + g));
-      vc[0] = load_vec(p + KV4_V + 16 * (4 * i + g));
-      vc[1] = load_vec(p + KV4_V + 1024 + 16 * (4 * i + g));
+      pg = page_of(a, run, b);
+      const unsigned char* p = block_in(a, run, b, pg);
+      kc[0] = load_vec(p + kv4_code_at(i, g, 0));
+      kc[1] = load_vec(p + kv4_code_at(16 + i, g, 0));
+      vc[0] = load_vec(p + kv4_code_at(i, g, 1));
+      vc[1] = load_vec(p + kv4_code_at(16 + i, g, 1));
       sc = *reinterpret_cast<const uint32_t*>(p + KV4_SC + 4 * lane);
     };
     // blocks that no row of the tile sees add nothing
-    const int b_end = min(b1, (vmax + KV4_KEYS - 1) / KV4_KEYS);
-    int b = b0 + wv;
+    const int b_end = min(run.b1, (vmax + KV4_KEYS - 1) / KV4_KEYS);
+    int b = run.b0 + wv;
     if (b < b_end) load_block(b);
     for (; b < b_end; b += 4) {
       u32x4 k0 = kc[0], k1 = kc[1], v0 = vc[0], v1 = vc[1];
@@ -520,40 +602,33 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       if (b + 4 < b_end) load_block(b + 4);
       const int kbase = b * KV4_KEYS;
       const bool masked = kbase + KV4_KEYS > vmin || page < 0;   // (uniform)
-      unsigned long long poison = 0;
       if (masked) {
         if (page < 0 && lane == 0) atomicOr(a.err, KV4_ERR_PAGE);
         // V rows that nobody may see, and groups that stand for NaN (they must not reach a row
-        // that does not see them, as 0 * NaN): zero codes; the rows that do see one are set below
+        // that does not see them, as 0 * NaN): zero codes; the rows that do see one are set here
         const int lim = page < 0 ? 0 : sq.len;
-        const bool gone0 = kbase + kv4_key(i, 0) >= lim, gone1 = kbase + kv4_key(i, 1) >= lim;
+        const bool gone0 = kbase + i >= lim, gone1 = kbase + 16 + i >= lim;
         const bool nan0 = !gone0 && ((s4 >> 16) & 255) == 255, nan1 = !gone1 && (s4 >> 24) == 255;
         if (gone0 || nan0) { v0 = (u32x4){0, 0, 0, 0}; s4 &= 0xff00ffffu; }
         if (gone1 || nan1) { v1 = (u32x4){0, 0, 0, 0}; s4 &= 0x00ffffffu; }
-        poison = __ballot(nan0 || nan1);
-        if (poison) {
-          // o of every row that sees such a key, in the values of that group
+        const float nan = __builtin_nanf("");
+        if (__ballot(nan0 || nan1)) {
 #pragma unroll 1
           for (int key = 0; key < KV4_KEYS; ++key) {
-            const int r = kv4_row(key);
-            const unsigned long long hit = __ballot((r >> 4) ? nan1 : nan0);
+            const unsigned long long hit = __ballot(key < 16 ? nan0 : nan1) >> (key & 15);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               if (kbase + key < vis[n])
                 static_for<0, 4>([&](auto group) {
                   constexpr int gr = group;
-                  if ((hit >> ((r & 15) + 16 * gr)) & 1) {
-                    o[n][2 * gr] = o[n][2 * gr + 1] =
-                        (floatx4){__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-                  }
+                  if ((hit >> (16 * gr)) & 1)
+                    o[n][2 * gr] = o[n][2 * gr + 1] = (floatx4){nan, nan, nan, nan};
                 });
           }
         }
       }
-      const float sk0 = M::kUnit * __uint_as_float((s4 & 255u) << 23);
-      const float sk1 = M::kUnit * __uint_as_float(((s4 >> 8) & 255u) << 23);
-      const float sv0 = M::kUnit * __uint_as_float(((s4 >> 16) & 255u) << 23);
-      const float sv1 = M::kUnit * __uint_as_float((s4 >> 24) << 23);
+      const float sk0 = M::kUnit * exponent(s4 & 255u), sk1 = M::kUnit * exponent((s4 >> 8) & 255u);
+      const float sv0 = M::kUnit * exponent((s4 >> 16) & 255u), sv1 = M::kUnit * exponent(s4 >> 24);
       floatx4 sa[NT], sb[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) sa[n] = sb[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
@@ -566,29 +641,32 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
           sb[n] = M::mfma(f1, qf[n][st], sb[n]);
         }
       });
+      __builtin_amdgcn_sched_barrier(0);   // (fewer operands in flight: 168 registers)
       static_for<0, 4>([&](auto step) {
         constexpr int st = step;
         *reinterpret_cast<v8*>(vwrite + 16 * st) = M::dequant(v0[st], sv0);
         *reinterpret_cast<v8*>(vwrite + 16 * VROW + 16 * st) = M::dequant(v1[st], sv1);
       });
-      // softmax of this lane's 8 keys (kbase + 8 g ..) for its row i of each tile
+      // softmax of this lane's 8 keys (4 g .. 4 g + 3 and 16 on) for its row i of each tile
       v8 pf[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float v[8];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          v[r] = sa[n][r] * scale;
-          v[4 + r] = sb[n][r] * scale;
+          v[r] = sa[n][r];
+          v[4 + r] = sb[n][r];
         }
         if (masked) {
+          asm volatile("");   // (a branch: as selects these are a part of every step)
           const int lim = page < 0 ? 0 : vis[n];
 #pragma unroll
           for (int r = 0; r < 8; ++r)
-            if (kbase + 8 * g + r >= lim) v[r] = -INFINITY;
+            if (kbase + 4 * g + (r & 3) + 16 * (r >> 2) >= lim) v[r] = -INFINITY;
         }
-        float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
-                          fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        // (scale > 0: the largest logit is the largest product's)
+        float top = scale * fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])),
+                                  fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
         if (!__all(top <= mrun[n] + KV4_SLACK)) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -599,11 +677,12 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
           for (int d = 0; d < 8; ++d) o[n][d] *= alpha;
           mrun[n] = mnew;
         }
-        const float ref = mrun[n] - KV4_LIFT;
+        const float ref = KV4_LIFT - mrun[n];
 #pragma unroll
         for (int r = 0; r < 8; r += 2) {
           const v2 p = __builtin_convertvector(
-              ((floatx2){__builtin_amdgcn_exp2f(v[r] - ref), __builtin_amdgcn_exp2f(v[r + 1] - ref)}), v2);
+              ((floatx2){__builtin_amdgcn_exp2f(__builtin_fmaf(v[r], scale, ref)),
+                         __builtin_amdgcn_exp2f(__builtin_fmaf(v[r + 1], scale, ref))}), v2);
           lrun[n] = M::sum2(p, lrun[n]);
           pf[n][r] = p.x;
           pf[n][r + 1] = p.y;
@@ -611,18 +690,15 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       }
       static_for<0, 8>([&](auto dt) {
         constexpr int d = dt;
-        typedef __attribute__((address_space(3))) short4_t* lp;
-        const short4_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vread + 32 * d));
-        const short4_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(vread + 16 * VROW + 32 * d));
-        typedef short short8_t __attribute__((ext_vector_type(8)));
-        const v8 vf = __builtin_bit_cast(
-            v8, (short8_t){t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w});
+        const v8 vf = read_vt<T>(vread + 32 * d, vread + 16 * VROW + 32 * d);
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n][d] = M::mfma(vf, pf[n], o[n][d]);
       });
     }
 
     // join the four waves: a row's reference is its largest, the states are brought to it
+    int ge = g;
+    asm volatile("" : "+v"(ge));   // (addresses of the end are not kept in registers over the loop)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       float l = lrun[n];
@@ -634,8 +710,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       }
     }
     __syncthreads();
-    const long long piece = kv4_piece(w, per, u0);
-    float* wsO = a.ws + piece * kv4_piece_floats(ROWS);
+    float* piece = a.ws + kv4_piece(walk.w, walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int c = 16 * n + i;
@@ -661,121 +736,496 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
                   *reinterpret_cast<const floatx4*>(lds + 3 * VWAVE + at);
       }
       __syncthreads();
-      const int r = tile * ROWS + c;
-      if (r < n_row) {
-        if (whole) {
-          const int tok = r / ratio;
-          const long long orow = (long long)(sq.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
-          const bool none = vis[n] <= 0;   // a row that sees no key: zeros, and the sum of none
-          T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * g;
+      const int r = run.tile * ROWS + c;
+      if (!run.whole) {   // (a.ws holds two pieces a worker; rows past the unit's are not read)
 #pragma unroll
-          for (int dd = 0; dd < 2; ++dd) {
-            typedef T v4 __attribute__((ext_vector_type(4)));
-            v4 x;
+        for (int dd = 0; dd < 2; ++dd)
+          *reinterpret_cast<floatx4*>(piece + ((n * 8 + 2 * wv + dd) * 64 + lane) * 4) = sum[dd];
+        if (wv == 0 && g == 0)
+          *reinterpret_cast<floatx2*>(piece + ROWS * KV4_D + 2 * c) = (floatx2){m, l};
+      } else if (r < n_row) {
+        const int tok = r / ratio;
+        const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + r - tok * ratio;
+        const bool none = vis[n] <= 0;   // a row that sees no key: zeros, and the sum of none
+        T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * ge;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l);
-            *reinterpret_cast<v4*>(op + 16 * (2 * wv + dd)) = x;
-          }
-          if (a.lse && wv == 0 && g == 0)
-            a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
-        } else {
-          // (a.ws holds two pieces a worker)
+        for (int dd = 0; dd < 2; ++dd) {
+          typedef T v4 __attribute__((ext_vector_type(4)));
+          v4 x;
 #pragma unroll
-          for (int dd = 0; dd < 2; ++dd)
-            *reinterpret_cast<floatx4*>(wsO + c * KV4_D + 16 * (2 * wv + dd) + 4 * g) = sum[dd];
-          if (wv == 0 && g == 0) {
-            wsO[ROWS * KV4_D + 2 * c] = m;
-            wsO[ROWS * KV4_D + 2 * c + 1] = l;
-          }
+          for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l);
+          *reinterpret_cast<v4*>(op + 16 * (2 * wv + dd)) = x;
         }
+        if (a.lse && wv == 0 && g == 0)
+          a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
       }
     }
     __syncthreads();   // mls is written again
   }
 }
 
-// A row of a unit that several workers share: their partial states joined in the order of the
-// keys.  One wave to a row, two values a lane.
-template <typename T>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+// ---- more query rows
+//
+// WQ waves of 32 rows each go over the same keys, two blocks a step (one block's chain of eight
+// dependent products leaves the matrix unit half idle, two interleaved fill it).  Blocks come as
+// they lie in the pool into a ring in LDS, TDEPTH steps of them on their way while one computes.
+// K goes from codes to operands in each wave's registers; V is converted once for all, a part by
+// each wave, into one of two LDS buffers; one barrier a step.  v_mfma 32x32x16, whose accumulator r
+// in lane (q, h) is key 8 (r / 4) + 4 h + r % 4 of the block.
+
+constexpr int TROW = 320;                 // bytes of a V row in LDS: 16 banks apart, so that the 4
+                                          // rows of a half wave's transposing read do not collide
+constexpr int VTILE = 32 * TROW;
+constexpr int TPAIR = 2 * KV4_BLOCK;
+constexpr int TDEPTH = 3;                 // steps loaded ahead
+constexpr int TRING = TDEPTH + 1;
+constexpr int TILE_LDS = TRING * TPAIR + 4 * VTILE;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+// 16 (4) bytes a lane from global memory into LDS at to + 16 (4) * lane, to uniform.  In assembly,
+// because the compiler waits for all loads of the builtin before it lets any LDS read go by; these
+// have no result registers, and the waits are wait_loads'.  (m0, which holds the LDS address, is
+// the compiler's to use: it is put back.)
+DFL_DEV void load_to_lds16(const unsigned char* from, unsigned char* to) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+}
+DFL_DEV void load_to_lds4(const unsigned char* from, unsigned char* to) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+}
+
+// Waits until at most n (uniform, 2 to 5) of this wave's loads are outstanding.
+DFL_DEV void wait_loads(int n) {
+  asm volatile("" ::: "memory");
+  if (n == 2) __builtin_amdgcn_s_waitcnt(2 | (7 << 4) | (15 << 8));
+  else if (n == 3) __builtin_amdgcn_s_waitcnt(3 | (7 << 4) | (15 << 8));
+  else if (n == 4) __builtin_amdgcn_s_waitcnt(4 | (7 << 4) | (15 << 8));
+  else __builtin_amdgcn_s_waitcnt(5 | (7 << 4) | (15 << 8));
+  asm volatile("" ::: "memory");
+}
+// Barrier that leaves loads on their way; LDS writes of this wave are done before it.
+DFL_DEV void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4) | (0 << 8));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, int WQ, bool WHOLE>
+__global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
+  typedef Mat<T> M;
+  typedef typename M::v8 v8;
+  typedef typename M::v2 v2;
+  constexpr int ROWS = 32 * WQ;
+  static_assert(WQ == 2 || WQ == 4, "the waves' shares of a step's loads and of V");
+  constexpr int VN = 4 / WQ;              // groups of V of a step that a lane converts
+  extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[];   // TILE_LDS bytes
+  unsigned char* const ring = tile_lds;                      // [TRING][TPAIR]
+  unsigned char* const vbuf = tile_lds + TRING * TPAIR;      // [2][2][VTILE]
+  const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ratio = a.n_heads / a.n_kv;
-  const int groups = tile_rows / 4;                 // workgroups of a unit
+  const float scale = a.scale_log2 * (1.f / M::kUnit);
+  // K: row i of the block, groups h and 2 + h
+  const int koff = 16 * lane;
+  const int soff = KV4_SC + 4 * ((i & 15) + 16 * h);
+  const int kshift = 8 * (i >> 4);
+  // V: group vg of row vr (and, with two waves, of row 16 + vr) of the step's block vu
+  const int vu = wv * VN >> 1;
+  const int vr = (WQ == 4 ? 16 * (wv & 1) : 0) + (lane & 15), vg = lane >> 4;
+  const int voff = vu * KV4_BLOCK + kv4_code_at(vr, vg, 1);
+  const int vsoff = vu * KV4_BLOCK + kv4_scale_at(vr, vg, 1);
+  const int vwrite = vu * VTILE + vr * TROW + 64 * vg;
+  const int vread = (4 * h + ((lane & 15) >> 2)) * TROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  const int loads = WQ == 2 ? 5 : wv < 2 ? 3 : 2;   // this wave's loads of a step
+
+  Walk walk;
+  Run run;
+  if (!walk_begin<WHOLE>(a, ROWS, walk)) return;
+  while (walk_next<WHOLE>(a, ROWS, walk, run)) {
+    const Kv4Seq& sq = run.sq;
+    const int n_row = sq.qlen * ratio;
+    const int row0 = run.tile * ROWS + 32 * wv;     // this wave's first row (may be past the last)
+    int le = lane;
+    asm volatile("" : "+v"(le));   // (addresses of a run's begin and end are not kept over others)
+    const int row = min(row0 + (le & 31), n_row - 1), tok = row / ratio;
+    v8 qf[8];
+    const T* qp = reinterpret_cast<const T*>(a.q) + (long long)(sq.q0 + tok) * a.q_row +
+                  (long long)(run.head * ratio + row - tok * ratio) * a.q_head + 32 * (le >> 5);
+#pragma unroll
+    for (int st = 0; st < 8; ++st) qf[st] = *reinterpret_cast<const v8*>(qp + 8 * (st & 3) + 64 * (st >> 2));
+    const int vis = attn_visible(a, sq, tok);
+    // fewest and most keys that rows of this wave see, and rows of the tile
+    const int wmin = attn_visible(a, sq, min(row0, n_row - 1) / ratio);
+    const int wmax = row0 < n_row ? attn_visible(a, sq, min(row0 + 31, n_row - 1) / ratio) : 0;
+    const int tmin = attn_visible(a, sq, run.tile * ROWS / ratio);
+    const int tmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
+    const int b_end = min(run.b1, (tmax + KV4_KEYS - 1) / KV4_KEYS);
+
+    floatx16 o[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = (floatx16){};
+    float mrun = -FLT_MAX, lrun = 0.f;
+
+    // The pages of blocks b, b + 1 (past the last block the last one again, so that the count of
+    // loads under way is always the same), and those blocks into place `slot` of the ring: this
+    // wave's load j of them.
+    struct Two { int p0, p1; };
+    auto pages = [&](int b) {
+      return Two{page_of(a, run, min(b, b_end - 1)), page_of(a, run, min(b + 1, b_end - 1))};
+    };
+    uint32_t absent = 0;   // bit j: block b + j of the loop lies in no page of the pool
+    struct From { const unsigned char *p0, *p1; };
+    auto from = [&](int b, int ahead, Two pg) {
+      absent |= ((pg.p0 < 0 ? 1u : 0u) | (pg.p1 < 0 ? 2u : 0u)) << ahead;
+      return From{block_in(a, run, min(b, b_end - 1), pg.p0), block_in(a, run, min(b + 1, b_end - 1), pg.p1)};
+    };
+    constexpr int LOADS = WQ == 2 ? 5 : 3;
+    auto issue = [&](const From& f, int slot, int j) {
+      unsigned char* to = ring + slot * TPAIR;
+      if (j == LOADS - 1) {   // the exponents of block wv
+        if (wv < 2) load_to_lds4((wv ? f.p1 : f.p0) + KV4_SC + 4 * lane, to + wv * KV4_BLOCK + KV4_SC);
+      } else {                // KiB wv (wv + 2) of block 0, then of block 1
+        const int u = WQ == 2 ? j >> 1 : j, kib = WQ == 2 ? wv + 2 * (j & 1) : wv;
+        load_to_lds16((u ? f.p1 : f.p0) + 1024 * kib + 16 * lane, to + u * KV4_BLOCK + 1024 * kib);
+      }
+    };
+    // V of the step that begins with block b, from place `slot` of the ring: codes and exponent,
+    // then into buffers `to`.  In a block that some row of the tile does not see whole: zeros for
+    // rows past the sequence and for NaN groups, as there 0 * NaN would reach rows that do not see
+    // them; the rows that do see a NaN are set when the block is used.
+    u32x4 vc[VN];
+    uint32_t ve[VN];
+    auto read_v = [&](int slot) {
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        vc[j] = *reinterpret_cast<const u32x4*>(ring + slot * TPAIR + voff + 256 * j);
+        ve[j] = ring[slot * TPAIR + vsoff + j];
+      }
+    };
+    auto write_v = [&](int b, int to, uint32_t gone2) {
+      const int kbase = (b + vu) * KV4_KEYS;
+      const bool gone = (gone2 >> vu) & 1;
+      if (kbase + KV4_KEYS > tmin || gone) {
+#pragma unroll
+        for (int j = 0; j < VN; ++j)
+          if (ve[j] == 255 || gone || kbase + vr + 16 * j >= sq.len) {
+            ve[j] = 0;
+            vc[j] = (u32x4){0, 0, 0, 0};
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const float s = M::kUnit * exponent(ve[j]);
+        unsigned char* at = vbuf + 2 * to * VTILE + vwrite + 16 * j * TROW;
+        static_for<0, 4>([&](auto word) {
+          constexpr int w = word;
+          *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[j][w], s);
+        });
+      }
+    };
+    int slot = 0, to = 0;  // of the step's blocks: in the ring, their V's buffers
+    Two page{0, 0};        // of the blocks that are loaded next, a step ahead
+    if (run.b0 < b_end) {
+      Two first[TDEPTH];
+#pragma unroll
+      for (int j = 0; j < TDEPTH; ++j) first[j] = pages(run.b0 + 2 * j);
+      page = pages(run.b0 + 2 * TDEPTH);
+#pragma unroll
+      for (int j = 0; j < TDEPTH; ++j) {
+        const From f = from(run.b0 + 2 * j, 2 * j, first[j]);
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) issue(f, j, k);
+      }
+    }
+    // The queries and the first blocks are there: from here on the ring's loads alone are counted.
+    // (The compiler's waits do not know of them; one statement, so that it has none in the loop.)
+    asm volatile("s_waitcnt vmcnt(0)"
+                 : "+v"(qf[0]), "+v"(qf[1]), "+v"(qf[2]), "+v"(qf[3]), "+v"(qf[4]), "+v"(qf[5]),
+                   "+v"(qf[6]), "+v"(qf[7]) :: "memory");
+    if (run.b0 < b_end) {
+      lds_barrier();
+      read_v(0);
+      write_v(run.b0, 0, absent);
+    }
+    for (int b = run.b0; b < b_end; b += 2) {
+      const int kbase = b * KV4_KEYS;
+      const int slot1 = slot + 1 == TRING ? 0 : slot + 1;
+      wait_loads(loads * (TDEPTH - 2));
+      // the next step's blocks and V of this one's are there, and nobody reads those of the last
+      // step any more
+      lds_barrier();
+      const int slot3 = slot == 0 ? TRING - 1 : slot - 1;
+      const From f = from(b + 2 * TDEPTH, 2 * TDEPTH, page);
+      // the second block may be past the run's last
+      const bool gone0 = absent & 1, gone1 = (absent & 2) || b + 1 >= b_end;
+      read_v(slot1);   // (after the last step that is a block read once too often)
+      if (kbase >= wmax) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) issue(f, slot3, j);
+        write_v(b + 2, to ^ 1, absent >> 2);
+      } else {
+        const unsigned char* kb = ring + slot * TPAIR;
+        const u32x4 k0 = *reinterpret_cast<const u32x4*>(kb + koff);
+        const u32x4 k2 = *reinterpret_cast<const u32x4*>(kb + KV4_BLOCK + koff);
+        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(kb + soff);
+        const uint32_t s2 = *reinterpret_cast<const uint32_t*>(kb + KV4_BLOCK + soff);
+        const u32x4 k1 = *reinterpret_cast<const u32x4*>(kb + koff + 1024);
+        const u32x4 k3 = *reinterpret_cast<const u32x4*>(kb + KV4_BLOCK + koff + 1024);
+        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(kb + soff + 128);
+        const uint32_t s3 = *reinterpret_cast<const uint32_t*>(kb + KV4_BLOCK + soff + 128);
+        const bool masked = kbase + 2 * KV4_KEYS > wmin || gone0 || gone1;
+        if (kbase + 2 * KV4_KEYS > tmin || gone0 || gone1) {
+          // groups h, 2 + h of row i of either block that stand for NaN
+          const bool there0 = !gone0 && kbase + i < sq.len;
+          const bool there1 = !gone1 && kbase + KV4_KEYS + i < sq.len;
+          const int sh = 16 + kshift;
+          const bool n0 = there0 && ((s0 >> sh) & 255) == 255, n1 = there0 && ((s1 >> sh) & 255) == 255;
+          const bool n2 = there1 && ((s2 >> sh) & 255) == 255, n3 = there1 && ((s3 >> sh) & 255) == 255;
+          if (__ballot(n0 || n1 || n2 || n3)) {
+            const float nan = __builtin_nanf("");
+#pragma unroll 1
+            for (int r = 0; r < 2 * KV4_KEYS; ++r) {
+              const unsigned long long lo = __ballot(r < 32 ? n0 : n2) >> (r & 31);
+              const unsigned long long hi = __ballot(r < 32 ? n1 : n3) >> (r & 31);
+              if (kbase + r < vis)
+                static_for<0, 4>([&](auto group) {
+                  constexpr int gr = group;
+                  if (((gr & 2 ? hi : lo) >> (32 * (gr & 1))) & 1)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) o[gr][k] = nan;
+                });
+            }
+          }
+        }
+        const float e0 = M::kUnit * exponent((s0 >> kshift) & 255u);
+        const float e1 = M::kUnit * exponent((s1 >> kshift) & 255u);
+        const float e2 = M::kUnit * exponent((s2 >> kshift) & 255u);
+        const float e3 = M::kUnit * exponent((s3 >> kshift) & 255u);
+        floatx16 s[2] = {};
+        static_for<0, 4>([&](auto step) {
+          constexpr int st = step;
+          s[0] = M::mfma(M::dequant(k0[st], e0), qf[st], s[0]);
+          s[1] = M::mfma(M::dequant(k2[st], e2), qf[st], s[1]);
+          if constexpr (st < LOADS) issue(f, slot3, st);
+        });
+        if constexpr (LOADS > 4) issue(f, slot3, 4);
+        static_for<0, 4>([&](auto step) {
+          constexpr int st = step;
+          s[0] = M::mfma(M::dequant(k1[st], e1), qf[4 + st], s[0]);
+          s[1] = M::mfma(M::dequant(k3[st], e3), qf[4 + st], s[1]);
+        });
+        write_v(b + 2, to ^ 1, absent >> 2);
+        if (masked) {
+          asm volatile("");   // (a branch: as selects these are a third of the loop)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int lim = (u ? gone1 : gone0) ? 0 : vis;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (kbase + 32 * u + 4 * h + (r & 3) + 8 * (r >> 2) >= lim) s[u][r] = -INFINITY;
+          }
+        }
+        float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+        top *= scale;
+        if (!__all(top <= mrun + KV4_SLACK)) {
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float mnew = top > mrun + KV4_SLACK ? top : mrun;
+          const float alpha = __builtin_amdgcn_exp2f(mrun - mnew);
+          lrun *= alpha;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] *= alpha;
+          mrun = mnew;
+        }
+        const float ref = KV4_LIFT - mrun;
+        const unsigned char* vb = vbuf + 2 * to * VTILE + vread;
+        static_for<0, 4>([&](auto quarter) {   // 16 keys each
+          constexpr int st = quarter & 1, u = quarter >> 1;
+          v8 vf[4], p;   // (the reads' latency passes while the weights are made)
+          static_for<0, 4>([&](auto dt) {
+            constexpr int d = dt;
+            const unsigned char* at = vb + u * VTILE + 16 * st * TROW + 64 * d;
+            vf[d] = read_vt<T>(at, at + 8 * TROW);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int r = 0; r < 8; r += 2) {
+            const v2 x = __builtin_convertvector(
+                ((floatx2){__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * st + r], scale, ref)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * st + r + 1], scale, ref))}), v2);
+            lrun = M::sum2(x, lrun);
+            p[r] = x.x;
+            p[r + 1] = x.y;
+          }
+          static_for<0, 4>([&](auto dt) {
+            constexpr int d = dt;
+            o[d] = M::mfma(vf[d], p, o[d]);
+          });
+        });
+      }
+      page = pages(b + 2 * TDEPTH + 2);
+      if ((absent & 3) && threadIdx.x == 0) atomicOr(a.err, KV4_ERR_PAGE);
+      absent >>= 2;
+      slot = slot1;
+      to ^= 1;
+    }
+    __builtin_amdgcn_s_waitcnt(0);   // (the loads past the last block)
+
+    lrun += __shfl_xor(lrun, 32, 64);
+    asm volatile("" : "+v"(le));
+    if (!run.whole) {
+      float* piece = a.ws + kv4_piece(walk.w, walk.per, run.r0) * kv4_piece_floats(ROWS);
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<floatx4*>(piece + (((wv * 4 + d) * 4 + k) * 64 + le) * 4) =
+              (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * (1.f / M::kUnit);
+      if (le < 32)
+        *reinterpret_cast<floatx2*>(piece + ROWS * KV4_D + 2 * (32 * wv + le)) = (floatx2){mrun, lrun};
+    } else if (row0 + (le & 31) < n_row) {
+      const int row = row0 + (le & 31), tok = row / ratio;
+      const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + row - tok * ratio;
+      const bool none = vis <= 0;   // a row that sees no key: zeros, and the sum of none
+      const float f = (1.f / M::kUnit) / lrun;
+      T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * (le >> 5);
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          typedef T v4 __attribute__((ext_vector_type(4)));
+          v4 x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[d][4 * k + j] * f);
+          *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
+        }
+      if (a.lse && le < 32)
+        a.lse[orow] = none ? -INFINITY : (mrun - KV4_LIFT + __log2f(lrun)) * 0.69314718056f;
+    }
+    __syncthreads();   // the buffers are written again
+  }
+}
+
+// Units that several workers share: their partial states joined in the order of the keys.  A
+// thread has 4 values of a row.  TILE: the partials are kv4_tile_kernel's.
+template <typename T, bool TILE>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
+  const int lane = threadIdx.x & 63;
+  const int ratio = a.n_heads / a.n_kv;
+  const int groups = tile_rows / 8;                 // workgroups of a unit
   const long long unit = blockIdx.x / groups;
-  const int c = (int)(blockIdx.x % groups) * 4 + wv;
+  const int f = (int)(blockIdx.x % groups) * 256 + threadIdx.x;   // which 4 values of the tile
+  const int c = TILE ? 32 * (f >> 10) + (lane & 31) : 16 * (f >> 9) + (lane & 15);
+  const int col = TILE ? 32 * ((f >> 8) & 3) + 8 * ((f >> 6) & 3) + 4 * (lane >> 5)
+                       : 16 * ((f >> 6) & 7) + 4 * (lane >> 4);
   long long before;
   const int s = __builtin_amdgcn_readfirstlane(attn_find<true>(a, tile_rows, unit, before));
   if (s >= a.n_seq) return;
   const Kv4Seq sq = attn_seq(a, s, tile_rows);
-  const long long u = unit - before;
-  const int head = (int)(u / sq.tiles), tile = (int)(u - (long long)head * sq.tiles);
+  const int u = (int)(unit - before);
+  const int head = u / sq.tiles, tile = u - head * sq.tiles;
   const int r = tile * tile_rows + c;
-  if (r >= sq.qlen * ratio) return;
-  // block numbers: those of the sequences before s, then of the units before this one
+  // places: those of the sequences before s, then of the units before this one
   long long t = 0, all = 0;
   for (int k = lane; k < a.n_seq; k += 64) {
     const long long cost = kv4_cost(attn_seq(a, k, tile_rows), a.n_kv);
     all += cost;
     if (k < s) t += cost;
   }
-  const long long total = wave_sum_ll(all);
-  const long long u0 = wave_sum_ll(t) + u * sq.nblk, u1 = u0 + sq.nblk;
-  const long long per = kv4_per(total, a.workers);
-  const long long w0 = u0 / per, w1 = (u1 - 1) / per;
-  if (w0 == w1) return;   // one worker had it all
+  const long long per = kv4_per(wave_sum_ll(all), a.workers);
+  const long long r0 = wave_sum_ll(t) + (long long)u * kv4_span(sq) + KV4_PAD;
+  const int w0 = (int)(r0 / per), w1 = (int)((r0 + sq.nblk - 1) / per);
+  if (w0 == w1 || r >= sq.qlen * ratio) return;   // one worker had it all; no such row
   const long long pf = kv4_piece_floats(tile_rows);
-  float m = -FLT_MAX;
-  for (long long w = w0 + lane; w <= w1; w += 64)
-    m = fmaxf(m, a.ws[kv4_piece(w, per, u0) * pf + tile_rows * KV4_D + 2 * c]);
-  m = wave_max(m);
-  float l = 0.f;
-  floatx2 o = {0.f, 0.f};
-  for (long long w = w0; w <= w1; ++w) {
-    const float* p = a.ws + kv4_piece(w, per, u0) * pf;
-    const float f = __builtin_amdgcn_exp2f(p[tile_rows * KV4_D + 2 * c] - m);
-    const floatx2 x = *reinterpret_cast<const floatx2*>(p + c * KV4_D + 2 * lane);
-    l += f * p[tile_rows * KV4_D + 2 * c + 1];
-    o.x += f * x.x;
-    o.y += f * x.y;
+  float m = -FLT_MAX, l = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 12;   // pieces in flight
+  for (int w = w0; w <= w1; w += N) {
+    floatx4 x[N];
+    floatx2 y[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float* p = a.ws + kv4_piece(min(w + j, w1), per, r0) * pf;
+      x[j] = *reinterpret_cast<const floatx4*>(p + 4 * f);
+      y[j] = *reinterpret_cast<const floatx2*>(p + tile_rows * KV4_D + 2 * c);
+      if (w + j > w1) {   // (0 * what lies there may be NaN)
+        x[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+        y[j] = (floatx2){-INFINITY, 0.f};
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) mn = fmaxf(mn, y[j].x);
+    const float k = __builtin_amdgcn_exp2f(m - mn);
+    o *= k;
+    l *= k;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float e = __builtin_amdgcn_exp2f(y[j].x - m);
+      l += e * y[j].y;
+      o += e * x[j];
+    }
   }
   const int tok = r / ratio;
   const long long orow = (long long)(sq.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
   const bool none = attn_visible(a, sq, tok) <= 0;
-  typedef T o2 __attribute__((ext_vector_type(2)));
-  *reinterpret_cast<o2*>(reinterpret_cast<T*>(a.out) + orow * KV4_D + 2 * lane) =
-      (o2){(T)(none ? 0.f : o.x / l), (T)(none ? 0.f : o.y / l)};
-  if (a.lse && lane == 0)
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[j] / l);
+  *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.out) + orow * KV4_D + col) = x;
+  if (a.lse && col == 0)
     a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
 }
 
-// Units that a launch can have at most.
-long long max_units(const Kv4AttnArgs& a, int tile_rows) {
-  const long long rows = (long long)a.n_rows * (a.n_heads / a.n_kv);
-  // a tile of a sequence holds a row of its own
-  const long long tiles = rows / tile_rows + (a.n_seq < a.n_rows ? a.n_seq : a.n_rows);
-  return tiles * a.n_kv;
+// Units that a launch can have at most: a tile holds a row of its sequence.
+long long max_units(int n_rows, int n_heads, int n_kv, int n_seq, int tile_rows) {
+  const long long rows = (long long)n_rows * (n_heads / n_kv);
+  return (rows / tile_rows + (n_seq < n_rows ? n_seq : n_rows)) * n_kv;
 }
 
+template <typename T, int WQ>
+void launch_tile(const Kv4AttnArgs& a, const Kv4Cut& c, dim3 grid, hipStream_t st) {
+  if (c.whole) hipLaunchKernelGGL((kv4_tile_kernel<T, WQ, true>), grid, dim3(64 * WQ), TILE_LDS, st, a);
+  else hipLaunchKernelGGL((kv4_tile_kernel<T, WQ, false>), grid, dim3(64 * WQ), TILE_LDS, st, a);
+}
 template <typename T>
-void attend(const Kv4AttnArgs& a, hipStream_t st) {
-  const int tr = kv4_tile_rows(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
-  const dim3 grid(a.workers), block(256);
-  if (tr == 16) hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a);
-  hipLaunchKernelGGL((kv4_merge_kernel<T>), dim3((unsigned)(max_units(a, tr) * (tr / 4))), block, 0, st, a,
-                     tr);
+void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
+  const long long units = max_units(a.n_rows, a.n_heads, a.n_kv, a.n_seq, c.tile_rows);
+  const dim3 grid(c.whole ? (unsigned)units : (unsigned)c.workers), block(256);
+  switch (c.tile_rows) {
+    case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a); break;
+    case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a); break;
+    case 64: launch_tile<T, 2>(a, c, grid, st); break;
+    default: launch_tile<T, 4>(a, c, grid, st);
+  }
+  if (c.whole) return;
+  const dim3 mgrid((unsigned)(units * (c.tile_rows / 8)));
+  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
+  else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);
 }
 
 }  // namespace
 
-int kv4_tile_rows(int n_rows, int n_heads, int n_kv, int n_seq) {
-  // rows of a kv head in a sequence, on average
-  const long long rows = ((long long)n_rows * (n_heads / n_kv) + n_seq - 1) / n_seq;
-  return rows <= 16 ? 16 : 32;
-}
-int kv4_workers(int n_rows, int n_heads, int n_kv, int n_seq) {
-  const int tr = kv4_tile_rows(n_rows, n_heads, n_kv, n_seq);
-  return KV4_CUS * (tr == 16 ? 3 : 2);
+Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
+  Kv4Cut c{};
+  const int ratio = n_heads / n_kv;
+  // rows of a kv head in a sequence, on average over those that can have any
+  const long long seqs = n_seq < n_rows ? n_seq : n_rows;
+  const long long rows = ((long long)n_rows * ratio + seqs - 1) / seqs;
+  c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : 2);
+  // Prompts, of several tiles a sequence and enough units for every workgroup to have some: a unit
+  // to a workgroup, the longest first
+  const long long tiles = (long long)n_rows * ratio / c.tile_rows;
+  c.whole = tiles >= 4ll * n_seq && tiles * n_kv >= 2ll * c.workers;
+  return c;
 }
 
 void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st) {
@@ -807,9 +1257,12 @@ void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st) {
   else if (a.dtype == 1) hipLaunchKernelGGL((kv4_read_kernel<1>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((kv4_read_kernel<2>), grid, block, 0, st, a);
 }
-void launch_kv4_attend(const Kv4AttnArgs& a, hipStream_t st) {
-  if (a.dtype == 1) attend<half_t>(a, st);
-  else attend<bf16_t>(a, st);
+void launch_kv4_attend(const Kv4AttnArgs& a_in, hipStream_t st) {
+  Kv4AttnArgs a = a_in;
+  const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
+  a.workers = c.workers;
+  if (a.dtype == 1) attend<half_t>(a, c, st);
+  else attend<bf16_t>(a, c, st);
 }
 
 }  // namespace dfl

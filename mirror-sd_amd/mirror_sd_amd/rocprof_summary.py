@@ -65,7 +65,7 @@ GROUPS = [
     ("RoPE angle table (prompt-sized ingest)", r"rope_table_kernel"),
     ("embed + norm", r"embed_norm_kernel"),
     ("argmax finalize", r"argmax_finalize_kernel"),
-    ("4-bit cache: attention", r"kv4_attn_kernel"),
+    ("4-bit cache: attention", r"kv4_(attn|tile)_kernel"),
     ("4-bit cache: attention merge", r"kv4_merge_kernel"),
     ("4-bit cache: step (tables, slots)", r"kv4_step_\w*kernel"),
     ("4-bit cache: rows in and out", r"kv4_(append|read)_kernel"),

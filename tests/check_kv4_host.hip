@@ -21,21 +21,18 @@ static bool says(const char* got, const char* needle) {
 }
 
 static void layout() {
-  std::vector<int> seen(32, 0), bytes(KV4_BLOCK, 0);
-  for (int k = 0; k < 32; ++k) {
-    const int r = kv4_row(k);
-    must(r >= 0 && r < 32 && !seen[r]++, "kv4_row is a permutation");
-    must(kv4_key(r & 15, r >> 4) == k, "kv4_key undoes kv4_row");
-    for (int v = 0; v < 2; ++v) {
-      for (int b = 0; b < 64; ++b) must(!bytes[v * KV4_V + r * 64 + b]++, "codes overlap");
+  std::vector<int> bytes(KV4_BLOCK, 0);
+  for (int r = 0; r < 32; ++r)
+    for (int v = 0; v < 2; ++v)
       for (int g = 0; g < 4; ++g) {
+        for (int b = 0; b < 16; ++b) must(!bytes[kv4_code_at(r, g, v) + b]++, "codes overlap");
         const int at = kv4_scale_at(r, g, v);
         must(at >= KV4_SC && at < KV4_BLOCK && !bytes[at]++, "exponent bytes overlap");
       }
-    }
-  }
   for (int b : bytes) must(b == 1, "a block has no gaps");
-  must(kv4_block_at(70000, 8, 7, 8, 7) == ((70000ll * 8 + 7) * 8 + 7) * KV4_BLOCK, "offsets past 32 bits");
+  must(kv4_block_at(kv4_block_no(70000, 8, 7, 3, 7)) == ((70000ull * 8 + 7) * 8 + 7) * KV4_BLOCK,
+       "offsets past 32 bits");
+  must(kv4_block_at(kv4_block_no(0x1ffffffu, 16, 15, 3, 7)) == 0xffffffffull * KV4_BLOCK, "the last block");
 }
 
 static void asks() {
@@ -66,7 +63,7 @@ static void split(const std::vector<int>& q, const std::vector<int>& lens, int h
     total += kv4_cost(s.back(), kv);
   }
   const long long per = kv4_per(total, workers);
-  must(per >= KV4_MIN_BLOCKS && per * workers >= total, "the workers cover the blocks");
+  must(per >= KV4_MIN_PLACES && per * workers >= total, "the workers cover the places");
   std::vector<int> done(total, 0), slot(2ll * workers, 0), want(2ll * workers, 0);
   for (long long w = 0; w < workers; ++w) {
     long long pos = w * per;
@@ -75,26 +72,30 @@ static void split(const std::vector<int>& q, const std::vector<int>& lens, int h
       long long before = 0;
       size_t i = 0;
       while (before + kv4_cost(s[i], kv) <= pos) before += kv4_cost(s[i++], kv);
-      const long long unit = (pos - before) / s[i].nblk, u0 = before + unit * s[i].nblk;
-      const long long b0 = pos - u0, b1 = s[i].nblk < b0 + (end - pos) ? s[i].nblk : b0 + (end - pos);
-      must(unit < (long long)s[i].tiles * kv && b1 > b0, "a unit of the sequence");
-      for (long long b = b0; b < b1; ++b) ++done[u0 + b];
+      const int span = kv4_span(s[i]);
+      const long long unit = (pos - before) / span, r0 = before + unit * span + KV4_PAD;
+      const long long b0 = pos > r0 ? pos - r0 : 0, b1 = s[i].nblk < end - r0 ? s[i].nblk : end - r0;
+      must(unit < (long long)s[i].tiles * kv, "a unit of the sequence");
+      pos = r0 + s[i].nblk;
+      if (b1 <= 0) continue;
+      must(b1 > b0, "a run is not empty");
+      for (long long b = b0; b < b1; ++b) ++done[r0 + b];
       if (b0 > 0 || b1 < s[i].nblk) {
-        const long long p = kv4_piece(w, per, u0);
+        const long long p = kv4_piece(w, per, r0);
         must(p >= 0 && p < 2ll * workers && !slot[p]++, "two pieces in one slot");
       }
-      pos += b1 - b0;
     }
   }
-  for (int d : done) must(d == 1, "each block once");
   long long u0 = 0;
   for (auto& x : s)
-    for (long long u = 0; u < (long long)x.tiles * kv; ++u, u0 += x.nblk) {
-      const long long w0 = u0 / per, w1 = (u0 + x.nblk - 1) / per;
+    for (long long u = 0; u < (long long)x.tiles * kv; ++u, u0 += kv4_span(x)) {
+      const long long r0 = u0 + KV4_PAD;
+      for (int k = 0; k < kv4_span(x); ++k) must(done[u0 + k] == (k >= KV4_PAD), "each block once");
+      const long long w0 = r0 / per, w1 = (r0 + x.nblk - 1) / per;
       if (w0 != w1)
-        for (long long w = w0; w <= w1; ++w) ++want[kv4_piece(w, per, u0)];
+        for (long long w = w0; w <= w1; ++w) ++want[kv4_piece(w, per, r0)];
     }
-  must(slot == want, "the merge reads what was written");
+  must(u0 == total && slot == want, "the merge reads what was written");
 }
 
 static void seqs() {
@@ -142,6 +143,7 @@ static void rules() {
   row([](Kv4RowsArgs& x) { x.dtype = 3; }, "dtype");
   row([](Kv4RowsArgs& x) { x.rows = -1; }, "negative");
   row([](Kv4RowsArgs& x) { x.n_kv = 0; }, "kv heads");
+  row([](Kv4RowsArgs& x) { x.n_kv = 1024; x.n_pages = 0x1ffffff; }, "pool pages");
   row([](Kv4RowsArgs& x) { x.k_row = 1028; }, "strides");
   row([](Kv4RowsArgs& x) { x.v_head = 4; }, "strides");
   row([](Kv4RowsArgs& x) { x.k = mem + 8; }, "aligned");
