@@ -1734,7 +1734,7 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
 int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq) {
   if (n_rows < 1 || n_heads < 1 || n_kv < 1 || n_seq < 1 || n_heads % n_kv) return 0;
   const Kv4Cut c = kv4_cut(n_rows, n_heads, n_kv, n_seq);
-  return c.whole ? 0 : 2ll * c.workers * kv4_piece_floats(c.tile_rows) * (long long)sizeof(float);
+  return kv4_ws_bytes(c.tile_rows, c.workers);
 }
 
 int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {

@@ -113,17 +113,30 @@ struct Kv4AttnArgs {
   int* err;
 };
 
-// The work of a launch.  Sequence s contributes, for each of its query tiles and kv heads, one
-// unit of nblk key blocks; units are numbered sequence by sequence, head by head.  A unit spans
-// KV4_PAD + nblk places: the first KV4_PAD stand for what a unit costs besides its blocks (finding
-// it, its queries, the first loads' latency, its result), so that a worker with many short units
-// has no more to do than one with a part of a long one.  Worker w takes the places
+// The work of a launch.  Sequence s contributes, for each kv head and each of its query tiles, one
+// unit; units are numbered sequence by sequence, head by head, tile by tile.  A unit takes up
+// KV4_PAD + nblk places in a row: the first KV4_PAD stand for what a unit costs besides its key
+// blocks (finding it, its queries, the first loads' latency, its result), so that a worker with
+// many short units has no more to do than one with a part of a long one; then one for each key
+// block that its rows see, and now and then one more.  Worker w takes the places
 // [w * per, (w + 1) * per); a unit whose blocks several workers share leaves one partial result
 // with each (slot kv4_piece), which the merge joins.
+//
+// The places of a head's tiles 0 .. t - 1 are KV4_PAD t + floor((slope t (t - 1) / 2 + base t) / m)
+// with m = 32 ratio.  Tile t sees ceil(v / 32) blocks, v = len - qlen + 1 + floor((tile_rows (t + 1)
+// - 1) / ratio) the keys that its last row's token sees; that is floor((slope t + base) / m) with
+// slope = tile_rows and base = ratio (len - qlen + 32) + tile_rows - 1, and the floor of a sum is
+// not below the sum of floors.  Where every row sees all keys, slope = 0 and base = ratio (len + 31).
+// (Keys before the first row at least 0, keys at least 1: every unit has a block, so that rows that
+// see nothing are written too.)
 constexpr int KV4_PAD = 8;
-struct Kv4Seq { int q0, qlen, len, tiles, nblk; bool bad; };
+struct Kv4Seq {
+  int q0, qlen, len, tiles;
+  long long slope, base, m;
+  bool bad;
+};
 DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_shift, int ratio,
-                      int tile_rows) {
+                      int tile_rows, bool causal) {
   Kv4Seq s;
   const long long cap = (long long)width << page_shift;
   s.bad = q0 < 0 || q1 < q0 || q1 > n_rows || len < 0 || (long long)len > cap;
@@ -131,15 +144,30 @@ DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_s
   s.qlen = s.bad ? 0 : q1 - q0;
   s.len = s.bad ? 0 : len;
   s.tiles = (int)(((long long)s.qlen * ratio + tile_rows - 1) / tile_rows);
-  // a sequence without keys still has its rows written: one block, all of it masked
-  s.nblk = s.qlen ? (s.len > 0 ? (s.len + KV4_KEYS - 1) / KV4_KEYS : 1) : 0;
+  const long long before = s.len > s.qlen ? s.len - s.qlen : 0;
+  s.slope = causal ? tile_rows : 0;
+  s.base = causal ? ratio * (before + KV4_KEYS) + tile_rows - 1
+                  : ratio * ((long long)(s.len > 1 ? s.len : 1) + KV4_KEYS - 1);
+  s.m = (long long)KV4_KEYS * ratio;
   return s;
 }
-DFL_HD int kv4_span(const Kv4Seq& s) { return KV4_PAD + s.nblk; }
-DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return (long long)s.tiles * n_kv * kv4_span(s); }
-constexpr int KV4_MIN_PLACES = 24;   // fewest places of a worker
+// slope t (t - 1) / 2 + base t
+DFL_HD long long kv4_sum(const Kv4Seq& s, long long t) { return s.slope * (t * (t - 1) / 2) + s.base * t; }
+DFL_HD long long kv4_div(long long n, long long d) {   // for 0 <= n, 0 < d (in 32 bits where it fits)
+  return n <= 0xffffffffll && d <= 0xffffffffll ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+}
+// Places of a head's first t tiles, and of a sequence's units.
+DFL_HD long long kv4_places(const Kv4Seq& s, long long t) {
+  return KV4_PAD * t + kv4_div(kv4_sum(s, t), s.m);
+}
+DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return n_kv * kv4_places(s, s.tiles); }
+// Whether tile t begins at or before place r of its head.
+DFL_HD bool kv4_begun(const Kv4Seq& s, long long t, long long r) {
+  return kv4_sum(s, t) < (r - KV4_PAD * t + 1) * s.m;
+}
+constexpr int KV4_MIN_PLACES = 16;   // fewest places of a worker
 DFL_HD long long kv4_per(long long total, int workers) {
-  const long long per = (total + workers - 1) / workers;
+  const long long per = kv4_div(total + workers - 1, workers);
   return per < KV4_MIN_PLACES ? KV4_MIN_PLACES : per;
 }
 // Partial slot of worker w for a shared unit whose first block is at place r0: a worker has at
@@ -150,13 +178,25 @@ DFL_HD long long kv4_piece(long long w, long long per, long long r0) {
 // Floats of one partial: O [tile rows][128] in the order of the kernel's registers, then (max,
 // sum) a row.
 DFL_HD long long kv4_piece_floats(int tile_rows) { return (long long)tile_rows * (KV4_D + 2); }
+// What a worker notes of a shared unit for the merge.
+struct Kv4Note { int w1, head, tile, q0, qlen, len, pad[2]; };
+// Bytes of a launch's workspace.
+DFL_HD long long kv4_ws_bytes(int tile_rows, int workers) {
+  return workers * (2 * kv4_piece_floats(tile_rows) * (long long)sizeof(float) + (long long)sizeof(Kv4Note));
+}
+// Whether every count above stays below 2^62, for any lengths that the launch can have.
+DFL_HD bool kv4_counts_fit(int n_rows, int ratio, int n_kv, int n_seq, int width, int page_shift) {
+  const double cap = (double)((long long)width << page_shift) + KV4_KEYS;
+  const double tiles = (double)n_rows * ratio / 16 + n_seq + 1;
+  const double sum = 128.0 * tiles * tiles + (ratio * cap + 128.0) * tiles;
+  return sum * (n_kv + 1) < 4e18;
+}
 
 // How a launch is cut (what its workspace holds follows from it).
 struct Kv4Cut {
   int tile_rows;   // query rows of a unit: 16 or 32 (each wave has them all and a fourth of the
                    // keys) or 64, 128 (each wave has 32 of them and all keys)
-  int workers;     // workgroups, or
-  bool whole;      // each unit whole to a workgroup of its own, no workspace
+  int workers;     // workgroups
 };
 Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq);
 
@@ -201,6 +241,8 @@ inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
   if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
   if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll)
     return "table width out of range";
+  if (!kv4_counts_fit(a.n_rows, a.n_heads / a.n_kv, a.n_kv, a.n_seq, a.width, a.page_shift))
+    return "too many query rows for so long a table";
   if (!(a.scale_log2 > 0.f) || a.scale_log2 > 1e30f) return "scale must be positive and finite";
   if (!a.q || !a.out || !a.starts || !a.lens || !a.table || !a.pool || !a.err) return "null pointer";
   auto mis = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };

@@ -389,63 +389,58 @@ DFL_DEV long long uniform(long long v) {
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((unsigned long long)v >> 32));
   return (long long)((unsigned long long)hi << 32 | lo);
 }
-DFL_DEV Kv4Seq attn_seq(const Kv4AttnArgs& a, int s, int tile_rows) {
-  return kv4_seq(a.starts[s], a.starts[s + 1], a.lens[s], a.n_rows, a.width, a.page_shift,
-                 a.n_heads / a.n_kv, tile_rows);
-}
-// The same for an s that is uniform.
-DFL_DEV Kv4Seq attn_seq_uniform(const Kv4AttnArgs& a, int s, int tile_rows) {
-  return kv4_seq(load_const(a.starts + s), load_const(a.starts + s + 1), load_const(a.lens + s),
-                 a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, tile_rows);
-}
 DFL_DEV long long wave_sum_ll(long long v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// Places of all units; every lane gets the sum.
-DFL_DEV long long attn_total(const Kv4AttnArgs& a, int tile_rows) {
+// Inclusive sum over the wave's lanes.
+DFL_DEV long long wave_scan_ll(long long v) {
   const int lane = threadIdx.x & 63;
-  long long t = 0;
-  for (int s = lane; s < a.n_seq; s += 64) {
-    const Kv4Seq q = attn_seq(a, s, tile_rows);
-    if (q.bad) atomicOr(a.err, KV4_ERR_PAGE);
-    t += kv4_cost(q, a.n_kv);
-  }
-  return wave_sum_ll(t);
-}
-// The sequence that holds place (UNITS: unit) pos, and the places (units) before it; n_seq if pos
-// is past the last.
-template <bool UNITS>
-DFL_DEV int attn_find(const Kv4AttnArgs& a, int tile_rows, long long pos, long long& before) {
-  const int lane = threadIdx.x & 63;
-  long long acc = 0;
-  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-    long long c = 0;
-    if (s0 + lane < a.n_seq) {
-      const Kv4Seq q = attn_seq(a, s0 + lane, tile_rows);
-      c = UNITS ? (long long)q.tiles * a.n_kv : kv4_cost(q, a.n_kv);
-    }
-    long long in = c;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const long long x = __shfl_up(in, o, 64);
-      if (lane >= o) in += x;
-    }
-    const unsigned long long past = __ballot(acc + in > pos);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      before = acc + __shfl(in - c, l, 64);
-      return s0 + l;
-    }
-    acc += __shfl(in, 63, 64);
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long x = __shfl_up(v, o, 64);
+    if (lane >= o) v += x;
   }
-  before = acc;
-  return a.n_seq;
+  return v;
 }
-// n / d for 0 <= n, 0 < d, in 32 bits where it fits (the wide division is a hundred instructions).
-DFL_DEV long long div_ll(long long n, int d) {
-  return n <= 0xffffffffll ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
+DFL_DEV int pick(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// Sequences one lane each, 64 at a time: sequence s0 + lane's row range and length, and its places.
+struct Lanes { int q0, q1, len; long long cost; };
+DFL_DEV Lanes attn_lanes(const Kv4AttnArgs& a, int tile_rows, int s0, bool report) {
+  const int s = s0 + (threadIdx.x & 63);
+  Lanes l{0, 0, 0, 0};
+  if (s < a.n_seq) {
+    l = Lanes{a.starts[s], a.starts[s + 1], a.lens[s], 0};
+    const Kv4Seq q = kv4_seq(l.q0, l.q1, l.len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv,
+                             tile_rows, a.causal);
+    if (q.bad && report) atomicOr(a.err, KV4_ERR_PAGE);
+    l.cost = kv4_cost(q, a.n_kv);
+  }
+  return l;
+}
+// The sequence among the 64 whose places hold pos (in: their inclusive sums, after acc places):
+// its number of them and the places before it; -1 if there is none.
+DFL_DEV int attn_among(const Lanes& l, long long in, long long acc, long long pos, long long& before) {
+  const unsigned long long past = __ballot(acc + in > pos);
+  if (!past) return -1;
+  const int k = __ffsll((unsigned long long)past) - 1;
+  before = uniform(acc + __shfl(in - l.cost, k, 64));
+  return k;
+}
+// The tile of a head at its place r: the last that has begun.  Every lane tries one, 64 at a time.
+DFL_DEV int attn_tile(const Kv4Seq& s, long long r) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = s.tiles;   // the tile is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 63) >> 6;
+    const int t = lo + lane * step;
+    const unsigned long long begun = __ballot(t < lo + n && kv4_begun(s, t, r));
+    const int k = max(0, __popcll(begun) - 1);
+    n = min(step, n - k * step);
+    lo += k * step;
+  }
+  return lo;
 }
 
 // Visible keys of a token of a sequence (they grow with the token).
@@ -453,64 +448,108 @@ DFL_DEV int attn_visible(const Kv4AttnArgs& a, const Kv4Seq& q, int token) {
   return a.causal ? max(0, min(q.len, q.len - q.qlen + token + 1)) : q.len;
 }
 
-// A worker's walk over its places: run after run of blocks [b0, b1) of a unit.
-struct Run {
+// A unit, and where its places are.
+struct Unit {
   Kv4Seq sq;
-  int s, head, tile, b0, b1;
-  bool whole;          // all of the unit's blocks
-  long long r0;        // place of the unit's first block
+  int s, head, tile, nblk;
+  long long r0;        // place of its first block
+  long long head0;     // place at which its head begins
 };
-struct Walk { long long pos, end, per, w; };
-template <bool WHOLE>
-DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k) {
-  k.w = blockIdx.x;
-  if constexpr (WHOLE) {
-    if (k.w == 0) attn_total(a, tile_rows);   // (for its error bit)
-    k.pos = k.w;
-    k.end = k.w + 1;
-    k.per = 1;
-  } else {
-    const long long total = uniform(attn_total(a, tile_rows));
-    k.per = kv4_per(total, a.workers);
-    k.pos = k.w * k.per;
-    k.end = min(total, k.pos + k.per);
-  }
-  return k.pos < k.end;
+DFL_DEV void unit_places(Unit& u) {
+  const long long p0 = kv4_places(u.sq, u.tile);
+  u.nblk = (int)(kv4_places(u.sq, u.tile + 1) - p0) - KV4_PAD;
+  u.r0 = u.head0 + p0 + KV4_PAD;
 }
-// The next run; false at the end.  (Everything here is uniform over the workgroup.)
-template <bool WHOLE>
-DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
-  while (k.pos < k.end) {
+// The unit of sequence s (row range and length q0, q1, len) at a place, the sequence's first being
+// at place `at`.
+DFL_DEV void unit_of(const Kv4AttnArgs& a, int tile_rows, int s, int q0, int q1, int len, long long at,
+                     long long pos, Unit& u) {
+  u.s = s;
+  u.sq = kv4_seq(q0, q1, len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, tile_rows, a.causal);
+  const long long of_head = kv4_places(u.sq, u.sq.tiles);
+  u.head = (int)kv4_div(pos - at, of_head);
+  u.head0 = at + u.head * of_head;
+  u.tile = u.sq.tiles > 1 ? __builtin_amdgcn_readfirstlane(attn_tile(u.sq, pos - u.head0)) : 0;
+  unit_places(u);
+}
+// The unit at a place (uniform); false if there is none.
+DFL_DEV bool unit_at(const Kv4AttnArgs& a, int tile_rows, long long pos, Unit& u) {
+  long long acc = 0;
+  for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+    const Lanes l = attn_lanes(a, tile_rows, s0, false);
+    const long long in = wave_scan_ll(l.cost);
     long long at;
-    r.s = __builtin_amdgcn_readfirstlane(attn_find<WHOLE>(a, tile_rows, k.pos, at));
-    if (r.s >= a.n_seq) return false;
-    at = uniform(at);
-    r.sq = attn_seq_uniform(a, r.s, tile_rows);
-    const int span = WHOLE ? 1 : kv4_span(r.sq);
-    const long long unit = div_ll(k.pos - at, span);
-    r.head = (int)div_ll(unit, r.sq.tiles);
-    r.tile = (int)(unit - (long long)r.head * r.sq.tiles);
-    r.whole = true;
-    if constexpr (WHOLE) {
-      // the last tiles of a prompt see the most keys: they go first
-      r.tile = r.sq.tiles - 1 - r.tile;
-      r.b0 = 0;
-      r.b1 = r.sq.nblk;
-      r.r0 = 0;
-      k.pos = k.end;
-    } else {
-      r.r0 = at + unit * span + KV4_PAD;
-      r.b0 = (int)max(0ll, k.pos - r.r0);
-      r.b1 = (int)min((long long)r.sq.nblk, k.end - r.r0);
-      r.whole = r.b0 == 0 && r.b1 == r.sq.nblk;
-      k.pos = r.r0 + r.sq.nblk;
-      if (r.b1 <= 0) continue;   // only places before the first block
+    const int k = attn_among(l, in, acc, pos, at);
+    if (k >= 0) {
+      unit_of(a, tile_rows, s0 + k, pick(l.q0, k), pick(l.q1, k), pick(l.len, k), at, pos, u);
+      return true;
     }
-    return true;
+    acc += uniform(__shfl(in, 63, 64));
   }
   return false;
 }
 
+// A worker's walk over its places: run after run of blocks [b0, b1) of a unit.
+struct Run : Unit {
+  int b0, b1;
+  bool whole;          // all of the unit's blocks
+};
+struct Walk { long long pos, end, per; };
+// Begins at the worker's first place; false if it has none.
+DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
+  const bool report = blockIdx.x == 0;
+  Lanes l = attn_lanes(a, tile_rows, 0, report);
+  long long in = wave_scan_ll(l.cost);
+  long long total = uniform(__shfl(in, 63, 64));
+  for (int s0 = 64; s0 < a.n_seq; s0 += 64)
+    total += uniform(wave_sum_ll(attn_lanes(a, tile_rows, s0, report).cost));
+  k.per = kv4_per(total, a.workers);
+  k.pos = blockIdx.x * k.per;
+  k.end = min(total, k.pos + k.per);
+  if (k.pos >= k.end) return false;
+  if (a.n_seq > 64) return unit_at(a, tile_rows, k.pos, r);
+  long long at;
+  const int s = attn_among(l, in, 0, k.pos, at);
+  if (s < 0) return false;
+  unit_of(a, tile_rows, s, pick(l.q0, s), pick(l.q1, s), pick(l.len, s), at, k.pos, r);
+  return true;
+}
+// The run of the unit at hand; false if only places before its first block are this worker's.
+DFL_DEV bool walk_run(const Walk& k, Run& r) {
+  r.b0 = (int)max(0ll, k.pos - r.r0);
+  r.b1 = (int)min((long long)r.nblk, k.end - r.r0);
+  r.whole = r.b0 == 0 && r.b1 == r.nblk;
+  return r.b1 > 0;
+}
+// On to the next unit; false at the end.  (Everything here is uniform over the workgroup.)
+DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
+  k.pos = r.r0 + r.nblk;
+  if (k.pos >= k.end) return false;
+  if (r.tile + 1 < r.sq.tiles) {
+    ++r.tile;
+  } else if (r.head + 1 < a.n_kv) {
+    r.head0 = k.pos;
+    ++r.head;
+    r.tile = 0;
+  } else {
+    return unit_at(a, tile_rows, k.pos, r);
+  }
+  unit_places(r);
+  return true;
+}
+// What the merge needs to know of the unit that a worker begins and others go on with (w1: the
+// last of them; -1: there is none).  The notes lie behind the partials.
+DFL_DEV Kv4Note* kv4_notes(const Kv4AttnArgs& a, int tile_rows) {
+  return reinterpret_cast<Kv4Note*>(a.ws + 2ll * a.workers * kv4_piece_floats(tile_rows));
+}
+DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows) {
+  if (threadIdx.x == 0) kv4_notes(a, tile_rows)[blockIdx.x].w1 = -1;
+}
+DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, long long per, const Run& r) {
+  if (threadIdx.x) return;
+  kv4_notes(a, tile_rows)[blockIdx.x] = Kv4Note{
+      (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, 0, 0};
+}
 // The page of block b of a run's keys; -1: there is no such page (its keys are absent).
 DFL_DEV int page_of(const Kv4AttnArgs& a, const Run& r, int b) {
   const int page = load_const(a.table + (long long)r.s * a.width + (b >> (a.page_shift - 5)));
@@ -550,8 +589,11 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 
   Walk walk;
   Run run;
-  if (!walk_begin<false>(a, ROWS, walk)) return;
-  while (walk_next<false>(a, ROWS, walk, run)) {
+  bool more = walk_begin(a, ROWS, walk, run);
+  walk_no_note(a, ROWS);
+  for (; more; more = walk_next(a, ROWS, walk, run)) {
+    if (!walk_run(walk, run)) break;   // (the worker's last places)
+    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, walk.per, run);
     const Kv4Seq& sq = run.sq;
     // query fragments: step st covers values 32 g + 8 st ..; visible keys of this lane's rows
     v8 qf[NT][4];
@@ -710,7 +752,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       }
     }
     __syncthreads();
-    float* piece = a.ws + kv4_piece(walk.w, walk.per, run.r0) * kv4_piece_floats(ROWS);
+    float* piece = a.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int c = 16 * n + i;
@@ -782,19 +824,19 @@ constexpr int TRING = TDEPTH + 1;
 constexpr int TILE_LDS = TRING * TPAIR + 4 * VTILE;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
-// 16 (4) bytes a lane from global memory into LDS at to + 16 (4) * lane, to uniform.  In assembly,
-// because the compiler waits for all loads of the builtin before it lets any LDS read go by; these
-// have no result registers, and the waits are wait_loads'.  (m0, which holds the LDS address, is
-// the compiler's to use: it is put back.)
-DFL_DEV void load_to_lds16(const unsigned char* from, unsigned char* to) {
+// 16 (4) bytes a lane from global memory, from + 16 (4) * lane, into LDS at to + 16 (4) * lane; from
+// and to uniform, at = 16 (4) * lane.  In assembly, because the compiler waits for all loads of the
+// builtin before it lets any LDS read go by; these have no result registers, and the waits are
+// wait_loads'.  (m0, which holds the LDS address, is the compiler's to use: it is put back.)
+DFL_DEV void load_to_lds16(const unsigned char* from, int at, unsigned char* to) {
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(at), "s"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
 }
-DFL_DEV void load_to_lds4(const unsigned char* from, unsigned char* to) {
+DFL_DEV void load_to_lds4(const unsigned char* from, int at, unsigned char* to) {
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0) : "v"(at), "s"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
 }
 
 // Waits until at most n (uniform, 2 to 5) of this wave's loads are outstanding.
@@ -814,7 +856,7 @@ DFL_DEV void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-template <typename T, int WQ, bool WHOLE>
+template <typename T, int WQ>
 __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
@@ -837,15 +879,19 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
   const int vu = wv * VN >> 1;
   const int vr = (WQ == 4 ? 16 * (wv & 1) : 0) + (lane & 15), vg = lane >> 4;
   const int voff = vu * KV4_BLOCK + kv4_code_at(vr, vg, 1);
-  const int vsoff = vu * KV4_BLOCK + kv4_scale_at(vr, vg, 1);
+  const int vsoff = vu * KV4_BLOCK + KV4_SC + 4 * ((lane & 15) + 16 * vg);   // word of rows vr, 16 + vr
+  const int vshift = 16 + (vr >> 1 & 8);
   const int vwrite = vu * VTILE + vr * TROW + 64 * vg;
   const int vread = (4 * h + ((lane & 15) >> 2)) * TROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
   const int loads = WQ == 2 ? 5 : wv < 2 ? 3 : 2;   // this wave's loads of a step
 
   Walk walk;
   Run run;
-  if (!walk_begin<WHOLE>(a, ROWS, walk)) return;
-  while (walk_next<WHOLE>(a, ROWS, walk, run)) {
+  bool more = walk_begin(a, ROWS, walk, run);
+  walk_no_note(a, ROWS);
+  for (; more; more = walk_next(a, ROWS, walk, run)) {
+    if (!walk_run(walk, run)) break;   // (the worker's last places)
+    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, walk.per, run);
     const Kv4Seq& sq = run.sq;
     const int n_row = sq.qlen * ratio;
     const int row0 = run.tile * ROWS + 32 * wv;     // this wave's first row (may be past the last)
@@ -858,9 +904,7 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
 #pragma unroll
     for (int st = 0; st < 8; ++st) qf[st] = *reinterpret_cast<const v8*>(qp + 8 * (st & 3) + 64 * (st >> 2));
     const int vis = attn_visible(a, sq, tok);
-    // fewest and most keys that rows of this wave see, and rows of the tile
-    const int wmin = attn_visible(a, sq, min(row0, n_row - 1) / ratio);
-    const int wmax = row0 < n_row ? attn_visible(a, sq, min(row0 + 31, n_row - 1) / ratio) : 0;
+    // fewest and most keys that rows of the tile see
     const int tmin = attn_visible(a, sq, run.tile * ROWS / ratio);
     const int tmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
     const int b_end = min(run.b1, (tmax + KV4_KEYS - 1) / KV4_KEYS);
@@ -870,27 +914,42 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
     for (int d = 0; d < 4; ++d) o[d] = (floatx16){};
     float mrun = -FLT_MAX, lrun = 0.f;
 
-    // The pages of blocks b, b + 1 (past the last block the last one again, so that the count of
-    // loads under way is always the same), and those blocks into place `slot` of the ring: this
-    // wave's load j of them.
-    struct Two { int p0, p1; };
-    auto pages = [&](int b) {
-      return Two{page_of(a, run, min(b, b_end - 1)), page_of(a, run, min(b + 1, b_end - 1))};
+    // Addresses of blocks, 64 at a time, a lane each (past the last block the last one again, so
+    // that the count of loads under way is always the same).
+    const int subs = a.page_shift - 5;
+    const int* trow = a.table + (long long)run.s * a.width;
+    const uint32_t per_page = (uint32_t)a.n_kv << subs, of_head = (uint32_t)run.head << subs;
+    int abase = 0;                       // the first of the 64
+    unsigned long long mine = 0, gone64 = 0;
+    auto addresses = [&](int b) {
+      const int k = max(0, min(b + lane, b_end - 1));   // (b_end may be 0: then nothing is loaded)
+      const int page = b_end > 0 ? trow[k >> subs] : 0;
+      const bool no = page < 0 || page >= a.n_pages;
+      mine = kv4_block_at((no ? 0u : (uint32_t)page * per_page) + of_head + (uint32_t)(k & ((1 << subs) - 1)));
+      gone64 = __ballot(no);
+      abase = b;
     };
     uint32_t absent = 0;   // bit j: block b + j of the loop lies in no page of the pool
     struct From { const unsigned char *p0, *p1; };
-    auto from = [&](int b, int ahead, Two pg) {
-      absent |= ((pg.p0 < 0 ? 1u : 0u) | (pg.p1 < 0 ? 2u : 0u)) << ahead;
-      return From{block_in(a, run, min(b, b_end - 1), pg.p0), block_in(a, run, min(b + 1, b_end - 1), pg.p1)};
+    auto from = [&](int b, int ahead) {
+      if (b - abase >= 64) addresses(b);
+      const int k = b - abase;           // (even: the pair is within the 64)
+      absent |= ((uint32_t)(gone64 >> k) & 3u) << ahead;
+      const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+      auto at = [&](int l) {
+        return a.pool + ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane(lo, l));
+      };
+      return From{at(k), at(k + 1)};
     };
     constexpr int LOADS = WQ == 2 ? 5 : 3;
     auto issue = [&](const From& f, int slot, int j) {
       unsigned char* to = ring + slot * TPAIR;
       if (j == LOADS - 1) {   // the exponents of block wv
-        if (wv < 2) load_to_lds4((wv ? f.p1 : f.p0) + KV4_SC + 4 * lane, to + wv * KV4_BLOCK + KV4_SC);
+        if (wv < 2) load_to_lds4((wv ? f.p1 : f.p0) + KV4_SC, 4 * lane, to + wv * KV4_BLOCK + KV4_SC);
       } else {                // KiB wv (wv + 2) of block 0, then of block 1
         const int u = WQ == 2 ? j >> 1 : j, kib = WQ == 2 ? wv + 2 * (j & 1) : wv;
-        load_to_lds16((u ? f.p1 : f.p0) + 1024 * kib + 16 * lane, to + u * KV4_BLOCK + 1024 * kib);
+        load_to_lds16((u ? f.p1 : f.p0) + 1024 * kib, 16 * lane, to + u * KV4_BLOCK + 1024 * kib);
       }
     };
     // V of the step that begins with block b, from place `slot` of the ring: codes and exponent,
@@ -898,28 +957,31 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
     // rows past the sequence and for NaN groups, as there 0 * NaN would reach rows that do not see
     // them; the rows that do see a NaN are set when the block is used.
     u32x4 vc[VN];
-    uint32_t ve[VN];
+    uint32_t ve;
     auto read_v = [&](int slot) {
+      ve = *reinterpret_cast<const uint32_t*>(ring + slot * TPAIR + vsoff);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
+      for (int j = 0; j < VN; ++j)
         vc[j] = *reinterpret_cast<const u32x4*>(ring + slot * TPAIR + voff + 256 * j);
-        ve[j] = ring[slot * TPAIR + vsoff + j];
-      }
     };
     auto write_v = [&](int b, int to, uint32_t gone2) {
       const int kbase = (b + vu) * KV4_KEYS;
       const bool gone = (gone2 >> vu) & 1;
+      uint32_t e[VN];
+#pragma unroll
+      for (int j = 0; j < VN; ++j) e[j] = (ve >> (vshift + 8 * j)) & 255u;
       if (kbase + KV4_KEYS > tmin || gone) {
+        asm volatile("");
 #pragma unroll
         for (int j = 0; j < VN; ++j)
-          if (ve[j] == 255 || gone || kbase + vr + 16 * j >= sq.len) {
-            ve[j] = 0;
+          if (e[j] == 255 || gone || kbase + vr + 16 * j >= sq.len) {
+            e[j] = 0;
             vc[j] = (u32x4){0, 0, 0, 0};
           }
       }
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
-        const float s = M::kUnit * exponent(ve[j]);
+        const float s = M::kUnit * exponent(e[j]);
         unsigned char* at = vbuf + 2 * to * VTILE + vwrite + 16 * j * TROW;
         static_for<0, 4>([&](auto word) {
           constexpr int w = word;
@@ -927,16 +989,29 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
         });
       }
     };
-    int slot = 0, to = 0;  // of the step's blocks: in the ring, their V's buffers
-    Two page{0, 0};        // of the blocks that are loaded next, a step ahead
-    if (run.b0 < b_end) {
-      Two first[TDEPTH];
+    // S^T of the two blocks in place `slot` of the ring: codes and exponents, then (quarter by
+    // quarter of the values) the products.
+    u32x4 kc[4];
+    uint32_t ke[4];
+    auto read_k = [&](int slot) {
+      const unsigned char* kb = ring + slot * TPAIR;
 #pragma unroll
-      for (int j = 0; j < TDEPTH; ++j) first[j] = pages(run.b0 + 2 * j);
-      page = pages(run.b0 + 2 * TDEPTH);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ke[2 * u + j] = *reinterpret_cast<const uint32_t*>(kb + u * KV4_BLOCK + soff + 128 * j);
+          kc[2 * u + j] = *reinterpret_cast<const u32x4*>(kb + u * KV4_BLOCK + koff + 1024 * j);
+        }
+    };
+    auto k_unit = [&](int j) { return M::kUnit * exponent((ke[j] >> kshift) & 255u); };
+    const bool idle = row0 >= n_row;   // a wave past the sequence's rows only loads and converts
+    int slot = 0, to = 0;  // of the step's blocks: in the ring, their V's buffers
+    floatx16 s[2] = {};
+    addresses(run.b0);
+    if (run.b0 < b_end) {
 #pragma unroll
       for (int j = 0; j < TDEPTH; ++j) {
-        const From f = from(run.b0 + 2 * j, 2 * j, first[j]);
+        const From f = from(run.b0 + 2 * j, 2 * j);
 #pragma unroll
         for (int k = 0; k < LOADS; ++k) issue(f, j, k);
       }
@@ -949,42 +1024,42 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
     if (run.b0 < b_end) {
       lds_barrier();
       read_v(0);
+      read_k(0);
       write_v(run.b0, 0, absent);
+      const float e[4] = {k_unit(0), k_unit(1), k_unit(2), k_unit(3)};
+      static_for<0, 8>([&](auto step) {
+        constexpr int st = step;
+        s[0] = M::mfma(M::dequant(kc[st >> 2][st & 3], e[st >> 2]), qf[st], s[0]);
+        s[1] = M::mfma(M::dequant(kc[2 + (st >> 2)][st & 3], e[2 + (st >> 2)]), qf[st], s[1]);
+      });
     }
-    for (int b = run.b0; b < b_end; b += 2) {
+    // A step (s: S^T of its two blocks): their weights, between which (they do not wait for each
+    // other) go the products of the next step's S^T t, then the products with V.
+    auto do_step = [&](int b, floatx16 (&s)[2], floatx16 (&t)[2]) __attribute__((always_inline)) {
       const int kbase = b * KV4_KEYS;
       const int slot1 = slot + 1 == TRING ? 0 : slot + 1;
       wait_loads(loads * (TDEPTH - 2));
       // the next step's blocks and V of this one's are there, and nobody reads those of the last
       // step any more
       lds_barrier();
-      const int slot3 = slot == 0 ? TRING - 1 : slot - 1;
-      const From f = from(b + 2 * TDEPTH, 2 * TDEPTH, page);
+      read_k(slot1);   // (after the last step those are blocks read once too often)
+      read_v(slot1);
+      const From f = from(b + 2 * TDEPTH, 2 * TDEPTH);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) issue(f, slot == 0 ? TRING - 1 : slot - 1, j);
       // the second block may be past the run's last
       const bool gone0 = absent & 1, gone1 = (absent & 2) || b + 1 >= b_end;
-      read_v(slot1);   // (after the last step that is a block read once too often)
-      if (kbase >= wmax) {
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) issue(f, slot3, j);
-        write_v(b + 2, to ^ 1, absent >> 2);
-      } else {
-        const unsigned char* kb = ring + slot * TPAIR;
-        const u32x4 k0 = *reinterpret_cast<const u32x4*>(kb + koff);
-        const u32x4 k2 = *reinterpret_cast<const u32x4*>(kb + KV4_BLOCK + koff);
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(kb + soff);
-        const uint32_t s2 = *reinterpret_cast<const uint32_t*>(kb + KV4_BLOCK + soff);
-        const u32x4 k1 = *reinterpret_cast<const u32x4*>(kb + koff + 1024);
-        const u32x4 k3 = *reinterpret_cast<const u32x4*>(kb + KV4_BLOCK + koff + 1024);
-        const uint32_t s1 = *reinterpret_cast<const uint32_t*>(kb + soff + 128);
-        const uint32_t s3 = *reinterpret_cast<const uint32_t*>(kb + KV4_BLOCK + soff + 128);
-        const bool masked = kbase + 2 * KV4_KEYS > wmin || gone0 || gone1;
+      if (!idle) {
         if (kbase + 2 * KV4_KEYS > tmin || gone0 || gone1) {
+          asm volatile("");   // (a branch: as selects the masks are a third of the loop)
           // groups h, 2 + h of row i of either block that stand for NaN
+          const unsigned char* kb = ring + slot * TPAIR + soff;
+          const int sh = 16 + kshift;
           const bool there0 = !gone0 && kbase + i < sq.len;
           const bool there1 = !gone1 && kbase + KV4_KEYS + i < sq.len;
-          const int sh = 16 + kshift;
-          const bool n0 = there0 && ((s0 >> sh) & 255) == 255, n1 = there0 && ((s1 >> sh) & 255) == 255;
-          const bool n2 = there1 && ((s2 >> sh) & 255) == 255, n3 = there1 && ((s3 >> sh) & 255) == 255;
+          auto nan_at = [&](int at) { return ((*reinterpret_cast<const uint32_t*>(kb + at) >> sh) & 255u) == 255u; };
+          const bool n0 = there0 && nan_at(0), n1 = there0 && nan_at(128);
+          const bool n2 = there1 && nan_at(KV4_BLOCK), n3 = there1 && nan_at(KV4_BLOCK + 128);
           if (__ballot(n0 || n1 || n2 || n3)) {
             const float nan = __builtin_nanf("");
 #pragma unroll 1
@@ -1000,27 +1075,6 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
                 });
             }
           }
-        }
-        const float e0 = M::kUnit * exponent((s0 >> kshift) & 255u);
-        const float e1 = M::kUnit * exponent((s1 >> kshift) & 255u);
-        const float e2 = M::kUnit * exponent((s2 >> kshift) & 255u);
-        const float e3 = M::kUnit * exponent((s3 >> kshift) & 255u);
-        floatx16 s[2] = {};
-        static_for<0, 4>([&](auto step) {
-          constexpr int st = step;
-          s[0] = M::mfma(M::dequant(k0[st], e0), qf[st], s[0]);
-          s[1] = M::mfma(M::dequant(k2[st], e2), qf[st], s[1]);
-          if constexpr (st < LOADS) issue(f, slot3, st);
-        });
-        if constexpr (LOADS > 4) issue(f, slot3, 4);
-        static_for<0, 4>([&](auto step) {
-          constexpr int st = step;
-          s[0] = M::mfma(M::dequant(k1[st], e1), qf[4 + st], s[0]);
-          s[1] = M::mfma(M::dequant(k3[st], e3), qf[4 + st], s[1]);
-        });
-        write_v(b + 2, to ^ 1, absent >> 2);
-        if (masked) {
-          asm volatile("");   // (a branch: as selects these are a third of the loop)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int lim = (u ? gone1 : gone0) ? 0 : vis;
@@ -1029,11 +1083,40 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
               if (kbase + 32 * u + 4 * h + (r & 3) + 8 * (r >> 2) >= lim) s[u][r] = -INFINITY;
           }
         }
-        float top = fmaxf(s[0][0], s[1][0]);
+        const float e[4] = {k_unit(0), k_unit(1), k_unit(2), k_unit(3)};
+        v8 p[4];
+        float sum = 0.f;
+        auto weights = [&](int q, float ref) __attribute__((always_inline)) {   // of 16 keys
+          const int u = q >> 1, r0 = 8 * (q & 1);
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
-        top *= scale;
-        if (!__all(top <= mrun + KV4_SLACK)) {
+          for (int r = 0; r < 8; r += 2) {
+            const v2 x = __builtin_convertvector(
+                ((floatx2){__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r0 + r], scale, ref)),
+                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r0 + r + 1], scale, ref))}), v2);
+            sum = M::sum2(x, sum);
+            p[q][r] = x.x;
+            p[q][r + 1] = x.y;
+          }
+        };
+        const float ref = KV4_LIFT - mrun;
+        t[0] = t[1] = (floatx16){};
+        static_for<0, 4>([&](auto quarter) {
+          constexpr int q = quarter;
+          static_for<0, 2>([&](auto half) {
+            constexpr int k = 2 * q + half;
+            t[0] = M::mfma(M::dequant(kc[k >> 2][k & 3], e[k >> 2]), qf[k], t[0]);
+            t[1] = M::mfma(M::dequant(kc[2 + (k >> 2)][k & 3], e[2 + (k >> 2)]), qf[k], t[1]);
+          });
+          weights(q, ref);
+        });
+        // Weights above 2^15 (the sum of 32 says so; an infinity and a NaN do too): the reference
+        // is raised where the largest logit is more than KV4_SLACK above it, and they are made
+        // again.  So no maximum is taken in the steps in which none is needed.
+        if (!__all(sum <= 1048576.f)) {
+          float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+          for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
+          top *= scale;
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           const float mnew = top > mrun + KV4_SLACK ? top : mrun;
           const float alpha = __builtin_amdgcn_exp2f(mrun - mnew);
@@ -1041,45 +1124,38 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
 #pragma unroll
           for (int d = 0; d < 4; ++d) o[d] *= alpha;
           mrun = mnew;
+          sum = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) weights(q, KV4_LIFT - mrun);
         }
-        const float ref = KV4_LIFT - mrun;
+        lrun += sum;
         const unsigned char* vb = vbuf + 2 * to * VTILE + vread;
-        static_for<0, 4>([&](auto quarter) {   // 16 keys each
-          constexpr int st = quarter & 1, u = quarter >> 1;
-          v8 vf[4], p;   // (the reads' latency passes while the weights are made)
+        static_for<0, 4>([&](auto quarter) {
+          constexpr int q = quarter, st = q & 1, u = q >> 1;
           static_for<0, 4>([&](auto dt) {
             constexpr int d = dt;
             const unsigned char* at = vb + u * VTILE + 16 * st * TROW + 64 * d;
-            vf[d] = read_vt<T>(at, at + 8 * TROW);
-          });
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int r = 0; r < 8; r += 2) {
-            const v2 x = __builtin_convertvector(
-                ((floatx2){__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * st + r], scale, ref)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * st + r + 1], scale, ref))}), v2);
-            lrun = M::sum2(x, lrun);
-            p[r] = x.x;
-            p[r + 1] = x.y;
-          }
-          static_for<0, 4>([&](auto dt) {
-            constexpr int d = dt;
-            o[d] = M::mfma(vf[d], p, o[d]);
+            o[d] = M::mfma(read_vt<T>(at, at + 8 * TROW), p[q], o[d]);
           });
         });
       }
-      page = pages(b + 2 * TDEPTH + 2);
+      write_v(b + 2, to ^ 1, absent >> 2);
       if ((absent & 3) && threadIdx.x == 0) atomicOr(a.err, KV4_ERR_PAGE);
       absent >>= 2;
       slot = slot1;
       to ^= 1;
+    };
+    floatx16 t[2];
+    for (int b = run.b0; b < b_end; b += 4) {
+      do_step(b, s, t);
+      if (b + 2 < b_end) do_step(b + 2, t, s);
     }
     __builtin_amdgcn_s_waitcnt(0);   // (the loads past the last block)
 
     lrun += __shfl_xor(lrun, 32, 64);
     asm volatile("" : "+v"(le));
     if (!run.whole) {
-      float* piece = a.ws + kv4_piece(walk.w, walk.per, run.r0) * kv4_piece_floats(ROWS);
+      float* piece = a.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -1111,36 +1187,22 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
   }
 }
 
-// Units that several workers share: their partial states joined in the order of the keys.  A
-// thread has 4 values of a row.  TILE: the partials are kv4_tile_kernel's.
+// Units that several workers share: their partial states joined in the order of the keys, by the
+// note of the worker that began with the unit.  A thread has 4 values of a row.  TILE: the partials
+// are kv4_tile_kernel's.
 template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
   const int lane = threadIdx.x & 63;
   const int ratio = a.n_heads / a.n_kv;
   const int groups = tile_rows / 8;                 // workgroups of a unit
-  const long long unit = blockIdx.x / groups;
+  const int w0 = blockIdx.x / groups;               // the worker
   const int f = (int)(blockIdx.x % groups) * 256 + threadIdx.x;   // which 4 values of the tile
   const int c = TILE ? 32 * (f >> 10) + (lane & 31) : 16 * (f >> 9) + (lane & 15);
   const int col = TILE ? 32 * ((f >> 8) & 3) + 8 * ((f >> 6) & 3) + 4 * (lane >> 5)
                        : 16 * ((f >> 6) & 7) + 4 * (lane >> 4);
-  long long before;
-  const int s = __builtin_amdgcn_readfirstlane(attn_find<true>(a, tile_rows, unit, before));
-  if (s >= a.n_seq) return;
-  const Kv4Seq sq = attn_seq(a, s, tile_rows);
-  const int u = (int)(unit - before);
-  const int head = u / sq.tiles, tile = u - head * sq.tiles;
-  const int r = tile * tile_rows + c;
-  // places: those of the sequences before s, then of the units before this one
-  long long t = 0, all = 0;
-  for (int k = lane; k < a.n_seq; k += 64) {
-    const long long cost = kv4_cost(attn_seq(a, k, tile_rows), a.n_kv);
-    all += cost;
-    if (k < s) t += cost;
-  }
-  const long long per = kv4_per(wave_sum_ll(all), a.workers);
-  const long long r0 = wave_sum_ll(t) + (long long)u * kv4_span(sq) + KV4_PAD;
-  const int w0 = (int)(r0 / per), w1 = (int)((r0 + sq.nblk - 1) / per);
-  if (w0 == w1 || r >= sq.qlen * ratio) return;   // one worker had it all; no such row
+  const Kv4Note& n = kv4_notes(a, tile_rows)[w0];
+  const int w1 = n.w1, head = n.head, r = n.tile * tile_rows + c;
+  if (w1 < 0 || r >= n.qlen * ratio) return;
   const long long pf = kv4_piece_floats(tile_rows);
   float m = -FLT_MAX, l = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
@@ -1150,7 +1212,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
     floatx2 y[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float* p = a.ws + kv4_piece(min(w + j, w1), per, r0) * pf;
+      const int k = min(w + j, w1);   // (that of the first lies behind its other one)
+      const float* p = a.ws + (2ll * k + (k == w0 ? 1 : 0)) * pf;
       x[j] = *reinterpret_cast<const floatx4*>(p + 4 * f);
       y[j] = *reinterpret_cast<const floatx2*>(p + tile_rows * KV4_D + 2 * c);
       if (w + j > w1) {   // (0 * what lies there may be NaN)
@@ -1173,8 +1236,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
     }
   }
   const int tok = r / ratio;
-  const long long orow = (long long)(sq.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
-  const bool none = attn_visible(a, sq, tok) <= 0;
+  const long long orow = (long long)(n.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
+  const bool none = a.causal ? n.len - n.qlen + tok < 0 : n.len == 0;
   typedef T v4 __attribute__((ext_vector_type(4)));
   v4 x;
 #pragma unroll
@@ -1184,29 +1247,15 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
     a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
 }
 
-// Units that a launch can have at most: a tile holds a row of its sequence.
-long long max_units(int n_rows, int n_heads, int n_kv, int n_seq, int tile_rows) {
-  const long long rows = (long long)n_rows * (n_heads / n_kv);
-  return (rows / tile_rows + (n_seq < n_rows ? n_seq : n_rows)) * n_kv;
-}
-
-template <typename T, int WQ>
-void launch_tile(const Kv4AttnArgs& a, const Kv4Cut& c, dim3 grid, hipStream_t st) {
-  if (c.whole) hipLaunchKernelGGL((kv4_tile_kernel<T, WQ, true>), grid, dim3(64 * WQ), TILE_LDS, st, a);
-  else hipLaunchKernelGGL((kv4_tile_kernel<T, WQ, false>), grid, dim3(64 * WQ), TILE_LDS, st, a);
-}
 template <typename T>
 void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
-  const long long units = max_units(a.n_rows, a.n_heads, a.n_kv, a.n_seq, c.tile_rows);
-  const dim3 grid(c.whole ? (unsigned)units : (unsigned)c.workers), block(256);
+  const dim3 grid(a.workers), block(256), mgrid((a.workers - 1) * (c.tile_rows / 8));
   switch (c.tile_rows) {
     case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a); break;
     case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a); break;
-    case 64: launch_tile<T, 2>(a, c, grid, st); break;
-    default: launch_tile<T, 4>(a, c, grid, st);
+    case 64: hipLaunchKernelGGL((kv4_tile_kernel<T, 2>), grid, dim3(128), TILE_LDS, st, a); break;
+    default: hipLaunchKernelGGL((kv4_tile_kernel<T, 4>), grid, block, TILE_LDS, st, a);
   }
-  if (c.whole) return;
-  const dim3 mgrid((unsigned)(units * (c.tile_rows / 8)));
   if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
   else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);
 }
@@ -1215,16 +1264,11 @@ void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
 
 Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
   Kv4Cut c{};
-  const int ratio = n_heads / n_kv;
   // rows of a kv head in a sequence, on average over those that can have any
   const long long seqs = n_seq < n_rows ? n_seq : n_rows;
-  const long long rows = ((long long)n_rows * ratio + seqs - 1) / seqs;
+  const long long rows = ((long long)n_rows * (n_heads / n_kv) + seqs - 1) / seqs;
   c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : 2);
-  // Prompts, of several tiles a sequence and enough units for every workgroup to have some: a unit
-  // to a workgroup, the longest first
-  const long long tiles = (long long)n_rows * ratio / c.tile_rows;
-  c.whole = tiles >= 4ll * n_seq && tiles * n_kv >= 2ll * c.workers;
+  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : c.tile_rows == 64 ? 4 : 2);
   return c;
 }
 

@@ -49,64 +49,88 @@ static void asks() {
   must(kv4_ask(0, 0, 0x7fffffe0, 0x3ffffff, 5, a), "the longest table");
 }
 
+// Keys that the last row of a tile sees, from the definition.
+static long long seen(const Kv4Seq& s, int ratio, int rows, int t, bool causal) {
+  long long last = (long long)(t + 1) * rows - 1;
+  if (last > (long long)s.qlen * ratio - 1) last = (long long)s.qlen * ratio - 1;
+  long long v = causal ? s.len - s.qlen + last / ratio + 1 : s.len;
+  return v < 0 ? 0 : v > s.len ? s.len : v;
+}
+
 // Every block of every unit is one worker's; the pieces of a shared unit are different slots, and
 // those that the merge reads are those that the workers write.
-static void split(const std::vector<int>& q, const std::vector<int>& lens, int heads, int kv, int rows, int workers) {
-  std::vector<Kv4Seq> s;
+static void split(const std::vector<int>& q, const std::vector<int>& lens, int heads, int kv, int rows, int workers,
+                  bool causal) {
+  struct U { long long r0; int nblk; };
+  std::vector<U> units;
   int at = 0, n = 0;
   for (int m : q) n += m;
   long long total = 0;
   for (size_t i = 0; i < q.size(); ++i) {
-    s.push_back(kv4_seq(at, at + q[i], lens[i], n, 1 << 20, 5, heads / kv, rows));
-    must(!s.back().bad, "the rows fit");
+    const Kv4Seq s = kv4_seq(at, at + q[i], lens[i], n, 1 << 20, 5, heads / kv, rows, causal);
+    must(!s.bad, "the rows fit");
     at += q[i];
-    total += kv4_cost(s.back(), kv);
+    const long long head = kv4_places(s, s.tiles);
+    for (int h = 0; h < kv; ++h)
+      for (int t = 0; t < s.tiles; ++t) {
+        const long long p0 = kv4_places(s, t), p1 = kv4_places(s, t + 1);
+        const int nblk = (int)(p1 - p0) - KV4_PAD;
+        const long long need = (seen(s, heads / kv, rows, t, causal) + 31) / 32;
+        must(nblk >= 1 && nblk >= need, "a place for each block");
+        must(lens[i] < q[i] || nblk <= need + 2, "few places besides");
+        for (long long r = p0; r < p1; r += r + 97 < p1 ? 97 : 1)
+          must(kv4_begun(s, t, r) && (t + 1 == s.tiles || !kv4_begun(s, t + 1, r)), "a place is its tile's");
+        units.push_back({total + h * head + p0 + KV4_PAD, nblk});
+      }
+    total += kv4_cost(s, kv);
   }
   const long long per = kv4_per(total, workers);
   must(per >= KV4_MIN_PLACES && per * workers >= total, "the workers cover the places");
   std::vector<int> done(total, 0), slot(2ll * workers, 0), want(2ll * workers, 0);
-  for (long long w = 0; w < workers; ++w) {
-    long long pos = w * per;
-    const long long end = pos + per < total ? pos + per : total;
-    while (pos < end) {   // as the kernel walks
-      long long before = 0;
-      size_t i = 0;
-      while (before + kv4_cost(s[i], kv) <= pos) before += kv4_cost(s[i++], kv);
-      const int span = kv4_span(s[i]);
-      const long long unit = (pos - before) / span, r0 = before + unit * span + KV4_PAD;
-      const long long b0 = pos > r0 ? pos - r0 : 0, b1 = s[i].nblk < end - r0 ? s[i].nblk : end - r0;
-      must(unit < (long long)s[i].tiles * kv, "a unit of the sequence");
-      pos = r0 + s[i].nblk;
+  long long end_of_last = 0;
+  for (const U& u : units) {
+    must(u.r0 - KV4_PAD == end_of_last, "units lie one behind the other");
+    end_of_last = u.r0 + u.nblk;
+    int shared = 0;
+    for (long long w = (u.r0 - KV4_PAD) / per; w * per < u.r0 + u.nblk; ++w) {   // as the walk cuts it
+      const long long pos = w * per > u.r0 - KV4_PAD ? w * per : u.r0 - KV4_PAD;
+      const long long end = (w + 1) * per < total ? (w + 1) * per : total;
+      const long long b0 = pos > u.r0 ? pos - u.r0 : 0, b1 = u.nblk < end - u.r0 ? u.nblk : end - u.r0;
       if (b1 <= 0) continue;
       must(b1 > b0, "a run is not empty");
-      for (long long b = b0; b < b1; ++b) ++done[r0 + b];
-      if (b0 > 0 || b1 < s[i].nblk) {
-        const long long p = kv4_piece(w, per, r0);
+      for (long long b = b0; b < b1; ++b) ++done[u.r0 + b];
+      if (b0 > 0 || b1 < u.nblk) {
+        const long long p = kv4_piece(w, per, u.r0);
         must(p >= 0 && p < 2ll * workers && !slot[p]++, "two pieces in one slot");
+        ++shared;
       }
     }
-  }
-  long long u0 = 0;
-  for (auto& x : s)
-    for (long long u = 0; u < (long long)x.tiles * kv; ++u, u0 += kv4_span(x)) {
-      const long long r0 = u0 + KV4_PAD;
-      for (int k = 0; k < kv4_span(x); ++k) must(done[u0 + k] == (k >= KV4_PAD), "each block once");
-      const long long w0 = r0 / per, w1 = (r0 + x.nblk - 1) / per;
-      if (w0 != w1)
-        for (long long w = w0; w <= w1; ++w) ++want[kv4_piece(w, per, r0)];
+    // the merge: the worker that begins inside the unit's blocks first
+    int merged = 0;
+    for (long long first = u.r0 / per; first * per < u.r0 + u.nblk; ++first) {
+      const long long pos = first * per;
+      if (first < 1 || pos <= u.r0 || pos - per > u.r0) continue;
+      must(++merged == 1, "one worker's affair");
+      for (long long w = first - 1; w <= (u.r0 + u.nblk - 1) / per; ++w) ++want[kv4_piece(w, per, u.r0)];
     }
-  must(u0 == total && slot == want, "the merge reads what was written");
+    must(merged == (shared > 0), "merged if shared");
+    for (int k = -KV4_PAD; k < u.nblk; ++k) must(done[u.r0 + k] == (k >= 0), "each block once");
+  }
+  must(end_of_last == total && slot == want, "the merge reads what was written");
 }
 
 static void seqs() {
   // row ranges and lengths that do not fit make a sequence without rows
-  for (auto t : {std::vector<int>{-1, 3, 5}, {3, 2, 5}, {0, 11, 5}, {0, 1, -1}, {0, 1, 97}, {0, 0x7fffffff, 1}}) {
-    const Kv4Seq s = kv4_seq(t[0], t[1], t[2], 10, 3, 5, 4, 16);
-    must(s.bad && s.qlen == 0 && s.tiles == 0 && kv4_cost(s, 8) == 0, "a bad sequence has no work");
-  }
-  const Kv4Seq e = kv4_seq(2, 3, 0, 10, 3, 5, 4, 16);
-  must(!e.bad && e.nblk == 1 && e.tiles == 1, "a row without keys is still written");
-  must(kv4_cost(kv4_seq(0, 0, 90, 10, 3, 5, 4, 16), 8) == 0, "a sequence without rows costs nothing");
+  for (auto t : {std::vector<int>{-1, 3, 5}, {3, 2, 5}, {0, 11, 5}, {0, 1, -1}, {0, 1, 97}, {0, 0x7fffffff, 1}})
+    for (bool causal : {false, true}) {
+      const Kv4Seq s = kv4_seq(t[0], t[1], t[2], 10, 3, 5, 4, 16, causal);
+      must(s.bad && s.qlen == 0 && s.tiles == 0 && kv4_cost(s, 8) == 0, "a bad sequence has no work");
+    }
+  const Kv4Seq e = kv4_seq(2, 3, 0, 10, 3, 5, 4, 16, false);
+  must(!e.bad && e.tiles == 1 && kv4_places(e, 1) == KV4_PAD + 1, "a row without keys is still written");
+  must(kv4_cost(kv4_seq(0, 0, 90, 10, 3, 5, 4, 16, true), 8) == 0, "a sequence without rows costs nothing");
+  must(kv4_counts_fit(1 << 20, 8, 8, 64, 1 << 15, 6), "large launches fit");
+  must(!kv4_counts_fit(0x7fffffff, 1024, 1, 65536, 0x3ffffff, 5), "launches past 62 bits do not");
 }
 
 static void rules() {
@@ -178,12 +202,15 @@ int main() {
   asks();
   seqs();
   for (int workers : {1, 3, 256, 768})
-    for (int rows : {16, 32, 64}) {
-      split({1}, {1}, 32, 8, rows, workers);
-      split({1}, {33000}, 32, 8, rows, workers);
-      split({32, 0, 7, 1, 300}, {500, 90, 0, 1, 4097}, 40, 8, rows, workers);
-      split({1, 1, 1, 1, 1, 1, 1}, {511, 512, 513, 16, 100000, 3, 2000}, 5, 1, rows, workers);
-    }
+    for (int rows : {16, 32, 64, 128})
+      for (bool causal : {false, true}) {
+        split({1}, {1}, 32, 8, rows, workers, causal);
+        split({1}, {33000}, 32, 8, rows, workers, causal);
+        split({32, 0, 7, 1, 300}, {500, 90, 0, 1, 4097}, 40, 8, rows, workers, causal);
+        split({1, 1, 1, 1, 1, 1, 1}, {511, 512, 513, 16, 100000, 3, 2000}, 5, 1, rows, workers, causal);
+        split({700, 64, 5}, {700, 3000, 2}, 21, 3, rows, workers, causal);
+        split({333}, {90}, 2, 2, rows, workers, causal);
+      }
   rules();
   std::printf("ok\n");
   return 0;
