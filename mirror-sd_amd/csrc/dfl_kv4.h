@@ -153,9 +153,10 @@ DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_s
 }
 // slope t (t - 1) / 2 + base t
 DFL_HD long long kv4_sum(const Kv4Seq& s, long long t) { return s.slope * (t * (t - 1) / 2) + s.base * t; }
-DFL_HD long long kv4_div(long long n, long long d) {   // for 0 <= n, 0 < d (in 32 bits where it fits)
-  return n <= 0xffffffffll && d <= 0xffffffffll ? (long long)((uint32_t)n / (uint32_t)d) : n / d;
-}
+// floor(n / d) for 0 <= n < 2^52, 0 < d: both are whole in a double, and a quotient below a whole
+// number is below it by at least 1 / d, more than the rounding.  (The wide whole-number division is
+// some 170 instructions, and there are seven of them.)
+DFL_HD long long kv4_div(long long n, long long d) { return (long long)((double)n / (double)d); }
 // Places of a head's first t tiles, and of a sequence's units.
 DFL_HD long long kv4_places(const Kv4Seq& s, long long t) {
   return KV4_PAD * t + kv4_div(kv4_sum(s, t), s.m);
@@ -184,12 +185,12 @@ struct Kv4Note { int w1, head, tile, q0, qlen, len, pad[2]; };
 DFL_HD long long kv4_ws_bytes(int tile_rows, int workers) {
   return workers * (2 * kv4_piece_floats(tile_rows) * (long long)sizeof(float) + (long long)sizeof(Kv4Note));
 }
-// Whether every count above stays below 2^62, for any lengths that the launch can have.
-DFL_HD bool kv4_counts_fit(int n_rows, int ratio, int n_kv, int n_seq, int width, int page_shift) {
+// Whether every count above stays below 2^52, for any lengths that the launch can have.
+DFL_HD bool kv4_counts_fit(int n_rows, int ratio, int n_kv, int n_seq, int width, int page_shift, int tile_rows) {
   const double cap = (double)((long long)width << page_shift) + KV4_KEYS;
-  const double tiles = (double)n_rows * ratio / 16 + n_seq + 1;
-  const double sum = 128.0 * tiles * tiles + (ratio * cap + 128.0) * tiles;
-  return sum * (n_kv + 1) < 4e18;
+  const double tiles = (double)n_rows * ratio / tile_rows + n_seq + 1;
+  const double sum = tile_rows * tiles * tiles + (ratio * cap + tile_rows) * tiles;
+  return sum < 4e15 && (sum / KV4_KEYS + KV4_PAD * tiles) * n_kv < 4e15;
 }
 
 // How a launch is cut (what its workspace holds follows from it).
@@ -198,7 +199,15 @@ struct Kv4Cut {
                    // keys) or 64, 128 (each wave has 32 of them and all keys)
   int workers;     // workgroups
 };
-Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq);
+inline Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
+  Kv4Cut c{};
+  // rows of a kv head in a sequence, on average over those that can have any
+  const long long seqs = n_seq < n_rows ? n_seq : n_rows;
+  const long long rows = ((long long)n_rows * (n_heads / n_kv) + seqs - 1) / seqs;
+  c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : c.tile_rows == 64 ? 4 : 2);
+  return c;
+}
 
 inline const char* check_kv4_pool(int n_kv, int page_shift, int n_pages) {
   if (n_kv < 1 || n_kv > 1024) return "kv heads outside [1, 1024]";
@@ -241,7 +250,8 @@ inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
   if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
   if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll)
     return "table width out of range";
-  if (!kv4_counts_fit(a.n_rows, a.n_heads / a.n_kv, a.n_kv, a.n_seq, a.width, a.page_shift))
+  if (a.n_rows > 0 && !kv4_counts_fit(a.n_rows, a.n_heads / a.n_kv, a.n_kv, a.n_seq, a.width, a.page_shift,
+                                      kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq).tile_rows))
     return "too many query rows for so long a table";
   if (!(a.scale_log2 > 0.f) || a.scale_log2 > 1e30f) return "scale must be positive and finite";
   if (!a.q || !a.out || !a.starts || !a.lens || !a.table || !a.pool || !a.err) return "null pointer";

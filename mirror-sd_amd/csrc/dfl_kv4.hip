@@ -1206,8 +1206,9 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
   const long long pf = kv4_piece_floats(tile_rows);
   float m = -FLT_MAX, l = 0.f;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  constexpr int N = 12;   // pieces in flight
-  for (int w = w0; w <= w1; w += N) {
+  // N pieces from w on, all loads under way together
+  auto join = [&](int w, auto count) __attribute__((always_inline)) {
+    constexpr int N = count;
     floatx4 x[N];
     floatx2 y[N];
 #pragma unroll
@@ -1216,14 +1217,16 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
       const float* p = a.ws + (2ll * k + (k == w0 ? 1 : 0)) * pf;
       x[j] = *reinterpret_cast<const floatx4*>(p + 4 * f);
       y[j] = *reinterpret_cast<const floatx2*>(p + tile_rows * KV4_D + 2 * c);
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
       if (w + j > w1) {   // (0 * what lies there may be NaN)
         x[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
         y[j] = (floatx2){-INFINITY, 0.f};
       }
+      mn = fmaxf(mn, y[j].x);
     }
-    float mn = m;
-#pragma unroll
-    for (int j = 0; j < N; ++j) mn = fmaxf(mn, y[j].x);
     const float k = __builtin_amdgcn_exp2f(m - mn);
     o *= k;
     l *= k;
@@ -1234,6 +1237,11 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
       l += e * y[j].y;
       o += e * x[j];
     }
+  };
+  if (w1 == w0 + 1) {
+    join(w0, std::integral_constant<int, 2>{});
+  } else {
+    for (int w = w0; w <= w1; w += 8) join(w, std::integral_constant<int, 8>{});
   }
   const int tok = r / ratio;
   const long long orow = (long long)(n.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
@@ -1261,16 +1269,6 @@ void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
 }
 
 }  // namespace
-
-Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
-  Kv4Cut c{};
-  // rows of a kv head in a sequence, on average over those that can have any
-  const long long seqs = n_seq < n_rows ? n_seq : n_rows;
-  const long long rows = ((long long)n_rows * (n_heads / n_kv) + seqs - 1) / seqs;
-  c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : c.tile_rows == 64 ? 4 : 2);
-  return c;
-}
 
 void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st) {
   if (a.n_seq <= 64 && a.max_rows <= 4096) {

@@ -129,8 +129,13 @@ static void seqs() {
   const Kv4Seq e = kv4_seq(2, 3, 0, 10, 3, 5, 4, 16, false);
   must(!e.bad && e.tiles == 1 && kv4_places(e, 1) == KV4_PAD + 1, "a row without keys is still written");
   must(kv4_cost(kv4_seq(0, 0, 90, 10, 3, 5, 4, 16, true), 8) == 0, "a sequence without rows costs nothing");
-  must(kv4_counts_fit(1 << 20, 8, 8, 64, 1 << 15, 6), "large launches fit");
-  must(!kv4_counts_fit(0x7fffffff, 1024, 1, 65536, 0x3ffffff, 5), "launches past 62 bits do not");
+  must(kv4_counts_fit(1 << 20, 8, 8, 64, 1 << 15, 6, 128), "large launches fit");
+  must(kv4_counts_fit(65536, 1024, 1, 1024, 1 << 14, 6, 128), "with a thousand heads to a kv head too");
+  must(!kv4_counts_fit(0x7fffffff, 1024, 1, 65536, 0x3ffffff, 5, 16), "launches past 52 bits do not");
+  for (long long d : {1ll, 3ll, 7ll, 1024ll, 32768ll, 1000003ll, (1ll << 40) + 1})
+    for (long long q : {0ll, 1ll, 2ll, 12345ll, (1ll << 52) / d - 2})
+      for (long long r : {0ll, 1ll, d / 2, d - 1})
+        if (q >= 0 && r < d && q * d + r < (1ll << 52)) must(kv4_div(q * d + r, d) == q, "division");
 }
 
 static void rules() {
