@@ -24,10 +24,19 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 // sequence, so a step that puts back what it takes leaves every table as it was.
 //
 // Phases, each over all sequences: scan (totals, then offsets), free, take, rows.  A phase reads
-// what the one before wrote, so they are launches of their own, or for a few sequences one
-// workgroup with barriers between them.
+// what the one before wrote, so for many sequences or rows they are launches of their own; up to
+// STEP_ONE_SEQS and STEP_ONE_ROWS one workgroup does them all, with the offsets in LDS.  In both
+// forms the pages and rows of all sequences are numbered through and found by a search in the
+// offsets, so that no thread waits for a long sequence.
+//
+// Bound by latencies: launches and a handful of reads that follow on each other.  One workgroup
+// against launches, us (sequences x new rows of each; every page put back and taken again):
+//   8 x 16 5.0, 11.6;  256 x 16 11.2, 18.2;  1024 x 8 16.5, 22.2;  8 x 1024 11.0, 13.7;
+//   1024 x 32 38.6, 20.4;  64 x 512 29.4, 16.2;  8 x 4096 22.5, 14.1.
 
-// Inclusive sums over the workgroup's threads of three counts at once.
+constexpr int STEP_ONE_SEQS = 1024, STEP_ONE_ROWS = 8192;
+
+// Sums over the workgroup's threads of three counts at once (inclusive), and their totals.
 struct Sum3 { long long a, b, c; };
 DFL_DEV Sum3 block_scan3(Sum3 v, Sum3* lds /* 16 */, Sum3& total) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
@@ -41,23 +50,113 @@ DFL_DEV Sum3 block_scan3(Sum3 v, Sum3* lds /* 16 */, Sum3& total) {
   __syncthreads();
   total = Sum3{0, 0, 0};
   for (int w = 0; w < nw; ++w) {
-    if (w < wv) { v.a += lds[w].a; v.b += lds[w].b; v.c += lds[w].c; }
-    total.a += lds[w].a; total.b += lds[w].b; total.c += lds[w].c;
+    const Sum3 x = lds[w];
+    if (w < wv) { v.a += x.a; v.b += x.b; v.c += x.c; }
+    total.a += x.a; total.b += x.b; total.c += x.c;
   }
   return v;
 }
 
-struct StepView { int *base, *f_at, *t_at; };
-DFL_DEV StepView step_view(const Kv4StepArgs& a) {
-  return StepView{a.scratch + 4, a.scratch + 4 + a.n_seq, a.scratch + 4 + 2 * a.n_seq};
-}
 DFL_DEV bool step_ask(const Kv4StepArgs& a, int s, Kv4Ask& q) {
   const int len = a.lens[s];
   return kv4_ask(len, a.keep ? a.keep[s] : len, a.grow ? a.grow[s] : 0, a.width, a.page_shift, q);
 }
+// Why a step cannot be done (0: it can), from its totals.
+DFL_DEV int step_error(const Kv4StepArgs& a, bool bad, const Sum3& all, int n_free) {
+  int err = bad ? KV4_ERR_LEN : 0;
+  // (freed pages beyond the pool, or a free count beyond it: the state is not a step's)
+  if (n_free < 0 || n_free > a.n_pages || n_free + all.a > a.n_pages) err |= KV4_ERR_PAGE;
+  else if (all.b > n_free + all.a) err |= KV4_ERR_POOL;
+  if (all.c > a.max_rows) err |= KV4_ERR_ROWS;
+  return err;
+}
+// The last of the ascending n numbers at (n > 0, at[0] <= v) that is not above v, of equals the last.
+DFL_DEV int step_search(const int* at, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (at[mid] <= v) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+// Offsets of all sequences: kept lengths, pages put back and taken before each (n_seq), new rows
+// before each (n_seq + 1).
+struct StepView { int *base, *f_at, *t_at, *starts; };
+// Page i of those put back: from its table onto the stack.
+DFL_DEV void step_free(const Kv4StepArgs& a, const StepView& v, int i, int top) {
+  const int s = step_search(v.f_at, a.n_seq, i);
+  int* at = a.table + (long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.f_at[s]);
+  const int p = *at;
+  if (p < 0 || p >= a.n_pages) atomicOr(a.err, KV4_ERR_PAGE);
+  a.free_pages[top - i] = p;
+  *at = -1;
+}
+// Page i of those taken: from the stack into its table.
+DFL_DEV void step_take(const Kv4StepArgs& a, const StepView& v, int i, int top) {
+  const int s = step_search(v.t_at, a.n_seq, i);
+  a.table[(long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.t_at[s])] = a.free_pages[top - i];
+  a.free_pages[top - i] = -1;
+}
+// Slot and position of new row r of sequence s.
+struct StepRow { int slot, pos; };
+DFL_DEV StepRow step_row(const Kv4StepArgs& a, const StepView& v, int s, int r) {
+  const int pos = v.base[s] + (r - v.starts[s]);
+  const int pg = a.table[(long long)s * a.width + (pos >> a.page_shift)];
+  const int in = pos & ((1 << a.page_shift) - 1);
+  return StepRow{pg < 0 || pg >= a.n_pages ? -1 : (pg << a.page_shift) + in, pos};
+}
 
-// One workgroup: status and totals into scratch[0 .. 3], offsets and starts; all or nothing.
-DFL_DEV void step_scan(const Kv4StepArgs& a, Sum3* lds) {
+// One workgroup, a thread to a sequence.  Eight sequences of up to 16 new rows: 11.1 us with the
+// offsets in memory and a wave to each sequence's pages, 5.2 so.
+__global__ __launch_bounds__(1024) void kv4_step_one_kernel(Kv4StepArgs a) {
+  __shared__ Sum3 lds[16];
+  __shared__ int offsets[4][STEP_ONE_SEQS + 1];
+  const StepView v{offsets[0], offsets[1], offsets[2], offsets[3]};
+  const int s = threadIdx.x, nt = blockDim.x;
+  Kv4Ask q{0, 0, 0, 0};
+  bool bad = false;
+  if (s < a.n_seq) bad = !step_ask(a, s, q);
+  const int n_free = *a.n_free;
+  Sum3 all;
+  const Sum3 in = block_scan3(Sum3{q.freed, q.taken, q.grow}, lds, all);
+  const int err = step_error(a, __syncthreads_or(bad), all, n_free);
+  if (s < a.n_seq) {
+    v.base[s] = q.keep;
+    v.f_at[s] = (int)(in.a - q.freed);
+    v.t_at[s] = (int)(in.b - q.taken);
+    a.starts[s] = v.starts[s] = err ? 0 : (int)(in.c - q.grow);
+  }
+  if (s == 0) {
+    a.starts[a.n_seq] = err ? 0 : (int)all.c;
+    if (err) atomicOr(a.err, err);
+    else *a.n_free = (int)(n_free + all.a - all.b);
+  }
+  const int rows = err ? 0 : (int)all.c;
+  if (!err) {
+    const int top = (int)(n_free + all.a) - 1;
+    __syncthreads();
+    for (int i = s; i < all.a; i += nt) step_free(a, v, i, top);
+    __syncthreads();
+    for (int i = s; i < all.b; i += nt) step_take(a, v, i, top);
+    if (s < a.n_seq) a.lens[s] = q.keep + q.grow;
+    __syncthreads();
+  }
+  for (int r = s; r < a.max_rows; r += nt) {
+    StepRow x{-1, -1};
+    if (r < rows) x = step_row(a, v, step_search(v.starts, a.n_seq, r), r);
+    a.slots[r] = x.slot;
+    a.positions[r] = x.pos;
+  }
+}
+
+// The same in launches.  scratch: error, pages put back and taken, free pages before; then the
+// offsets but for the rows', which are a.starts.
+DFL_DEV StepView step_view(const Kv4StepArgs& a) {
+  return StepView{a.scratch + 4, a.scratch + 4 + a.n_seq, a.scratch + 4 + 2 * a.n_seq, a.starts};
+}
+__global__ __launch_bounds__(1024) void kv4_step_scan_kernel(Kv4StepArgs a) {
+  __shared__ Sum3 lds[16];
+  const StepView v = step_view(a);
   const int nt = blockDim.x;
   Sum3 all{0, 0, 0};
   int bad = 0;
@@ -66,34 +165,21 @@ DFL_DEV void step_scan(const Kv4StepArgs& a, Sum3* lds) {
     Kv4Ask q{0, 0, 0, 0};
     if (s < a.n_seq && !step_ask(a, s, q)) bad = 1;
     Sum3 t;
-    block_scan3(Sum3{q.freed, q.taken, q.grow}, lds, t);
-    all.a += t.a; all.b += t.b; all.c += t.c;
-  }
-  bad = __syncthreads_or(bad);
-  const int n_free = *a.n_free;
-  int err = bad ? KV4_ERR_LEN : 0;
-  // (freed pages beyond the pool, or a free count beyond it: the state is not a step's)
-  if (n_free < 0 || n_free > a.n_pages || n_free + all.a > a.n_pages) err |= KV4_ERR_PAGE;
-  else if (all.b > n_free + all.a) err |= KV4_ERR_POOL;
-  if (all.c > a.max_rows) err |= KV4_ERR_ROWS;
-  const StepView v = step_view(a);
-  Sum3 at{0, 0, 0};
-  for (int s0 = 0; s0 < a.n_seq; s0 += nt) {
-    const int s = s0 + threadIdx.x;
-    Kv4Ask q{0, 0, 0, 0};
-    if (s < a.n_seq) step_ask(a, s, q);
-    Sum3 t;
     const Sum3 in = block_scan3(Sum3{q.freed, q.taken, q.grow}, lds, t);
     if (s < a.n_seq) {
       v.base[s] = q.keep;
-      v.f_at[s] = (int)(at.a + in.a - q.freed);
-      v.t_at[s] = (int)(at.b + in.b - q.taken);
-      a.starts[s] = err ? 0 : (int)(at.c + in.c - q.grow);
+      v.f_at[s] = (int)(all.a + in.a - q.freed);
+      v.t_at[s] = (int)(all.b + in.b - q.taken);
+      v.starts[s] = (int)(all.c + in.c - q.grow);
     }
-    at.a += t.a; at.b += t.b; at.c += t.c;
+    all.a += t.a; all.b += t.b; all.c += t.c;
   }
+  const int n_free = *a.n_free;
+  const int err = step_error(a, __syncthreads_or(bad), all, n_free);
+  if (err)   // no rows
+    for (int s = threadIdx.x; s < a.n_seq; s += nt) v.starts[s] = 0;
   if (threadIdx.x == 0) {
-    a.starts[a.n_seq] = err ? 0 : (int)all.c;
+    v.starts[a.n_seq] = err ? 0 : (int)all.c;
     a.scratch[0] = err;
     a.scratch[1] = (int)all.a;
     a.scratch[2] = (int)all.b;
@@ -101,92 +187,67 @@ DFL_DEV void step_scan(const Kv4StepArgs& a, Sum3* lds) {
     if (err) atomicOr(a.err, err);
   }
 }
-// Waves wave, wave + n_waves, ..: one sequence each.
-DFL_DEV void step_free(const Kv4StepArgs& a, int wave, int n_waves) {
-  if (a.scratch[0]) return;
-  const int lane = threadIdx.x & 63;
-  const int top = a.scratch[3] + a.scratch[1] - 1;
-  const StepView v = step_view(a);
-  for (int s = wave; s < a.n_seq; s += n_waves) {
-    const int pk = kv4_pages(v.base[s], a.page_shift);
-    const int n = kv4_pages(a.lens[s], a.page_shift) - pk;
-    int* row = a.table + (long long)s * a.width + pk;
-    for (int j = lane; j < n; j += 64) {
-      const int p = row[j];
-      if (p < 0 || p >= a.n_pages) atomicOr(a.err, KV4_ERR_PAGE);
-      a.free_pages[top - (v.f_at[s] + j)] = p;
-      row[j] = -1;
-    }
-  }
-}
-DFL_DEV void step_take(const Kv4StepArgs& a, int wave, int n_waves) {
-  if (a.scratch[0]) return;
-  const int lane = threadIdx.x & 63;
-  const int top = a.scratch[3] + a.scratch[1] - 1;
-  const StepView v = step_view(a);
-  for (int s = wave; s < a.n_seq; s += n_waves) {
-    const int keep = v.base[s], grow = a.starts[s + 1] - a.starts[s];
-    const int pk = kv4_pages(keep, a.page_shift);
-    const int n = kv4_pages(keep + grow, a.page_shift) - pk;
-    int* row = a.table + (long long)s * a.width + pk;
-    for (int j = lane; j < n; j += 64) {
-      const int i = top - (v.t_at[s] + j);
-      row[j] = a.free_pages[i];
-      a.free_pages[i] = -1;
-    }
-    if (lane == 0) a.lens[s] = keep + grow;
-  }
-  if (wave == 0 && lane == 0) *a.n_free = a.scratch[3] + a.scratch[1] - a.scratch[2];
-}
-// Rows t, t + n, .. of the slot map; those past the step's rows get -1.
-DFL_DEV void step_rows(const Kv4StepArgs& a, long long t, long long n) {
-  const StepView v = step_view(a);
-  const int total = a.starts[a.n_seq];
-  for (long long r = t; r < a.max_rows; r += n) {
-    int slot = -1, pos = -1;
-    if (r < total) {
-      int lo = 0, hi = a.n_seq;   // the last sequence that starts at or before r
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.starts[mid] <= r) lo = mid; else hi = mid;
-      }
-      pos = v.base[lo] + (int)(r - a.starts[lo]);
-      const int pg = a.table[(long long)lo * a.width + (pos >> a.page_shift)];
-      const int mask = (1 << a.page_shift) - 1;
-      slot = pg < 0 || pg >= a.n_pages ? -1 : (pg << a.page_shift) + (pos & mask);
-    }
-    a.slots[r] = slot;
-    a.positions[r] = pos;
-  }
-}
-
-__global__ __launch_bounds__(1024) void kv4_step_scan_kernel(Kv4StepArgs a) {
-  __shared__ Sum3 lds[16];
-  step_scan(a, lds);
-}
 __global__ __launch_bounds__(256) void kv4_step_free_kernel(Kv4StepArgs a) {
-  step_free(a, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
+  if (a.scratch[0]) return;
+  const StepView v = step_view(a);
+  const int n = a.scratch[1], top = a.scratch[3] + n - 1;
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) step_free(a, v, i, top);
 }
 __global__ __launch_bounds__(256) void kv4_step_take_kernel(Kv4StepArgs a) {
-  step_take(a, blockIdx.x * 4 + (threadIdx.x >> 6), gridDim.x * 4);
+  if (a.scratch[0]) return;
+  const StepView v = step_view(a);
+  const int n = a.scratch[2], top = a.scratch[3] + a.scratch[1] - 1, t = blockIdx.x * 256 + threadIdx.x;
+  for (int i = t; i < n; i += gridDim.x * 256) step_take(a, v, i, top);
+  for (int s = t; s < a.n_seq; s += gridDim.x * 256) a.lens[s] = v.base[s] + (v.starts[s + 1] - v.starts[s]);
+  if (t == 0) *a.n_free = a.scratch[3] + a.scratch[1] - n;
 }
+// 1024 rows a workgroup, 4 a thread; the sequences of the first and the last are found first, 64
+// places at a time, those between them are few.  Two million rows of 1024 sequences: 17 us with a
+// search of all sequences for each row, 11.2 so (16 MB, 3.3 us of a copy's time).
+constexpr int STEP_ROWS = 1024;
 __global__ __launch_bounds__(256) void kv4_step_rows_kernel(Kv4StepArgs a) {
-  step_rows(a, (long long)blockIdx.x * 256 + threadIdx.x, (long long)gridDim.x * 256);
-}
-__global__ __launch_bounds__(1024) void kv4_step_small_kernel(Kv4StepArgs a) {
-  __shared__ Sum3 lds[16];
-  step_scan(a, lds);
-  __syncthreads();
-  step_free(a, threadIdx.x >> 6, blockDim.x >> 6);
-  __syncthreads();
-  step_take(a, threadIdx.x >> 6, blockDim.x >> 6);
-  __syncthreads();
-  step_rows(a, threadIdx.x, blockDim.x);
+  const StepView v = step_view(a);
+  const int lane = threadIdx.x & 63, rows = v.starts[a.n_seq];
+  for (long long c = (long long)blockIdx.x * STEP_ROWS; c < a.max_rows; c += (long long)gridDim.x * STEP_ROWS) {
+    const int c0 = (int)c;   // (at most 2^31 - 1024)
+    int s = 0, last = 0;
+    if (c0 < rows) {
+      const int r1 = min(c0 + (STEP_ROWS - 1), rows - 1);
+      int n = a.n_seq, m = a.n_seq;   // sequences that s and last are still among
+      while (n > 1 || m > 1) {
+        const int i = (n + 63) >> 6, j = (m + 63) >> 6;
+        const bool x = lane * i < n && v.starts[s + min(lane * i, n - 1)] <= c0;
+        const bool y = lane * j < m && v.starts[last + min(lane * j, m - 1)] <= r1;
+        const int k = max(0, __popcll(__ballot(x)) - 1) * i, l = max(0, __popcll(__ballot(y)) - 1) * j;
+        s += k; n = min(i, n - k);
+        last += l; m = min(j, m - l);
+      }
+    }
+    StepRow x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = c0 + 256 * k + threadIdx.x;
+      x[k] = StepRow{-1, -1};
+      if (r < rows) x[k] = step_row(a, v, s + step_search(v.starts + s, last - s + 1, r), r);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = c0 + 256 * k + threadIdx.x;
+      if (r < a.max_rows) {
+        a.slots[r] = x[k].slot;
+        a.positions[r] = x[k].pos;
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------ rows in and out
 //
-// 16 threads to a row of one head, 8 values (one code word) each; a group is a quad of lanes.
+// A workgroup has 32 rows of one head's keys or values, 8 lanes a row; a lane has 8 values of the
+// row's first half and 8 of its second, so that each load of a wave takes 8 times 128 bytes (fp16)
+// in a row and each store of codes the 16-byte groups of 8 rows.  Groups are four lanes.  65521
+// rows of 8 heads (bf16, 268 MB to 71 MB): 82 us to append, 72 to read, 4.2 and 4.7 TB/s (copies
+// reach 5.1); 16 lanes a row, each of 8 values in a row, took 112 and 111.
 
 template <int DT> struct RowT;
 template <> struct RowT<0> { typedef float t; };
@@ -206,7 +267,7 @@ DFL_DEV void load8(const void* base, long long at, float (&x)[8]) {
   }
 }
 
-// Where slot's row lies; false (and the error bit) for a slot outside the pool, -1 is no error.
+// Where a slot's row lies; false (and the error bit) for a slot outside the pool, -1 is no error.
 DFL_DEV bool slot_at(const Kv4RowsArgs& a, int slot, int head, unsigned char*& blk, int& r) {
   if (slot < 0 || slot >= (a.n_pages << a.page_shift)) {
     if (slot != -1) atomicOr(a.err, KV4_ERR_SLOT);
@@ -218,84 +279,86 @@ DFL_DEV bool slot_at(const Kv4RowsArgs& a, int slot, int head, unsigned char*& b
   return true;
 }
 
+constexpr int ROWS_WG = 32;   // rows of a workgroup
+
 template <int DT>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4RowsArgs a) {
-  const long long n = (long long)a.rows * 2 * a.n_kv * 16;
-  const long long step = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const int part = (int)i & 15;
-    const long long item = i >> 4;
-    const int head = (int)(item % a.n_kv);
-    const long long rv = item / a.n_kv;
-    const int v = (int)rv & 1;
-    const long long row = rv >> 1;
+  const int head = blockIdx.x >> 1, v = blockIdx.x & 1;
+  const int part = threadIdx.x & 7;
+  for (long long row = (long long)blockIdx.y * ROWS_WG + (threadIdx.x >> 3); row < a.rows;
+       row += (long long)gridDim.y * ROWS_WG) {
     unsigned char* blk;
     int r;
-    const bool ok = slot_at(a, a.slots[row], head, blk, r);   // (one answer for the quad's lanes)
-    if (!ok) continue;
-    float x[8];
-    load8<DT>(v ? a.v : a.k, row * (v ? a.v_row : a.k_row) + head * (v ? a.v_head : a.k_head) + 8 * part, x);
-    // |x| orders as its bits do; an infinity or a NaN is at or past 0x7f800000
-    int top = 0;
+    if (!slot_at(a, a.slots[row], head, blk, r)) continue;   // (one answer for the row's lanes)
+    const long long at = row * (v ? a.v_row : a.k_row) + head * (v ? a.v_head : a.k_head) + 8 * part;
+    float x[2][8];
+    load8<DT>(v ? a.v : a.k, at, x[0]);
+    load8<DT>(v ? a.v : a.k, at + 64, x[1]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, (int)(__float_as_uint(x[j]) & 0x7fffffffu));
-    top = max(top, __shfl_xor(top, 1, 64));
-    top = max(top, __shfl_xor(top, 2, 64));
-    const bool bad = top >= 0x7f800000;
-    const int b = bad ? 255 : max(0, (top >> 23) - 2 + ((top & 0x7fffff) > 0x600000 ? 1 : 0));
-    const float s = __uint_as_float((uint32_t)b << 23);   // (the conversion reads the exponent alone)
-    uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
-    *reinterpret_cast<uint32_t*>(blk + kv4_code_at(r, part >> 2, v) + 4 * (part & 3)) = bad ? 0u : w;
-    if ((part & 3) == 0) blk[kv4_scale_at(r, part >> 2, v)] = (unsigned char)b;
+    for (int half = 0; half < 2; ++half) {
+      // |x| orders as its bits do; an infinity or a NaN is at or past 0x7f800000
+      int top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, (int)(__float_as_uint(x[half][j]) & 0x7fffffffu));
+      top = max(top, __shfl_xor(top, 1, 64));
+      top = max(top, __shfl_xor(top, 2, 64));
+      const bool bad = top >= 0x7f800000;
+      const int b = bad ? 255 : max(0, (top >> 23) - 2 + ((top & 0x7fffff) > 0x600000 ? 1 : 0));
+      const float s = __uint_as_float((uint32_t)b << 23);   // (the conversion reads the exponent alone)
+      uint32_t w = 0;
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[half][0], x[half][1], s, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[half][2], x[half][3], s, 1);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[half][4], x[half][5], s, 2);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[half][6], x[half][7], s, 3);
+      const int g = 2 * half + (part >> 2);
+      *reinterpret_cast<uint32_t*>(blk + kv4_code_at(r, g, v) + 4 * (part & 3)) = bad ? 0u : w;
+      if ((part & 3) == 0) blk[kv4_scale_at(r, g, v)] = (unsigned char)b;
+    }
   }
 }
 
 template <int DT>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsArgs a) {
-  const long long n = (long long)a.rows * 2 * a.n_kv * 16;
-  const long long step = (long long)gridDim.x * 256;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const int part = (int)i & 15;
-    const long long item = i >> 4;
-    const int head = (int)(item % a.n_kv);
-    const long long rv = item / a.n_kv;
-    const int v = (int)rv & 1;
-    const long long row = rv >> 1;
+  const int head = blockIdx.x >> 1, v = blockIdx.x & 1;
+  const int part = threadIdx.x & 7;
+  for (long long row = (long long)blockIdx.y * ROWS_WG + (threadIdx.x >> 3); row < a.rows;
+       row += (long long)gridDim.y * ROWS_WG) {
     unsigned char* blk;
     int r;
-    uint32_t w = 0;
-    float s = 1.f;
-    if (slot_at(a, a.slots[row], head, blk, r)) {
-      w = *reinterpret_cast<const uint32_t*>(blk + kv4_code_at(r, part >> 2, v) + 4 * (part & 3));
-      s = __uint_as_float((uint32_t)blk[kv4_scale_at(r, part >> 2, v)] << 23);
-    }
+    const bool ok = slot_at(a, a.slots[row], head, blk, r);
     typedef typename RowT<DT>::t E;
     E* out = reinterpret_cast<E*>(v ? a.ov : a.ok) + (row * a.n_kv + head) * KV4_D + 8 * part;
-    if constexpr (DT == 0) {
-      const floatx2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
-      const floatx2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
-      const floatx2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
-      const floatx2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
-      reinterpret_cast<floatx4*>(out)[0] = (floatx4){p0.x, p0.y, p1.x, p1.y};
-      reinterpret_cast<floatx4*>(out)[1] = (floatx4){p2.x, p2.y, p3.x, p3.y};
-    } else {
-      u32x4 o;
-      if constexpr (DT == 1) {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
-      } else {
-        o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
-        o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
-        o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
-        o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int g = 2 * half + (part >> 2);
+      uint32_t w = 0;
+      float s = 1.f;
+      if (ok) {
+        w = *reinterpret_cast<const uint32_t*>(blk + kv4_code_at(r, g, v) + 4 * (part & 3));
+        s = __uint_as_float((uint32_t)blk[kv4_scale_at(r, g, v)] << 23);
       }
-      *reinterpret_cast<u32x4*>(out) = o;
+      if constexpr (DT == 0) {
+        const floatx2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 0);
+        const floatx2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 1);
+        const floatx2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 2);
+        const floatx2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, s, 3);
+        reinterpret_cast<floatx4*>(out + 64 * half)[0] = (floatx4){p0.x, p0.y, p1.x, p1.y};
+        reinterpret_cast<floatx4*>(out + 64 * half)[1] = (floatx4){p2.x, p2.y, p3.x, p3.y};
+      } else {
+        u32x4 o;
+        if constexpr (DT == 1) {
+          o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0));
+          o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1));
+          o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2));
+          o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3));
+        } else {
+          o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+          o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+          o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+          o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+        }
+        *reinterpret_cast<u32x4*>(out + 64 * half) = o;
+      }
     }
   }
 }
@@ -1271,21 +1334,23 @@ void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
 }  // namespace
 
 void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st) {
-  if (a.n_seq <= 64 && a.max_rows <= 4096) {
-    hipLaunchKernelGGL(kv4_step_small_kernel, dim3(1), dim3(1024), 0, st, a);
+  if (a.n_seq <= STEP_ONE_SEQS && a.max_rows <= STEP_ONE_ROWS) {
+    const int threads = a.n_seq <= 256 && a.max_rows <= 1024 ? 256 : 1024;
+    hipLaunchKernelGGL(kv4_step_one_kernel, dim3(1), dim3(threads), 0, st, a);
     return;
   }
+  // (what a step moves is known on the device alone: at most the pool's pages)
+  const dim3 pages(min(1024, (max(a.n_pages, a.n_seq) + 255) / 256)), block(256);
   hipLaunchKernelGGL(kv4_step_scan_kernel, dim3(1), dim3(1024), 0, st, a);
-  const int wgs = min(1024, (a.n_seq + 3) / 4);
-  hipLaunchKernelGGL(kv4_step_free_kernel, dim3(wgs), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(kv4_step_take_kernel, dim3(wgs), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(kv4_step_free_kernel, pages, block, 0, st, a);
+  hipLaunchKernelGGL(kv4_step_take_kernel, pages, block, 0, st, a);
   if (a.max_rows > 0)
-    hipLaunchKernelGGL(kv4_step_rows_kernel, dim3(min(2048, (a.max_rows + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(kv4_step_rows_kernel, dim3(min(65536, a.max_rows / STEP_ROWS + 1)), block, 0, st, a);
 }
 
 static dim3 rows_grid(const Kv4RowsArgs& a) {
-  const long long wgs = ((long long)a.rows * 2 * a.n_kv * 16 + 255) / 256;
-  return dim3((unsigned)(wgs < 65536 ? wgs : 65536));
+  const long long chunks = ((long long)a.rows + ROWS_WG - 1) / ROWS_WG;
+  return dim3(2 * a.n_kv, (unsigned)(chunks < 65535 ? chunks : 65535));
 }
 void launch_kv4_append(const Kv4RowsArgs& a, hipStream_t st) {
   const dim3 grid = rows_grid(a), block(256);

@@ -21,6 +21,7 @@ acceptance feels it, the verified output does not.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple, Optional
 
@@ -28,6 +29,7 @@ from . import _lib
 
 __all__ = ["KV4Cache", "KV4Step"]
 
+_NOTHING = contextlib.nullcontext()
 HEAD_DIM = 128
 BLOCK_ROWS, BLOCK_BYTES = 32, 4352
 
@@ -86,15 +88,19 @@ class KV4Cache:
         self.n_free = torch.full((1,), self.n_pages, **ints)
         self._err = torch.zeros(1, **ints)
         self._scratch = self._L.dfl_kv4_step_scratch(self.max_seqs)
+        # (the handle alone: torch.cuda.current_stream() makes an object of it, 2 us a call)
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
         self._codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
     # ------------------------------------------------------------------ checks
     def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return self._raw_stream(self.device.index)
 
     def _guard(self):
+        """Makes the cache's device the current one, if it is not."""
         import torch
+        if torch.cuda.current_device() == self.device.index:
+            return _NOTHING
         return torch.cuda.device(self.device)
 
     def _layer(self, layer: int) -> int:
@@ -105,6 +111,9 @@ class KV4Cache:
     def _ints(self, t, n: Optional[int], what: str):
         """An int32 tensor [n] (any length if n is None) on the cache's device."""
         import torch
+        if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and
+                t.device == self.device and t.is_contiguous() and (n is None or t.shape[0] == n)):
+            return t
         if not isinstance(t, torch.Tensor):
             t = torch.as_tensor(t, dtype=torch.int32)
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
@@ -153,8 +162,8 @@ class KV4Cache:
             keep = None if keep is None else self._ints(keep, n, "keep")
             buf = torch.empty(n + 1 + 2 * max_rows + self._scratch, dtype=torch.int32,
                               device=self.device)
-            starts, slots = buf[:n + 1], buf[n + 1:n + 1 + max_rows]
-            positions = buf[n + 1 + max_rows:n + 1 + 2 * max_rows]
+            starts, slots, positions, _ = buf.split_with_sizes((n + 1, max_rows, max_rows,
+                                                                self._scratch))
             at = buf.data_ptr()
             _lib.check(self._L.dfl_kv4_step(
                 n, self.page, self.width, self.n_pages, _lib.ptr(keep), _lib.ptr(grow),
@@ -225,14 +234,12 @@ class KV4Cache:
             lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
             ws_bytes = self._L.dfl_kv4_attend_ws(n, heads, self.n_kv_heads, self.max_seqs)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self.device)
-            a = _lib.DflKv4Attn(
-                q=q.data_ptr(), out=out.data_ptr(), lse=_lib.ptr(lse), q_row=q.stride(0),
-                q_head=q.stride(1), dtype=self._codes[q.dtype], n_rows=n, n_heads=heads,
-                n_kv=self.n_kv_heads, n_seq=self.max_seqs, causal=int(bool(causal)),
-                scale=HEAD_DIM ** -0.5 if scale is None else float(scale),
-                starts=starts.data_ptr(), lens=self.lens.data_ptr(), table=self.table.data_ptr(),
-                width=self.width, page=self.page, n_pages=self.n_pages, pool=self._layer(layer),
-                ws=ws.data_ptr(), ws_bytes=ws_bytes, err_flags=self._err.data_ptr())
+            a = _lib.DflKv4Attn(   # (in the order of its fields: names cost 3 us)
+                q.data_ptr(), out.data_ptr(), _lib.ptr(lse), q.stride(0), q.stride(1),
+                self._codes[q.dtype], n, heads, self.n_kv_heads, self.max_seqs, bool(causal),
+                HEAD_DIM ** -0.5 if scale is None else float(scale), starts.data_ptr(),
+                self.lens.data_ptr(), self.table.data_ptr(), self.width, self.page, self.n_pages,
+                self._layer(layer), ws.data_ptr(), ws_bytes, self._err.data_ptr())
             _lib.check(self._L.dfl_kv4_attend(ctypes.byref(a), self._stream()), "dfl_kv4_attend")
         return (out, lse) if return_lse else out
 
