@@ -133,7 +133,7 @@ constexpr int KV4_PAD = 8;
 struct Kv4Seq {
   int q0, qlen, len, tiles;
   long long slope, base, m;
-  bool bad;
+  int bad;
 };
 DFL_HD Kv4Seq kv4_seq(int q0, int q1, int len, int n_rows, int width, int page_shift, int ratio,
                       int tile_rows, bool causal) {

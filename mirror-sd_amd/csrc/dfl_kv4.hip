@@ -446,32 +446,36 @@ DFL_DEV float exponent(uint32_t b) { return __uint_as_float(b << 23); }
 DFL_DEV int load_const(const int* p) {
   return *reinterpret_cast<const __attribute__((address_space(4))) int*>(reinterpret_cast<uintptr_t>(p));
 }
-// A value that is the same in all lanes, as the compiler cannot know: into scalar registers.
-DFL_DEV long long uniform(long long v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((unsigned long long)v >> 32));
+// The lane's number, anew: what is made of it in a walk's steps is not kept in registers between them.
+DFL_DEV int lane_again() {
+  int lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+DFL_DEV long long lane_value(long long v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * lane, (int)v);
+  const uint32_t hi = __builtin_amdgcn_ds_bpermute(4 * lane, (int)(v >> 32));
   return (long long)((unsigned long long)hi << 32 | lo);
 }
-DFL_DEV long long wave_sum_ll(long long v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-// Inclusive sum over the wave's lanes.
+// Inclusive sum over the wave's lanes, and a lane's.
 DFL_DEV long long wave_scan_ll(long long v) {
-  const int lane = threadIdx.x & 63;
+  const int lane = lane_again();
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const long long x = __shfl_up(v, o, 64);
+    const long long x = lane_value(v, lane - o);
     if (lane >= o) v += x;
   }
   return v;
+}
+DFL_DEV long long pick_ll(long long v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (long long)((unsigned long long)hi << 32 | lo);
 }
 DFL_DEV int pick(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 // Sequences one lane each, 64 at a time: sequence s0 + lane's row range and length, and its places.
 struct Lanes { int q0, q1, len; long long cost; };
 DFL_DEV Lanes attn_lanes(const Kv4AttnArgs& a, int tile_rows, int s0, bool report) {
-  const int s = s0 + (threadIdx.x & 63);
+  const int s = s0 + lane_again();
   Lanes l{0, 0, 0, 0};
   if (s < a.n_seq) {
     l = Lanes{a.starts[s], a.starts[s + 1], a.lens[s], 0};
@@ -488,12 +492,12 @@ DFL_DEV int attn_among(const Lanes& l, long long in, long long acc, long long po
   const unsigned long long past = __ballot(acc + in > pos);
   if (!past) return -1;
   const int k = __ffsll((unsigned long long)past) - 1;
-  before = uniform(acc + __shfl(in - l.cost, k, 64));
+  before = acc + pick_ll(in - l.cost, k);
   return k;
 }
 // The tile of a head at its place r: the last that has begun.  Every lane tries one, 64 at a time.
 DFL_DEV int attn_tile(const Kv4Seq& s, long long r) {
-  const int lane = threadIdx.x & 63;
+  const int lane = lane_again();
   int lo = 0, n = s.tiles;   // the tile is in [lo, lo + n)
   while (n > 1) {
     const int step = (n + 63) >> 6;
@@ -547,7 +551,7 @@ DFL_DEV bool unit_at(const Kv4AttnArgs& a, int tile_rows, long long pos, Unit& u
       unit_of(a, tile_rows, s0 + k, pick(l.q0, k), pick(l.q1, k), pick(l.len, k), at, pos, u);
       return true;
     }
-    acc += uniform(__shfl(in, 63, 64));
+    acc += pick_ll(in, 63);
   }
   return false;
 }
@@ -555,7 +559,7 @@ DFL_DEV bool unit_at(const Kv4AttnArgs& a, int tile_rows, long long pos, Unit& u
 // A worker's walk over its places: run after run of blocks [b0, b1) of a unit.
 struct Run : Unit {
   int b0, b1;
-  bool whole;          // all of the unit's blocks
+  int whole;           // all of the unit's blocks
 };
 struct Walk { long long pos, end, per; };
 // Begins at the worker's first place; false if it has none.
@@ -563,9 +567,9 @@ DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
   const bool report = blockIdx.x == 0;
   Lanes l = attn_lanes(a, tile_rows, 0, report);
   long long in = wave_scan_ll(l.cost);
-  long long total = uniform(__shfl(in, 63, 64));
+  long long total = pick_ll(in, 63);
   for (int s0 = 64; s0 < a.n_seq; s0 += 64)
-    total += uniform(wave_sum_ll(attn_lanes(a, tile_rows, s0, report).cost));
+    total += pick_ll(wave_scan_ll(attn_lanes(a, tile_rows, s0, report).cost), 63);
   k.per = kv4_per(total, a.workers);
   k.pos = blockIdx.x * k.per;
   k.end = min(total, k.pos + k.per);
@@ -605,11 +609,11 @@ DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
 DFL_DEV Kv4Note* kv4_notes(const Kv4AttnArgs& a, int tile_rows) {
   return reinterpret_cast<Kv4Note*>(a.ws + 2ll * a.workers * kv4_piece_floats(tile_rows));
 }
-DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows) {
-  if (threadIdx.x == 0) kv4_notes(a, tile_rows)[blockIdx.x].w1 = -1;
+DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows, int wave) {
+  if (wave == 0 && lane_again() == 0) kv4_notes(a, tile_rows)[blockIdx.x].w1 = -1;
 }
-DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, long long per, const Run& r) {
-  if (threadIdx.x) return;
+DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, int wave, long long per, const Run& r) {
+  if (wave || lane_again()) return;
   kv4_notes(a, tile_rows)[blockIdx.x] = Kv4Note{
       (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, 0, 0};
 }
@@ -653,10 +657,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
   Walk walk;
   Run run;
   bool more = walk_begin(a, ROWS, walk, run);
-  walk_no_note(a, ROWS);
+  walk_no_note(a, ROWS, wv);
   for (; more; more = walk_next(a, ROWS, walk, run)) {
     if (!walk_run(walk, run)) break;   // (the worker's last places)
-    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, walk.per, run);
+    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
     const Kv4Seq& sq = run.sq;
     // query fragments: step st covers values 32 g + 8 st ..; visible keys of this lane's rows
     v8 qf[NT][4];
@@ -887,28 +891,26 @@ constexpr int TRING = TDEPTH + 1;
 constexpr int TILE_LDS = TRING * TPAIR + 4 * VTILE;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
-// 16 (4) bytes a lane from global memory, from + 16 (4) * lane, into LDS at to + 16 (4) * lane; from
-// and to uniform, at = 16 (4) * lane.  In assembly, because the compiler waits for all loads of the
-// builtin before it lets any LDS read go by; these have no result registers, and the waits are
-// wait_loads'.  (m0, which holds the LDS address, is the compiler's to use: it is put back.)
-DFL_DEV void load_to_lds16(const unsigned char* from, int at, unsigned char* to) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(at), "s"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+// 16 (4) bytes a lane from global memory, from + 16 lane (from + past + 4 lane), into LDS at to + 16
+// lane (to + 4 lane); from, to and past uniform, at = 16 lane.  In assembly, because the compiler
+// waits for all loads of the builtin before it lets any LDS read go by; these have no result
+// registers, and the waits are wait_loads'.
+DFL_DEV void load_to_lds16(const unsigned char* from, int at, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :: "v"(at), "s"(from), "s"(to) : "memory", "m0");
 }
-DFL_DEV void load_to_lds4(const unsigned char* from, int at, unsigned char* to) {
-  uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-               : "=&s"(m0) : "v"(at), "s"(from), "s"((uint32_t)(uintptr_t)(lds_ptr_t)to) : "memory");
+DFL_DEV void load_to_lds4(const unsigned char* from, int past, int at, uint32_t to) {
+  uint32_t at4;
+  asm volatile("s_mov_b32 m0, %3\n\tv_lshrrev_b32 %0, 2, %1\n\tv_add_u32 %0, %4, %0\n\t"
+               "global_load_lds_dword %0, %2"
+               : "=&v"(at4) : "v"(at), "s"(from), "s"(to), "s"(past) : "memory", "m0");
 }
 
-// Waits until at most n (uniform, 2 to 5) of this wave's loads are outstanding.
-DFL_DEV void wait_loads(int n) {
+// Waits until at most N of this wave's loads are outstanding.
+template <int N>
+DFL_DEV void wait_loads() {
   asm volatile("" ::: "memory");
-  if (n == 2) __builtin_amdgcn_s_waitcnt(2 | (7 << 4) | (15 << 8));
-  else if (n == 3) __builtin_amdgcn_s_waitcnt(3 | (7 << 4) | (15 << 8));
-  else if (n == 4) __builtin_amdgcn_s_waitcnt(4 | (7 << 4) | (15 << 8));
-  else __builtin_amdgcn_s_waitcnt(5 | (7 << 4) | (15 << 8));
+  __builtin_amdgcn_s_waitcnt(N | (7 << 4) | (15 << 8));
   asm volatile("" ::: "memory");
 }
 // Barrier that leaves loads on their way; LDS writes of this wave are done before it.
@@ -919,8 +921,92 @@ DFL_DEV void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Q in 6 bits, thrice.  The matrix instructions that take 4-bit operands as they lie, with a power
+// of two for each 32 of them, want the other operand in 8 bits or fewer, and are with 6 bits as
+// fast as without: 64 values in the time that 16-bit ones need for 16.  So a group x of 32 values
+// of Q (times the softmax's scale) is split into x = (p0 + p1 / 16 + p2 / 512) 2^b, each part the
+// nearest of the numbers with 4 bits of which 7.5 is the largest: with a <= 7.5 for the largest
+// |x| = a 2^b, what p0 leaves is at most 1/4, 4 units of p1, which leaves at most 1/8, 4 units of
+// p2, which leaves at most 1/8 of its own, 2^-12 2^b.  As a > 3.75, every value is held to 2^-13.9
+// of its group's largest; fp16 Q rounded to 11 bits beforehand has up to 2^-12 of each value.
+typedef int int8v_t __attribute__((ext_vector_type(8)));
+typedef unsigned uint6v_t __attribute__((ext_vector_type(6)));
+typedef float float32v_t __attribute__((ext_vector_type(32)));
+struct Q6 { uint6v_t part[3]; uint32_t exps; };   // exps: an exponent byte for each part
+// Values 2 i in lo, 2 i + 1 in hi, divided by 2^(b - 127).  (In assembly: the builtin's result may be
+// put into registers of its operands, which the instruction still reads when it has written them.)
+DFL_DEV uint6v_t to_fp6(floatx16 lo, floatx16 hi, uint32_t b) {
+  uint6v_t r;
+  asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(r) : "v"(lo), "v"(hi), "v"(b << 23));
+  return r;
+}
+DFL_DEV float32v_t from_fp6(uint6v_t x, uint32_t b) {
+  float32v_t r;
+  asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(r) : "v"(x), "v"(b << 23));
+  return r;
+}
+template <typename V8>
+DFL_DEV Q6 split_q(const V8 (&x)[4], float scale) {
+  floatx16 lo, hi;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    lo[i] = scale * (float)x[i >> 2][2 * (i & 3)];
+    hi[i] = scale * (float)x[i >> 2][2 * (i & 3) + 1];
+    top = max(max(top, __float_as_uint(lo[i]) & 0x7fffffffu), __float_as_uint(hi[i]) & 0x7fffffffu);
+  }
+  // (10: p2's exponent must not go below that of the byte 0.  Groups below 2^-115 keep fewer bits.)
+  const uint32_t b = max(10, (int)(top >> 23) - 2 + ((top & 0x7fffff) > 0x700000 ? 1 : 0));
+  Q6 q;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const uint32_t bk = k == 0 ? b : k == 1 ? b - 4 : b - 9;
+    q.part[k] = to_fp6(lo, hi, bk);
+    if (k < 2) {
+      const float32v_t held = from_fp6(q.part[k], bk);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        lo[i] -= held[2 * i];
+        hi[i] -= held[2 * i + 1];
+      }
+    }
+  }
+  // an infinity or a NaN, or what the scale makes one, is a NaN in all products of the row
+  q.exps = top >= 0x7f800000u ? 0xffffffu : b | (b - 4) << 8 | (b - 9) << 16;
+  return q;
+}
+// c + K Q^T of 64 values a row: 32 keys of K as they are cached, a lane's key and half of the
+// values, and the exponent in ke's lowest byte.
+template <int PART>
+DFL_DEV floatx16 mfma_part(u32x4 k, uint32_t ke, const Q6& q, floatx16 c) {
+  const int8v_t x = {(int)k.x, (int)k.y, (int)k.z, (int)k.w};
+  const uint6v_t p = q.part[PART];
+  const int8v_t y = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5]};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, 0, (int)ke, PART, (int)q.exps);
+}
+
+// What all lanes hold alike, into scalar registers.
+template <typename S>
+DFL_DEV S scalars(const S& v) {
+  constexpr int N = sizeof(S) / 4;
+  static_assert(sizeof(S) % 4 == 0, "words");
+  struct Words { int w[N]; };
+  Words x = __builtin_bit_cast(Words, v);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x.w[i] = __builtin_amdgcn_readfirstlane(x.w[i]);
+  return __builtin_bit_cast(S, x);
+}
+// The kernel's arguments, read again: what a run's begin and end need of them is not kept in scalar
+// registers over its steps, which have few.
+DFL_DEV const Kv4AttnArgs& args_again() {
+  auto p = reinterpret_cast<const __attribute__((address_space(4))) Kv4AttnArgs*>(
+      (uintptr_t)__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return *(const Kv4AttnArgs*)p;
+}
+
 template <typename T, int WQ>
-__global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v2 v2;
@@ -932,41 +1018,53 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
   unsigned char* const vbuf = tile_lds + TRING * TPAIR;      // [2][2][VTILE]
   const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ratio = a.n_heads / a.n_kv;
-  const float scale = a.scale_log2 * (1.f / M::kUnit);
-  // K: row i of the block, groups h and 2 + h
+  // K: row i of a block, groups h and 2 + h.  V: of block vu of the step the same, or, of four waves,
+  // group h or 2 + h.
   const int koff = 16 * lane;
-  const int soff = KV4_SC + 4 * ((i & 15) + 16 * h);
-  const int kshift = 8 * (i >> 4);
-  // V: group vg of row vr (and, with two waves, of row 16 + vr) of the step's block vu
-  const int vu = wv * VN >> 1;
-  const int vr = (WQ == 4 ? 16 * (wv & 1) : 0) + (lane & 15), vg = lane >> 4;
-  const int voff = vu * KV4_BLOCK + kv4_code_at(vr, vg, 1);
-  const int vsoff = vu * KV4_BLOCK + KV4_SC + 4 * ((lane & 15) + 16 * vg);   // word of rows vr, 16 + vr
-  const int vshift = 16 + (vr >> 1 & 8);
-  const int vwrite = vu * VTILE + vr * TROW + 64 * vg;
+  const int soff = KV4_SC + 4 * ((i & 15) + 16 * h) + (i >> 4);   // K's exponent (V's is 2 further)
+  const int vu = WQ == 2 ? wv : wv >> 1, vj = WQ == 2 ? 0 : wv & 1;
+  const int vwrite = i * TROW + 64 * h;
   const int vread = (4 * h + ((lane & 15) >> 2)) * TROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-  const int loads = WQ == 2 ? 5 : wv < 2 ? 3 : 2;   // this wave's loads of a step
 
-  Walk walk;
-  Run run;
-  bool more = walk_begin(a, ROWS, walk, run);
-  walk_no_note(a, ROWS);
-  for (; more; more = walk_next(a, ROWS, walk, run)) {
+  // (as with the arguments: a wave's place in its walk is kept in LDS over a run's steps)
+  struct Kept { Walk walk; Run run; };
+  __shared__ Kept kept_of[WQ];
+  Kept& kept = kept_of[wv];
+  bool more;
+  {
+    Walk walk;
+    Run run;
+    more = walk_begin(args, ROWS, walk, run);
+    kept = Kept{walk, run};
+  }
+  walk_no_note(args, ROWS, wv);
+  while (more) {
+    Walk walk = scalars(kept.walk);
+    Run run = scalars(kept.run);
+    const Kv4AttnArgs& a = args_again();
+    const int ratio = a.n_heads / a.n_kv;
     if (!walk_run(walk, run)) break;   // (the worker's last places)
-    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, walk.per, run);
+    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
+    kept.run = run;
     const Kv4Seq& sq = run.sq;
     const int n_row = sq.qlen * ratio;
     const int row0 = run.tile * ROWS + 32 * wv;     // this wave's first row (may be past the last)
-    int le = lane;
-    asm volatile("" : "+v"(le));   // (addresses of a run's begin and end are not kept over others)
+    int le = lane_again();   // (addresses of a run's begin and end are not kept over others)
     const int row = min(row0 + (le & 31), n_row - 1), tok = row / ratio;
-    v8 qf[8];
+    v8 qin[2][4];   // groups h and 2 + h of the row
     const T* qp = reinterpret_cast<const T*>(a.q) + (long long)(sq.q0 + tok) * a.q_row +
                   (long long)(run.head * ratio + row - tok * ratio) * a.q_head + 32 * (le >> 5);
 #pragma unroll
-    for (int st = 0; st < 8; ++st) qf[st] = *reinterpret_cast<const v8*>(qp + 8 * (st & 3) + 64 * (st >> 2));
-    const int vis = attn_visible(a, sq, tok);
+    for (int st = 0; st < 8; ++st) qin[st >> 2][st & 3] = *reinterpret_cast<const v8*>(qp + 8 * (st & 3) + 64 * (st >> 2));
+    // keys that the lane's row sees (made again where it is needed: rarely)
+    auto visible = [&]() __attribute__((always_inline)) {
+      const int l = lane_again();
+      const Kv4AttnArgs& e = args_again();
+      const Run r = scalars(kept.run);
+      const Kv4Seq& q = r.sq;
+      const int ratio = e.n_heads / e.n_kv;
+      return attn_visible(e, q, min(r.tile * ROWS + 32 * wv + (l & 31), q.qlen * ratio - 1) / ratio);
+    };
     // fewest and most keys that rows of the tile see
     const int tmin = attn_visible(a, sq, run.tile * ROWS / ratio);
     const int tmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
@@ -975,7 +1073,10 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
     floatx16 o[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] = (floatx16){};
-    float mrun = -FLT_MAX, lrun = 0.f;
+    float lrun = -INFINITY;   // (the row has no weight yet)
+    // What the logits are summed onto: KV4_LIFT less the reference (in all 16: the instruction's
+    // operand), 0 while the row has no weight.
+    floatx16 ref = {};
 
     // Addresses of blocks, 64 at a time, a lane each (past the last block the last one again, so
     // that the count of loads under way is always the same).
@@ -983,144 +1084,145 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
     const int* trow = a.table + (long long)run.s * a.width;
     const uint32_t per_page = (uint32_t)a.n_kv << subs, of_head = (uint32_t)run.head << subs;
     int abase = 0;                       // the first of the 64
-    unsigned long long mine = 0, gone64 = 0;
+    uint32_t mine = 0;                   // (their numbers: a register less)
+    // Blocks before this one are in pages of the pool, in the run, and seen whole by all rows of the
+    // tile; steps past it look closer.
+    int full = min(b_end, tmin / KV4_KEYS);
+    auto no_page = [&](int page) { return page < 0 || page >= a.n_pages; };
+    auto absent = [&](int b) { return b >= b_end || no_page(load_const(trow + (b >> subs))); };
     auto addresses = [&](int b) {
-      const int k = max(0, min(b + lane, b_end - 1));   // (b_end may be 0: then nothing is loaded)
+      const int k = max(0, min(b + lane_again(), b_end - 1));   // (b_end may be 0: then nothing is loaded)
       const int page = b_end > 0 ? trow[k >> subs] : 0;
-      const bool no = page < 0 || page >= a.n_pages;
-      mine = kv4_block_at((no ? 0u : (uint32_t)page * per_page) + of_head + (uint32_t)(k & ((1 << subs) - 1)));
-      gone64 = __ballot(no);
+      const bool no = no_page(page);
+      mine = (no ? 0u : (uint32_t)page * per_page) + of_head + (uint32_t)(k & ((1 << subs) - 1));
       abase = b;
+      if (__ballot(no)) {
+        full = 0;
+        int bit = KV4_ERR_PAGE;
+        asm volatile("" : "+v"(bit));   // (no register for it over the steps)
+        if (no) atomicOr(a.err, bit);
+      }
     };
-    uint32_t absent = 0;   // bit j: block b + j of the loop lies in no page of the pool
-    struct From { const unsigned char *p0, *p1; };
-    auto from = [&](int b, int ahead) {
-      if (b - abase >= 64) addresses(b);
-      const int k = b - abase;           // (even: the pair is within the 64)
-      absent |= ((uint32_t)(gone64 >> k) & 3u) << ahead;
-      const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
-      auto at = [&](int l) {
-        return a.pool + ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 |
-                         (uint32_t)__builtin_amdgcn_readlane(lo, l));
-      };
-      return From{at(k), at(k + 1)};
-    };
+    // A wave's loads of the step that begins with block b, into a place of the ring: KiB wv (and, of
+    // two waves, wv + 2) of both blocks, and the exponents of block wv % 2 (of four waves two load
+    // the same, so that all count alike).
     constexpr int LOADS = WQ == 2 ? 5 : 3;
-    auto issue = [&](const From& f, int slot, int j) {
-      unsigned char* to = ring + slot * TPAIR;
-      if (j == LOADS - 1) {   // the exponents of block wv
-        if (wv < 2) load_to_lds4((wv ? f.p1 : f.p0) + KV4_SC, 4 * lane, to + wv * KV4_BLOCK + KV4_SC);
-      } else {                // KiB wv (wv + 2) of block 0, then of block 1
-        const int u = WQ == 2 ? j >> 1 : j, kib = WQ == 2 ? wv + 2 * (j & 1) : wv;
-        load_to_lds16((u ? f.p1 : f.p0) + 1024 * kib, 16 * lane, to + u * KV4_BLOCK + 1024 * kib);
+    const unsigned char* const pool_w = a.pool + 1024 * wv;
+    const uint32_t ring_w = (uint32_t)(uintptr_t)(lds_ptr_t)ring + 1024 * wv;
+    auto issue = [&](int b, int place) __attribute__((always_inline)) {
+      if (__builtin_expect(b - abase >= 64, 0)) addresses(b);
+      const int k = b - abase;           // (even: the pair is within the 64)
+      const unsigned char* const p0 = pool_w + kv4_block_at((uint32_t)__builtin_amdgcn_readlane(mine, k));
+      const unsigned char* const p1 = pool_w + kv4_block_at((uint32_t)__builtin_amdgcn_readlane(mine, k + 1));
+      const uint32_t to = ring_w + place;
+      load_to_lds16(p0, koff, to);
+      load_to_lds16(p1, koff, to + KV4_BLOCK);
+      if constexpr (WQ == 2) {
+        load_to_lds16(p0 + 2048, koff, to + 2048);
+        load_to_lds16(p1 + 2048, koff, to + KV4_BLOCK + 2048);
       }
+      const uintptr_t p = wv & 1 ? (uintptr_t)p1 : (uintptr_t)p0;
+      load_to_lds4(reinterpret_cast<const unsigned char*>(p), KV4_SC - 1024 * wv, koff,
+                   to + (wv & 1) * KV4_BLOCK + KV4_SC - 1024 * wv);
     };
-    // V of the step that begins with block b, from place `slot` of the ring: codes and exponent,
-    // then into buffers `to`.  In a block that some row of the tile does not see whole: zeros for
-    // rows past the sequence and for NaN groups, as there 0 * NaN would reach rows that do not see
-    // them; the rows that do see a NaN are set when the block is used.
-    u32x4 vc[VN];
+    // V of the step that begins with block b, from a place of the ring: codes and exponent, then
+    // into buffers `to`.  In a block that some row of the tile does not see whole: zeros for rows
+    // past the sequence and for NaN groups, as there 0 * NaN would reach rows that do not see them;
+    // the rows that do see a NaN are set when the block is used.
+    u32x4 vc;
     uint32_t ve;
-    auto read_v = [&](int slot) {
-      ve = *reinterpret_cast<const uint32_t*>(ring + slot * TPAIR + vsoff);
-#pragma unroll
-      for (int j = 0; j < VN; ++j)
-        vc[j] = *reinterpret_cast<const u32x4*>(ring + slot * TPAIR + voff + 256 * j);
+    auto read_v = [&](int place, int j) __attribute__((always_inline)) {
+      const unsigned char* vb = ring + place + vu * KV4_BLOCK;
+      ve = vb[128 * (vj + j) + soff + 2];
+      vc = *reinterpret_cast<const u32x4*>(vb + 2048 + 1024 * (vj + j) + koff);
     };
-    auto write_v = [&](int b, int to, uint32_t gone2) {
-      const int kbase = (b + vu) * KV4_KEYS;
-      const bool gone = (gone2 >> vu) & 1;
-      uint32_t e[VN];
-#pragma unroll
-      for (int j = 0; j < VN; ++j) e[j] = (ve >> (vshift + 8 * j)) & 255u;
-      if (kbase + KV4_KEYS > tmin || gone) {
-        asm volatile("");
-#pragma unroll
-        for (int j = 0; j < VN; ++j)
-          if (e[j] == 255 || gone || kbase + vr + 16 * j >= sq.len) {
-            e[j] = 0;
-            vc[j] = (u32x4){0, 0, 0, 0};
-          }
+    auto mask_v = [&](int b) __attribute__((always_inline)) {
+      if (__builtin_expect(b + 2 > full, 0)) {
+        const bool gone = absent(b + vu);
+        if (ve == 255 || gone || (b + vu) * KV4_KEYS + (lane_again() & 31) >= sq.len) {
+          ve = 0;
+          vc = (u32x4){0, 0, 0, 0};
+        }
       }
+    };
+    auto write_v = [&](auto word, int j, int to, int row) __attribute__((always_inline)) {
+      constexpr int w = word;
+      unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * (vj + j) + row;
+      *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[w], M::kUnit * exponent(ve));
+    };
+    auto convert_v = [&](int place, int b, int to) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
-        const float s = M::kUnit * exponent(e[j]);
-        unsigned char* at = vbuf + 2 * to * VTILE + vwrite + 16 * j * TROW;
-        static_for<0, 4>([&](auto word) {
-          constexpr int w = word;
-          *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[j][w], s);
-        });
+        read_v(place, j);
+        mask_v(b);
+        const int l = lane_again();
+        static_for<0, 4>([&](auto w) { write_v(w, j, to, (l & 31) * TROW + 64 * (l >> 5)); });
       }
     };
-    // S^T of the two blocks in place `slot` of the ring: codes and exponents, then (quarter by
-    // quarter of the values) the products.
+    // S^T of the two blocks in a place of the ring: codes and exponents, then the products.
+    Q6 qf[2];
     u32x4 kc[4];
     uint32_t ke[4];
-    auto read_k = [&](int slot) {
-      const unsigned char* kb = ring + slot * TPAIR;
+    auto read_k = [&](int place) __attribute__((always_inline)) {
+      const unsigned char* kb = ring + place;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          ke[2 * u + j] = *reinterpret_cast<const uint32_t*>(kb + u * KV4_BLOCK + soff + 128 * j);
+          ke[2 * u + j] = kb[u * KV4_BLOCK + soff + 128 * j];
           kc[2 * u + j] = *reinterpret_cast<const u32x4*>(kb + u * KV4_BLOCK + koff + 1024 * j);
         }
     };
-    auto k_unit = [&](int j) { return M::kUnit * exponent((ke[j] >> kshift) & 255u); };
+    // Product n of 12 for the S^T t of both blocks, begun on ref: half the values, one part of Q.
+    auto product = [&](auto n, floatx16 (&t)[2]) __attribute__((always_inline)) {
+      constexpr int st = decltype(n)::value / 6, part = 2 - decltype(n)::value % 6 / 2, u = decltype(n)::value & 1;
+      t[u] = mfma_part<part>(kc[2 * u + st], ke[2 * u + st], qf[st],
+                             decltype(n)::value < 2 ? ref : t[u]);
+    };
     const bool idle = row0 >= n_row;   // a wave past the sequence's rows only loads and converts
-    int slot = 0, to = 0;  // of the step's blocks: in the ring, their V's buffers
     floatx16 s[2] = {};
     addresses(run.b0);
     if (run.b0 < b_end) {
 #pragma unroll
-      for (int j = 0; j < TDEPTH; ++j) {
-        const From f = from(run.b0 + 2 * j, 2 * j);
-#pragma unroll
-        for (int k = 0; k < LOADS; ++k) issue(f, j, k);
-      }
+      for (int j = 0; j < TDEPTH; ++j) issue(run.b0 + 2 * j, j * TPAIR);
     }
-    // The queries and the first blocks are there: from here on the ring's loads alone are counted.
-    // (The compiler's waits do not know of them; one statement, so that it has none in the loop.)
-    asm volatile("s_waitcnt vmcnt(0)"
-                 : "+v"(qf[0]), "+v"(qf[1]), "+v"(qf[2]), "+v"(qf[3]), "+v"(qf[4]), "+v"(qf[5]),
-                   "+v"(qf[6]), "+v"(qf[7]) :: "memory");
+    qf[0] = split_q(qin[0], a.scale_log2);
+    qf[1] = split_q(qin[1], a.scale_log2);
+    // The queries are there: from here on the ring's loads alone are counted.  (The compiler's waits
+    // do not know of them; one statement, so that it has none in the loop.)
+    asm volatile(""
+                 : "+v"(qf[0].part[0]), "+v"(qf[0].part[1]), "+v"(qf[0].part[2]), "+v"(qf[0].exps),
+                   "+v"(qf[1].part[0]), "+v"(qf[1].part[1]), "+v"(qf[1].part[2]), "+v"(qf[1].exps) :: "memory");
     if (run.b0 < b_end) {
+      wait_loads<LOADS * (TDEPTH - 1)>();
       lds_barrier();
-      read_v(0);
       read_k(0);
-      write_v(run.b0, 0, absent);
-      const float e[4] = {k_unit(0), k_unit(1), k_unit(2), k_unit(3)};
-      static_for<0, 8>([&](auto step) {
-        constexpr int st = step;
-        s[0] = M::mfma(M::dequant(kc[st >> 2][st & 3], e[st >> 2]), qf[st], s[0]);
-        s[1] = M::mfma(M::dequant(kc[2 + (st >> 2)][st & 3], e[2 + (st >> 2)]), qf[st], s[1]);
-      });
+      convert_v(0, run.b0, 0);
+      static_for<0, 12>([&](auto n) { product(n, s); });
     }
-    // A step (s: S^T of its two blocks): their weights, between which (they do not wait for each
-    // other) go the products of the next step's S^T t, then the products with V.
-    auto do_step = [&](int b, floatx16 (&s)[2], floatx16 (&t)[2]) __attribute__((always_inline)) {
-      const int kbase = b * KV4_KEYS;
-      const int slot1 = slot + 1 == TRING ? 0 : slot + 1;
-      wait_loads(loads * (TDEPTH - 2));
+    // Step `odd` of a pair (s: S^T of its two blocks): their weights, between which (they do not wait
+    // for each other) go the products of the next step's S^T t, then the products with V.  A pair of
+    // steps has half of the ring (h0, the other is h1; bytes), a step one of V's buffers.
+    int h0 = 0, h1 = 2 * TPAIR;
+    auto do_step = [&](auto which, int b, floatx16 (&s)[2], floatx16 (&t)[2]) __attribute__((always_inline)) {
+      constexpr int odd = which, to = odd;
+      const int kbase = b * KV4_KEYS, next = odd ? h1 : h0 + TPAIR;
+      wait_loads<LOADS * (TDEPTH - 2)>();
       // the next step's blocks and V of this one's are there, and nobody reads those of the last
       // step any more
       lds_barrier();
-      read_k(slot1);   // (after the last step those are blocks read once too often)
-      read_v(slot1);
-      const From f = from(b + 2 * TDEPTH, 2 * TDEPTH);
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) issue(f, slot == 0 ? TRING - 1 : slot - 1, j);
-      // the second block may be past the run's last
-      const bool gone0 = absent & 1, gone1 = (absent & 2) || b + 1 >= b_end;
-      if (!idle) {
-        if (kbase + 2 * KV4_KEYS > tmin || gone0 || gone1) {
-          asm volatile("");   // (a branch: as selects the masks are a third of the loop)
+      read_k(next);   // (after the last step those are blocks read once too often)
+      issue(b + 2 * TDEPTH, odd ? h0 : h1 + TPAIR);
+      if (__builtin_expect(!idle, 1)) {
+        if (__builtin_expect(b + 2 > full, 0)) {
+          const bool gone0 = absent(b), gone1 = absent(b + 1);
+          const int vis = visible();   // (volatile: a branch; as selects the masks are a third of the loop)
           // groups h, 2 + h of row i of either block that stand for NaN
-          const unsigned char* kb = ring + slot * TPAIR + soff;
-          const int sh = 16 + kshift;
+          const unsigned char* kb = ring + h0 + odd * TPAIR + soff;
+          const int l = lane_again(), i = l & 31, h = l >> 5;
           const bool there0 = !gone0 && kbase + i < sq.len;
           const bool there1 = !gone1 && kbase + KV4_KEYS + i < sq.len;
-          auto nan_at = [&](int at) { return ((*reinterpret_cast<const uint32_t*>(kb + at) >> sh) & 255u) == 255u; };
+          auto nan_at = [&](int at) { return kb[at + 2] == 255; };
           const bool n0 = there0 && nan_at(0), n1 = there0 && nan_at(128);
           const bool n2 = there1 && nan_at(KV4_BLOCK), n3 = there1 && nan_at(KV4_BLOCK + 128);
           if (__ballot(n0 || n1 || n2 || n3)) {
@@ -1146,105 +1248,127 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs a) {
               if (kbase + 32 * u + 4 * h + (r & 3) + 8 * (r >> 2) >= lim) s[u][r] = -INFINITY;
           }
         }
-        const float e[4] = {k_unit(0), k_unit(1), k_unit(2), k_unit(3)};
-        v8 p[4];
+        v8 p[4], vf[2][4];
         float sum = 0.f;
-        auto weights = [&](int q, float ref) __attribute__((always_inline)) {   // of 16 keys
-          const int u = q >> 1, r0 = 8 * (q & 1);
+        auto weights = [&](int n) __attribute__((always_inline)) {   // two of 32
+          const int u = n >> 3, r = 2 * (n & 7);
+          const v2 x = __builtin_convertvector(
+              ((floatx2){__builtin_amdgcn_exp2f(s[u][r]), __builtin_amdgcn_exp2f(s[u][r + 1])}), v2);
+          sum = M::sum2(x, sum);
+          p[n >> 2][r & 7] = x.x;
+          p[n >> 2][(r & 7) + 1] = x.y;
+        };
+        const unsigned char* vb = vbuf + 2 * to * VTILE + vread;
+        auto read_vf = [&](int q) __attribute__((always_inline)) {   // operands of V for 16 keys
 #pragma unroll
-          for (int r = 0; r < 8; r += 2) {
-            const v2 x = __builtin_convertvector(
-                ((floatx2){__builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r0 + r], scale, ref)),
-                           __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r0 + r + 1], scale, ref))}), v2);
-            sum = M::sum2(x, sum);
-            p[q][r] = x.x;
-            p[q][r + 1] = x.y;
+          for (int d = 0; d < 4; ++d) {
+            const unsigned char* at = vb + (q >> 1) * VTILE + 16 * (q & 1) * TROW + 64 * d;
+            vf[q & 1][d] = read_vt<T>(at, at + 8 * TROW);
           }
         };
-        const float ref = KV4_LIFT - mrun;
-        t[0] = t[1] = (floatx16){};
-        static_for<0, 4>([&](auto quarter) {
-          constexpr int q = quarter;
-          static_for<0, 2>([&](auto half) {
-            constexpr int k = 2 * q + half;
-            t[0] = M::mfma(M::dequant(kc[k >> 2][k & 3], e[k >> 2]), qf[k], t[0]);
-            t[1] = M::mfma(M::dequant(kc[2 + (k >> 2)][k & 3], e[2 + (k >> 2)]), qf[k], t[1]);
-          });
-          weights(q, ref);
+        // (the order is held by the barriers: left to itself the compiler puts all products first and
+        // each read right before its use, which costs 2.1 instead of %STEP% us a step)
+        static_for<0, 12>([&](auto n) {
+          constexpr int k = n;
+          product(n, t);
+          static_for<16 * k / 12, 16 * (k + 1) / 12>([&](auto w) { weights(w); });
+          __builtin_amdgcn_sched_barrier(0);
         });
-        // Weights above 2^15 (the sum of 32 says so; an infinity and a NaN do too): the reference
-        // is raised where the largest logit is more than KV4_SLACK above it, and they are made
-        // again.  So no maximum is taken in the steps in which none is needed.
-        if (!__all(sum <= 1048576.f)) {
+        // Weights above 2^15 (the sum of 32 says so; an infinity and a NaN do too), or none so far:
+        // the reference is raised where the largest logit is more than KV4_SLACK above it, or set,
+        // and they are made again.  So no maximum is taken in the steps in which none is needed.
+        if (__builtin_expect(!__all((sum <= 1048576.f) & (lrun + sum >= 0.f)), 0)) {
           float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
           for (int r = 1; r < 16; ++r) top = fmaxf(fmaxf(top, s[0][r]), s[1][r]);
-          top *= scale;
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float mnew = top > mrun + KV4_SLACK ? top : mrun;
-          const float alpha = __builtin_amdgcn_exp2f(mrun - mnew);
-          lrun *= alpha;
+          top = fmaxf(top, __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane_again() ^ 32), __float_as_int(top))));
+          top -= KV4_LIFT;
+          const bool none = lrun == -INFINITY;   // (both lanes of the row)
+          const float up = top > KV4_SLACK || (none && top > -INFINITY) ? top : 0.f;
+          const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(-up);
+          lrun = none && top > -INFINITY ? 0.f : lrun * alpha;
 #pragma unroll
           for (int d = 0; d < 4; ++d) o[d] *= alpha;
-          mrun = mnew;
+          ref -= up;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            s[u] -= up;
+            t[u] -= up;
+          }
           sum = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) weights(q, KV4_LIFT - mrun);
+          for (int n = 0; n < 16; ++n) weights(n);
         }
         lrun += sum;
-        const unsigned char* vb = vbuf + 2 * to * VTILE + vread;
+        read_vf(0);   // (after the logits and K, whose registers these take)
         static_for<0, 4>([&](auto quarter) {
-          constexpr int q = quarter, st = q & 1, u = q >> 1;
+          constexpr int q = quarter, j = q >> 1;
+          if constexpr (q < 3) read_vf(q + 1);
+          if constexpr (j < VN && (q & 1) == 0) read_v(next, j);
+          if constexpr (j < VN && (q & 1) == 1) mask_v(b + 2);
+          __builtin_amdgcn_sched_barrier(0);
           static_for<0, 4>([&](auto dt) {
             constexpr int d = dt;
-            const unsigned char* at = vb + u * VTILE + 16 * st * TROW + 64 * d;
-            o[d] = M::mfma(read_vt<T>(at, at + 8 * TROW), p[q], o[d]);
+            o[d] = M::mfma(vf[q & 1][d], p[q], o[d]);
+            if constexpr (j < VN && (q & 1) == 1) write_v(dt, j, to ^ 1, vwrite);
+            __builtin_amdgcn_sched_barrier(0);
           });
         });
+      } else {
+        convert_v(next, b + 2, to ^ 1);
       }
-      write_v(b + 2, to ^ 1, absent >> 2);
-      if ((absent & 3) && threadIdx.x == 0) atomicOr(a.err, KV4_ERR_PAGE);
-      absent >>= 2;
-      slot = slot1;
-      to ^= 1;
     };
     floatx16 t[2];
     for (int b = run.b0; b < b_end; b += 4) {
-      do_step(b, s, t);
-      if (b + 2 < b_end) do_step(b + 2, t, s);
+      do_step(std::integral_constant<int, 0>{}, b, s, t);
+      if (__builtin_expect(b + 2 < b_end, 1)) do_step(std::integral_constant<int, 1>{}, b + 2, t, s);
+      const int h = h0;
+      h0 = h1;
+      h1 = h;
     }
     __builtin_amdgcn_s_waitcnt(0);   // (the loads past the last block)
 
-    lrun += __shfl_xor(lrun, 32, 64);
-    asm volatile("" : "+v"(le));
-    if (!run.whole) {
-      float* piece = a.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
+    {
+      const Kv4AttnArgs& e = args_again();
+      walk = scalars(kept.walk);
+      run = scalars(kept.run);
+      const Kv4Seq& sq = run.sq;
+      const int ratio = e.n_heads / e.n_kv, n_row = sq.qlen * ratio, row0 = run.tile * ROWS + 32 * wv;
+      lrun += __shfl_xor(lrun, 32, 64);
+      const float mrun = lrun == -INFINITY ? -FLT_MAX : KV4_LIFT - ref[0];
+      if (lrun == -INFINITY) lrun = 0.f;
+      le = lane_again();
+      if (!run.whole) {
+        float* piece = e.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          *reinterpret_cast<floatx4*>(piece + (((wv * 4 + d) * 4 + k) * 64 + le) * 4) =
-              (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * (1.f / M::kUnit);
-      if (le < 32)
-        *reinterpret_cast<floatx2*>(piece + ROWS * KV4_D + 2 * (32 * wv + le)) = (floatx2){mrun, lrun};
-    } else if (row0 + (le & 31) < n_row) {
-      const int row = row0 + (le & 31), tok = row / ratio;
-      const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + row - tok * ratio;
-      const bool none = vis <= 0;   // a row that sees no key: zeros, and the sum of none
-      const float f = (1.f / M::kUnit) / lrun;
-      T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * (le >> 5);
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<floatx4*>(piece + (((wv * 4 + d) * 4 + k) * 64 + le) * 4) =
+                (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * (1.f / M::kUnit);
+        if (le < 32)
+          *reinterpret_cast<floatx2*>(piece + ROWS * KV4_D + 2 * (32 * wv + le)) = (floatx2){mrun, lrun};
+      } else if (row0 + (le & 31) < n_row) {
+        const int row = row0 + (le & 31), tok = row / ratio;
+        const long long orow = (long long)(sq.q0 + tok) * e.n_heads + (run.head - tok) * ratio + row;
+        const bool none = attn_visible(e, sq, tok) <= 0;   // a row that sees no key: zeros, and the sum of none
+        const float f = (1.f / M::kUnit) / lrun;
+        T* op = reinterpret_cast<T*>(e.out) + orow * KV4_D + 4 * (le >> 5);
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          typedef T v4 __attribute__((ext_vector_type(4)));
-          v4 x;
+          for (int k = 0; k < 4; ++k) {
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            v4 x;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[d][4 * k + j] * f);
-          *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
-        }
-      if (a.lse && le < 32)
-        a.lse[orow] = none ? -INFINITY : (mrun - KV4_LIFT + __log2f(lrun)) * 0.69314718056f;
+            for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[d][4 * k + j] * f);
+            *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
+          }
+        if (e.lse && le < 32)
+          e.lse[orow] = none ? -INFINITY : (mrun - KV4_LIFT + __log2f(lrun)) * 0.69314718056f;
+      }
+      more = walk_next(e, ROWS, walk, run);
+      kept = Kept{walk, run};
     }
     __syncthreads();   // the buffers are written again
   }

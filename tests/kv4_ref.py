@@ -71,15 +71,17 @@ class Plan:
 
 
 def attend(q, k, v, causal, scale):
-    """q [m, heads, 128], k and v [n, kv, 128], float64 -> (out, lse, bound): bound [m, heads] holds
-    (sum w |v| over the values' largest, largest scale * sum |q k| of a visible key)."""
+    """q [m, heads, 128], k and v [n, kv, 128], float64 -> (out, lse, mass, size): mass [m, heads,
+    128] is sum w |v| / sum w, size [2, m, heads] the largest over the visible keys of scale * sum
+    |q k| and of scale * sum |g k|, g the largest |q| of the value's group of 32."""
     m, heads, _ = q.shape
     n, kv, _ = k.shape
     r = heads // kv
     out = np.zeros((m, heads, 128))
     lse = np.full((m, heads), -np.inf)
     mass = np.zeros((m, heads, 128))
-    size = np.zeros((m, heads))
+    size = np.zeros((2, m, heads))
+    group = np.abs(q).reshape(m, heads, 4, 32).max(-1).repeat(32, -1)
     for h in range(heads):
         if n == 0:
             break
@@ -97,12 +99,14 @@ def attend(q, k, v, causal, scale):
             out[t, h] = w @ vv[:see] / w.sum()
             mass[t, h] = w @ np.abs(vv[:see]) / w.sum()
             lse[t, h] = top + np.log(w.sum())
-            size[t, h] = scale * (np.abs(q[t, h]) @ np.abs(kk[:see]).T).max()
+            size[0, t, h] = scale * (np.abs(q[t, h]) @ np.abs(kk[:see]).T).max()
+            size[1, t, h] = scale * (group[t, h] @ np.abs(kk[:see]).T).max()
     return out, lse, mass, size
 
 
-def attend_tolerance(out, lse, mass, size, n, half_step):
-    """How far a result may be off, by arithmetic.  half_step = eps / 2 of the query's type.
+def attend_tolerance(out, lse, mass, size, n, half_step, split=True):
+    """How far a result may be off, by arithmetic.  half_step = eps / 2 of the query's type; split:
+    the query goes into the product as three 6-bit parts (tiles of more than 32 rows).
 
     Logits: 128 products summed in fp32, each sum off by at most 2^-23 (MFMA sums may truncate), of
     at most `size` in all; the product with scale * log2(e), the difference to the reference and
@@ -111,7 +115,16 @@ def attend_tolerance(out, lse, mass, size, n, half_step):
     of the rounded ones.  The chain of fp32 sums over n keys has n / 32 steps in a wave, and some 64
     more between waves and workers.  With o = sum w v / sum w, weights off by f each move o by at
     most 2 f sum w |v| / sum w; the result rounds once more.  Weights below 2^-34 of the largest
-    may vanish (fp16): n 2^-34 of the mass, which is at least 1 / n of the largest value's."""
-    d = 2.0 ** -23 * (132 * size + 8 + n / 32 + 64) + n * 2.0 ** -34
+    may vanish (fp16): n 2^-34 of the mass, which is at least 1 / n of the largest value's.
+
+    The parts of a query have 4 bits: x = (p0 + p1 / 16 + p2 / 512) 2^b with 3.75 2^b < g <= 7.5 2^b
+    for the largest |x| = g of 32.  p0 leaves at most 1/4 (half a step of 1/2), which is 4 units of
+    p1; p1 leaves at most 1/8 (half a step of 1/4 below 4), which is 4 units of p2; p2 leaves 1/8
+    of its unit, 2^(b - 12) <= 2^-12 / 3.75 g.  A logit is off by at most that times size[1].  Its
+    384 products add up on the reference's exponent (a logit and KV4_LIFT = 9 in log2, 7), so that
+    each of their sums is off by 2^-23 of that, too."""
+    d = 2.0 ** -23 * (132 * size[0] + 8 + n / 32 + 64) + n * 2.0 ** -34
+    if split:
+        d += 2.0 ** -12 / 3.75 * size[1] + 2.0 ** -23 * 384 * (2 * size[0] + 7)
     tol = half_step * np.abs(out) + (2 * half_step + 2 * d)[..., None] * mass + 2.0 ** -24
     return tol, half_step + 2 * d + 2.0 ** -20 * np.maximum(1, np.abs(lse))

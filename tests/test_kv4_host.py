@@ -176,7 +176,7 @@ def test_plain_attention_against_torch():
     g = torch.Generator().manual_seed(0)
     q, k, v = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 6, 128), (9, 2, 128), (9, 2, 128)))
     for causal in (False, True):
-        out, lse, _, size = R.attend(q.numpy(), k.numpy(), v.numpy(), causal, 0.1)
+        out, lse, _, (size, _) = R.attend(q.numpy(), k.numpy(), v.numpy(), causal, 0.1)
         s = torch.einsum("mhd,nhd->hmn", q, k.repeat_interleave(3, 1)) * 0.1
         if causal:
             s = s.masked_fill(torch.ones(5, 9, dtype=torch.bool).triu(5), -float("inf"))
