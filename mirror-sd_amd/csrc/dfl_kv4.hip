@@ -562,6 +562,13 @@ struct Run : Unit {
   int whole;           // all of the unit's blocks
 };
 struct Walk { long long pos, end, per; };
+// Which worker a workgroup is.  Workgroups go to the 8 dies of the chip in turn, each with an L2 of
+// its own, and workers that follow on each other read the same keys (the tiles of a head): so
+// each die has an eighth of all places, one after the other.  (Two prompts of 4096 and 777 rows:
+// 219 us in turn, 216 so.)
+DFL_DEV int worker_of(const Kv4AttnArgs& a, int workgroup) {   // (a.workers: a multiple of 8)
+  return (workgroup & 7) * (a.workers >> 3) + (workgroup >> 3);
+}
 // Begins at the worker's first place; false if it has none.
 DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
   const bool report = blockIdx.x == 0;
@@ -571,7 +578,7 @@ DFL_DEV bool walk_begin(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
   for (int s0 = 64; s0 < a.n_seq; s0 += 64)
     total += pick_ll(wave_scan_ll(attn_lanes(a, tile_rows, s0, report).cost), 63);
   k.per = kv4_per(total, a.workers);
-  k.pos = blockIdx.x * k.per;
+  k.pos = worker_of(a, blockIdx.x) * k.per;
   k.end = min(total, k.pos + k.per);
   if (k.pos >= k.end) return false;
   if (a.n_seq > 64) return unit_at(a, tile_rows, k.pos, r);
@@ -610,11 +617,11 @@ DFL_DEV Kv4Note* kv4_notes(const Kv4AttnArgs& a, int tile_rows) {
   return reinterpret_cast<Kv4Note*>(a.ws + 2ll * a.workers * kv4_piece_floats(tile_rows));
 }
 DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows, int wave) {
-  if (wave == 0 && lane_again() == 0) kv4_notes(a, tile_rows)[blockIdx.x].w1 = -1;
+  if (wave == 0 && lane_again() == 0) kv4_notes(a, tile_rows)[worker_of(a, blockIdx.x)].w1 = -1;
 }
 DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, int wave, long long per, const Run& r) {
   if (wave || lane_again()) return;
-  kv4_notes(a, tile_rows)[blockIdx.x] = Kv4Note{
+  kv4_notes(a, tile_rows)[worker_of(a, blockIdx.x)] = Kv4Note{
       (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, 0, 0};
 }
 // The page of block b of a run's keys; -1: there is no such page (its keys are absent).
@@ -819,7 +826,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       }
     }
     __syncthreads();
-    float* piece = a.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
+    float* piece = a.ws + kv4_piece(worker_of(a, blockIdx.x), walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int c = 16 * n + i;
@@ -1145,19 +1152,13 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
         }
       }
     };
-    auto write_v = [&](auto word, int j, int to, int row) __attribute__((always_inline)) {
-      constexpr int w = word;
-      unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * (vj + j) + row;
-      *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[w], M::kUnit * exponent(ve));
-    };
-    auto convert_v = [&](int place, int b, int to) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        read_v(place, j);
-        mask_v(b);
-        const int l = lane_again();
-        static_for<0, 4>([&](auto w) { write_v(w, j, to, (l & 31) * TROW + 64 * (l >> 5)); });
-      }
+    auto write_v = [&](int j, int to) __attribute__((always_inline)) {
+      unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * (vj + j) + vwrite;
+      const float unit = M::kUnit * exponent(ve);
+      static_for<0, 4>([&](auto word) {
+        constexpr int w = word;
+        *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[w], unit);
+      });
     };
     // S^T of the two blocks in a place of the ring: codes and exponents, then the products.
     Q6 qf[2];
@@ -1179,6 +1180,14 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
       t[u] = mfma_part<part>(kc[2 * u + st], ke[2 * u + st], qf[st],
                              decltype(n)::value < 2 ? ref : t[u]);
     };
+    auto convert_v = [&](int place, int b, int to) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {   // (the first has been read)
+        if (j > 0) read_v(place, j);
+        mask_v(b);
+        write_v(j, to);
+      }
+    };
     const bool idle = row0 >= n_row;   // a wave past the sequence's rows only loads and converts
     floatx16 s[2] = {};
     addresses(run.b0);
@@ -1196,6 +1205,7 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
     if (run.b0 < b_end) {
       wait_loads<LOADS * (TDEPTH - 1)>();
       lds_barrier();
+      read_v(0, 0);
       read_k(0);
       convert_v(0, run.b0, 0);
       static_for<0, 12>([&](auto n) { product(n, s); });
@@ -1207,12 +1217,15 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
     auto do_step = [&](auto which, int b, floatx16 (&s)[2], floatx16 (&t)[2]) __attribute__((always_inline)) {
       constexpr int odd = which, to = odd;
       const int kbase = b * KV4_KEYS, next = odd ? h1 : h0 + TPAIR;
+      __builtin_amdgcn_s_setprio(0);
       wait_loads<LOADS * (TDEPTH - 2)>();
       // the next step's blocks and V of this one's are there, and nobody reads those of the last
       // step any more
       lds_barrier();
-      read_k(next);   // (after the last step those are blocks read once too often)
+      read_v(next, 0);   // (after the last step those are blocks read once too often)
+      read_k(next);
       issue(b + 2 * TDEPTH, odd ? h0 : h1 + TPAIR);
+      convert_v(next, b + 2, to ^ 1);   // (while K is on its way from LDS)
       if (__builtin_expect(!idle, 1)) {
         if (__builtin_expect(b + 2 > full, 0)) {
           const bool gone0 = absent(b), gone1 = absent(b + 1);
@@ -1268,12 +1281,16 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
         };
         // (the order is held by the barriers: left to itself the compiler puts all products first and
         // each read right before its use, which costs 2.1 instead of %STEP% us a step)
+        constexpr int AHEAD = 4;   // weights made while K is on its way
+        static_for<0, AHEAD>([&](auto w) { weights(w); });
+        __builtin_amdgcn_sched_barrier(0);
         static_for<0, 12>([&](auto n) {
           constexpr int k = n;
           product(n, t);
-          static_for<16 * k / 12, 16 * (k + 1) / 12>([&](auto w) { weights(w); });
+          static_for<AHEAD + (16 - AHEAD) * k / 12, AHEAD + (16 - AHEAD) * (k + 1) / 12>([&](auto w) { weights(w); });
           __builtin_amdgcn_sched_barrier(0);
         });
+        read_vf(0);
         // Weights above 2^15 (the sum of 32 says so; an infinity and a NaN do too), or none so far:
         // the reference is raised where the largest logit is more than KV4_SLACK above it, or set,
         // and they are made again.  So no maximum is taken in the steps in which none is needed.
@@ -1300,22 +1317,15 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
           for (int n = 0; n < 16; ++n) weights(n);
         }
         lrun += sum;
-        read_vf(0);   // (after the logits and K, whose registers these take)
+        __builtin_amdgcn_s_setprio(1);   // (before the other workgroup's conversions: 1%)
         static_for<0, 4>([&](auto quarter) {
-          constexpr int q = quarter, j = q >> 1;
+          constexpr int q = quarter;
           if constexpr (q < 3) read_vf(q + 1);
-          if constexpr (j < VN && (q & 1) == 0) read_v(next, j);
-          if constexpr (j < VN && (q & 1) == 1) mask_v(b + 2);
           __builtin_amdgcn_sched_barrier(0);
-          static_for<0, 4>([&](auto dt) {
-            constexpr int d = dt;
-            o[d] = M::mfma(vf[q & 1][d], p[q], o[d]);
-            if constexpr (j < VN && (q & 1) == 1) write_v(dt, j, to ^ 1, vwrite);
-            __builtin_amdgcn_sched_barrier(0);
-          });
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] = M::mfma(vf[q & 1][d], p[q], o[d]);
+          __builtin_amdgcn_sched_barrier(0);
         });
-      } else {
-        convert_v(next, b + 2, to ^ 1);
       }
     };
     floatx16 t[2];
@@ -1339,7 +1349,7 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
       if (lrun == -INFINITY) lrun = 0.f;
       le = lane_again();
       if (!run.whole) {
-        float* piece = e.ws + kv4_piece(blockIdx.x, walk.per, run.r0) * kv4_piece_floats(ROWS);
+        float* piece = e.ws + kv4_piece(worker_of(e, blockIdx.x), walk.per, run.r0) * kv4_piece_floats(ROWS);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -1382,8 +1392,9 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
   const int lane = threadIdx.x & 63;
   const int ratio = a.n_heads / a.n_kv;
   const int groups = tile_rows / 8;                 // workgroups of a unit
-  const int w0 = blockIdx.x / groups;               // the worker
-  const int f = (int)(blockIdx.x % groups) * 256 + threadIdx.x;   // which 4 values of the tile
+  // (the worker, whose partials its own die's L2 may still hold)
+  const int w0 = (blockIdx.x & 7) * (a.workers >> 3) + (blockIdx.x >> 3) / groups;
+  const int f = (int)((blockIdx.x >> 3) % groups) * 256 + threadIdx.x;   // which 4 values of the tile
   const int c = TILE ? 32 * (f >> 10) + (lane & 31) : 16 * (f >> 9) + (lane & 15);
   const int col = TILE ? 32 * ((f >> 8) & 3) + 8 * ((f >> 6) & 3) + 4 * (lane >> 5)
                        : 16 * ((f >> 6) & 7) + 4 * (lane >> 4);
@@ -1444,7 +1455,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
 
 template <typename T>
 void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
-  const dim3 grid(a.workers), block(256), mgrid((a.workers - 1) * (c.tile_rows / 8));
+  const dim3 grid(a.workers), block(256), mgrid(a.workers * (c.tile_rows / 8));
   switch (c.tile_rows) {
     case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a); break;
     case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a); break;

@@ -290,6 +290,50 @@ def test_long_caches():
         check(c, q, [0, 2, 3], held, lens, False, out, lse, scale=0.02)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("q_rows,heads", [(1, 8), (2, 80), (4, 80), (16, 56), (33, 40)])
+def test_all_workers_share_units(q_rows, heads, dtype):
+    """Enough keys that every workgroup has some and most units have several (in each of the tiles):
+    nine ragged sequences of 70 thousand rows in all, against 64 bits on the GPU."""
+    lens = [4100, 16001, 9000, 33, 12345, 0, 7777, 20011, 1500]
+    c = make(n_kv_heads=8, max_seqs=9, max_len=20480, page=64, n_pages=sum(R.pages(n, 64) for n in lens))
+    step = c.step(grow=lens)
+    g = torch.Generator("cuda").manual_seed(q_rows)
+    x = torch.randn((sum(lens), 2, 8, 128), generator=g, device="cuda", dtype=torch.float32).to(DT[dtype])
+    c.append(x[:, 0], x[:, 1], step.slots)
+    k, v = (t.double() for t in c.read(step.slots, dtype=torch.float32))
+    m_of = [min(q_rows, n) for n in lens]
+    starts = np.concatenate(([0], np.cumsum(m_of))).tolist()
+    q = queries(starts[-1], heads, 5, DT[dtype])
+    r = heads // 8
+    for causal in (False, True):
+        out = c.attend(q, starts, causal=causal)
+        at = 0
+        for s, n in enumerate(lens):
+            m = m_of[s]
+            if m == 0:
+                continue
+            see = torch.arange(n, device="cuda") < (n - m + torch.arange(m, device="cuda") + 1)[:, None]
+            see = see if causal else torch.ones_like(see)
+            for h in range(8):
+                kh, vh = k[at:at + n, h].contiguous(), v[at:at + n, h].contiguous()
+                qh = q[starts[s]:starts[s + 1], h * r:(h + 1) * r].double()
+                group = qh.abs().reshape(m, r, 4, 32).amax(-1).repeat_interleave(32, -1)
+                sees = see[:, None].expand(m, r, n).reshape(m * r, n)
+                z = (qh.reshape(m * r, 128) @ kh.T * 128 ** -0.5).masked_fill(~sees, -torch.inf)
+                top = z.amax(1, keepdim=True)
+                w = torch.exp(z - top)
+                l = w.sum(1, keepdim=True)
+                size = [(y.reshape(m * r, 128) @ kh.abs().T * 128 ** -0.5 * sees).amax(1) for y in (qh.abs(), group)]
+                tol, _ = R.attend_tolerance(
+                    (w @ vh / l).cpu().numpy(), (top + l.log())[:, 0].cpu().numpy(), (w @ vh.abs() / l).cpu().numpy(),
+                    torch.stack(size).cpu().numpy(), n, torch.finfo(q.dtype).eps / 2, split=q_rows * r > 32)
+                off = (out[starts[s]:starts[s + 1], h * r:(h + 1) * r].double().reshape(m * r, 128) - w @ vh / l).abs()
+                assert (off.cpu().numpy() <= tol).all(), (s, h, causal)
+            at += n
+    assert c.errors() == 0
+
+
 @pytest.mark.parametrize("q_rows", [1, 24])
 def test_pool_past_32_bits(q_rows):
     """Pages whose bytes lie past 2^32 from the pool's start, in the second layer too."""
