@@ -129,7 +129,11 @@ struct Kv4AttnArgs {
 // not below the sum of floors.  Where every row sees all keys, slope = 0 and base = ratio (len + 31).
 // (Keys before the first row at least 0, keys at least 1: every unit has a block, so that rows that
 // see nothing are written too.)
-constexpr int KV4_PAD = 8;
+//
+// KV4_PAD 8, 10 and 12 (KV4_MIN_PLACES 12, 12, 14) as measured, us: eight blocks of 32 rows over
+// 5000 keys (32 heads on 8) 48.6, 47.3, 45.5; sixteen of 8 rows over 300 keys 16.7, 17.3, 18.2; one
+// token over 2000 keys 12.6, 12.8, 14.8; 64 tokens over 1000 keys 26.0, 24.0, 24.5.
+constexpr int KV4_PAD = 10;
 struct Kv4Seq {
   int q0, qlen, len, tiles;
   long long slope, base, m;
@@ -166,7 +170,9 @@ DFL_HD long long kv4_cost(const Kv4Seq& s, int n_kv) { return n_kv * kv4_places(
 DFL_HD bool kv4_begun(const Kv4Seq& s, long long t, long long r) {
   return kv4_sum(s, t) < (r - KV4_PAD * t + 1) * s.m;
 }
-constexpr int KV4_MIN_PLACES = 16;   // fewest places of a worker
+// Fewest places of a worker: 10, 12, 16 and 32 take, us, for one token over 500 keys 10.4, 9.8, 10.9,
+// 14.3, for a block of 32 rows over 500 keys 21.6, 21.8, 24.1, 34.0.
+constexpr int KV4_MIN_PLACES = 12;
 DFL_HD long long kv4_per(long long total, int workers) {
   const long long per = kv4_div(total + workers - 1, workers);
   return per < KV4_MIN_PLACES ? KV4_MIN_PLACES : per;
@@ -196,7 +202,7 @@ DFL_HD bool kv4_counts_fit(int n_rows, int ratio, int n_kv, int n_seq, int width
 // How a launch is cut (what its workspace holds follows from it).
 struct Kv4Cut {
   int tile_rows;   // query rows of a unit: 16 or 32 (each wave has them all and a fourth of the
-                   // keys) or 64, 128 (each wave has 32 of them and all keys)
+                   // keys) or 128 (each wave has 32 of them and all keys)
   int workers;     // workgroups
 };
 inline Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
@@ -204,8 +210,13 @@ inline Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
   // rows of a kv head in a sequence, on average over those that can have any
   const long long seqs = n_seq < n_rows ? n_seq : n_rows;
   const long long rows = ((long long)n_rows * (n_heads / n_kv) + seqs - 1) / seqs;
-  c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : c.tile_rows == 64 ? 4 : 2);
+  // us, eight sequences of 5000 keys, 8 kv heads: 16 rows in tiles of 16 and 32 22.2, 27.1; 32 rows
+  // in tiles of 32 27.9, 40 rows in tiles of 128 41.0; tiles of 64 (two waves, else as those of 128)
+  // took 40.4 and at 64 rows 40.3 for 41.5.  Workgroups for each CU: as many as fit at once with
+  // tiles of 32 and 128 (LDS and registers); of four that fit with 16, three: 64 ragged tokens take
+  // 93 us with two, 89, 100 with four; sixteen tokens over 65 thousand keys 214, 216, 253.
+  c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+  c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : 2);
   return c;
 }
 

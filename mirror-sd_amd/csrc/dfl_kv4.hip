@@ -882,7 +882,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 
 // ---- more query rows
 //
-// WQ waves of 32 rows each go over the same keys, two blocks a step (one block's chain of eight
+// Four waves of 32 rows each go over the same keys, two blocks a step (one block's chain of eight
 // dependent products leaves the matrix unit half idle, two interleaved fill it).  Blocks come as
 // they lie in the pool into a ring in LDS, TDEPTH steps of them on their way while one computes.
 // K goes from codes to operands in each wave's registers; V is converted once for all, a part by
@@ -1012,30 +1012,27 @@ DFL_DEV const Kv4AttnArgs& args_again() {
   return *(const Kv4AttnArgs*)p;
 }
 
-template <typename T, int WQ>
-__global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
+template <typename T>
+__global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
   typedef typename M::v2 v2;
-  constexpr int ROWS = 32 * WQ;
-  static_assert(WQ == 2 || WQ == 4, "the waves' shares of a step's loads and of V");
-  constexpr int VN = 4 / WQ;              // groups of V of a step that a lane converts
+  constexpr int ROWS = 128;
   extern __shared__ __attribute__((aligned(1024))) unsigned char tile_lds[];   // TILE_LDS bytes
   unsigned char* const ring = tile_lds;                      // [TRING][TPAIR]
   unsigned char* const vbuf = tile_lds + TRING * TPAIR;      // [2][2][VTILE]
   const int lane = threadIdx.x & 63, i = lane & 31, h = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // K: row i of a block, groups h and 2 + h.  V: of block vu of the step the same, or, of four waves,
-  // group h or 2 + h.
+  // K: row i of a block, groups h and 2 + h.  V: of block vu of the step row i, group 2 vj + h.
   const int koff = 16 * lane;
   const int soff = KV4_SC + 4 * ((i & 15) + 16 * h) + (i >> 4);   // K's exponent (V's is 2 further)
-  const int vu = WQ == 2 ? wv : wv >> 1, vj = WQ == 2 ? 0 : wv & 1;
+  const int vu = wv >> 1, vj = wv & 1;
   const int vwrite = i * TROW + 64 * h;
   const int vread = (4 * h + ((lane & 15) >> 2)) * TROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 
   // (as with the arguments: a wave's place in its walk is kept in LDS over a run's steps)
   struct Kept { Walk walk; Run run; };
-  __shared__ Kept kept_of[WQ];
+  __shared__ Kept kept_of[4];
   Kept& kept = kept_of[wv];
   bool more;
   {
@@ -1110,10 +1107,9 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
         if (no) atomicOr(a.err, bit);
       }
     };
-    // A wave's loads of the step that begins with block b, into a place of the ring: KiB wv (and, of
-    // two waves, wv + 2) of both blocks, and the exponents of block wv % 2 (of four waves two load
-    // the same, so that all count alike).
-    constexpr int LOADS = WQ == 2 ? 5 : 3;
+    // A wave's loads of the step that begins with block b, into a place of the ring: KiB wv of both
+    // blocks, and the exponents of block wv % 2 (two waves load the same, so that all count alike).
+    constexpr int LOADS = 3;
     const unsigned char* const pool_w = a.pool + 1024 * wv;
     const uint32_t ring_w = (uint32_t)(uintptr_t)(lds_ptr_t)ring + 1024 * wv;
     auto issue = [&](int b, int place) __attribute__((always_inline)) {
@@ -1124,10 +1120,6 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
       const uint32_t to = ring_w + place;
       load_to_lds16(p0, koff, to);
       load_to_lds16(p1, koff, to + KV4_BLOCK);
-      if constexpr (WQ == 2) {
-        load_to_lds16(p0 + 2048, koff, to + 2048);
-        load_to_lds16(p1 + 2048, koff, to + KV4_BLOCK + 2048);
-      }
       const uintptr_t p = wv & 1 ? (uintptr_t)p1 : (uintptr_t)p0;
       load_to_lds4(reinterpret_cast<const unsigned char*>(p), KV4_SC - 1024 * wv, koff,
                    to + (wv & 1) * KV4_BLOCK + KV4_SC - 1024 * wv);
@@ -1138,10 +1130,10 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
     // the rows that do see a NaN are set when the block is used.
     u32x4 vc;
     uint32_t ve;
-    auto read_v = [&](int place, int j) __attribute__((always_inline)) {
+    auto read_v = [&](int place) __attribute__((always_inline)) {
       const unsigned char* vb = ring + place + vu * KV4_BLOCK;
-      ve = vb[128 * (vj + j) + soff + 2];
-      vc = *reinterpret_cast<const u32x4*>(vb + 2048 + 1024 * (vj + j) + koff);
+      ve = vb[128 * vj + soff + 2];
+      vc = *reinterpret_cast<const u32x4*>(vb + 2048 + 1024 * vj + koff);
     };
     auto mask_v = [&](int b) __attribute__((always_inline)) {
       if (__builtin_expect(b + 2 > full, 0)) {
@@ -1152,8 +1144,9 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
         }
       }
     };
-    auto write_v = [&](int j, int to) __attribute__((always_inline)) {
-      unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * (vj + j) + vwrite;
+    auto convert_v = [&](int b, int to) __attribute__((always_inline)) {
+      mask_v(b);
+      unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * vj + vwrite;
       const float unit = M::kUnit * exponent(ve);
       static_for<0, 4>([&](auto word) {
         constexpr int w = word;
@@ -1180,14 +1173,6 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
       t[u] = mfma_part<part>(kc[2 * u + st], ke[2 * u + st], qf[st],
                              decltype(n)::value < 2 ? ref : t[u]);
     };
-    auto convert_v = [&](int place, int b, int to) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < VN; ++j) {   // (the first has been read)
-        if (j > 0) read_v(place, j);
-        mask_v(b);
-        write_v(j, to);
-      }
-    };
     const bool idle = row0 >= n_row;   // a wave past the sequence's rows only loads and converts
     floatx16 s[2] = {};
     addresses(run.b0);
@@ -1205,9 +1190,9 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
     if (run.b0 < b_end) {
       wait_loads<LOADS * (TDEPTH - 1)>();
       lds_barrier();
-      read_v(0, 0);
+      read_v(0);
       read_k(0);
-      convert_v(0, run.b0, 0);
+      convert_v(run.b0, 0);
       static_for<0, 12>([&](auto n) { product(n, s); });
     }
     // Step `odd` of a pair (s: S^T of its two blocks): their weights, between which (they do not wait
@@ -1222,10 +1207,10 @@ __global__ __launch_bounds__(64 * WQ, 2) void kv4_tile_kernel(Kv4AttnArgs args) 
       // the next step's blocks and V of this one's are there, and nobody reads those of the last
       // step any more
       lds_barrier();
-      read_v(next, 0);   // (after the last step those are blocks read once too often)
+      read_v(next);   // (after the last step those are blocks read once too often)
       read_k(next);
       issue(b + 2 * TDEPTH, odd ? h0 : h1 + TPAIR);
-      convert_v(next, b + 2, to ^ 1);   // (while K is on its way from LDS)
+      convert_v(b + 2, to ^ 1);   // (while K is on its way from LDS)
       if (__builtin_expect(!idle, 1)) {
         if (__builtin_expect(b + 2 > full, 0)) {
           const bool gone0 = absent(b), gone1 = absent(b + 1);
@@ -1459,8 +1444,7 @@ void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
   switch (c.tile_rows) {
     case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a); break;
     case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a); break;
-    case 64: hipLaunchKernelGGL((kv4_tile_kernel<T, 2>), grid, dim3(128), TILE_LDS, st, a); break;
-    default: hipLaunchKernelGGL((kv4_tile_kernel<T, 4>), grid, block, TILE_LDS, st, a);
+    default: hipLaunchKernelGGL((kv4_tile_kernel<T>), grid, block, TILE_LDS, st, a);
   }
   if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
   else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);

@@ -207,7 +207,7 @@ int main() {
   asks();
   seqs();
   for (int workers : {1, 3, 256, 768})
-    for (int rows : {16, 32, 64, 128})
+    for (int rows : {16, 32, 128})
       for (bool causal : {false, true}) {
         split({1}, {1}, 32, 8, rows, workers, causal);
         split({1}, {33000}, 32, 8, rows, workers, causal);
