@@ -369,15 +369,14 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsArgs a) {
 //
 // A unit is a tile of query rows (row = token * ratio + head in group) of one sequence and kv
 // head; a workgroup takes a run of key blocks of a unit (32 keys each).  Of a block:
-//   S^T = K Q^T   matrix instructions with keys on the M axis, K converted from codes in registers
-//                 (two values an instruction, which applies their power of two: exact);
+//   S^T = K Q^T   matrix instructions with keys on the M axis;
 //   softmax       fp32, log2 domain, the reference maximum raised only when a block exceeds it by
 //                 more than KV4_SLACK; weights rounded to the type of Q, and summed as rounded;
 //   O^T += V^T P  V converted in registers, written to LDS as rows, read back transposed
 //                 (ds_read_b64_tr_b16); P from the S^T accumulators as they lie: the rows of V that
 //                 a lane's weights stand for are those whose keys its accumulators hold.
 // Two kernels: kv4_attn_kernel for up to 32 rows (single tokens, small blocks), where HBM and
-// latency count, and kv4_tile_kernel for more.
+// latency count, and kv4_tile_kernel for more, where the matrix and vector units do.
 
 constexpr float KV4_SLACK = 6.f;
 // Weights are 2^(s - m + KV4_LIFT) <= 2^15 for a reference m: fp16 then keeps 2^-23 of the
@@ -640,6 +639,10 @@ DFL_DEV const unsigned char* block_in(const Kv4AttnArgs& a, const Run& r, int b,
 // The four waves of a workgroup take every fourth block of a run each, a wave's whole work on a
 // block in its own registers and its own 9 KiB of LDS (no barrier in the loop); their states are
 // joined at the run's end.  The next block's codes load while this one computes.
+//
+// Long caches are bound by HBM: sixteen tokens of 64 heads over 65 thousand keys each (1.14 GB) take
+// 203 us, 5.6 TB/s; 64 ragged tokens (379 MB) 80, 4.7.  One token over 500 keys takes 7.4 us, a
+// chain of latencies: launch, lengths, pages, blocks, join.
 
 constexpr int VROW = 288;                 // bytes of a V row in LDS: 8 banks apart, so that the 8
                                           // rows of a half wave's transposing read do not collide
@@ -862,7 +865,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       } else if (r < n_row) {
         const int tok = r / ratio;
         const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + r - tok * ratio;
-        const bool none = vis[n] <= 0;   // a row that sees no key: zeros, and the sum of none
+        const bool none = l == 0.f;   // a row that sees no key: zeros, and the sum of none
         T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * ge;
 #pragma unroll
         for (int dd = 0; dd < 2; ++dd) {
@@ -882,12 +885,24 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 
 // ---- more query rows
 //
-// Four waves of 32 rows each go over the same keys, two blocks a step (one block's chain of eight
-// dependent products leaves the matrix unit half idle, two interleaved fill it).  Blocks come as
-// they lie in the pool into a ring in LDS, TDEPTH steps of them on their way while one computes.
-// K goes from codes to operands in each wave's registers; V is converted once for all, a part by
-// each wave, into one of two LDS buffers; one barrier a step.  v_mfma 32x32x16, whose accumulator r
-// in lane (q, h) is key 8 (r / 4) + 4 h + r % 4 of the block.
+// Four waves of 32 rows each go over the same keys, two blocks a step (one block's chain of products
+// leaves the matrix unit half idle, two interleaved fill it).  Blocks come as they lie in the pool
+// into a ring in LDS, TDEPTH steps of them on their way while one computes.  K goes into the
+// products as it is cached (see split_q); V is converted once for all, a part by each wave, into
+// one of two LDS buffers; one barrier a step.  Accumulator r of lane (q, h) is key 8 (r / 4) + 4 h +
+// r % 4 of the block.
+//
+// The logits are summed onto the negative reference, so that a weight is the power of what the
+// products leave.  S^T of the next step is made between the weights of this one.
+//
+// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 206 us
+// and 15 for the merge, 818 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
+// A step of both workgroups takes 1.8 us, 3400 cycles: for each SIMD 1790 of products and 1700 of
+// vector instructions, for the CU 1900 of LDS.  No one of them is full: two waves a SIMD do not
+// fill each other's gaps, and there are no registers for a third.  Eight blocks of 32 rows over
+// 811 .. 7844 keys: 37 us and 11; of the 37 3 go to finding the first unit, 4.3 to its queries and
+// first blocks, 20 to the steps, and both kernels move 36 MB of partials.  With K converted in
+// registers as V is (64 conversions for each 32 keys and wave), the prompts took 233, the blocks 54.
 
 constexpr int TROW = 320;                 // bytes of a V row in LDS: 16 banks apart, so that the 4
                                           // rows of a half wave's transposing read do not collide
@@ -1265,7 +1280,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
           }
         };
         // (the order is held by the barriers: left to itself the compiler puts all products first and
-        // each read right before its use, which costs 2.1 instead of %STEP% us a step)
+        // each read right before its use; eight blocks then take 52 us for 51)
         constexpr int AHEAD = 4;   // weights made while K is on its way
         static_for<0, AHEAD>([&](auto w) { weights(w); });
         __builtin_amdgcn_sched_barrier(0);
@@ -1302,7 +1317,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
           for (int n = 0; n < 16; ++n) weights(n);
         }
         lrun += sum;
-        __builtin_amdgcn_s_setprio(1);   // (before the other workgroup's conversions: 1%)
+        __builtin_amdgcn_s_setprio(1);   // (before the other workgroup's conversions: eight blocks 49.7 -> 48.9 us)
         static_for<0, 4>([&](auto quarter) {
           constexpr int q = quarter;
           if constexpr (q < 3) read_vf(q + 1);
@@ -1346,7 +1361,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
       } else if (row0 + (le & 31) < n_row) {
         const int row = row0 + (le & 31), tok = row / ratio;
         const long long orow = (long long)(sq.q0 + tok) * e.n_heads + (run.head - tok) * ratio + row;
-        const bool none = attn_visible(e, sq, tok) <= 0;   // a row that sees no key: zeros, and the sum of none
+        const bool none = lrun == 0.f;   // a row that sees no key: zeros, and the sum of none
         const float f = (1.f / M::kUnit) / lrun;
         T* op = reinterpret_cast<T*>(e.out) + orow * KV4_D + 4 * (le >> 5);
 #pragma unroll
@@ -1371,7 +1386,9 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
 
 // Units that several workers share: their partial states joined in the order of the keys, by the
 // note of the worker that began with the unit.  A thread has 4 values of a row.  TILE: the partials
-// are kv4_tile_kernel's.
+// are kv4_tile_kernel's.  Bound by them: eight blocks leave 550 of 66 KB, 10.6 us with the launch.
+// Two partials (most of a prompt's) or eight are loaded at once: one by one two prompts' took 30 us
+// for 16.  Which they are is in notes: every workgroup finding its unit by itself took 40 us more.
 template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
   const int lane = threadIdx.x & 63;
@@ -1428,7 +1445,7 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
   }
   const int tok = r / ratio;
   const long long orow = (long long)(n.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
-  const bool none = a.causal ? n.len - n.qlen + tok < 0 : n.len == 0;
+  const bool none = l == 0.f;
   typedef T v4 __attribute__((ext_vector_type(4)));
   v4 x;
 #pragma unroll

@@ -334,6 +334,31 @@ def test_all_workers_share_units(q_rows, heads, dtype):
     assert c.errors() == 0
 
 
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+def test_all_keys_absent(q_rows, heads):
+    """A sequence all of whose pages are outside the pool is one without keys, however it is cut."""
+    from mirror_sd_amd import kv4
+    c = make(max_seqs=3, n_pages=200, page=32, max_len=4096)
+    lens = [40, 3000, 40]
+    _, held, _ = fill(c, lens, 4, torch.float16)
+    q = queries(3 * q_rows, heads, 3, torch.float16)
+    starts = [0, q_rows, 2 * q_rows, 3 * q_rows]
+    good = c.attend(q, starts)
+    c.table[1, :60] = -1                                    # keys 0 .. 1919: the first seen is a late one
+    out = c.attend(q, starts)
+    kv = held[40 + 1920:3040]
+    o, l, mass, size = R.attend(q[q_rows:2 * q_rows].double().cpu().numpy(), kv[:, 0], kv[:, 1], False, 128 ** -0.5)
+    tol, _ = R.attend_tolerance(o, l, mass, size, 3000, 2.0 ** -11)
+    assert (np.abs(out[q_rows:2 * q_rows].double().cpu().numpy() - o) <= tol).all()
+    assert c.errors() == kv4.ERR_PAGE
+    c.table[1] = -1
+    out, lse = c.attend(q, starts, return_lse=True)
+    assert c.errors() == kv4.ERR_PAGE
+    a, b = starts[1], starts[2]
+    assert (out[a:b] == 0).all() and torch.isneginf(lse[a:b]).all()
+    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
+
+
 @pytest.mark.parametrize("q_rows", [1, 24])
 def test_pool_past_32_bits(q_rows):
     """Pages whose bytes lie past 2^32 from the pool's start, in the second layer too."""
