@@ -895,8 +895,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 // The logits are summed onto the negative reference, so that a weight is the power of what the
 // products leave.  S^T of the next step is made between the weights of this one.
 //
-// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 206 us
-// and 15 for the merge, 818 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
+// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 200 us
+// with the merge's 15, 840 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
 // A step of both workgroups takes 1.8 us, 3400 cycles: for each SIMD 1790 of products and 1700 of
 // vector instructions, for the CU 1900 of LDS.  No one of them is full: two waves a SIMD do not
 // fill each other's gaps, and there are no registers for a third.  Eight blocks of 32 rows over

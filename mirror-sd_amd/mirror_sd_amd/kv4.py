@@ -118,10 +118,12 @@ class KV4Cache:
             t = torch.as_tensor(t, dtype=torch.int32)
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
             raise ValueError(f"{what} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
-        if t.dtype.is_floating_point or t.dtype in (torch.bool, torch.complex64, torch.complex128):
+        if t.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
             raise ValueError(f"{what} must be integers, got {t.dtype}")
         if t.is_cuda and t.device != self.device:
             raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
+        if t.dtype == torch.int64:   # (what 32 bits do not hold stays out of range)
+            t = t.clamp(-2**31, 2**31 - 1)
         return t.to(self.device, torch.int32).contiguous()
 
     def _rows(self, t, heads: Optional[int], what: str):

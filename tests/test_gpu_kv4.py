@@ -635,6 +635,22 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+def test_integers_wider_than_32_bits():
+    """Numbers that 32 bits do not hold are out of range, not what their low bits say."""
+    from mirror_sd_amd import kv4
+    c = make()
+    wide = torch.full((4,), 2**32 + 1, dtype=torch.int64, device="cuda")
+    step = c.step(grow=wide, max_rows=8)
+    assert c.errors() == kv4.ERR_LENGTH and step.starts.tolist() == [0] * 5 and c.lens.tolist() == [0] * 4
+    x = torch.ones((4, 2, 128), dtype=torch.float16, device="cuda")
+    c.append(x, x, wide)
+    assert c.errors() == kv4.ERR_SLOT and int(c.pool.max()) == 0
+    c.append(x, x, -wide)
+    assert c.errors() == kv4.ERR_SLOT and int(c.pool.max()) == 0
+    with pytest.raises(ValueError, match="integers"):
+        c.append(x, x, torch.zeros(4, device="cuda"))
+
+
 def test_refusals_on_the_device():
     c = make()
     with pytest.raises(ValueError, match="max_rows"):
