@@ -318,7 +318,7 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
  * Weights are rounded to q's dtype, all else is held in fp32, but for queries where a sequence has
  * more than 32 rows (tokens * n_heads / n_kv) for each kv head, on average: there scale * log2(e) *
  * q, which must be finite in fp32, goes into the products in parts that hold it to 2^-13.9 of the
- * largest of its 32 values.  With fp16 queries, cached values beyond +-131008 read as infinities
+ * largest of its 32 values (2^-129 if that is more).  With fp16 queries, cached values beyond +-131008 read as infinities
  * (keys and values of up to 32 rows, values of more).  ws: dfl_kv4_attend_ws(...) bytes for the same arguments,
  * 16-byte aligned, any content, not shared with a call that may run at the same time. */
 typedef struct dfl_kv4_attn {

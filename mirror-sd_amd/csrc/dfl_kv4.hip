@@ -605,7 +605,20 @@ DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
     ++r.head;
     r.tile = 0;
   } else {
-    return unit_at(a, tile_rows, k.pos, r);
+    // the next sequence that has rows begins here
+    for (int s0 = r.s + 1;; s0 += 64) {
+      if (s0 >= a.n_seq) return false;
+      const Lanes l = attn_lanes(a, tile_rows, s0, false);
+      const unsigned long long some = __ballot(l.cost > 0);
+      if (!some) continue;
+      const int i = __ffsll(some) - 1;
+      r.s = s0 + i;
+      r.sq = kv4_seq(pick(l.q0, i), pick(l.q1, i), pick(l.len, i), a.n_rows, a.width, a.page_shift,
+                     a.n_heads / a.n_kv, tile_rows, a.causal);
+      r.head = r.tile = 0;
+      r.head0 = k.pos;
+      break;
+    }
   }
   unit_places(r);
   return true;
