@@ -908,8 +908,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 // The logits are summed onto the negative reference, so that a weight is the power of what the
 // products leave.  S^T of the next step is made between the weights of this one.
 //
-// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 200 us
-// with the merge's 15, 840 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
+// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 205 us
+// with the merge's 15, 820 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
 // A step of both workgroups takes 1.8 us, 3400 cycles: for each SIMD 1790 of products and 1700 of
 // vector instructions, for the CU 1900 of LDS.  No one of them is full: two waves a SIMD do not
 // fill each other's gaps, and there are no registers for a third.  Eight blocks of 32 rows over
@@ -1305,8 +1305,9 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
         });
         read_vf(0);
         // Weights above 2^15 (the sum of 32 says so; an infinity and a NaN do too), or none so far:
-        // the reference is raised where the largest logit is more than KV4_SLACK above it, or set,
-        // and they are made again.  So no maximum is taken in the steps in which none is needed.
+        // the row's reference is raised to the largest logit (more than KV4_SLACK above it), or set,
+        // and they are made again.  So no maximum is taken in the steps in which none is needed, and
+        // a row's references do not depend on the other rows.
         if (__builtin_expect(!__all((sum <= 1048576.f) & (lrun + sum >= 0.f)), 0)) {
           float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
@@ -1314,7 +1315,9 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
           top = fmaxf(top, __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (lane_again() ^ 32), __float_as_int(top))));
           top -= KV4_LIFT;
           const bool none = lrun == -INFINITY;   // (both lanes of the row)
-          const float up = top > KV4_SLACK || (none && top > -INFINITY) ? top : 0.f;
+          const unsigned long long past = __ballot(!(sum <= 1048576.f));
+          const bool over = (past | past >> 32 | past << 32) >> lane_again() & 1;
+          const float up = (over && top > KV4_SLACK) || (none && top > -INFINITY) ? top : 0.f;
           const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(-up);
           lrun = none && top > -INFINITY ? 0.f : lrun * alpha;
 #pragma unroll

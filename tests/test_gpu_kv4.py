@@ -335,6 +335,34 @@ def test_all_workers_share_units(q_rows, heads, dtype):
 
 
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+def test_extreme_magnitudes(q_rows, heads):
+    """Keys of 2^90 under queries of 2^-88 (and the other way round), values of 2^100: powers of two
+    change nothing but the exponents.  A query whose values differ by 2^40 within a group."""
+    for up, down in ((90, -88), (-100, 101)):
+        c = make(max_seqs=2, n_pages=40, page=32, max_len=512)
+        lens = [77, 300]
+        step = c.step(grow=lens)
+        x = rows(sum(lens), 2, 8, torch.bfloat16)
+        x[:, 0] *= 2.0 ** up
+        x[:, 1] *= 2.0 ** 100
+        c.append(x[:, 0], x[:, 1], step.slots)
+        held = R.values(x.double().cpu().numpy())
+        q = queries(2 * q_rows, heads, 6, torch.bfloat16)
+        q[:, :, ::5] *= 2.0 ** -40
+        q *= 2.0 ** down
+        starts = [0, q_rows, 2 * q_rows]
+        out, lse = c.attend(q, starts, causal=True, return_lse=True)
+        check(c, q, starts, held, lens, True, out, lse)
+    # an infinity or a NaN in a query is its rows' alone
+    q[1, 1, 3], q[-1, 0, 100] = float("inf"), float("nan")
+    again = c.attend(q, starts, causal=True)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[1, 1] = bad[-1, 0] = True
+    assert torch.isnan(again[bad]).all() and torch.equal(again[~bad], out[~bad])
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
 def test_all_keys_absent(q_rows, heads):
     """A sequence all of whose pages are outside the pool is one without keys, however it is cut."""
     from mirror_sd_amd import kv4
