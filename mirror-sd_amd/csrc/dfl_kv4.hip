@@ -565,7 +565,8 @@ struct Walk { long long pos, end, per; };
 // its own, and workers that follow on each other read the same keys (the tiles of a head): so
 // each die has an eighth of all places, one after the other.  (Two prompts of 4096 and 777 rows:
 // 219 us in turn, 216 so.)
-DFL_DEV int worker_of(const Kv4AttnArgs& a, int workgroup) {   // (a.workers: a multiple of 8)
+static_assert(KV4_CUS % 8 == 0, "workers in eight parts");
+DFL_DEV int worker_of(const Kv4AttnArgs& a, int workgroup) {
   return (workgroup & 7) * (a.workers >> 3) + (workgroup >> 3);
 }
 // Begins at the worker's first place; false if it has none.

@@ -600,14 +600,15 @@ def test_results_join_over_keys():
     assert float((joined - o).abs().max()) <= 2 * 3 * 2.0 ** -11 * 10 and float((both - l).abs().max()) <= 2.0 ** -9
 
 
-def test_captured_steps():
+@pytest.mark.parametrize("heads,n", [(4, 12), (40, 12), (4, 9000)])
+def test_captured_steps(heads, n):
     """A step, its rows and its attention in a graph, replayed with other lengths and rows between
-    eager work; a second graph beside it."""
+    eager work; a second graph beside it.  (40 heads: tiles of 128 rows; 9000 rows, nearly all of
+    them spare: a step in several launches.)"""
     caches = [make(max_seqs=3, n_pages=30, page=32) for _ in range(2)]
-    n = 12
     grow, keep = (torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(2))
     x = rows(n, 2, 0)
-    q = queries(n, 4, 0, torch.float16)
+    q = queries(n, heads, 0, torch.float16)
     graphs, outs = [], []
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -635,7 +636,7 @@ def test_captured_steps():
         grow.copy_(torch.tensor(gr, dtype=torch.int32))
         keep.copy_(torch.tensor(k, dtype=torch.int32))
         x.copy_(rows(n, 2, turn))
-        q.copy_(queries(n, 4, turn, torch.float16))
+        q.copy_(queries(n, heads, turn, torch.float16))
         graphs[turn % 2].replay()
         got, out = outs[turn % 2]
         e = caches[1].step(grow=grow, keep=keep, max_rows=n)
