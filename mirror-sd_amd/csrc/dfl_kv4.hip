@@ -909,14 +909,14 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 // The logits are summed onto the negative reference, so that a weight is the power of what the
 // products leave.  S^T of the next step is made between the weights of this one.
 //
-// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 205 us
-// with the merge's 15, 820 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
+// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 210 us
+// with the merge's 15, 800 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
 // A step of both workgroups takes 1.8 us, 3400 cycles: for each SIMD 1790 of products and 1700 of
 // vector instructions, for the CU 1900 of LDS.  No one of them is full: two waves a SIMD do not
 // fill each other's gaps, and there are no registers for a third.  Eight blocks of 32 rows over
 // 811 .. 7844 keys: 37 us and 11; of the 37 3 go to finding the first unit, 4.3 to its queries and
 // first blocks, 20 to the steps, and both kernels move 36 MB of partials.  With K converted in
-// registers as V is (64 conversions for each 32 keys and wave), the prompts took 233, the blocks 54.
+// registers as V is (64 conversions a step and wave), the prompts took 233 us, the blocks 54 in all.
 
 constexpr int TROW = 320;                 // bytes of a V row in LDS: 16 banks apart, so that the 4
                                           // rows of a half wave's transposing read do not collide
