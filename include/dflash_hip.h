@@ -284,8 +284,10 @@ int dfl_device_errors(dfl_ctx* ctx, int32_t* flags, void* stream);
  * places past a sequence's pages and free places past *n_free that the step gives up become -1.
  * Out: starts [n_seq + 1] (the new rows of sequence s are starts[s] .. starts[s+1] - 1), and for
  * each new row its slot and its position (the row's number in its sequence), max_rows of each;
- * those past starts[n_seq] are -1.  A step that cannot be done (bits 3, 4, 5, 7) changes nothing,
- * and gives no rows.  scratch: dfl_kv4_step_scratch(n_seq) int32, any content, not shared with a
+ * those past starts[n_seq] are -1.  A step that cannot be done (bits 3, 4, 5; bit 7 for a *n_free
+ * that does not fit, or a page id outside the pool that the step would put back, take, or add rows
+ * to) changes nothing, and gives no rows (free places past *n_free, which hold no page, may become
+ * -1).  scratch: dfl_kv4_step_scratch(n_seq) int32, any content, not shared with a
  * step that may run at the same time. */
 int dfl_kv4_step(int32_t n_seq, int32_t page, int32_t width, int32_t n_pages, const int32_t* keep,
                  const int32_t* grow, int32_t* lens, int32_t* table, int32_t* free_pages,

@@ -40,7 +40,7 @@ constexpr int KV4_ERR_LEN = 8;       // step: a length out of range
 constexpr int KV4_ERR_POOL = 16;     // step: not enough free pages
 constexpr int KV4_ERR_ROWS = 32;     // step: more new rows than the slot map holds
 constexpr int KV4_ERR_SLOT = 64;     // append, read: a slot outside the pool
-constexpr int KV4_ERR_PAGE = 128;    // attend, step: a page, length or row range out of bounds
+constexpr int KV4_ERR_PAGE = 128;    // attend, step: a page, length, row range or free count out of bounds
 
 // Offsets in a block, of K (v = 0) or V (v = 1): the 16 code bytes of group g of row r, and its
 // exponent byte.
@@ -66,9 +66,9 @@ struct Kv4StepArgs {
   int* scratch;                // kv4_step_scratch(n_seq) ints
   int* err;
 };
-// scratch: status, freed and taken totals, free pages before; then [n_seq] kept lengths, freed
-// and taken pages before each sequence
-DFL_HD long long kv4_step_scratch(int n_seq) { return 4 + 3ll * n_seq; }
+// scratch: the scan's error, freed and taken totals, free pages before, the check's error; then
+// [n_seq] kept lengths, freed and taken pages before each sequence
+DFL_HD long long kv4_step_scratch(int n_seq) { return 5 + 3ll * n_seq; }
 
 // What one sequence asks of a step; false if a length is out of range.
 struct Kv4Ask { int keep, grow, freed, taken; };

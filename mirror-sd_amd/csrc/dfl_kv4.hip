@@ -23,16 +23,21 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 // the first sequence's first page on top, and are handed out again from the top, sequence by
 // sequence, so a step that puts back what it takes leaves every table as it was.
 //
-// Phases, each over all sequences: scan (totals, then offsets), free, take, rows.  A phase reads
-// what the one before wrote, so for many sequences or rows they are launches of their own; up to
-// STEP_ONE_SEQS and STEP_ONE_ROWS one workgroup does them all, with the offsets in LDS.  In both
-// forms the pages and rows of all sequences are numbered through and found by a search in the
-// offsets, so that no thread waits for a long sequence.
+// Phases, each over all sequences: scan (totals, then offsets), check, move, rows.  The check looks
+// at every page id that the step will touch, and puts the pages that come back on the stack, above
+// its top as it was; only when all are pages of the pool does anything else change (if not, those
+// places of the stack, which hold no page, are cleared).  A phase reads what the one before wrote,
+// so for many sequences or rows they are launches of their own; up to STEP_ONE_SEQS and
+// STEP_ONE_ROWS one workgroup does them all, with the offsets in LDS.  In both forms the pages and
+// rows of all sequences are numbered through and found by a search in the offsets, so that no thread
+// waits for a long sequence.
 //
 // Bound by latencies: launches and a handful of reads that follow on each other.  One workgroup
 // against launches, us (sequences x new rows of each; every page put back and taken again):
-//   8 x 16 5.0, 11.6;  256 x 16 11.2, 18.2;  1024 x 8 16.5, 22.2;  8 x 1024 11.0, 13.7;
-//   1024 x 32 38.6, 20.4;  64 x 512 29.4, 16.2;  8 x 4096 22.5, 14.1.
+//   8 x 16 5.2, 12.4;  256 x 16 11.6, 19.1;  1024 x 8 16.9, 23.3;  8 x 1024 11.3, 14.5;
+//   1024 x 32 39.5, 22.2;  64 x 512 29.3, 15.9;  8 x 4096 22.3, 14.5.
+// (Of these the check takes 0.2 in one workgroup, where a thread keeps what it has looked at in
+// registers, and 1 in launches.)
 
 constexpr int STEP_ONE_SEQS = 1024, STEP_ONE_ROWS = 8192;
 
@@ -82,32 +87,50 @@ DFL_DEV int step_search(const int* at, int n, int v) {
 // Offsets of all sequences: kept lengths, pages put back and taken before each (n_seq), new rows
 // before each (n_seq + 1).
 struct StepView { int *base, *f_at, *t_at, *starts; };
-// Page i of those put back: from its table onto the stack.
-DFL_DEV void step_free(const Kv4StepArgs& a, const StepView& v, int i, int top) {
-  const int s = step_search(v.f_at, a.n_seq, i);
-  int* at = a.table + (long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.f_at[s]);
-  const int p = *at;
-  if (p < 0 || p >= a.n_pages) atomicOr(a.err, KV4_ERR_PAGE);
-  a.free_pages[top - i] = p;
-  *at = -1;
+// Move i of a step: page i of those put back and page i of those taken, which is the same one if
+// both are there (they have one place on the stack, `top` less i with the stack's top after all
+// are put back).
+struct StepMove {
+  int *from, *to;   // its places in the tables (null: it comes from the stack, it stays there)
+  int page;
+  bool again;       // the step puts another page into `from`
+};
+// on_stack: the pages put back are on the stack already.
+DFL_DEV StepMove step_look(const Kv4StepArgs& a, const StepView& v, int i, int freed, int taken, int top, bool on_stack) {
+  StepMove m{nullptr, nullptr, 0, false};
+  if (i < freed) {
+    const int s = step_search(v.f_at, a.n_seq, i), at = kv4_pages(v.base[s], a.page_shift) + (i - v.f_at[s]);
+    m.again = at < kv4_pages(v.base[s] + (v.starts[s + 1] - v.starts[s]), a.page_shift);
+    m.from = a.table + (long long)s * a.width + at;
+  }
+  if (i < freed || i < taken) m.page = m.from && !on_stack ? *m.from : a.free_pages[top - i];
+  if (i < taken) {
+    const int s = step_search(v.t_at, a.n_seq, i);
+    m.to = a.table + (long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.t_at[s]);
+  }
+  return m;
 }
-// Page i of those taken: from the stack into its table.
-DFL_DEV void step_take(const Kv4StepArgs& a, const StepView& v, int i, int top) {
-  const int s = step_search(v.t_at, a.n_seq, i);
-  a.table[(long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.t_at[s])] = a.free_pages[top - i];
-  a.free_pages[top - i] = -1;
+DFL_DEV void step_move(const Kv4StepArgs& a, const StepMove& m, int i, int top) {
+  if (m.from && !m.again) *m.from = -1;
+  if (m.to) *m.to = m.page;
+  if (m.from || m.to) a.free_pages[top - i] = m.to ? -1 : m.page;
 }
+// The page that new rows of sequence s go on in; 0 if there is none.
+DFL_DEV int step_kept(const Kv4StepArgs& a, const StepView& v, int s) {
+  if (v.starts[s] == v.starts[s + 1] || !(v.base[s] & ((1 << a.page_shift) - 1))) return 0;
+  return a.table[(long long)s * a.width + (v.base[s] >> a.page_shift)];
+}
+DFL_DEV bool step_page_ok(const Kv4StepArgs& a, int page) { return page >= 0 && page < a.n_pages; }
 // Slot and position of new row r of sequence s.
 struct StepRow { int slot, pos; };
 DFL_DEV StepRow step_row(const Kv4StepArgs& a, const StepView& v, int s, int r) {
   const int pos = v.base[s] + (r - v.starts[s]);
   const int pg = a.table[(long long)s * a.width + (pos >> a.page_shift)];
-  const int in = pos & ((1 << a.page_shift) - 1);
-  return StepRow{pg < 0 || pg >= a.n_pages ? -1 : (pg << a.page_shift) + in, pos};
+  return StepRow{(pg << a.page_shift) + (pos & ((1 << a.page_shift) - 1)), pos};
 }
 
 // One workgroup, a thread to a sequence.  Eight sequences of up to 16 new rows: 11.1 us with the
-// offsets in memory and a wave to each sequence's pages, 5.2 so.
+// offsets in memory and a wave to each sequence's pages, 5.3 so.
 __global__ __launch_bounds__(1024) void kv4_step_one_kernel(Kv4StepArgs a) {
   __shared__ Sum3 lds[16];
   __shared__ int offsets[4][STEP_ONE_SEQS + 1];
@@ -119,28 +142,42 @@ __global__ __launch_bounds__(1024) void kv4_step_one_kernel(Kv4StepArgs a) {
   const int n_free = *a.n_free;
   Sum3 all;
   const Sum3 in = block_scan3(Sum3{q.freed, q.taken, q.grow}, lds, all);
-  const int err = step_error(a, __syncthreads_or(bad), all, n_free);
-  if (s < a.n_seq) {
-    v.base[s] = q.keep;
-    v.f_at[s] = (int)(in.a - q.freed);
-    v.t_at[s] = (int)(in.b - q.taken);
-    a.starts[s] = v.starts[s] = err ? 0 : (int)(in.c - q.grow);
+  int err = step_error(a, __syncthreads_or(bad), all, n_free);
+  if (!err) {
+    if (s < a.n_seq) {
+      v.base[s] = q.keep;
+      v.f_at[s] = (int)(in.a - q.freed);
+      v.t_at[s] = (int)(in.b - q.taken);
+      v.starts[s] = (int)(in.c - q.grow);
+    }
+    if (s == 0) v.starts[a.n_seq] = (int)all.c;
+    const int freed = (int)all.a, taken = (int)all.b, moves = max(freed, taken), top = n_free + freed - 1;
+    __syncthreads();
+    const int kept = s < a.n_seq ? step_kept(a, v, s) : 0;
+    const StepMove m = step_look(a, v, s, freed, taken, top, false);
+    bool ok = step_page_ok(a, kept) && step_page_ok(a, m.page);
+    for (int i = s + nt; i < moves; i += nt) {   // (the first is in registers)
+      const int page = step_look(a, v, i, freed, taken, top, false).page;
+      ok = step_page_ok(a, page) && ok;
+      if (i < freed) a.free_pages[top - i] = page;
+    }
+    if (__syncthreads_or(!ok)) {
+      err = KV4_ERR_PAGE;
+      for (int i = s + nt; i < freed; i += nt) a.free_pages[top - i] = -1;
+    } else {
+      step_move(a, m, s, top);
+      for (int i = s + nt; i < moves; i += nt) step_move(a, step_look(a, v, i, freed, taken, top, true), i, top);
+      if (s < a.n_seq) a.lens[s] = q.keep + q.grow;
+      if (s == 0) *a.n_free = (int)(n_free + all.a - all.b);
+      __syncthreads();
+    }
   }
+  if (s < a.n_seq) a.starts[s] = err ? 0 : v.starts[s];
   if (s == 0) {
     a.starts[a.n_seq] = err ? 0 : (int)all.c;
     if (err) atomicOr(a.err, err);
-    else *a.n_free = (int)(n_free + all.a - all.b);
   }
   const int rows = err ? 0 : (int)all.c;
-  if (!err) {
-    const int top = (int)(n_free + all.a) - 1;
-    __syncthreads();
-    for (int i = s; i < all.a; i += nt) step_free(a, v, i, top);
-    __syncthreads();
-    for (int i = s; i < all.b; i += nt) step_take(a, v, i, top);
-    if (s < a.n_seq) a.lens[s] = q.keep + q.grow;
-    __syncthreads();
-  }
   for (int r = s; r < a.max_rows; r += nt) {
     StepRow x{-1, -1};
     if (r < rows) x = step_row(a, v, step_search(v.starts, a.n_seq, r), r);
@@ -149,10 +186,10 @@ __global__ __launch_bounds__(1024) void kv4_step_one_kernel(Kv4StepArgs a) {
   }
 }
 
-// The same in launches.  scratch: error, pages put back and taken, free pages before; then the
-// offsets but for the rows', which are a.starts.
+// The same in launches.  scratch: the scan's error, pages put back and taken, free pages before, the
+// check's error; then the offsets but for the rows', which are a.starts.
 DFL_DEV StepView step_view(const Kv4StepArgs& a) {
-  return StepView{a.scratch + 4, a.scratch + 4 + a.n_seq, a.scratch + 4 + 2 * a.n_seq, a.starts};
+  return StepView{a.scratch + 5, a.scratch + 5 + a.n_seq, a.scratch + 5 + 2 * a.n_seq, a.starts};
 }
 __global__ __launch_bounds__(1024) void kv4_step_scan_kernel(Kv4StepArgs a) {
   __shared__ Sum3 lds[16];
@@ -176,30 +213,46 @@ __global__ __launch_bounds__(1024) void kv4_step_scan_kernel(Kv4StepArgs a) {
   }
   const int n_free = *a.n_free;
   const int err = step_error(a, __syncthreads_or(bad), all, n_free);
-  if (err)   // no rows
-    for (int s = threadIdx.x; s < a.n_seq; s += nt) v.starts[s] = 0;
   if (threadIdx.x == 0) {
-    v.starts[a.n_seq] = err ? 0 : (int)all.c;
+    v.starts[a.n_seq] = (int)all.c;
     a.scratch[0] = err;
     a.scratch[1] = (int)all.a;
     a.scratch[2] = (int)all.b;
     a.scratch[3] = n_free;
+    a.scratch[4] = 0;
     if (err) atomicOr(a.err, err);
   }
 }
-__global__ __launch_bounds__(256) void kv4_step_free_kernel(Kv4StepArgs a) {
+__global__ __launch_bounds__(256) void kv4_step_check_kernel(Kv4StepArgs a) {
   if (a.scratch[0]) return;
   const StepView v = step_view(a);
-  const int n = a.scratch[1], top = a.scratch[3] + n - 1;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) step_free(a, v, i, top);
+  const int n_free = a.scratch[3], freed = a.scratch[1], taken = a.scratch[2], top = n_free + freed - 1;
+  const int t = blockIdx.x * 256 + threadIdx.x, nt = gridDim.x * 256;
+  bool ok = true;
+  for (int s = t; s < a.n_seq; s += nt) ok = step_page_ok(a, step_kept(a, v, s)) && ok;
+  for (int i = t; i < max(freed, taken); i += nt) {
+    const int page = step_look(a, v, i, freed, taken, top, false).page;
+    ok = step_page_ok(a, page) && ok;
+    if (i < freed) a.free_pages[top - i] = page;
+  }
+  if (!ok) {
+    atomicOr(a.scratch + 4, KV4_ERR_PAGE);
+    atomicOr(a.err, KV4_ERR_PAGE);
+  }
 }
-__global__ __launch_bounds__(256) void kv4_step_take_kernel(Kv4StepArgs a) {
-  if (a.scratch[0]) return;
+__global__ __launch_bounds__(256) void kv4_step_move_kernel(Kv4StepArgs a) {
   const StepView v = step_view(a);
-  const int n = a.scratch[2], top = a.scratch[3] + a.scratch[1] - 1, t = blockIdx.x * 256 + threadIdx.x;
-  for (int i = t; i < n; i += gridDim.x * 256) step_take(a, v, i, top);
-  for (int s = t; s < a.n_seq; s += gridDim.x * 256) a.lens[s] = v.base[s] + (v.starts[s + 1] - v.starts[s]);
-  if (t == 0) *a.n_free = a.scratch[3] + a.scratch[1] - n;
+  const int n_free = a.scratch[3], freed = a.scratch[1], taken = a.scratch[2], top = n_free + freed - 1;
+  const int t = blockIdx.x * 256 + threadIdx.x, nt = gridDim.x * 256;
+  if (a.scratch[0] | a.scratch[4]) {   // no rows, and the stack as it was
+    for (int s = t; s <= a.n_seq; s += nt) v.starts[s] = 0;
+    if (!a.scratch[0])
+      for (int i = t; i < freed; i += nt) a.free_pages[top - i] = -1;
+    return;
+  }
+  for (int i = t; i < max(freed, taken); i += nt) step_move(a, step_look(a, v, i, freed, taken, top, true), i, top);
+  for (int s = t; s < a.n_seq; s += nt) a.lens[s] = v.base[s] + (v.starts[s + 1] - v.starts[s]);
+  if (t == 0) *a.n_free = n_free + freed - taken;
 }
 // 1024 rows a workgroup, 4 a thread; the sequences of the first and the last are found first, 64
 // places at a time, those between them are few.  Two million rows of 1024 sequences: 17 us with a
@@ -1495,8 +1548,8 @@ void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st) {
   // (what a step moves is known on the device alone: at most the pool's pages)
   const dim3 pages(min(1024, (max(a.n_pages, a.n_seq) + 255) / 256)), block(256);
   hipLaunchKernelGGL(kv4_step_scan_kernel, dim3(1), dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(kv4_step_free_kernel, pages, block, 0, st, a);
-  hipLaunchKernelGGL(kv4_step_take_kernel, pages, block, 0, st, a);
+  hipLaunchKernelGGL(kv4_step_check_kernel, pages, block, 0, st, a);
+  hipLaunchKernelGGL(kv4_step_move_kernel, pages, block, 0, st, a);
   if (a.max_rows > 0)
     hipLaunchKernelGGL(kv4_step_rows_kernel, dim3(min(65536, a.max_rows / STEP_ROWS + 1)), block, 0, st, a);
 }

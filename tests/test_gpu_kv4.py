@@ -204,6 +204,66 @@ def test_a_step_that_cannot_be_done_changes_nothing(n_seq):
     compare_plan(c, plan, c.step(grow=[9] * n_seq), plan.step([9] * n_seq, [33] * n_seq, 9 * n_seq)[0])
 
 
+def state(c):
+    return [t.clone() for t in (c.lens, c.table, c.free, c.n_free)]
+
+
+@pytest.mark.parametrize("n_seq,spare", [(4, 0), (70, 0), (4, 9000), (1100, 0)])
+def test_a_step_that_meets_a_bad_page_changes_nothing(n_seq, spare):
+    """Page ids outside the pool where a step would put them back, take them or go on in them: the
+    step gives no rows, says so and leaves everything as it was.  (9000 spare rows, 1100 sequences:
+    the step in launches.)  Ids that the step does not touch are none of its business."""
+    from mirror_sd_amd import kv4
+    n_pages = 3 * n_seq + 4
+    c = make(n_kv_heads=1, n_pages=n_pages, max_seqs=n_seq, max_len=128, page=32)
+    plan = R.Plan(n_seq, 32, 4, n_pages)
+    lens = [40 + s % 3 * 15 for s in range(n_seq)]           # 2 or 3 pages, the last partly filled
+    c.step(grow=lens)
+    plan.step(lens, [0] * n_seq, sum(lens))
+    last = n_seq - 1
+    places = {
+        "put back": lambda: c.table[last, 1:2],
+        "taken": lambda: c.free[int(c.n_free) - 1:int(c.n_free)],
+        "last of those taken": lambda: c.free[int(c.n_free) - 2:int(c.n_free) - 1],
+        "gone on in": lambda: c.table[last, 1:2],
+    }
+    for what, place in places.items():
+        keep, grow = list(lens), [0] * n_seq
+        if what == "put back":
+            keep[last] = 31
+        elif what == "gone on in":
+            keep[last], grow[last] = 35, 3                   # rows 35 .. 37 lie in its second page
+        else:
+            grow[0], grow[last] = 64, 5                      # 2 pages for the first alone
+            assert R.pages(keep[last] + 5, 32) == R.pages(keep[last], 32)
+        rows_ = sum(grow) + spare
+        at = place()
+        good = at.clone()
+        for page in (-1, n_pages, 2**31 - 1, -2**31):
+            at.fill_(page)
+            before = state(c)
+            step = c.step(grow=grow, keep=keep, max_rows=rows_)
+            assert c.errors() == kv4.ERR_PAGE, (what, page)
+            assert step.starts.tolist() == [0] * (n_seq + 1), (what, page)
+            assert step.slots.tolist() == step.positions.tolist() == [-1] * rows_, (what, page)
+            for now, then in zip(state(c), before):
+                assert torch.equal(now, then), (what, page)
+        at.copy_(good)
+    # a bad id in the rows that stay, and below those that are taken
+    c.table[last, 0], c.free[0] = -1, n_pages
+    keep, grow = list(lens), [0] * n_seq
+    keep[0], grow[0] = 33, 2
+    step = c.step(grow=grow, keep=keep, max_rows=2 + spare)
+    assert c.errors() == 0 and int(step.slots[0]) == int(c.table[0, 1]) * 32 + 1
+    c.table[last, 0], c.free[0] = plan.table[last][0], plan.free[0]
+    plan.step(grow, keep, 2)
+    # and the next step is that of a sound cache
+    keep, grow = list(plan.lens), [5] * n_seq
+    want, err = plan.step(grow, keep, 5 * n_seq + spare)
+    compare_plan(c, plan, c.step(grow=grow, keep=keep, max_rows=5 * n_seq + spare), want)
+    assert c.errors() == err == 0
+
+
 # ------------------------------------------------------------------ attention
 
 
