@@ -108,18 +108,29 @@ class KV4Cache:
             raise ValueError(f"layer {layer} outside [0, {self.n_layers})")
         return self.pool.data_ptr() + layer * self.pool.stride(0)
 
+    @staticmethod
+    def _integers(t, what: str):
+        """A tensor of integers as they are given (a list's as 64 bits)."""
+        import torch
+        if not isinstance(t, torch.Tensor):
+            t = torch.as_tensor(t)
+            if t.numel() == 0:
+                t = t.to(torch.int32)
+        if t.dtype in (torch.uint16, torch.uint32):
+            t = t.to(torch.int64)
+        if t.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
+            raise ValueError(f"{what} must be integers, got {t.dtype}")
+        return t
+
     def _ints(self, t, n: Optional[int], what: str):
         """An int32 tensor [n] (any length if n is None) on the cache's device."""
         import torch
         if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and
                 t.device == self.device and t.is_contiguous() and (n is None or t.shape[0] == n)):
             return t
-        if not isinstance(t, torch.Tensor):
-            t = torch.as_tensor(t, dtype=torch.int32)
+        t = self._integers(t, what)
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
             raise ValueError(f"{what} must be [{'n' if n is None else n}], got {tuple(t.shape)}")
-        if t.dtype not in (torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64):
-            raise ValueError(f"{what} must be integers, got {t.dtype}")
         if t.is_cuda and t.device != self.device:
             raise ValueError(f"{what} is on {t.device}, the cache on {self.device}")
         if t.dtype == torch.int64:   # (what 32 bits do not hold stays out of range)
@@ -155,7 +166,9 @@ class KV4Cache:
         if max_rows is None:
             if isinstance(grow, torch.Tensor) and grow.is_cuda:
                 raise ValueError("max_rows is needed with lengths on the device")
-            max_rows = 0 if grow is None else max(0, int(torch.as_tensor(grow).sum()))
+            if grow is not None:
+                grow = self._integers(grow, "grow")
+            max_rows = 0 if grow is None else max(0, int(grow.sum()))
         if not 0 <= max_rows < 2**31:
             raise ValueError(f"max_rows {max_rows} out of range")
         n = self.max_seqs

@@ -140,6 +140,24 @@ def test_cache_refuses_what_does_not_fit():
         c.step(grow=[1, 2, 3], max_rows=-1)
 
 
+def test_counts_from_the_host_are_what_they_say():
+    """Lists and arrays: what 32 bits do not hold stays out of range (not its low bits, and never the
+    -1 that skips a row), fractions and truth values are refused as on the device."""
+    c = _cache()
+    lo, hi = -2**31, 2**31 - 1
+    for given, want in [([3, -1], [3, -1]), ([], []), ((5,), [5]), (range(3), [0, 1, 2]), ([2**32 + 5, -2**40], [hi, lo]),
+                        (np.array([2**32 + 5, -2**32 - 1, 7]), [hi, lo, 7]), (np.array([7, -1], np.int16), [7, -1]),
+                        (np.array([7, 2**32 - 1], np.uint32), [7, hi]), (np.array([2**16 - 1], np.uint16), [65535]),
+                        (np.zeros(0, np.int64), [])]:
+        got = c._ints(given, None, "slots")
+        assert got.dtype == torch.int32 and got.tolist() == want, given
+    for bad in ([0.5], np.array([2.0]), np.zeros(2), [True], np.array([False]), np.array([1], np.uint64)):
+        with pytest.raises(ValueError, match="integers"):
+            c._ints(bad, None, "slots")
+    with pytest.raises(ValueError, match="integers"):
+        c.step(grow=[0.5, 0.25, 0.25])
+
+
 def test_rows_are_read_in_place_where_they_can_be():
     c = _cache()
     wide = torch.zeros((5, 1024), dtype=torch.float16)
