@@ -259,10 +259,14 @@ class KV4Cache:
         return (out, lse) if return_lse else out
 
     def errors(self) -> int:
-        """Error bits since the last call (waits for the device): ERR_LENGTH a length out of
-        range, ERR_POOL too few free pages, ERR_ROWS more new rows than max_rows, ERR_SLOT a slot
-        outside the pool, ERR_PAGE pages, lengths or row ranges that do not fit each other."""
+        """Error bits since the last call (waits for the device, all its streams): ERR_LENGTH a
+        length out of range, ERR_POOL too few free pages, ERR_ROWS more new rows than max_rows,
+        ERR_SLOT a slot outside the pool, ERR_PAGE pages, lengths or row ranges that do not fit each
+        other."""
+        import torch
+        torch.cuda.synchronize(self.device)
         e = int(self._err.item())
         if e:
             self._err.zero_()
+            torch.cuda.synchronize(self.device)   # (before the bits of a later call on any stream)
         return e

@@ -724,6 +724,28 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+def test_errors_of_another_stream():
+    """errors() waits for calls on every stream, and clears before any later one."""
+    from mirror_sd_amd import kv4
+    c = make(n_pages=3)
+    x = rows(2, 2, 0)
+    bad = torch.tensor([5, 96], dtype=torch.int32, device="cuda")
+    ok = bad - 5
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                    # some 10 ms
+            c.append(x[:, 0], x[:, 1], bad)
+        assert c.errors() == kv4.ERR_SLOT
+        with torch.cuda.stream(side):
+            c.append(x[:, 0], x[:, 1], bad)
+        assert c.errors() == kv4.ERR_SLOT and c.errors() == 0
+    with torch.cuda.stream(side):
+        c.append(x[:, 0], x[:, 1], ok)
+    assert c.errors() == 0
+
+
 def test_integers_wider_than_32_bits():
     """Numbers that 32 bits do not hold are out of range, not what their low bits say."""
     from mirror_sd_amd import kv4
