@@ -314,9 +314,10 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
  * aligned; fp16 or bf16); query head h reads kv head h / (n_heads / n_kv).  Every row sees all
  * lens[s] cached rows of its sequence, or with causal != 0 row t of the sequence's m rows the
  * first lens[s] - m + t + 1.  out [n_rows][n_heads][128] (dtype of q) = softmax(scale * q.k) v;
- * lse [n_rows][n_heads] fp32 (or NULL) = log sum exp(scale * q.k).  A row that sees no key gives
- * zeros and -infinity; rows of no sequence are left as they were.  What a row does not see does
- * not reach it, whatever it holds.  Keys in a page outside the pool count as absent (bit 7).
+ * lse [n_rows][n_heads] fp32 (or NULL) = log sum exp(scale * q.k).  out may be q (q_row n_heads * 128,
+ * q_head 128) and overlaps nothing else.  A row that sees no key gives zeros and -infinity; rows of
+ * no sequence are left as they were.  What a row does not see does not reach it, whatever it holds.
+ * Keys in a page outside the pool count as absent (bit 7).
  * Weights are rounded to q's dtype, all else is held in fp32, but for queries where a sequence has
  * more than 32 rows (tokens * n_heads / n_kv) for each kv head, on average: there scale * log2(e) *
  * q, which must be finite in fp32, goes into the products in parts that hold it to 2^-13.9 of the

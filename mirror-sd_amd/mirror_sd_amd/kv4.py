@@ -228,10 +228,11 @@ class KV4Cache:
         ``lens[s]`` rows of its sequence (a draft block), or with ``causal`` row t of m the first
         ``lens[s] - m + t + 1`` (tokens, prompts).  ``scale`` defaults to 128^-0.5.
 
-        Returns [n, heads, 128] (``out`` if given: contiguous, same dtype), with ``return_lse`` also
-        the fp32 log of the sum of exponentials [n, heads], by which results over different keys
-        can be joined.  A row that sees no key gives zeros and -inf.  Rows that belong to no
-        sequence are not written (what ``out`` held, else anything)."""
+        Returns [n, heads, 128] (``out`` if given: contiguous, same dtype; q itself, or memory that
+        does not overlap it), with ``return_lse`` also the fp32 log of the sum of exponentials
+        [n, heads], by which results over different keys can be joined.  A row that sees no key
+        gives zeros and -inf.  Rows that belong to no sequence are not written (what ``out`` held,
+        else anything)."""
         import torch
         q = self._rows(q, None, "q")
         n, heads = q.shape[0], q.shape[1]
@@ -242,6 +243,11 @@ class KV4Cache:
         if out is not None and (out.shape != q.shape or out.dtype != q.dtype or
                                 out.device != self.device or not out.is_contiguous()):
             raise ValueError("out must be contiguous, of q's shape, dtype and device")
+        if out is not None and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):
+            at, size = q.data_ptr(), q.element_size()
+            past = at + size * (1 + sum((n - 1) * s for n, s in zip(q.shape, q.stride())))
+            if n and out.data_ptr() < past and at < out.data_ptr() + size * out.numel():
+                raise ValueError("out overlaps q (it may be q itself)")
         with self._guard():
             starts = self._ints(starts, self.max_seqs + 1, "starts")
             if out is None:

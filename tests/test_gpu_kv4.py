@@ -589,6 +589,19 @@ def test_queries_in_place_of_a_projection():
     check(c, q, [0, 3, 5], held, [70, 33], True, out)
 
 
+@pytest.mark.parametrize("q_rows,heads", [(1, 4), (5, 8), (30, 12)])
+def test_results_in_the_queries_place(q_rows, heads):
+    c = make(max_seqs=2, n_pages=80, max_len=1500)
+    fill(c, [1400, 33], 5, torch.float16)
+    q = queries(2 * q_rows, heads, 0, torch.float16)
+    starts = [0, q_rows, 2 * q_rows]
+    want = c.attend(q, starts, causal=True)
+    buf = torch.cat((q, q))
+    assert torch.equal(c.attend(buf[:2 * q_rows], starts, causal=True, out=buf[2 * q_rows:]), want)   # side by side
+    assert torch.equal(buf[:2 * q_rows], q)
+    assert c.attend(q, starts, causal=True, out=q) is q and torch.equal(q, want)
+
+
 # ------------------------------------------------------------------ together
 
 

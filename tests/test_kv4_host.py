@@ -158,6 +158,16 @@ def test_counts_from_the_host_are_what_they_say():
         c.step(grow=[0.5, 0.25, 0.25])
 
 
+def test_results_over_queries_that_are_still_read_are_refused():
+    c = _cache()
+    starts = torch.zeros(4, dtype=torch.int32)
+    buf = torch.zeros((9, 6, 128), dtype=torch.float16)
+    for q, out in [(buf[:4], buf[1:5]), (buf[3:7], buf[:4]), (buf[:8:2], buf[4:8]),
+                   (buf.view(9, 768)[:, :512].unflatten(1, (4, 128)), buf.view(-1)[512:512 + 9 * 512].view(9, 4, 128)[:9])]:
+        with pytest.raises(ValueError, match="overlap"):
+            c.attend(q, starts, out=out)
+
+
 def test_rows_are_read_in_place_where_they_can_be():
     c = _cache()
     wide = torch.zeros((5, 1024), dtype=torch.float16)
