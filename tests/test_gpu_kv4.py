@@ -394,6 +394,89 @@ def test_all_workers_share_units(q_rows, heads, dtype):
     assert c.errors() == 0
 
 
+def spare_rows(n_rows, n_seq, ratio, tile):
+    """Rows of no sequence behind n_rows, so that the call takes tiles of `tile` rows."""
+    most = {16: 16, 32: 32, 128: 1 << 20}[tile] * n_seq // ratio
+    least = {16: 1, 32: 16 * n_seq // ratio + 1, 128: 32 * n_seq // ratio + 1}[tile]
+    assert n_rows <= most, "the rows alone take larger tiles"
+    return max(0, least - n_rows)
+
+
+def many(n_seq, kind):
+    """Rows and lengths of n_seq sequences, most of them idle unless kind is "all"."""
+    rng = np.random.default_rng(n_seq)
+    lens = rng.integers(0, 90, n_seq)
+    lens[::17] = rng.integers(90, 1200, len(lens[::17]))
+    seams = [i for i in (0, 62, 63, 64, 65, 127, 128, 129, n_seq - 1) if i < n_seq]
+    if kind == "all":
+        on = np.arange(n_seq)
+    elif kind == "seams":
+        on = np.array(seams)
+    elif kind == "ends":                                    # 64 and more without rows between them
+        on = np.array([0, n_seq - 1])
+    else:
+        on = np.array([n_seq - 1])
+    m = np.zeros(n_seq, int)
+    m[on] = rng.integers(1, 4, len(on))
+    lens[n_seq - 1] = 700
+    return m, lens
+
+
+@pytest.mark.parametrize("tile", [16, 32, 128])
+@pytest.mark.parametrize("n_seq,kind", [(65, "all"), (65, "last"), (130, "seams"), (130, "ends"), (200, "all"),
+                                        (200, "last"), (1000, "seams"), (1000, "ends"), (1000, "all")])
+def test_more_than_64_sequences(n_seq, kind, tile):
+    """Work over more sequences than a wave looks at once, idle ones at the seams of 64 and whole 64s
+    of them between; the tile size is forced by rows of no sequence, which stay as they were."""
+    from mirror_sd_amd import kv4
+    m, lens = many(n_seq, kind)
+    heads, kv = 4, 2
+    c = make(n_kv_heads=kv, max_seqs=n_seq, max_len=1216, page=32, n_pages=int(sum(-(-lens // 32))) + 1)
+    _, held, _ = fill(c, lens.tolist(), n_seq, torch.bfloat16)
+    starts = np.concatenate(([0], np.cumsum(m))).tolist()
+    n = starts[-1] + spare_rows(starts[-1], n_seq, heads // kv, tile)
+    q = queries(n, heads, 1, torch.bfloat16)
+    for causal in (False, True):
+        out, lse = c.attend(q, starts, causal=causal, out=torch.full_like(q, 7.0), return_lse=True)
+        check(c, q, starts, held, lens.tolist(), causal, out, lse)
+        assert (out[starts[-1]:] == 7.0).all()
+    assert c.errors() == 0
+    # a length and a row range that do not fit, past the first 64: those sequences have no rows
+    bad = n_seq - 1
+    a = starts[bad]
+    for field in ("lens", "starts"):
+        st, keep = list(starts), c.lens.clone()
+        if field == "lens":
+            c.lens[bad] = 1217
+        else:
+            st[n_seq] = n + 1
+        got = c.attend(q, st, causal=True, out=torch.full_like(q, 7.0))
+        assert c.errors() == kv4.ERR_PAGE and (got[a:] == 7.0).all(), field
+        check(c, q, starts[:n_seq] + [a], held, lens.tolist(), True, got)
+        c.lens.copy_(keep)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("tile,heads,kv,n_seq,m,n", [
+    (16, 16, 2, 140, 141, 170), (32, 8, 1, 140, 421, 430), (128, 8, 1, 1, 1100, 1100), (128, 16, 2, 2, 1061, 1300)])
+def test_more_than_64_tiles(tile, heads, kv, n_seq, m, n, dtype):
+    """A sequence of more tiles than a wave looks at once, an odd number of rows in the last of
+    them, between sequences of a row."""
+    lens = [5 + s % 40 for s in range(n_seq)]
+    rows_ = [1] * n_seq
+    at = n_seq // 2
+    lens[at], rows_[at] = n, m
+    assert -(-m * heads // kv // tile) > 64
+    c = make(n_kv_heads=kv, max_seqs=n_seq, max_len=1312, page=32, n_pages=sum(R.pages(l, 32) for l in lens))
+    _, held, _ = fill(c, lens, n, DT[dtype])
+    starts = np.concatenate(([0], np.cumsum(rows_))).tolist()
+    q = queries(starts[-1] + spare_rows(starts[-1], n_seq, heads // kv, tile), heads, 1, DT[dtype])
+    for causal in (False, True):
+        out, lse = c.attend(q, starts, causal=causal, return_lse=True)
+        check(c, q, starts, held, lens, causal, out, lse)
+    assert c.errors() == 0
+
+
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
 def test_extreme_magnitudes(q_rows, heads):
     """Keys of 2^90 under queries of 2^-88 (and the other way round), values of 2^100: powers of two
