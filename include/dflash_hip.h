@@ -318,12 +318,16 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
  * q_head 128) and overlaps nothing else.  A row that sees no key gives zeros and -infinity; rows of
  * no sequence are left as they were.  What a row does not see does not reach it, whatever it holds.
  * Keys in a page outside the pool count as absent (bit 7).
- * Weights are rounded to q's dtype, all else is held in fp32, but for queries where a sequence has
- * more than 32 rows (tokens * n_heads / n_kv) for each kv head, on average: there scale * log2(e) *
- * q, which must be finite in fp32, goes into the products in parts that hold it to 2^-13.9 of the
- * largest of its 32 values (2^-129 if that is more).  With fp16 queries, cached values beyond +-131008 read as infinities
- * (keys and values of up to 32 rows, values of more).  ws: dfl_kv4_attend_ws(...) bytes for the same arguments,
- * 16-byte aligned, any content, not shared with a call that may run at the same time. */
+ * Weights are rounded to q's dtype; logits, sums and states are fp32.  Which of two kernels runs
+ * follows from the sizes alone.  Up to 32 rows for each kv head and sequence (n_rows * n_heads / n_kv
+ * / min(n_seq, n_rows), with all rows and sequences of the call, idle or not) queries and keys go
+ * into the products as they are.  Past that, scale * log2(e) * q, which must be finite in fp32, goes
+ * in as three parts that hold a value to 2^-13.9 of the largest of its group of 32 (2^-129 if that is
+ * more): within half a step of fp16 (2^-11 of a value) for values down to 1/7 of that largest, of
+ * bf16 (2^-8) down to 1/59; smaller ones lose bits that q gave.  With fp16 queries cached values (V,
+ * not keys) beyond +-131008 read as infinities, and are rounded to multiples of 2^-23.  Keys of a
+ * group that is below 2^-124 may count as zero.  ws: dfl_kv4_attend_ws(...) bytes for the same
+ * arguments, 16-byte aligned, any content, not shared with a call that may run at the same time. */
 typedef struct dfl_kv4_attn {
   const void* q;
   void* out;

@@ -442,6 +442,9 @@ template <> struct Mat<half_t> {
   // Codes convert to half their value: a group whose largest fp16 value is above 3.5 * 2^14 holds
   // 2^16, past fp16's range.  (The product keeps the exponent 255 of NaN.)
   static constexpr float kUnit = 0.5f;
+  // Whether codes of a group with exponent byte b, halved, may not be numbers of fp16 (those of 105,
+  // down to 2^-24, to 141, up to 49152, are; groups of zeros have 0, which stands for 2^-127).
+  static DFL_DEV bool past(uint32_t b) { return (b - 105u > 141u - 105u) & (b != 0); }
   typedef half8_t v8;
   typedef half2_t v2;
   static DFL_DEV floatx4 mfma(v8 a, v8 b, floatx4 c) {
@@ -463,6 +466,7 @@ template <> struct Mat<half_t> {
 };
 template <> struct Mat<bf16_t> {
   static constexpr float kUnit = 1.f;
+  static DFL_DEV bool past(uint32_t) { return false; }   // (all of them are bf16's)
   typedef bf16x8_t v8;
   typedef bf16x2_t v2;
   static DFL_DEV floatx4 mfma(v8 a, v8 b, floatx4 c) {
@@ -813,20 +817,53 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
           }
         }
       }
-      const float sk0 = M::kUnit * exponent(s4 & 255u), sk1 = M::kUnit * exponent((s4 >> 8) & 255u);
+      const uint32_t e0 = s4 & 255u, e1 = (s4 >> 8) & 255u;
       const float sv0 = M::kUnit * exponent((s4 >> 16) & 255u), sv1 = M::kUnit * exponent(s4 >> 24);
       floatx4 sa[NT], sb[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) sa[n] = sb[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
-      static_for<0, 4>([&](auto step) {
-        constexpr int st = step;
-        const v8 f0 = M::dequant(k0[st], sk0), f1 = M::dequant(k1[st], sk1);
+      // Keys past fp16's range, in a cache that was filled from bf16 or fp32: as bf16, which holds
+      // them, against Q in two parts of bf16, which hold every fp16 value.  To see that there are none
+      // costs, us: eight blocks of 8 rows 26.3 for 25.8, one token over 500 keys 10.6 for 10.3 (code);
+      // this path for all blocks 27.7 and 10.9.
+      const bool wide = __ballot(M::past(e0) | M::past(e1)) != 0;
+      if (__builtin_expect(wide, 0)) {
+        typedef Mat<bf16_t> W;
+        static_for<0, 4>([&](auto step) {
+          constexpr int st = step;
+          const bf16x8_t f0 = W::dequant(k0[st], exponent(e0)), f1 = W::dequant(k1[st], exponent(e1));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            u32x4 qw = __builtin_bit_cast(u32x4, qf[n][st]);
+            asm volatile("" : "+v"(qw));   // (made here, not kept over the loop)
+            const v8 x = __builtin_bit_cast(v8, qw);
+            bf16x8_t hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              hi[j] = (bf16_t)(float)x[j];
+              lo[j] = (bf16_t)((float)x[j] - (float)hi[j]);
+            }
+            sa[n] = W::mfma(f0, hi, W::mfma(f0, lo, sa[n]));
+            sb[n] = W::mfma(f1, hi, W::mfma(f1, lo, sb[n]));
+          }
+        });
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          sa[n] = M::mfma(f0, qf[n][st], sa[n]);
-          sb[n] = M::mfma(f1, qf[n][st], sb[n]);
+          sa[n] *= M::kUnit;
+          sb[n] *= M::kUnit;
         }
-      });
+      } else {
+        const float sk0 = M::kUnit * exponent(e0), sk1 = M::kUnit * exponent(e1);
+        static_for<0, 4>([&](auto step) {
+          constexpr int st = step;
+          const v8 f0 = M::dequant(k0[st], sk0), f1 = M::dequant(k1[st], sk1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            sa[n] = M::mfma(f0, qf[n][st], sa[n]);
+            sb[n] = M::mfma(f1, qf[n][st], sb[n]);
+          }
+        });
+      }
       __builtin_amdgcn_sched_barrier(0);   // (fewer operands in flight: 168 registers)
       static_for<0, 4>([&](auto step) {
         constexpr int st = step;

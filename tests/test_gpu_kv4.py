@@ -506,6 +506,39 @@ def test_extreme_magnitudes(q_rows, heads):
 
 
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+@pytest.mark.parametrize("up,down,scale", [(20, -18, None), (30, -20, 2.0 ** -11), (-26, 12, 1400.0), (-60, 12, 2.0 ** 48 / 11),
+                                           (15, -14, None), (-20, 8, 300.0)])
+def test_keys_past_the_range_of_fp16_queries(q_rows, heads, up, down, scale):
+    """Keys that fp16 does not hold (the cache was filled from bf16) under fp16 queries: they weigh as
+    they are, whatever the tile, all of them or the values of one group of 32 in some of the rows."""
+    lens = [77, 300]
+    starts = [0, q_rows, 2 * q_rows]
+    scale = 128 ** -0.5 if scale is None else scale
+    for part in (slice(0, 128), slice(32, 64)):
+        c = make(max_seqs=2, n_pages=40, page=32, max_len=512)
+        step = c.step(grow=lens)
+        x = rows(sum(lens), 2, 8, torch.bfloat16)
+        q = queries(2 * q_rows, heads, 6, torch.float16)
+        if part.stop < 128:                                  # the other groups' logits stay small
+            x[:, 0] *= 2.0 ** -4 * min(1.0, 128 ** -0.5 / scale)
+            x[::3, 0, :, part] = 0                           # (groups of zeros, with an exponent of zero)
+        x[:, 0, :, part] *= 2.0 ** up
+        q[:, :, part] *= 2.0 ** down
+        assert torch.isfinite(q).all()
+        c.append(x[:, 0], x[:, 1], step.slots)
+        held = R.values(x.double().cpu().numpy())
+        out, lse = c.attend(q, starts, causal=True, scale=scale, return_lse=True)
+        check(c, q, starts, held, lens, True, out, lse, scale=scale)
+    # NaN keys among them
+    x[77 + 200, 0, 1, 40] = float("nan")
+    c.append(x[:, 0], x[:, 1], step.slots)
+    again = c.attend(q, starts, causal=True, scale=scale)
+    assert torch.equal(again[:q_rows], out[:q_rows]) and torch.isnan(again[q_rows:, heads // 2:]).all()
+    assert torch.equal(again[q_rows:, :heads // 2], out[q_rows:, :heads // 2])
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
 def test_all_keys_absent(q_rows, heads):
     """A sequence all of whose pages are outside the pool is one without keys, however it is cut."""
     from mirror_sd_amd import kv4
