@@ -442,6 +442,8 @@ template <> struct Mat<half_t> {
   // Codes convert to half their value: a group whose largest fp16 value is above 3.5 * 2^14 holds
   // 2^16, past fp16's range.  (The product keeps the exponent 255 of NaN.)
   static constexpr float kUnit = 0.5f;
+  static constexpr uint32_t kVNan = 142;   // (the largest code is 4 or 6: halved, 2^16 or more)
+  static constexpr float kVUp = 0x1p113f;  // 2^(255 - kVNan)
   // Whether codes of a group with exponent byte b, halved, may not be numbers of fp16 (those of 105,
   // down to 2^-24, to 141, up to 49152, are; groups of zeros have 0, which stands for 2^-127).
   static DFL_DEV bool past(uint32_t b) { return (b - 105u > 141u - 105u) & (b != 0); }
@@ -466,6 +468,8 @@ template <> struct Mat<half_t> {
 };
 template <> struct Mat<bf16_t> {
   static constexpr float kUnit = 1.f;
+  static constexpr uint32_t kVNan = 253;   // (2^128 or more)
+  static constexpr float kVUp = 0x1p2f;
   static DFL_DEV bool past(uint32_t) { return false; }   // (all of them are bf16's)
   typedef bf16x8_t v8;
   typedef bf16x2_t v2;
@@ -497,6 +501,13 @@ DFL_DEV typename Mat<T>::v8 read_vt(const unsigned char* lo, const unsigned char
   return __builtin_bit_cast(typename Mat<T>::v8, (short8_t){a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w});
 }
 DFL_DEV float exponent(uint32_t b) { return __uint_as_float(b << 23); }
+// What V converts with.  A group of exponent byte M::kVNan or more has a value past the type's range:
+// it is NaN as a whole, so that its infinity does not reach rows that do not see it, as 0 * infinity
+// (where some row does not, groups that are NaN are left out and set by hand).
+template <typename M>
+DFL_DEV float v_unit(uint32_t b) {
+  return exponent(b) * M::kVUp * (M::kUnit / M::kVUp);
+}
 
 // An int that no kernel writes while this one runs, at a uniform address: a scalar load.
 DFL_DEV int load_const(const int* p) {
@@ -798,7 +809,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
         // that does not see them, as 0 * NaN): zero codes; the rows that do see one are set here
         const int lim = page < 0 ? 0 : sq.len;
         const bool gone0 = kbase + i >= lim, gone1 = kbase + 16 + i >= lim;
-        const bool nan0 = !gone0 && ((s4 >> 16) & 255) == 255, nan1 = !gone1 && (s4 >> 24) == 255;
+        const bool nan0 = !gone0 && ((s4 >> 16) & 255) >= M::kVNan, nan1 = !gone1 && (s4 >> 24) >= M::kVNan;
         if (gone0 || nan0) { v0 = (u32x4){0, 0, 0, 0}; s4 &= 0xff00ffffu; }
         if (gone1 || nan1) { v1 = (u32x4){0, 0, 0, 0}; s4 &= 0x00ffffffu; }
         const float nan = __builtin_nanf("");
@@ -818,7 +829,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
         }
       }
       const uint32_t e0 = s4 & 255u, e1 = (s4 >> 8) & 255u;
-      const float sv0 = M::kUnit * exponent((s4 >> 16) & 255u), sv1 = M::kUnit * exponent(s4 >> 24);
+      const float sv0 = v_unit<M>((s4 >> 16) & 255u), sv1 = v_unit<M>(s4 >> 24);
       floatx4 sa[NT], sb[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) sa[n] = sb[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
@@ -1257,7 +1268,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
     auto mask_v = [&](int b) __attribute__((always_inline)) {
       if (__builtin_expect(b + 2 > full, 0)) {
         const bool gone = absent(b + vu);
-        if (ve == 255 || gone || (b + vu) * KV4_KEYS + (lane_again() & 31) >= sq.len) {
+        if (ve >= M::kVNan || gone || (b + vu) * KV4_KEYS + (lane_again() & 31) >= sq.len) {
           ve = 0;
           vc = (u32x4){0, 0, 0, 0};
         }
@@ -1266,7 +1277,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
     auto convert_v = [&](int b, int to) __attribute__((always_inline)) {
       mask_v(b);
       unsigned char* at = vbuf + (2 * to + vu) * VTILE + 128 * vj + vwrite;
-      const float unit = M::kUnit * exponent(ve);
+      const float unit = v_unit<M>(ve);
       static_for<0, 4>([&](auto word) {
         constexpr int w = word;
         *reinterpret_cast<v8*>(at + 16 * w) = M::dequant(vc[w], unit);
@@ -1339,7 +1350,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
           const int l = lane_again(), i = l & 31, h = l >> 5;
           const bool there0 = !gone0 && kbase + i < sq.len;
           const bool there1 = !gone1 && kbase + KV4_KEYS + i < sq.len;
-          auto nan_at = [&](int at) { return kb[at + 2] == 255; };
+          auto nan_at = [&](int at) { return kb[at + 2] >= M::kVNan; };
           const bool n0 = there0 && nan_at(0), n1 = there0 && nan_at(128);
           const bool n2 = there1 && nan_at(KV4_BLOCK), n3 = there1 && nan_at(KV4_BLOCK + 128);
           if (__ballot(n0 || n1 || n2 || n3)) {

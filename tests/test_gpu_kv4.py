@@ -539,6 +539,69 @@ def test_keys_past_the_range_of_fp16_queries(q_rows, heads, up, down, scale):
 
 
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+def test_values_past_the_range_of_fp16_queries(q_rows, heads):
+    """Small values are rounded to multiples of 2^-23: each is off by 2^-24 at most, and so is their
+    mean."""
+    lens = [77, 300]
+    starts = [0, q_rows, 2 * q_rows]
+    q = queries(2 * q_rows, heads, 6, torch.float16)
+    for e in (-18, -21, -26, -40):
+        c = make(max_seqs=2, n_pages=40, page=32, max_len=512)
+        step = c.step(grow=lens)
+        x = rows(sum(lens), 2, 8, torch.bfloat16)
+        x[:, 1] *= 2.0 ** e
+        c.append(x[:, 0], x[:, 1], step.slots)
+        held = R.values(x.double().cpu().numpy())
+        out = c.attend(q, starts, causal=True)
+        for s in range(2):
+            kv = held[77 * s:77 + 300 * s]
+            a, b = starts[s], starts[s + 1]
+            o, l, mass, size = R.attend(q[a:b].double().cpu().numpy(), kv[:, 0], kv[:, 1], True, 128 ** -0.5)
+            tol, _ = R.attend_tolerance(o, l, mass, size, lens[s], 2.0 ** -11)
+            assert (np.abs(out[a:b].double().cpu().numpy() - o) <= tol + 2.0 ** -24).all(), e
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+@pytest.mark.parametrize("dtype,most,past", [("fp16", 114688.0, 115712.0), ("bf16", 2.95e38, 3.0e38)])
+def test_largest_values_of_the_query_type(q_rows, heads, dtype, most, past):
+    """Values up to 7 * 2^14 (fp16 queries; 7 * 2^125 with bf16) count; a group of 32 with one past that
+    is NaN for the rows that see it, and reaches no other."""
+    lens = [77, 300]
+    starts = [0, q_rows, 2 * q_rows]
+    q = queries(2 * q_rows, heads, 6, DT[dtype])
+    c = make(max_seqs=2, n_pages=40, page=32, max_len=512)
+    step = c.step(grow=lens)
+    x = rows(sum(lens), 2, 8, torch.bfloat16)
+    hidden = 77 + 298 if q_rows > 1 else 40                  # seen by the last two rows, or (page by page) by all
+    x[hidden, 1, 1, 5] = most
+    x[3, 1, 0, 127] = -most                                  # in a block that all rows see
+    c.append(x[:, 0], x[:, 1], step.slots)
+    held = R.values(x.double().cpu().numpy())
+    good, lse = c.attend(q, starts, causal=True, return_lse=True)
+    for s in range(2):
+        kv = held[77 * s:77 + 300 * s]
+        a, b = starts[s], starts[s + 1]
+        o, l, mass, size = R.attend(q[a:b].double().cpu().numpy(), kv[:, 0], kv[:, 1], True, 128 ** -0.5)
+        tol, _ = R.attend_tolerance(o, l, mass, size, lens[s], torch.finfo(DT[dtype]).eps / 2)
+        fits = np.abs(o) <= (65000 if dtype == "fp16" else 2.0 ** 112 / 300)
+        assert (np.abs(good[a:b].double().cpu().numpy() - o) <= tol)[fits].all() and fits.mean() > 0.9
+    x[hidden, 1, 1, 5], x[3, 1, 0, 127] = past, -past
+    c.append(x[:, 0], x[:, 1], step.slots)
+    assert torch.isfinite(x.float()).all()
+    again, lse2 = c.attend(q, starts, causal=True, return_lse=True)
+    nan = torch.zeros(again.shape, dtype=torch.bool, device="cuda")
+    nan[:q_rows, :heads // 2, 96:] = True
+    if q_rows > 1:
+        nan[-2:, heads // 2:, :32] = True
+    else:
+        nan[:1, heads // 2:, :32] = True
+    assert torch.equal(torch.isnan(again), nan)
+    assert torch.equal(again[~nan], good[~nan]) and torch.equal(lse2, lse)
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
 def test_all_keys_absent(q_rows, heads):
     """A sequence all of whose pages are outside the pool is one without keys, however it is cut."""
     from mirror_sd_amd import kv4
