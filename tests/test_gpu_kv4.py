@@ -505,6 +505,30 @@ def test_extreme_magnitudes(q_rows, heads):
     assert c.errors() == 0
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("ratio", [20, 300])
+@pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
+def test_queries_with_outlier_channels(q_rows, heads, ratio, dtype):
+    """A channel of each group of 32 far above the rest, as norm gains leave them: within the bound of
+    the parts of 6 bits past 32 rows, and of the type alone up to there."""
+    lens = [77, 700]
+    starts = [0, q_rows, 2 * q_rows]
+    c = make(max_seqs=2, n_pages=60, page=32)
+    _, held, _ = fill(c, lens, ratio, DT[dtype])
+    q = queries(2 * q_rows, heads, 6, torch.float32) * min(1.0, 20 / ratio)
+    q[:, :, 7::32] *= ratio
+    q = q.to(DT[dtype])
+    out, lse = c.attend(q, starts, causal=True, return_lse=True)
+    check(c, q, starts, held, lens, True, out, lse)
+    # and where the rest alone decides: the channel's keys are zero
+    x = rows(sum(lens), 2, 5, DT[dtype])
+    x[:, 0, :, 7::32] = 0
+    c.step(keep=[0, 0])
+    c.append(x[:, 0], x[:, 1], c.step(grow=lens).slots)
+    out, lse = c.attend(q, starts, causal=True, return_lse=True)
+    check(c, q, starts, R.values(x.double().cpu().numpy()), lens, True, out, lse)
+
+
 @pytest.mark.parametrize("q_rows,heads", [(1, 2), (5, 8), (30, 12)])
 @pytest.mark.parametrize("up,down,scale", [(20, -18, None), (30, -20, 2.0 ** -11), (-26, 12, 1400.0), (-60, 12, 2.0 ** 48 / 11),
                                            (15, -14, None), (-20, 8, 300.0)])
