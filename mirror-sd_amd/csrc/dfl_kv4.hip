@@ -36,10 +36,15 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 // against launches, us (sequences x new rows of each; every page put back and taken again):
 //   8 x 16 5.2, 12.4;  256 x 16 11.6, 19.1;  1024 x 8 16.9, 23.3;  8 x 1024 11.3, 14.5;
 //   1024 x 32 39.5, 22.2;  64 x 512 29.3, 15.9;  8 x 4096 22.3, 14.5.
-// (Of these the check takes 0.2 in one workgroup, where a thread keeps what it has looked at in
-// registers, and 1 in launches.)
+// (Of these the check takes 0.2 in one workgroup, where a thread keeps the move that it has looked at
+// in registers, and 1 in launches.)
 
 constexpr int STEP_ONE_SEQS = 1024, STEP_ONE_ROWS = 8192;
+// Steps of one workgroup that move more pages than it has threads: a thread has STEP_N moves under
+// way at once, and STEP_L threads clear what a table gives up.  64 tables of 256 pages put back 36 us
+// (one move at once 53), 1024 of 64 61 (79); STEP_L 4, 8, 16, 64: 1024 of 8 16.5, 17.2, 18.7, 28.6,
+// one of 1000 13.9, 10.8, 9.2, 7.9.
+constexpr int STEP_N = 4, STEP_L = 16;
 
 // Sums over the workgroup's threads of three counts at once (inclusive), and their totals.
 struct Sum3 { long long a, b, c; };
@@ -87,40 +92,104 @@ DFL_DEV int step_search(const int* at, int n, int v) {
 // Offsets of all sequences: kept lengths, pages put back and taken before each (n_seq), new rows
 // before each (n_seq + 1).
 struct StepView { int *base, *f_at, *t_at, *starts; };
-// Move i of a step: page i of those put back and page i of those taken, which is the same one if
-// both are there (they have one place on the stack, `top` less i with the stack's top after all
-// are put back).
-struct StepMove {
-  int *from, *to;   // its places in the tables (null: it comes from the stack, it stays there)
-  int page;
-  bool again;       // the step puts another page into `from`
+// Moves i, i + n, .. of a step, N of them at once (the searches do not wait for each other): page i of
+// those put back and page i of those taken, which is the same one if both are there (they have one
+// place on the stack, `top` less i with the stack's top after all are put back).
+template <int N> struct StepMoves {
+  int *from[N], *to[N];   // their places in the tables (null: from the stack, it stays there)
+  int page[N];
+  bool again[N];          // the step puts another page into `from`
 };
-// on_stack: the pages put back are on the stack already.
-DFL_DEV StepMove step_look(const Kv4StepArgs& a, const StepView& v, int i, int freed, int taken, int top, bool on_stack) {
-  StepMove m{nullptr, nullptr, 0, false};
-  if (i < freed) {
-    const int s = step_search(v.f_at, a.n_seq, i), at = kv4_pages(v.base[s], a.page_shift) + (i - v.f_at[s]);
-    m.again = at < kv4_pages(v.base[s] + (v.starts[s + 1] - v.starts[s]), a.page_shift);
-    m.from = a.table + (long long)s * a.width + at;
-  }
-  if (i < freed || i < taken) m.page = m.from && !on_stack ? *m.from : a.free_pages[top - i];
-  if (i < taken) {
-    const int s = step_search(v.t_at, a.n_seq, i);
-    m.to = a.table + (long long)s * a.width + kv4_pages(v.base[s], a.page_shift) + (i - v.t_at[s]);
-  }
-  return m;
+template <int N>
+DFL_DEV void step_search(const int* at, int n_seq, int i, int n, int past, int (&s)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) s[k] = 0;
+  for (int step = n_seq > 1 ? 1 << (31 - __clz(n_seq - 1)) : 0; step; step >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int mid = min(s[k] + step, n_seq - 1);
+      if (at[mid] <= min(i + k * n, past - 1)) s[k] = mid;
+    }
 }
-DFL_DEV void step_move(const Kv4StepArgs& a, const StepMove& m, int i, int top) {
-  if (m.from && !m.again) *m.from = -1;
-  if (m.to) *m.to = m.page;
-  if (m.from || m.to) a.free_pages[top - i] = m.to ? -1 : m.page;
+// Where pages that are put back come from.
+template <int N>
+DFL_DEV void step_from(const Kv4StepArgs& a, const StepView& v, int i, int n, int freed, StepMoves<N>& m) {
+  int s[N];
+  step_search<N>(v.f_at, a.n_seq, i, n, freed, s);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = kv4_pages(v.base[s[k]], a.page_shift) + (i + k * n - v.f_at[s[k]]);
+    m.again[k] = at < kv4_pages(v.base[s[k]] + (v.starts[s[k] + 1] - v.starts[s[k]]), a.page_shift);
+    m.from[k] = i + k * n < freed ? a.table + (long long)s[k] * a.width + at : nullptr;
+  }
+}
+// Where pages that are taken go.
+template <int N>
+DFL_DEV void step_to(const Kv4StepArgs& a, const StepView& v, int i, int n, int taken, StepMoves<N>& m) {
+  int s[N];
+  step_search<N>(v.t_at, a.n_seq, i, n, taken, s);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = kv4_pages(v.base[s[k]], a.page_shift) + (i + k * n - v.t_at[s[k]]);
+    m.to[k] = i + k * n < taken ? a.table + (long long)s[k] * a.width + at : nullptr;
+  }
+}
+DFL_DEV bool step_page_ok(const Kv4StepArgs& a, int page) { return page >= 0 && page < a.n_pages; }
+// The pages, and whether all are the pool's.
+template <int N>
+DFL_DEV bool step_look(const Kv4StepArgs& a, const StepView& v, int i, int n, int freed, int taken, int top, StepMoves<N>& m) {
+  step_from<N>(a, v, i, n, freed, m);
+  bool ok = true;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    m.page[k] = m.from[k] ? *m.from[k] : i + k * n < taken ? a.free_pages[top - (i + k * n)] : 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) ok = step_page_ok(a, m.page[k]) && ok;
+  return ok;
+}
+// With the pages that are put back on the stack.
+template <int N>
+DFL_DEV bool step_put(const Kv4StepArgs& a, const StepView& v, int i, int n, int freed, int taken, int top) {
+  StepMoves<N> m;
+  const bool ok = step_look<N>(a, v, i, n, freed, taken, top, m);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (m.from[k]) a.free_pages[top - (i + k * n)] = m.page[k];
+  return ok;
+}
+template <int N>
+DFL_DEV void step_move(const Kv4StepArgs& a, int i, int n, int top, const StepMoves<N>& m) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (m.from[k] && !m.again[k]) *m.from[k] = -1;
+    if (m.to[k]) *m.to[k] = m.page[k];
+    if (m.from[k] || m.to[k]) a.free_pages[top - (i + k * n)] = m.to[k] ? -1 : m.page[k];
+  }
+}
+// After step_put: the pages that are taken, and the places that are given up.
+template <int N>
+DFL_DEV void step_take(const Kv4StepArgs& a, const StepView& v, int i, int n, int taken, int top) {
+  StepMoves<N> m;
+  step_to<N>(a, v, i, n, taken, m);
+#pragma unroll
+  for (int k = 0; k < N; ++k) m.page[k] = m.to[k] ? a.free_pages[top - (i + k * n)] : 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (m.to[k]) {
+      *m.to[k] = m.page[k];
+      a.free_pages[top - (i + k * n)] = -1;
+    }
+}
+DFL_DEV void step_clear(const Kv4StepArgs& a, const StepView& v, int i, int freed) {
+  StepMoves<1> m;
+  step_from<1>(a, v, i, 0, freed, m);
+  if (!m.again[0]) *m.from[0] = -1;
 }
 // The page that new rows of sequence s go on in; 0 if there is none.
 DFL_DEV int step_kept(const Kv4StepArgs& a, const StepView& v, int s) {
   if (v.starts[s] == v.starts[s + 1] || !(v.base[s] & ((1 << a.page_shift) - 1))) return 0;
   return a.table[(long long)s * a.width + (v.base[s] >> a.page_shift)];
 }
-DFL_DEV bool step_page_ok(const Kv4StepArgs& a, int page) { return page >= 0 && page < a.n_pages; }
 // Slot and position of new row r of sequence s.
 struct StepRow { int slot, pos; };
 DFL_DEV StepRow step_row(const Kv4StepArgs& a, const StepView& v, int s, int r) {
@@ -154,19 +223,30 @@ __global__ __launch_bounds__(1024) void kv4_step_one_kernel(Kv4StepArgs a) {
     const int freed = (int)all.a, taken = (int)all.b, moves = max(freed, taken), top = n_free + freed - 1;
     __syncthreads();
     const int kept = s < a.n_seq ? step_kept(a, v, s) : 0;
-    const StepMove m = step_look(a, v, s, freed, taken, top, false);
-    bool ok = step_page_ok(a, kept) && step_page_ok(a, m.page);
-    for (int i = s + nt; i < moves; i += nt) {   // (the first is in registers)
-      const int page = step_look(a, v, i, freed, taken, top, false).page;
-      ok = step_page_ok(a, page) && ok;
-      if (i < freed) a.free_pages[top - i] = page;
+    bool ok = true;
+    StepMoves<1> m;   // (of few moves, in registers)
+    if (moves <= nt) {
+      ok = step_look<1>(a, v, s, nt, freed, taken, top, m);
+      step_to<1>(a, v, s, nt, taken, m);
+    } else {
+      for (int i = s; i < moves; i += STEP_N * nt) ok = step_put<STEP_N>(a, v, i, nt, freed, taken, top) && ok;
     }
+    ok = step_page_ok(a, kept) && ok;
     if (__syncthreads_or(!ok)) {
       err = KV4_ERR_PAGE;
-      for (int i = s + nt; i < freed; i += nt) a.free_pages[top - i] = -1;
+      if (moves > nt)
+        for (int i = s; i < freed; i += nt) a.free_pages[top - i] = -1;
     } else {
-      step_move(a, m, s, top);
-      for (int i = s + nt; i < moves; i += nt) step_move(a, step_look(a, v, i, freed, taken, top, true), i, top);
+      if (moves <= nt) step_move<1>(a, s, nt, top, m);
+      else {
+        for (int i = s; i < taken; i += STEP_N * nt) step_take<STEP_N>(a, v, i, nt, taken, top);
+        for (int k = s / STEP_L; k < a.n_seq; k += nt / STEP_L) {   // (stores: nothing waits)
+          const int kept_k = kv4_pages(v.base[k], a.page_shift);
+          const int from = kv4_pages(v.base[k] + (v.starts[k + 1] - v.starts[k]), a.page_shift);
+          const int past = kept_k + (k + 1 < a.n_seq ? v.f_at[k + 1] : freed) - v.f_at[k];
+          for (int at = from + s % STEP_L; at < past; at += STEP_L) a.table[(long long)k * a.width + at] = -1;
+        }
+      }
       if (s < a.n_seq) a.lens[s] = q.keep + q.grow;
       if (s == 0) *a.n_free = (int)(n_free + all.a - all.b);
       __syncthreads();
@@ -230,11 +310,7 @@ __global__ __launch_bounds__(256) void kv4_step_check_kernel(Kv4StepArgs a) {
   const int t = blockIdx.x * 256 + threadIdx.x, nt = gridDim.x * 256;
   bool ok = true;
   for (int s = t; s < a.n_seq; s += nt) ok = step_page_ok(a, step_kept(a, v, s)) && ok;
-  for (int i = t; i < max(freed, taken); i += nt) {
-    const int page = step_look(a, v, i, freed, taken, top, false).page;
-    ok = step_page_ok(a, page) && ok;
-    if (i < freed) a.free_pages[top - i] = page;
-  }
+  for (int i = t; i < max(freed, taken); i += nt) ok = step_put<1>(a, v, i, nt, freed, taken, top) && ok;
   if (!ok) {
     atomicOr(a.scratch + 4, KV4_ERR_PAGE);
     atomicOr(a.err, KV4_ERR_PAGE);
@@ -250,7 +326,8 @@ __global__ __launch_bounds__(256) void kv4_step_move_kernel(Kv4StepArgs a) {
       for (int i = t; i < freed; i += nt) a.free_pages[top - i] = -1;
     return;
   }
-  for (int i = t; i < max(freed, taken); i += nt) step_move(a, step_look(a, v, i, freed, taken, top, true), i, top);
+  for (int i = t; i < taken; i += nt) step_take<1>(a, v, i, nt, taken, top);
+  for (int i = t; i < freed; i += nt) step_clear(a, v, i, freed);
   for (int s = t; s < a.n_seq; s += nt) a.lens[s] = v.base[s] + (v.starts[s + 1] - v.starts[s]);
   if (t == 0) *a.n_free = n_free + freed - taken;
 }

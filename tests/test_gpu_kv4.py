@@ -264,6 +264,37 @@ def test_a_step_that_meets_a_bad_page_changes_nothing(n_seq, spare):
     assert c.errors() == err == 0
 
 
+@pytest.mark.parametrize("n_seq", [3, 70, 1000])
+def test_steps_that_move_many_pages(n_seq):
+    """More pages than a workgroup has threads, put back and taken with few new rows; a bad id among
+    the last of them changes nothing."""
+    from mirror_sd_amd import kv4
+    rng = np.random.default_rng(n_seq)
+    width = 3000 // n_seq + 6
+    n_pages = n_seq * width + 3
+    c = make(n_kv_heads=1, n_pages=n_pages, max_seqs=n_seq, max_len=width * 32, page=32)
+    plan = R.Plan(n_seq, 32, width, n_pages)
+    full = rng.integers(width * 32 - 90, width * 32 + 1, n_seq).tolist()
+    zero = [0] * n_seq
+    for few in ((8000 // n_seq) * np.ones(n_seq, int), rng.integers(0, 8, n_seq), np.array(zero)):
+        want, err = plan.step(full, zero, sum(full))         # (in launches)
+        compare_plan(c, plan, c.step(grow=full, keep=zero), want)
+        keep = np.minimum(rng.integers(0, 100, n_seq), np.array(full))
+        few = np.minimum(few, width * 32 - keep)
+        s, at = n_seq - 1, width - 3
+        good = int(c.table[s, at])
+        c.table[s, at] = n_pages
+        before = state(c)
+        step = c.step(grow=few.tolist(), keep=keep.tolist(), max_rows=8192)
+        assert c.errors() == kv4.ERR_PAGE and step.starts.tolist() == [0] * (n_seq + 1)
+        assert int(step.slots.max()) == -1
+        assert all(torch.equal(x, y) for x, y in zip(state(c), before))
+        c.table[s, at] = good
+        want, err = plan.step(few.tolist(), keep.tolist(), 8192)
+        compare_plan(c, plan, c.step(grow=few.tolist(), keep=keep.tolist(), max_rows=8192), want)
+        assert c.errors() == err == 0
+
+
 # ------------------------------------------------------------------ attention
 
 
