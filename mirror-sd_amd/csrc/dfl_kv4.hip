@@ -708,8 +708,9 @@ struct Run : Unit {
 struct Walk { long long pos, end, per; };
 // Which worker a workgroup is.  Workgroups go to the 8 dies of the chip in turn, each with an L2 of
 // its own, and workers that follow on each other read the same keys (the tiles of a head): so
-// each die has an eighth of all places, one after the other.  (Two prompts of 4096 and 777 rows:
-// 219 us in turn, 216 so.)
+// each die has an eighth of all places, one after the other.  (In turn, and
+// so, us: one token over 500 keys 11.0, 10.6; 32 rows of 40 heads over 32800 keys 55.4, 53.6; two
+// prompts of 4096 and 777 rows 196, 190.)
 static_assert(KV4_CUS % 8 == 0, "workers in eight parts");
 DFL_DEV int worker_of(const Kv4AttnArgs& a, int workgroup) {
   return (workgroup & 7) * (a.workers >> 3) + (workgroup >> 3);
@@ -1087,8 +1088,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
 // The logits are summed onto the negative reference, so that a weight is the power of what the
 // products leave.  S^T of the next step is made between the weights of this one.
 //
-// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 210 us
-// with the merge's 15, 800 TF of their 168 GF (a large product of 16-bit matrices reaches 1210).
+// Two workgroups a CU (LDS and 256 registers).  Two prompts of 4096 and 777 rows, 32 heads: 185 to
+// 210 us by card with the merge's 15, 800 to 910 TF (a large product of 16-bit matrices reaches 1210).
 // A step of both workgroups takes 1.8 us, 3400 cycles: for each SIMD 1790 of products and 1700 of
 // vector instructions, for the CU 1900 of LDS.  No one of them is full: two waves a SIMD do not
 // fill each other's gaps, and there are no registers for a third.  Eight blocks of 32 rows over
@@ -1142,7 +1143,13 @@ DFL_DEV void lds_barrier() {
 // nearest of the numbers with 4 bits of which 7.5 is the largest: with a <= 7.5 for the largest
 // |x| = a 2^b, what p0 leaves is at most 1/4, 4 units of p1, which leaves at most 1/8, 4 units of
 // p2, which leaves at most 1/8 of its own, 2^-12 2^b.  As a > 3.75, every value is held to 2^-13.9
-// of its group's largest; fp16 Q rounded to 11 bits beforehand has up to 2^-12 of each value.
+// of its group's largest: finer than half a step of fp16 (2^-11 of a value) down to 1/7 of that
+// largest, of bf16 (2^-8) down to 1/59, and coarser for the small values beside a large one.  Under
+// fp16 queries with a channel of each group 20 to 1000 times the rest (4000 keys, logits of some 5)
+// results are off by 2.9e-4 of their norm, by 2.0e-4 if Q is held as it is, which is what rounding
+// them to fp16 takes alone; under normal queries by 2.9e-4 and 2.7e-4.  A fourth part would bring the
+// 2.9e-4 to 2.1e-4 (2^-18.9), and take eight blocks from 45.6 to 48.4 us, fp16 prompts from 190 to
+// 207: it needs the reference's registers, so that the logits begin at zero.
 typedef int int8v_t __attribute__((ext_vector_type(8)));
 typedef unsigned uint6v_t __attribute__((ext_vector_type(6)));
 typedef float float32v_t __attribute__((ext_vector_type(32)));
