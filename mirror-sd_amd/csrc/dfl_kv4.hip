@@ -518,6 +518,7 @@ template <typename T> struct Mat;
 template <> struct Mat<half_t> {
   // Codes convert to half their value: a group whose largest fp16 value is above 3.5 * 2^14 holds
   // 2^16, past fp16's range.  (The product keeps the exponent 255 of NaN.)
+  // V below 2^-21 are rounded to steps of 2^-23, half an output's smallest step off at most.
   static constexpr float kUnit = 0.5f;
   static constexpr uint32_t kVNan = 142;   // (the largest code is 4 or 6: halved, 2^16 or more)
   static constexpr float kVUp = 0x1p113f;  // 2^(255 - kVNan)

@@ -971,6 +971,105 @@ def test_another_stream():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("spare", [0, 1_200_000])
+def test_the_most_sequences(spare):
+    """65536 sequences, every third idle, the others of one key: a row's result is that key's value
+    (its weight and its sum are one number).  Then 40 keys for the last of them.  (1.2 million spare
+    rows: tiles of 32.)"""
+    n_seq = 65536
+    c = make(n_kv_heads=1, max_seqs=n_seq, max_len=64, n_pages=n_seq + 8, page=32)
+    grow = torch.ones(n_seq, dtype=torch.int32, device="cuda")
+    grow[1::3] = 0                                            # (the last, 65535, has a row)
+    n = int(grow.sum())
+    step = c.step(grow=grow, max_rows=n)
+    x = rows(n, 1, 3)
+    c.append(x[:, 0], x[:, 1], step.slots)
+    q = queries(n + spare, 1, 1, torch.float16) if spare == 0 else torch.ones((n + spare, 1, 128), dtype=torch.float16, device="cuda")
+    out = c.attend(q, step.starts, causal=True, out=torch.full_like(q, 5.0))
+    assert c.errors() == 0 and torch.equal(out[:n], c.read(step.slots)[1]) and (out[n:] == 5.0).all()
+    more = torch.zeros_like(grow)
+    more[-1] = 39
+    last = c.step(grow=more, max_rows=39)
+    y = rows(39, 1, 4)
+    c.append(y[:, 0], y[:, 1], last.slots)
+    again = c.attend(q, step.starts, causal=True)
+    assert c.errors() == 0 and torch.equal(again[:n - 1], out[:n - 1])
+    held = R.values(torch.cat((x[n - 1:], y)).double().cpu().numpy())
+    check(c, q[n - 1:n], [0, 1], held, [40], True, again[n - 1:n])
+
+
+@pytest.mark.parametrize("heads", [4, 40])
+def test_two_calls_at_once(heads):
+    """Attention over one cache from two streams, eager and replayed, while a third fills another."""
+    c, d = make(max_seqs=3, n_pages=80), make(max_seqs=3, n_pages=80)
+    fill(c, [700, 33, 900], 1, torch.float16)
+    x = rows(1500, 2, 5)
+    qs = [queries(27, heads, i, torch.float16) for i in range(2)]
+    starts = torch.tensor([0, 9, 13, 27], dtype=torch.int32, device="cuda")
+    want = [c.attend(q, starts, causal=bool(i)) for i, q in enumerate(qs)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        replayed = c.attend(qs[1], starts, causal=True)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for turn in range(20):
+        got = []
+        with torch.cuda.stream(streams[0]):
+            got += [(c.attend(qs[0], starts), want[0]) for _ in range(3)]
+        with torch.cuda.stream(streams[1]):
+            replayed.zero_()
+            g.replay()
+            got += [(c.attend(qs[1], starts, causal=True), want[1]), (replayed, want[1])]
+        with torch.cuda.stream(streams[2]):
+            slots = d.step(grow=[500, 500, 500], keep=[0, 0, 0]).slots
+            d.append(x[:, 0], x[:, 1], slots)
+        torch.cuda.synchronize()
+        for a, b in got:
+            assert torch.equal(a, b), turn
+    assert c.errors() == d.errors() == 0
+
+
+def test_more_rows_than_a_launch_has_workgroups():
+    """2.2 million rows in one call (65535 workgroups of 32 take some of them twice), as in parts."""
+    n = 2_200_003
+    c, d = (make(n_kv_heads=1, max_seqs=1, n_pages=n // 256 + 9, page=256) for _ in range(2))
+    g = torch.Generator("cuda").manual_seed(0)
+    x = torch.randn((n, 2, 1, 128), generator=g, device="cuda", dtype=torch.float16)
+    slots = torch.randperm((n // 256 + 9) * 256, generator=g, device="cuda")[:n].to(torch.int32)
+    c.append(x[:, 0], x[:, 1], slots)
+    for a, b in ((0, 1_000_000), (1_000_000, 2_097_120), (2_097_120, n)):
+        d.append(x[a:b, 0], x[a:b, 1], slots[a:b])
+    assert torch.equal(c.pool, d.pool)
+    k, v = c.read(slots)
+    for at in (0, 1_048_575, 2_097_120, n - 40):
+        want = R.values(x[at:at + 40].double().cpu().numpy())
+        same(k[at:at + 40], want[:, 0])
+        same(v[at:at + 40], want[:, 1])
+    for a, b in ((0, 1_500_000), (1_500_000, n)):
+        pk, pv = c.read(slots[a:b])
+        assert torch.equal(k[a:b], pk) and torch.equal(v[a:b], pv)
+    assert c.errors() == 0
+
+
+def test_a_step_of_70_million_rows():
+    page, lens = 256, [35_000_123, 1, 0, 35_200_000]
+    n_pages = sum(R.pages(n, page) for n in lens) + 1
+    c = make(n_kv_heads=1, n_pages=n_pages, max_seqs=4, max_len=36_000_000, page=page)
+    step = c.step(grow=lens, max_rows=sum(lens) + 77)
+    assert step.starts.tolist() == [0, 35_000_123, 35_000_124, 35_000_124, sum(lens)] and c.errors() == 0
+    assert (step.slots[sum(lens):] == -1).all() and (step.positions[sum(lens):] == -1).all()
+    at = 0
+    for s, n in enumerate(lens):
+        pos = torch.arange(n, device="cuda", dtype=torch.int32)
+        assert torch.equal(step.positions[at:at + n], pos)
+        assert torch.equal(step.slots[at:at + n], c.table[s].long()[pos.long() // page].int() * page + pos % page)
+        at += n
+    used = torch.cat([c.table[s, :R.pages(n, page)] for s, n in enumerate(lens)])
+    assert used.unique().numel() == used.numel() == n_pages - int(c.n_free) and int(used.min()) >= 0
+    c.step(keep=[0] * 4)
+    assert int(c.n_free) == n_pages and int(c.table.max()) == -1 and c.errors() == 0
+
+
 def test_errors_of_another_stream():
     """errors() waits for calls on every stream, and clears before any later one."""
     from mirror_sd_amd import kv4
