@@ -326,9 +326,8 @@ int dfl_kv4_read(const int32_t* slots, int32_t rows, int32_t n_kv, int32_t page,
  * more): within half a step of fp16 (2^-11 of a value) for values down to 1/7 of that largest, of
  * bf16 (2^-8) down to 1/59; smaller ones lose bits that q gave.  With fp16 queries cached values (V,
  * not keys) are rounded to multiples of 2^-23; a group of 32 of them with one past +-7 * 2^14 (bf16
- * queries: 7 * 2^125) reads as NaN.  Results of values past 2^112 / lens[s] may overflow.
- * Keys of a group that is below 2^-124 may count as zero.
- * ws: dfl_kv4_attend_ws(...) bytes for the same
+ * queries: 7 * 2^125) reads as NaN.  Results of values past 2^112 / lens[s] may overflow.  Keys of a
+ * group that is below 2^-124 may count as zero.  ws: dfl_kv4_attend_ws(...) bytes for the same
  * arguments, 16-byte aligned, any content, not shared with a call that may run at the same time. */
 typedef struct dfl_kv4_attn {
   const void* q;
