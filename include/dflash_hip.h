@@ -347,6 +347,47 @@ typedef struct dfl_kv4_attn {
 int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream);
 int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq);
 
+/* ---- Verification of drafted blocks (the reference's caller compares argmax ids on the host,
+ * generate.py:614-728; this is its form for sampled tokens, on the device) ----
+ *
+ * Rows starts[s] .. starts[s+1] - 1 of target [n_rows][vocab] are the target's logits behind the
+ * tokens of sequence s's block: ids [n_rows] holds the block, its first row the last verified
+ * token, the others drafted ones.  draft (or NULL) holds for each drafted row the logits that its
+ * token was drawn from (as dfl_draft_block's out_logits; a sequence's first row is not read).
+ * dtypes: 0 fp32, 1 fp16, 2 bf16; rows target_row, draft_row elements apart, aligned to their type
+ * alone.  With p the softmax of a target row divided by its sequence's temperature, q the draft's
+ * (below 1e-5 all weight is on the largest logit, the first of equals; without draft logits all of
+ * q's is on the drafted token), the token x of row t is accepted if uniforms[t] * q(x) < p(x), p
+ * that of row t - 1.  temps, draft_temps: [n_seq] device numbers, or NULL: temp, draft_temp for all.
+ * Out: accepted [n_seq] the drafted tokens accepted one after another; next_ids [n_seq] a token
+ * drawn behind them, from max(p - q, 0) after a rejection (from p where that is zero), from p
+ * after none: the first whose running sum, in the order of ids, exceeds uniforms[starts[s]] times
+ * the whole; chances [n_rows] min(1, p(x) / q(x)), 1 in a sequence's first row.
+ * The sequence's new text is its accepted tokens and next_ids; its cache keeps accepted + 1 rows of
+ * the block.  uniforms are of [0, 1).  Tests and draws are those of sums in 64 bits; chances are
+ * off by some 2^-20 (2^-16 at most).  -infinity masks a token.  A row that holds a NaN or +infinity, or nothing
+ * above -infinity, has no distribution: its test fails with chance 0, a draw that needs it gives -1.
+ * An id outside [0, vocab) has probability 0.  Sequences without rows, or whose range does not fit,
+ * get 0 accepted and -1; rows of no sequence are left as they were.  starts must ascend (else the
+ * results are any, but nothing outside the buffers is read or written).
+ * ws: dfl_verify_ws(args) bytes (its ws and ws_bytes are not looked at), 16-byte aligned, any
+ * content, not shared with a call that may run at the same time. */
+typedef struct dfl_verify_args {
+  const void *target, *draft;
+  int64_t target_row, draft_row;
+  int32_t target_dtype, draft_dtype;
+  int32_t n_rows, vocab, n_seq;
+  float temp, draft_temp;
+  const int32_t *ids, *starts;
+  const float *uniforms, *temps, *draft_temps;
+  int32_t *accepted, *next_ids;
+  float* chances;
+  void* ws;
+  int64_t ws_bytes;
+} dfl_verify_args;
+int dfl_verify(const dfl_verify_args* args, void* stream);
+int64_t dfl_verify_ws(const dfl_verify_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@
 #include "dfl_kernels.h"
 #include "dfl_check.h"
 #include "dfl_kv4.h"
+#include "dfl_verify.h"
 #include "dfl_sk_plan.h"
 #include "dfl_tile_plan.h"
 
@@ -1768,6 +1769,52 @@ int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
     return fail(DFL_EINVAL, "dfl_kv4_attend: workspace of " + std::to_string(need) + " bytes needed");
   launch_kv4_attend(a, (hipStream_t)stream);
   return check_launch("dfl_kv4_attend");
+}
+
+// ---- verification of drafted blocks: context-free entry points over dfl_verify.hip ----
+
+static VerifyArgs verify_args(const dfl_verify_args* in) {
+  VerifyArgs a{};
+  a.target = in->target;
+  a.draft = in->draft;
+  a.target_row = in->target_row;
+  a.draft_row = in->draft_row;
+  a.target_dtype = in->target_dtype;
+  a.draft_dtype = in->draft_dtype;
+  a.n_rows = in->n_rows;
+  a.vocab = in->vocab;
+  a.n_seq = in->n_seq;
+  a.ids = in->ids;
+  a.starts = in->starts;
+  a.uniforms = in->uniforms;
+  a.temps = in->temps;
+  a.draft_temps = in->draft_temps;
+  a.temp = in->temp;
+  a.draft_temp = in->draft_temp;
+  a.accepted = in->accepted;
+  a.next_ids = in->next_ids;
+  a.chances = in->chances;
+  a.ws = in->ws;
+  return a;
+}
+
+int64_t dfl_verify_ws(const dfl_verify_args* args) {
+  if (!args) return 0;
+  VerifyArgs a = verify_args(args);
+  if (check_verify(a)) return 0;
+  vf_cut(a);
+  return vf_ws(a).bytes;
+}
+
+int dfl_verify(const dfl_verify_args* args, void* stream) {
+  if (!args) return fail(DFL_EINVAL, "dfl_verify: null argument");
+  const VerifyArgs a = verify_args(args);
+  if (const char* e = check_verify(a)) return fail(DFL_EINVAL, std::string("dfl_verify: ") + e);
+  const int64_t need = dfl_verify_ws(args);
+  if (!a.ws || (reinterpret_cast<uintptr_t>(a.ws) & 15) || args->ws_bytes < need)
+    return fail(DFL_EINVAL, "dfl_verify: an aligned workspace of " + std::to_string(need) + " bytes needed");
+  launch_verify(a, (hipStream_t)stream);
+  return check_launch("dfl_verify");
 }
 
 }  // extern "C"

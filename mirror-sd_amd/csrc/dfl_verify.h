@@ -1,0 +1,102 @@
+// Verification of drafted blocks against the target's distributions: sizes, workspace, host checks.
+// Everything here but the launcher is plain host code too, so that it can be tested on a CPU.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace dfl {
+
+struct VerifyArgs {
+  const void *target, *draft;        // [n_rows][vocab] logits; draft may be null
+  long long target_row, draft_row;   // row strides in elements
+  int target_dtype, draft_dtype;     // 0 fp32, 1 fp16, 2 bf16
+  int n_rows, vocab, n_seq;
+  const int *ids, *starts;
+  const float* uniforms;
+  const float *temps, *draft_temps;  // [n_seq], or null: one for all
+  float temp, draft_temp;
+  int *accepted, *next_ids;
+  float* chances;
+  void* ws;
+  // from here on set by the launcher
+  int t_chunks, d_chunks;            // parts of a row in the first pass, for each matrix
+  int draw_chunks;                   // parts of a row in the draw
+  int vecs;                          // 16-byte loads of a thread and part
+};
+
+constexpr int VF_THREADS = 256;
+constexpr int VF_DRAW = 2048;        // values of a part in the draw: 8 a thread
+constexpr int VF_MAX_VOCAB = 1 << 24, VF_MAX_ROWS = 1 << 24, VF_MAX_SEQS = 65536;
+
+inline int vf_elems(int dtype) { return dtype == 0 ? 4 : 8; }   // values of 16 bytes
+// Parts of a row, whose first value may lie up to vf_elems - 1 values behind a 16-byte boundary.
+inline int vf_chunks(int vocab, int dtype, int vecs) {
+  const long long e = vf_elems(dtype), part = VF_THREADS * e * vecs;
+  return (int)((vocab + e - 1 + part - 1) / part);
+}
+inline int vf_draw_chunks(int vocab) { return (vocab + VF_DRAW - 1) / VF_DRAW; }
+
+// What the first pass leaves of a part of a row: its largest logit and, softmax, the sum of its
+// weights relative to that one's (offset_of), greedy, the largest's first place.  A sum or
+// place that is no number marks a row without a distribution.
+struct VfPart { float top, pad; double sum; };
+// What a sequence's draw needs.
+struct VfDraw {
+  int kind;          // 0: nothing to draw; 1: from p but for one token; 2: from max(p - q, 0)
+  int row, draft;    // rows of target and draft
+  int not_this;      // the token that is left out (-1: none)
+  float p_top, q_top;   // the rows' largest logits
+  double pc, qc;        // log2(e) / T
+};
+struct VfWs { long long parts, draws, sums, states, bytes; };   // offsets
+inline VfWs vf_ws(const VerifyArgs& a) {
+  VfWs w{};
+  long long at = 0;
+  auto take = [&](long long n) { const long long p = at; at += (n + 15) / 16 * 16; return p; };
+  w.parts = take((long long)a.n_rows * (a.t_chunks + a.d_chunks) * (long long)sizeof(VfPart));
+  w.draws = take((long long)a.n_seq * (long long)sizeof(VfDraw));
+  w.sums = take(3ll * a.n_seq * a.draw_chunks * 8);   // p, q, max(p - q, 0)
+  w.states = take(4ll * a.n_rows);
+  w.bytes = at;
+  return w;
+}
+// How the call is cut.
+inline void vf_cut(VerifyArgs& a) {
+  const long long bytes = (long long)a.n_rows * a.vocab * ((a.target_dtype ? 2 : 4) +
+                                                           (a.draft ? (a.draft_dtype ? 2 : 4) : 0));
+  a.vecs = bytes <= (32ll << 20) ? 2 : 8;
+  a.t_chunks = vf_chunks(a.vocab, a.target_dtype, a.vecs);
+  a.d_chunks = a.draft ? vf_chunks(a.vocab, a.draft_dtype, a.vecs) : 0;
+  a.draw_chunks = vf_draw_chunks(a.vocab);
+}
+
+inline const char* check_verify(const VerifyArgs& a) {
+  if (a.n_rows < 0 || a.n_rows > VF_MAX_ROWS) return "rows outside [0, 2^24]";
+  if (a.vocab < 1 || a.vocab > VF_MAX_VOCAB) return "vocabulary outside [1, 2^24]";
+  if (a.n_seq < 1 || a.n_seq > VF_MAX_SEQS) return "sequences outside [1, 65536]";
+  if (a.target_dtype < 0 || a.target_dtype > 2 || (a.draft && (a.draft_dtype < 0 || a.draft_dtype > 2)))
+    return "dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)";
+  VerifyArgs cut = a;
+  vf_cut(cut);
+  if ((long long)a.n_rows * (cut.t_chunks + cut.d_chunks) > 0x7fffffffll ||
+      (long long)a.n_seq * cut.draw_chunks > 0x7fffffffll)
+    return "too many rows for so large a vocabulary";
+  if (!a.starts || !a.accepted || !a.next_ids) return "null pointer";
+  if (a.n_rows > 0 && (!a.target || !a.ids || !a.uniforms || !a.chances)) return "null pointer";
+  if (a.n_rows > 1 && (a.target_row < a.vocab || (a.draft && a.draft_row < a.vocab)))
+    return "rows overlap (a row stride below the vocabulary)";
+  auto mis = [](const void* p, int dtype) {
+    return (reinterpret_cast<uintptr_t>(p) & (dtype ? 1 : 3)) != 0;
+  };
+  if (mis(a.target, a.target_dtype) || mis(a.draft, a.draft_dtype)) return "logits are not aligned to their type";
+  auto number = [](float t) { return t >= 0.f && t <= 3.4028235e38f; };
+  if (!a.temps && !number(a.temp)) return "temperature must be finite and not negative";
+  if (a.draft && !a.draft_temps && !number(a.draft_temp))
+    return "draft temperature must be finite and not negative";
+  return nullptr;
+}
+
+void launch_verify(const VerifyArgs& a, hipStream_t st);
+
+}  // namespace dfl

@@ -8,7 +8,7 @@ include/dflash_hip.h).
 from .config import DFlashConfig, Workload, build_target_layer_ids, extract_context_feature, workload
 
 __all__ = ["DFlashConfig", "DFlashDraftModel", "DFlashKVCache", "KV4Cache", "Workload",
-           "build_target_layer_ids", "extract_context_feature", "workload", "sample"]
+           "build_target_layer_ids", "extract_context_feature", "workload", "sample", "verify_draft"]
 
 
 def __getattr__(name):
@@ -19,4 +19,7 @@ def __getattr__(name):
     if name == "KV4Cache":
         from .kv4 import KV4Cache
         return KV4Cache
+    if name == "verify_draft":
+        from .verify import verify_draft
+        return verify_draft
     raise AttributeError(name)

@@ -45,6 +45,18 @@ class DflKv4Attn(ctypes.Structure):
     ]
 
 
+class DflVerify(ctypes.Structure):
+    _fields_ = [
+        ("target", c_void_p), ("draft", c_void_p), ("target_row", c_int64),
+        ("draft_row", c_int64), ("target_dtype", c_int32), ("draft_dtype", c_int32),
+        ("n_rows", c_int32), ("vocab", c_int32), ("n_seq", c_int32), ("temp", ctypes.c_float),
+        ("draft_temp", ctypes.c_float), ("ids", c_void_p), ("starts", c_void_p),
+        ("uniforms", c_void_p), ("temps", c_void_p), ("draft_temps", c_void_p),
+        ("accepted", c_void_p), ("next_ids", c_void_p), ("chances", c_void_p), ("ws", c_void_p),
+        ("ws_bytes", c_int64),
+    ]
+
+
 PtrArray7 = c_void_p * 7
 
 # name -> (restype, argtypes); every symbol declared in include/dflash_hip.h
@@ -106,6 +118,8 @@ SIGNATURES = {
                                c_void_p, c_void_p, c_void_p, c_void_p]),
     "dfl_kv4_attend": (c_int32, [ctypes.POINTER(DflKv4Attn), c_void_p]),
     "dfl_kv4_attend_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "dfl_verify": (c_int32, [ctypes.POINTER(DflVerify), c_void_p]),
+    "dfl_verify_ws": (c_int64, [ctypes.POINTER(DflVerify)]),
 }
 
 _lib = None
