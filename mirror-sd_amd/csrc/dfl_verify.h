@@ -21,19 +21,20 @@ struct VerifyArgs {
   void* ws;
   // from here on set by the launcher
   int t_chunks, d_chunks;            // parts of a row in the first pass, for each matrix
+  int t_rounds, d_rounds;            // rounds of a part
   int draw_chunks;                   // parts of a row in the draw
-  int vecs;                          // 16-byte loads of a thread and part
 };
 
 constexpr int VF_THREADS = 256;
+constexpr int VF_VECS = 2;           // 16-byte loads of a thread and round
 constexpr int VF_DRAW = 2048;        // values of a part in the draw: 8 a thread
 constexpr int VF_MAX_VOCAB = 1 << 24, VF_MAX_ROWS = 1 << 24, VF_MAX_SEQS = 65536;
 
 inline int vf_elems(int dtype) { return dtype == 0 ? 4 : 8; }   // values of 16 bytes
-// Parts of a row, whose first value may lie up to vf_elems - 1 values behind a 16-byte boundary.
-inline int vf_chunks(int vocab, int dtype, int vecs) {
-  const long long e = vf_elems(dtype), part = VF_THREADS * e * vecs;
-  return (int)((vocab + e - 1 + part - 1) / part);
+// Rounds of a row (one at least).
+inline int vf_rounds(int vocab, int dtype) {
+  const int round = VF_THREADS * vf_elems(dtype) * VF_VECS;
+  return (vocab + round - 1) / round;
 }
 inline int vf_draw_chunks(int vocab) { return (vocab + VF_DRAW - 1) / VF_DRAW; }
 
@@ -47,7 +48,9 @@ struct VfDraw {
   int row, draft;    // rows of target and draft
   int not_this;      // the token that is left out (-1: none)
   float p_top, q_top;   // the rows' largest logits
+  float u, pad;
   double pc, qc;        // log2(e) / T
+  double ratio;         // sum of p's weights over that of q's (kind 2)
 };
 struct VfWs { long long parts, draws, sums, states, bytes; };   // offsets
 inline VfWs vf_ws(const VerifyArgs& a) {
@@ -61,13 +64,19 @@ inline VfWs vf_ws(const VerifyArgs& a) {
   w.bytes = at;
   return w;
 }
-// How the call is cut.
+// How the call is cut: into parts of as many rounds as leave VF_PARTS of them, what the chip holds at
+// once.  1024, 2048 and 4096 parts, us: 8 blocks of 32 rows without a draft's logits 41, 45, 51; 48
+// ragged ones of a vocabulary of 32003 58, 58, 69; one block of 16 rows 41 with each.
+constexpr int VF_PARTS = 1024;
 inline void vf_cut(VerifyArgs& a) {
-  const long long bytes = (long long)a.n_rows * a.vocab * ((a.target_dtype ? 2 : 4) +
-                                                           (a.draft ? (a.draft_dtype ? 2 : 4) : 0));
-  a.vecs = bytes <= (32ll << 20) ? 2 : 8;
-  a.t_chunks = vf_chunks(a.vocab, a.target_dtype, a.vecs);
-  a.d_chunks = a.draft ? vf_chunks(a.vocab, a.draft_dtype, a.vecs) : 0;
+  const int t = vf_rounds(a.vocab, a.target_dtype), d = a.draft ? vf_rounds(a.vocab, a.draft_dtype) : 0;
+  const long long each = (long long)a.n_rows * (t + d) / VF_PARTS;
+  auto cut = [&](int rounds, int& per, int& chunks) {
+    per = each < 1 ? 1 : each < rounds ? (int)each : rounds > 1 ? rounds : 1;
+    chunks = rounds ? (rounds + per - 1) / per : 0;
+  };
+  cut(t, a.t_rounds, a.t_chunks);
+  cut(d, a.d_rounds, a.d_chunks);
   a.draw_chunks = vf_draw_chunks(a.vocab);
 }
 

@@ -44,13 +44,12 @@ DFL_DEV double scale_of(const float* temps, float temp, int s) {
   const float t = temps ? temps[s] : temp;
   return t >= GREEDY ? LOG2E / (double)fminf(t, 1e30f) : 0.0;
 }
-// 2^x to the last bits: the series of 2^f around a whole number, |f| <= 1/2, to f^13 (the next term
-// is below 2^-57).  A third of the library's code; 0 for -infinity, NaN for NaN.
+// 2^x: the series of 2^f around a whole number, |f| <= 1/2, to f^12 (the next term is below 2^-52 of
+// it), half of the library's code.  0 for -infinity; any number for NaN.
 DFL_DEV double pow2_64(double x) {
-  x = x < -1100.0 ? -1100.0 : x;
+  x = fmax(x, -2000.0);
   const double k = __builtin_rint(x), f = x - k;
-  double p = 1.3691488853904128e-12;
-  p = __builtin_fma(p, f, 2.5678435993488206e-11);
+  double p = 2.5678435993488206e-11;
   p = __builtin_fma(p, f, 4.4455382718708116e-10);
   p = __builtin_fma(p, f, 7.054911620801123e-09);
   p = __builtin_fma(p, f, 1.01780860092397e-07);
@@ -96,105 +95,170 @@ DFL_DEV double moved_sum(double sum, float top, float to, double scale) {
   return sum == 0.0 || top == to ? sum : sum * pow2_64(((double)top - to) * scale + (offset_of(to, scale) - offset_of(top, scale)));
 }
 
+// Two parts joined (in the order of their places).
+DFL_DEV VfPart join(const VfPart& x, const VfPart& y, double scale) {
+  if (scale == 0.0) {
+    if (!(x.sum == x.sum) || !(y.sum == y.sum)) return VfPart{fmaxf(x.top, y.top), 0.f, __builtin_nan("")};
+    return y.top > x.top || (y.top == x.top && y.sum < x.sum) ? y : x;
+  }
+  const float top = fmaxf(x.top, y.top);
+  return VfPart{top, 0.f, moved_sum(x.sum, x.top, top, scale) + moved_sum(y.sum, y.top, top, scale)};
+}
 // ---- first pass: parts of rows
 //
-// A thread has VECS loads of 16 bytes, all under way together; a wave has its own reference.
-template <int DT, int VECS>
-DFL_DEV void part_of_row(const VerifyArgs& a, const void* base, long long stride, int row, int chunk,
-                         double scale, VfPart& out, float (&lds)[2][4]) {
+// A workgroup goes over its part of a row in rounds of VECS loads of 16 bytes a thread; the next
+// round's loads are on their way while this one's exponentials are made.
+
+template <int DT> struct Vec {
   typedef typename LogitT<DT>::t E;
-  constexpr int N = DT == 0 ? 4 : 8;
+  static constexpr int N = DT == 0 ? 4 : 8;   // values of 16 bytes
   typedef E vec __attribute__((ext_vector_type(N)));
-  const E* p = reinterpret_cast<const E*>(base) + row * stride;
-  const int pad = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(E));
-  const int e0 = chunk * (VF_THREADS * VECS * N) - pad + N * threadIdx.x;   // this thread's first value
-  vec x[VECS];
-  if (chunk > 0 && (chunk + 1) * (VF_THREADS * VECS * N) - pad <= a.vocab) {
+};
+// Vectors v, v + VF_THREADS, .. of a row's `n`; -infinity past the last.
+template <int DT, int VECS>
+DFL_DEV void load_round(const typename Vec<DT>::vec* p, int v, int n, bool inside, typename Vec<DT>::vec (&x)[VECS]) {
+  if (inside) {
 #pragma unroll
-    for (int j = 0; j < VECS; ++j)
-      x[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p + e0 + j * (VF_THREADS * N)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      const int e = e0 + j * (VF_THREADS * N);
-      if (e >= 0 && e + N <= a.vocab) {
-        x[j] = *reinterpret_cast<const vec*>(p + e);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[j][i] = e + i >= 0 && e + i < a.vocab ? p[e + i] : (E)-INFINITY;
-      }
-    }
+    for (int j = 0; j < VECS; ++j) x[j] = __builtin_nontemporal_load(p + v + j * VF_THREADS);
+    return;
   }
-  const int wv = threadIdx.x >> 6;
-  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
+#pragma unroll
+    for (int i = 0; i < Vec<DT>::N; ++i) x[j][i] = (typename Vec<DT>::E)-INFINITY;
+    if (v + j * VF_THREADS < n) x[j] = p[v + j * VF_THREADS];
+  }
+}
+// The weights' sum of a wave's part, relative to a logit that is raised to the largest so far when
+// that is more than twice its weight.
+struct SoftState {
+  float top, at, ref;   // this lane's largest; the logit that weights are relative to, and fl(c at)
+  float sum[4];
+};
+template <int VECS, int N, typename V>
+DFL_DEV void soft_round(const V (&x)[VECS], SoftState& s, float c, float d, double scale) {
+  float top = s.top;
 #pragma unroll
   for (int j = 0; j < VECS; ++j)
 #pragma unroll
     for (int i = 0; i < N; ++i) top = fmaxf(top, (float)x[j][i]);
-  if (scale == 0.0) {   // the largest and its first place
-    bool bad = false;
-    int at = INT32_MAX;
-    top = wave_max(top);
+  s.top = top;
+  if (!__all(is_moderate(s.ref) ? top * c <= s.ref + 1.f : top <= s.at)) {
+    const float to = wave_max(top);
+    if (to > s.at) {
+      if (s.at > -INFINITY) {
+        const float k = (float)moved_sum(1.0, s.at, to, scale);
 #pragma unroll
-    for (int j = VECS - 1; j >= 0; --j)
-#pragma unroll
-      for (int i = N - 1; i >= 0; --i) {
-        const float v = (float)x[j][i];
-        bad |= !(v < INFINITY);
-        if (v == top) at = e0 + j * (VF_THREADS * N) + i;
+        for (int i = 0; i < 4; ++i) s.sum[i] *= k;
       }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
-    at = __ballot(bad) ? -1 : max(at, 0);   // (of a wave without values it is no place)
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-      lds[0][wv] = top;
-      lds[1][wv] = __int_as_float(at);
+      s.at = to;
+      s.ref = to * c;
     }
-    __syncthreads();
-    out = VfPart{-INFINITY, 0.f, 0.0};
-    for (int w = 0; w < 4; ++w) {
-      const int i = __float_as_int(lds[1][w]);
-      if (i < 0) out.sum = __builtin_nan("");
-      const float m = lds[0][w];
-      if (m > out.top || (m == out.top && i < out.sum)) {
-        out.top = m;
-        if (out.sum == out.sum) out.sum = i;
-      }
-    }
-    return;
   }
-  top = wave_max(top);
-  const float c = scale_hi(scale), d = (float)(scale - (double)c), ref = top * c;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (__builtin_expect(is_moderate(ref), 1)) {
+  if (__builtin_expect(is_moderate(s.ref), 1)) {
 #pragma unroll
     for (int j = 0; j < VECS; ++j)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float v = (float)x[j][i];
-        sum[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(v, d, __builtin_fmaf(v, c, -ref)));
+        s.sum[i & 3] += __builtin_amdgcn_exp2f(__builtin_fmaf(v, d, __builtin_fmaf(v, c, -s.ref)));
       }
-  } else {   // nothing but -infinity, or large logits
+  } else {   // nothing but -infinity so far, or large logits
     const float both = (float)scale;
 #pragma unroll
     for (int j = 0; j < VECS; ++j)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float v = (float)x[j][i];
-        sum[i & 3] += v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v - top) * both);
+        s.sum[i & 3] += v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v - s.at) * both);
       }
   }
-  const float s = wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+}
+// (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not wanted)
+template <int DT, int VECS, typename F>
+DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stride, int row, int chunk, int rounds,
+                           F scale_at, float (&lds)[2][4]) {
+  typedef Vec<DT> V;
+  constexpr int ROUND = VF_THREADS * VECS;   // vectors
+  const typename V::E* p = reinterpret_cast<const typename V::E*>(base) + row * stride;
+  // whole vectors of the row, and the values before and behind them (the first part takes those)
+  const int head = min(a.vocab, (int)(-(reinterpret_cast<uintptr_t>(p) / sizeof(typename V::E)) & (V::N - 1)));
+  const int n = (a.vocab - head) / V::N, tail = head + n * V::N;
+  const typename V::vec* body = reinterpret_cast<const typename V::vec*>(p + head);
+  const int begin = chunk * rounds * ROUND, end = min(begin + rounds * ROUND, n);
+  const int tid = threadIdx.x, wv = threadIdx.x >> 6;
+  auto inside = [&](int v) { return v + ROUND <= n; };
+  // (threads 0 .. 7: the values before; 8 .. 15: those behind)
+  const int edge = tid < V::N ? tid : tail + tid - V::N;
+  const bool at_edge = chunk == 0 && (tid < V::N ? tid < head : edge < a.vocab && tid < 2 * V::N);
+  typename V::vec x[VECS], y[VECS];
+  load_round<DT, VECS>(body, begin + tid, n, inside(begin), x);
+  const float extra = at_edge ? (float)p[edge] : -INFINITY;
+  const double scale = scale_at();
+  VfPart out{-INFINITY, 0.f, 0.0};
+  if (scale < 0.0) return out;
+  if (scale == 0.0) {   // the largest and its first place
+    bool bad = false;
+    float top = -INFINITY;
+    int at = INT32_MAX;
+    auto take = [&](float v, int place) {
+      bad |= !(v < INFINITY);
+      if (v > top) {
+        top = v;
+        at = place;
+      }
+    };
+    if (tid < V::N) take(extra, edge);
+    for (int v = begin; v < end; v += ROUND) {
+      if (v + ROUND < end) load_round<DT, VECS>(body, v + ROUND + tid, n, inside(v + ROUND), y);
+#pragma unroll
+      for (int j = 0; j < VECS; ++j)
+#pragma unroll
+        for (int i = 0; i < V::N; ++i)
+          take((float)x[j][i], head + (v + tid + j * VF_THREADS) * V::N + i);
+#pragma unroll
+      for (int j = 0; j < VECS; ++j) x[j] = y[j];
+    }
+    if (tid >= V::N) take(extra, edge);
+    const float of_wave = wave_max(top);
+    if (top != of_wave) at = INT32_MAX;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+    if (__ballot(bad)) at = -1;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      lds[0][wv] = of_wave;
+      lds[1][wv] = __int_as_float(at);
+    }
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+      const int i = __float_as_int(lds[1][w]);
+      out = join(out, VfPart{lds[0][w], 0.f, i < 0 ? __builtin_nan("") : (double)i}, 0.0);
+    }
+    return out;
+  }
+  const float c = scale_hi(scale), d = (float)(scale - (double)c);
+  SoftState s{-INFINITY, -INFINITY, -INFINITY, {0.f, 0.f, 0.f, 0.f}};
+  if (chunk == 0 && n * V::N < a.vocab) {
+    const floatx2 one[1] = {{extra, extra}};
+    soft_round<1, 1>(one, s, c, d, scale);
+  }
+  for (int v = begin; v < end; v += ROUND) {
+    if (v + ROUND < end) load_round<DT, VECS>(body, v + ROUND + tid, n, inside(v + ROUND), y);
+    soft_round<VECS, V::N>(x, s, c, d, scale);
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) x[j] = y[j];
+  }
+  const float top = wave_max(s.top), sum = wave_sum((s.sum[0] + s.sum[1]) + (s.sum[2] + s.sum[3]));
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     lds[0][wv] = top;
-    lds[1][wv] = s;
+    lds[1][wv] = top == s.at ? sum : (float)moved_sum(sum, s.at, top, scale);
   }
   __syncthreads();
-  out = VfPart{lds[0][0], 0.f, 0.0};
-  for (int w = 1; w < 4; ++w) out.top = fmaxf(out.top, lds[0][w]);
+  for (int w = 0; w < 4; ++w) out.top = fmaxf(out.top, lds[0][w]);
   for (int w = 0; w < 4; ++w) out.sum += moved_sum(lds[1][w], lds[0][w], out.top, scale);
+  return out;
 }
 
 template <int VECS>
@@ -205,16 +269,18 @@ __global__ __launch_bounds__(VF_THREADS) void verify_parts_kernel(VerifyArgs a, 
     const bool drafted = i >= t_items;
     const uint32_t chunks = drafted ? a.d_chunks : a.t_chunks, k = drafted ? i - t_items : i;
     const int row = (int)(k / chunks), chunk = (int)(k - row * chunks);
-    const int s = seq_of(a, row);
-    if (s < 0 || (drafted && a.starts[s] == row)) continue;   // (a first row has no draft)
-    const double scale = drafted ? scale_of(a.draft_temps, a.draft_temp, s) : scale_of(a.temps, a.temp, s);
+    auto scale = [&]() {
+      const int s = seq_of(a, row);
+      if (s < 0 || (drafted && a.starts[s] == row)) return -1.0;   // (a first row has no draft)
+      return drafted ? scale_of(a.draft_temps, a.draft_temp, s) : scale_of(a.temps, a.temp, s);
+    };
     const void* base = drafted ? a.draft : a.target;
     const long long stride = drafted ? a.draft_row : a.target_row;
-    const int dt = drafted ? a.draft_dtype : a.target_dtype;
+    const int dt = drafted ? a.draft_dtype : a.target_dtype, rounds = drafted ? a.d_rounds : a.t_rounds;
     VfPart out;
-    if (dt == 0) part_of_row<0, VECS>(a, base, stride, row, chunk, scale, out, lds);
-    else if (dt == 1) part_of_row<1, VECS>(a, base, stride, row, chunk, scale, out, lds);
-    else part_of_row<2, VECS>(a, base, stride, row, chunk, scale, out, lds);
+    if (dt == 0) out = part_of_row<0, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
+    else if (dt == 1) out = part_of_row<1, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
+    else out = part_of_row<2, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
     if (threadIdx.x == 0) parts[i] = out;
   }
 }
@@ -223,36 +289,33 @@ __global__ __launch_bounds__(VF_THREADS) void verify_parts_kernel(VerifyArgs a, 
 //
 // A workgroup to a sequence, a wave to a row.
 
-// Two parts joined (in the order of their places).
-DFL_DEV VfPart join(const VfPart& x, const VfPart& y, double scale) {
-  if (scale == 0.0) {
-    if (!(x.sum == x.sum) || !(y.sum == y.sum)) return VfPart{fmaxf(x.top, y.top), 0.f, __builtin_nan("")};
-    return y.top > x.top || (y.top == x.top && y.sum < x.sum) ? y : x;
-  }
-  const float top = fmaxf(x.top, y.top);
-  return VfPart{top, 0.f, moved_sum(x.sum, x.top, top, scale) + moved_sum(y.sum, y.top, top, scale)};
-}
 // The parts of a row joined, by a wave: what VfPart is, of the whole row.
-DFL_DEV VfPart join_parts(const VfPart* parts, int chunks, double scale) {
+DFL_DEV VfPart own_part(const VfPart* parts, int chunks) {   // (a lane's first, for join_parts)
   const int lane = threadIdx.x & 63;
-  VfPart r{-INFINITY, 0.f, 0.0};
-  for (int i = lane; i < chunks; i += 64) r = join(r, parts[i], scale);
+  return lane < chunks ? parts[lane] : VfPart{-INFINITY, 0.f, 0.0};
+}
+DFL_DEV VfPart join_parts(const VfPart* parts, int chunks, double scale, VfPart r) {
+  for (int i = (threadIdx.x & 63) + 64; i < chunks; i += 64) r = join(r, parts[i], scale);
+  const float top = wave_max(r.top);
+  if (scale == 0.0) {
+    int at = r.top == top ? (int)r.sum : INT32_MAX;   // (of a NaN any)
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const VfPart x{__shfl_xor(r.top, o, 64), 0.f, __shfl_xor(r.sum, o, 64)};
-    r = lane & o ? join(x, r, scale) : join(r, x, scale);   // (the same in both of a pair)
+    for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+    return VfPart{top, 0.f, __ballot(!(r.sum == r.sum)) ? __builtin_nan("") : (double)at};
   }
-  return r;
+  r.sum = moved_sum(r.sum, r.top, top, scale);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) r.sum += __shfl_xor(r.sum, o, 64);
+  return VfPart{top, 0.f, r.sum};
 }
 DFL_DEV bool has_distribution(const VfPart& r, bool greedy) {
   return greedy ? r.sum == r.sum && r.top > -INFINITY : r.sum > 0.0 && r.sum < INFINITY;
 }
-// The probability of a token (any lane alone).
-DFL_DEV double chance_of(const void* base, int dtype, long long stride, int vocab, int row, int x,
-                         double scale, const VfPart& r) {
+// The probability of token x, whose logit is l, in a row (x outside the vocabulary: 0).
+DFL_DEV double chance_of(float l, int x, int vocab, double scale, const VfPart& r) {
   if (x < 0 || x >= vocab) return 0.0;
   if (scale == 0.0) return (double)x == r.sum ? 1.0 : 0.0;
-  return pow2_64(((double)logit_at(base, dtype, row * stride + x) - r.top) * scale + offset_of(r.top, scale)) / r.sum;
+  return pow2_64(((double)l - r.top) * scale + offset_of(r.top, scale)) / r.sum;
 }
 // Sum over the workgroup's threads in 64 bits, the same in all.
 DFL_DEV double block_sum64(double v, double* lds /* 16 */) {
@@ -268,14 +331,14 @@ DFL_DEV double block_sum64(double v, double* lds /* 16 */) {
 // The probability of a token with the sum in 64 bits, by the whole workgroup.
 DFL_DEV double chance64(const void* base, int dtype, long long stride, int vocab, int row, int x, double scale,
                         const VfPart& r, double* lds) {
-  if (scale == 0.0 || x < 0 || x >= vocab) return chance_of(base, dtype, stride, vocab, row, x, scale, r);
+  if (scale == 0.0 || x < 0 || x >= vocab) return chance_of(0.f, x, vocab, scale, r);
   double v = 0.0;
   for (int i = threadIdx.x; i < vocab; i += blockDim.x)
     v += pow2_64(((double)logit_at(base, dtype, row * stride + i) - r.top) * scale);
   return pow2_64(((double)logit_at(base, dtype, row * stride + x) - r.top) * scale) / block_sum64(v, lds);
 }
 
-constexpr int JUDGE = 1024;
+constexpr int JUDGE = 1024, JUDGE_KEPT = 64;
 enum { ROW_YES = 0, ROW_NO = 1, ROW_CLOSE = 2 };
 // What the first pass's sums (each off by 2^-16 at most: exponents of at most 40 that matter, each
 // rounded twice, 2^-17.6, the power's 2^-22, a thread's additions 2^-18) can change in a quotient.
@@ -284,7 +347,7 @@ constexpr double VF_CLOSE = 0x1p-14;
 __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const VfPart* parts, VfDraw* draws,
                                                              int* states) {
   __shared__ double lds[JUDGE / 64];
-  __shared__ int found;
+  __shared__ VfPart p_kept[JUDGE_KEPT], q_kept[JUDGE_KEPT];   // of the sequence's first rows
   const int s = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int q0 = a.starts[s], q1 = a.starts[s + 1];
   VfDraw draw{};
@@ -298,26 +361,36 @@ __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const
   }
   const double pc = scale_of(a.temps, a.temp, s), qc = a.draft ? scale_of(a.draft_temps, a.draft_temp, s) : 0.0;
   const VfPart* d_parts = parts + (long long)a.n_rows * a.t_chunks;
-  auto target = [&](int row) { return join_parts(parts + (long long)row * a.t_chunks, a.t_chunks, pc); };
-  auto drafted = [&](int row) { return join_parts(d_parts + (long long)row * a.d_chunks, a.d_chunks, qc); };
-  auto p_of = [&](int row, int x, const VfPart& r) {
-    return chance_of(a.target, a.target_dtype, a.target_row, a.vocab, row, x, pc, r);
+  auto t_at = [&](int row) { return parts + (long long)row * a.t_chunks; };
+  auto d_at = [&](int row) { return d_parts + (long long)row * a.d_chunks; };
+  auto target = [&](int row) {
+    return row - q0 < JUDGE_KEPT ? p_kept[row - q0] : join_parts(t_at(row), a.t_chunks, pc, own_part(t_at(row), a.t_chunks));
   };
-  auto q_of = [&](int row, int x, const VfPart& r) {
-    return chance_of(a.draft, a.draft_dtype, a.draft_row, a.vocab, row, x, qc, r);
+  auto drafted = [&](int row) {
+    return row - q0 < JUDGE_KEPT ? q_kept[row - q0] : join_parts(d_at(row), a.d_chunks, qc, own_part(d_at(row), a.d_chunks));
   };
   for (int row = q0 + wv; row < q1; row += JUDGE / 64) {
+    // (the first row has no test: its wave joins the last one's target, which no test needs)
+    const int before = row > q0 ? row - 1 : q1 - 1;
+    const bool with_draft = a.draft && row > q0;
+    // loads that do not wait for each other, then those of the token's logits
+    VfPart pr = own_part(t_at(before), a.t_chunks), qr{0.f, 0.f, 0.0};
+    if (with_draft) qr = own_part(d_at(row), a.d_chunks);
+    const int x = a.ids[row];
+    const double u = a.uniforms[row];
+    const bool in = x >= 0 && x < a.vocab;
+    const float pl = in ? logit_at(a.target, a.target_dtype, before * a.target_row + x) : 0.f;
+    const float ql = in && with_draft ? logit_at(a.draft, a.draft_dtype, row * a.draft_row + x) : 0.f;
+    pr = join_parts(t_at(before), a.t_chunks, pc, pr);
+    if (with_draft) qr = join_parts(d_at(row), a.d_chunks, qc, qr);
     int state = ROW_YES;
     double chance = 1.0;
     if (row > q0) {
-      const int x = a.ids[row];
-      const VfPart pr = target(row - 1), qr = a.draft ? drafted(row) : VfPart{0.f, 0.f, (double)x};
       if (!has_distribution(pr, pc == 0.0) || (a.draft && !has_distribution(qr, qc == 0.0))) {
         state = ROW_NO;
         chance = 0.0;
       } else {
-        const double p = p_of(row - 1, x, pr), q = a.draft ? q_of(row, x, qr) : 1.0;
-        const double u = a.uniforms[row];
+        const double p = chance_of(pl, x, a.vocab, pc, pr), q = a.draft ? chance_of(ql, x, a.vocab, qc, qr) : 1.0;
         chance = p > 0.0 ? fmin(1.0, p / fmax(q, 1e-300)) : 0.0;
         state = u * q < p ? ROW_YES : ROW_NO;
         if ((pc != 0.0 || qc != 0.0) && fabs(u * q - p) <= VF_CLOSE * p && p > 0.0) state = ROW_CLOSE;
@@ -326,20 +399,19 @@ __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const
     if (lane == 0) {
       a.chances[row] = (float)chance;
       states[row] = state;
+      if (before - q0 < JUDGE_KEPT) p_kept[before - q0] = pr;
+      if (row - q0 < JUDGE_KEPT) q_kept[row - q0] = qr;
     }
   }
   int stop = q0;   // the first rejected row, or the end
+  __syncthreads();
   while (true) {
-    __syncthreads();
-    if (threadIdx.x == 0) found = q1;
-    __syncthreads();
-    for (int row = stop + threadIdx.x; row < q1; row += JUDGE)
-      if (states[row] != ROW_YES) {
-        atomicMin(&found, row);
-        break;
-      }
-    __syncthreads();
-    stop = found;
+    while (stop < q1) {   // (every wave the same, 64 rows at a time)
+      const int row = stop + lane;
+      const unsigned long long no = __ballot(row < q1 && states[row] != ROW_YES);
+      stop = no ? stop + __ffsll(no) - 1 : min(stop + 64, q1);
+      if (no) break;
+    }
     if (stop >= q1 || states[stop] == ROW_NO) break;
     // too close for the sums in 32 bits
     const int x = a.ids[stop];
@@ -354,6 +426,7 @@ __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const
   const VfPart pr = target(last);
   draw.row = last;
   draw.draft = stop;
+  draw.u = a.uniforms[q0];
   draw.not_this = -1;
   draw.pc = pc;
   draw.qc = qc;
@@ -380,11 +453,32 @@ __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const
 //
 // Parts of VF_DRAW tokens, 8 in a row to a thread, in 64 bits.
 
+// Logits i0 .. i0 + 7 of a row (-infinity past its end).  Rows may begin at any value's address; the
+// card loads 16 bytes from those too.
+template <typename E>
+DFL_DEV void logits8(const E* p, int vocab, int i0, float (&x)[8]) {
+  constexpr int N = 16 / sizeof(E);
+  typedef E vec __attribute__((ext_vector_type(N), aligned(sizeof(E))));
+  if (i0 + 8 <= vocab) {
+#pragma unroll
+    for (int j = 0; j < 8 / N; ++j) {
+      const vec v = reinterpret_cast<const vec*>(p + i0)[j];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[N * j + i] = (float)v[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i0 + i < vocab ? (float)p[i0 + i] : -INFINITY;
+  }
+}
 DFL_DEV void weights8(const void* base, int dtype, long long stride, int vocab, int row, int i0, double scale,
                       float top, double (&w)[8]) {
+  float x[8];
+  if (dtype == 0) logits8(reinterpret_cast<const float*>(base) + row * stride, vocab, i0, x);
+  else if (dtype == 1) logits8(reinterpret_cast<const half_t*>(base) + row * stride, vocab, i0, x);
+  else logits8(reinterpret_cast<const bf16_t*>(base) + row * stride, vocab, i0, x);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    w[i] = i0 + i < vocab ? pow2_64(((double)logit_at(base, dtype, row * stride + i0 + i) - top) * scale) : 0.0;
+  for (int i = 0; i < 8; ++i) w[i] = pow2_64(((double)x[i] - top) * scale);
 }
 DFL_DEV void p_weights(const VerifyArgs& a, const VfDraw& d, int i0, double (&w)[8]) {
   weights8(a.target, a.target_dtype, a.target_row, a.vocab, d.row, i0, d.pc, d.p_top, w);
@@ -421,33 +515,70 @@ __global__ __launch_bounds__(VF_THREADS) void verify_sums_kernel(VerifyArgs a, c
     }
   }
 }
-DFL_DEV double sum_of(const double* at, int n, double* lds) {
-  double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) v += at[i];
-  return block_sum64(v, lds);
+DFL_DEV void sums_of(const double* x, const double* y, int n, double (*lds)[2], double& sx, double& sy) {
+  sx = sy = 0.0;
+  for (int i = threadIdx.x; i < n; i += VF_THREADS) {
+    sx += x[i];
+    sy += y[i];
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    sx += __shfl_xor(sx, o, 64);
+    sy += __shfl_xor(sy, o, 64);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    lds[threadIdx.x >> 6][0] = sx;
+    lds[threadIdx.x >> 6][1] = sy;
+  }
+  __syncthreads();
+  sx = sy = 0.0;
+  for (int w = 0; w < VF_THREADS / 64; ++w) {
+    sx += lds[w][0];
+    sy += lds[w][1];
+  }
 }
-// max(p - q, 0)
-DFL_DEV void left_weights(const VerifyArgs& a, const VfDraw& d, int i0, double zp, double zq, double (&w)[8]) {
+// max(p - q, 0) times the sum of p's weights; ratio: that over the sum of q's.
+DFL_DEV void left_weights(const VerifyArgs& a, const VfDraw& d, int i0, double ratio, double (&w)[8]) {
   double q[8];
   p_weights(a, d, i0, w);
   q_weights(a, d, i0, q);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = fmax(w[i] / zp - q[i] / zq, 0.0);
+  for (int i = 0; i < 8; ++i) w[i] = fmax(w[i] - q[i] * ratio, 0.0);
 }
-__global__ __launch_bounds__(VF_THREADS) void verify_left_kernel(VerifyArgs a, const VfDraw* draws, double* sums) {
-  __shared__ double lds[4];
+__global__ __launch_bounds__(VF_THREADS) void verify_left_kernel(VerifyArgs a, VfDraw* draws, double* sums) {
+  __shared__ double lds[4][2];
   const long long all = (long long)a.n_seq * a.draw_chunks;
   for (long long i = blockIdx.x; i < all; i += gridDim.x) {
     const int s = (int)(i / a.draw_chunks), chunk = (int)(i - (long long)s * a.draw_chunks);
-    const VfDraw d = draws[s];
+    const VfDraw d = draws[s];   // (but its ratio)
     if (d.kind != 2) continue;
-    const double zp = sum_of(sums + i - chunk, a.draw_chunks, lds);
-    const double zq = sum_of(sums + all + i - chunk, a.draw_chunks, lds);
+    double zp, zq;
+    sums_of(sums + i - chunk, sums + all + i - chunk, a.draw_chunks, lds, zp, zq);
     double w[8];
-    left_weights(a, d, chunk * VF_DRAW + 8 * threadIdx.x, zp, zq, w);
-    const double r = block_sum64(sum8(w), lds);
-    if (threadIdx.x == 0) sums[2 * all + i] = r;
+    left_weights(a, d, chunk * VF_DRAW + 8 * threadIdx.x, zp / zq, w);
+    const double r = block_sum64(sum8(w), lds[0]);
+    if (threadIdx.x == 0) {
+      sums[2 * all + i] = r;
+      if (chunk == 0) draws[s].ratio = zp / zq;
+    }
   }
+}
+// The first thread of the workgroup for which `hit`, and the last for which `any`; -1: there is none.
+struct Ends { int first, last; };
+DFL_DEV Ends block_ends(bool hit, bool any, Ends* lds /* 4 */) {
+  const unsigned long long h = __ballot(hit), y = __ballot(any);
+  const int wv = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+    lds[wv] = Ends{h ? 64 * wv + __ffsll(h) - 1 : -1, y ? 64 * wv + 63 - __clzll((long long)y) : -1};
+  __syncthreads();
+  Ends e{-1, -1};
+  for (int w = 0; w < VF_THREADS / 64; ++w) {
+    if (e.first < 0) e.first = lds[w].first;
+    e.last = max(e.last, lds[w].last);
+  }
+  return e;
 }
 // Sum over the threads before this one, and the whole.
 DFL_DEV double block_before64(double v, double* lds /* 4 */, double& all) {
@@ -472,85 +603,72 @@ DFL_DEV double block_before64(double v, double* lds /* 4 */, double& all) {
 }
 __global__ __launch_bounds__(VF_THREADS) void verify_draw_kernel(VerifyArgs a, const VfDraw* draws, const double* sums) {
   __shared__ double lds[4];
-  __shared__ int first, last;
-  const int s = blockIdx.x;
+  __shared__ Ends ends[4];
+  const int s = blockIdx.x, n = a.draw_chunks;
+  const long long all = (long long)a.n_seq * n;
+  const double* p_sums = sums + (long long)s * n;
+  // (loaded before it is known which are wanted: they do not wait for each other)
+  const int mine = min((int)threadIdx.x, n - 1);
+  const double x_p = p_sums[mine], x_left = a.draft ? p_sums[2 * all + mine] : 0.0;
   VfDraw d = draws[s];
   if (!d.kind) return;
-  const long long all = (long long)a.n_seq * a.draw_chunks, at = (long long)s * a.draw_chunks;
-  double zp = 1.0, zq = 1.0;
-  const double* parts = sums + at;
-  if (d.kind == 2) {
-    zp = sum_of(parts, a.draw_chunks, lds);
-    zq = sum_of(sums + all + at, a.draw_chunks, lds);
-    parts = sums + 2 * all + at;
-  }
-  double whole = sum_of(parts, a.draw_chunks, lds);
+  const double* parts = d.kind == 2 ? p_sums + 2 * all : p_sums;
+  double whole = 0.0;
+  // running sums of the parts, VF_THREADS at a time (a vocabulary of half a million: once)
+  double x = 0.0, b = 0.0;
+  auto scan = [&](int c0) {
+    const int c = c0 + (int)threadIdx.x;
+    x = c >= n ? 0.0 : c0 ? parts[c] : d.kind == 2 ? x_left : x_p;
+    double some;
+    b = block_before64(x, lds, some);
+    return some;
+  };
+  for (int c0 = 0; c0 < n; c0 += VF_THREADS) whole += scan(c0);
   if (!(whole > 0.0)) {
     if (d.kind == 1) {   // all of p's weight is on the token that is left out
       if (threadIdx.x == 0) a.next_ids[s] = d.not_this;
       return;
     }
     d.kind = 1;          // p and q are the same
-    parts = sums + at;
-    whole = zp;
+    parts = p_sums;
+    whole = 0.0;
+    for (int c0 = 0; c0 < n; c0 += VF_THREADS) whole += scan(c0);
   }
-  const double v = (double)a.uniforms[a.starts[s]] * whole;
+  const double v = (double)d.u * whole;
   // the part in which the running sum exceeds v (the last that has any weight if none does)
-  if (threadIdx.x == 0) {
-    first = INT32_MAX;
-    last = 0;
-  }
-  double done = 0.0, before = 0.0;
-  int mine = -1;
-  for (int c0 = 0; c0 < a.draw_chunks; c0 += VF_THREADS) {
-    const int c = c0 + threadIdx.x;
-    const double x = c < a.draw_chunks ? parts[c] : 0.0;
-    double some;
-    const double b = done + block_before64(x, lds, some);
-    if (x > 0.0) {
-      if (b + x > v) atomicMin(&first, c);
-      atomicMax(&last, c);
+  int chunk = -1, last = 0;
+  double done = 0.0;
+  for (int c0 = 0; c0 < n && chunk < 0; c0 += VF_THREADS) {
+    double some = 0.0;
+    if (n > VF_THREADS) some = scan(c0);
+    const Ends e = block_ends(x > 0.0 && done + b + x > v, x > 0.0, ends);
+    if (e.first >= 0) {
+      chunk = c0 + e.first;
+      if ((int)threadIdx.x == e.first) lds[0] = done + b;
     }
+    if (e.last >= 0) last = c0 + e.last;
     done += some;
-    __syncthreads();
-    const int hit = first;
-    if (hit != INT32_MAX) {
-      if (c == hit) {
-        mine = c;
-        before = b;
-      }
-      break;
-    }
   }
   __syncthreads();
-  const int chunk = first != INT32_MAX ? first : last;
-  const bool past = first == INT32_MAX;
-  if (mine >= 0) lds[0] = before;
-  __syncthreads();
-  const double rest = past ? INFINITY : v - lds[0];
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    first = INT32_MAX;
-    last = 0;
-  }
+  const double rest = chunk < 0 ? INFINITY : v - lds[0];
+  if (chunk < 0) chunk = last;
   const int i0 = chunk * VF_DRAW + 8 * threadIdx.x;
   double w[8], some;
-  if (d.kind == 2) left_weights(a, d, i0, zp, zq, w);
+  if (d.kind == 2) left_weights(a, d, i0, d.ratio, w);
   else p_weights(a, d, i0, w);
   double sum = block_before64(sum8(w), lds, some);
-  int hit = INT32_MAX, any = -1;
+  int hit = -1, any = -1;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     sum += w[i];
     if (w[i] > 0.0) {
-      if (hit == INT32_MAX && sum > rest) hit = i0 + i;
+      if (hit < 0 && sum > rest) hit = i0 + i;
       any = i0 + i;
     }
   }
-  if (hit != INT32_MAX) atomicMin(&first, hit);
-  if (any >= 0) atomicMax(&last, any);
-  __syncthreads();
-  if (threadIdx.x == 0) a.next_ids[s] = first != INT32_MAX ? first : last;
+  const Ends e = block_ends(hit >= 0, any >= 0, ends);
+  const int thread = e.first >= 0 ? e.first : max(e.last, 0);
+  if ((int)threadIdx.x == thread) a.next_ids[s] = e.first >= 0 ? hit : any;
 }
 
 }  // namespace
@@ -567,15 +685,14 @@ void launch_verify(const VerifyArgs& a_in, hipStream_t st) {
   const long long items = (long long)a.n_rows * (a.t_chunks + a.d_chunks);
   const dim3 block(VF_THREADS), grid((unsigned)(items < (1 << 20) ? items : 1 << 20));
   if (items > 0) {
-    if (a.vecs == 2) hipLaunchKernelGGL((verify_parts_kernel<2>), grid, block, 0, st, a, parts);
-    else hipLaunchKernelGGL((verify_parts_kernel<8>), grid, block, 0, st, a, parts);
+    hipLaunchKernelGGL((verify_parts_kernel<VF_VECS>), grid, block, 0, st, a, parts);
   }
   hipLaunchKernelGGL(verify_judge_kernel, dim3(a.n_seq), dim3(JUDGE), 0, st, a, (const VfPart*)parts, draws, states);
   if (a.n_rows == 0) return;
   const long long draws_n = (long long)a.n_seq * a.draw_chunks;
   const dim3 dgrid((unsigned)(draws_n < (1 << 20) ? draws_n : 1 << 20));
   hipLaunchKernelGGL(verify_sums_kernel, dgrid, block, 0, st, a, (const VfDraw*)draws, sums);
-  if (a.draft) hipLaunchKernelGGL(verify_left_kernel, dgrid, block, 0, st, a, (const VfDraw*)draws, sums);
+  if (a.draft) hipLaunchKernelGGL(verify_left_kernel, dgrid, block, 0, st, a, draws, sums);
   hipLaunchKernelGGL(verify_draw_kernel, dim3(a.n_seq), block, 0, st, a, (const VfDraw*)draws, (const double*)sums);
 }
 

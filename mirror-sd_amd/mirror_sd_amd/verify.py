@@ -19,7 +19,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 from typing import NamedTuple
 
 from . import _lib
@@ -39,9 +38,14 @@ class Verdict(NamedTuple):
     chances: "torch.Tensor"
 
 
+_CODES: dict = {}
+
+
 def _codes():
-    import torch
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    return _CODES
 
 
 def _logits(t, what):
@@ -49,13 +53,17 @@ def _logits(t, what):
         raise ValueError(f"{what} must be [n, vocab], got {tuple(t.shape)}")
     if t.dtype not in _codes():
         raise ValueError(f"{what} must be fp32, fp16 or bf16, got {t.dtype}")
-    if t.stride(1) != 1 and t.shape[1] > 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if not t.is_contiguous() and (t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < t.shape[1]):
         t = t.contiguous()   # (the kernels read rows of values next to each other)
     return t
 
 
 def _ints(t, n, what, device):
+    """An int32 tensor [n] (any length if n is None) on the logits' device."""
     import torch
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.device == device and
+            t.is_contiguous() and (n is None or t.shape[0] == n)):
+        return t
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
         if t.numel() == 0:
@@ -73,17 +81,27 @@ def _ints(t, n, what, device):
     return t.to(device, torch.int32).contiguous()
 
 
+def _numbers(t, n, what, device):
+    """An fp32 tensor [n] on the logits' device."""
+    import torch
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.dim() == 1 and t.shape[0] == n and
+            t.device == device and t.is_contiguous()):
+        return t
+    t = torch.as_tensor(t)
+    if t.dim() != 1 or t.shape[0] != n or not t.dtype.is_floating_point:
+        raise ValueError(f"{what} must be [{n}] numbers, got {t.dtype} {tuple(t.shape)}")
+    if t.is_cuda and t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the logits on {device}")
+    return t
+
+
 def _temps(t, n_seq, what, device):
     """(one number for all, None) or (0, a device tensor [n_seq])."""
     import torch
     if isinstance(t, torch.Tensor) and t.dim() == 1:
-        if t.shape[0] != n_seq or not t.dtype.is_floating_point:
-            raise ValueError(f"{what} must be a number or [{n_seq}] numbers, got {t.dtype} {tuple(t.shape)}")
-        if t.is_cuda and t.device != device:
-            raise ValueError(f"{what} is on {t.device}, the logits on {device}")
-        return 0.0, t.to(device, torch.float32).contiguous()
+        return 0.0, _numbers(t, n_seq, what, device).to(device, torch.float32).contiguous()
     t = float(t)
-    if not (0.0 <= t <= 3.4e38 and math.isfinite(t)):
+    if not 0.0 <= t <= 3.4e38:
         raise ValueError(f"{what} must be finite and not negative, got {t}")
     return t, None
 
@@ -120,10 +138,6 @@ def verify_draft(target_logits, ids, starts, uniforms, temperature=1.0, draft_lo
         draft_logits = _logits(draft_logits, "draft_logits")
         if draft_logits.shape != target_logits.shape or draft_logits.device != dev:
             raise ValueError("draft_logits must have the shape and device of target_logits")
-    if isinstance(uniforms, torch.Tensor) and uniforms.is_cuda and uniforms.device != dev:
-        raise ValueError(f"uniforms are on {uniforms.device}, the logits on {dev}")
-    if draft_temperature is None:
-        draft_temperature = temperature
     L = _lib.load()
     with _NOTHING if torch.cuda.current_device() == dev.index else torch.cuda.device(dev):
         starts = _ints(starts, None, "starts", dev)
@@ -131,28 +145,30 @@ def verify_draft(target_logits, ids, starts, uniforms, temperature=1.0, draft_lo
         if n_seq < 1:
             raise ValueError("starts must hold at least one sequence (two numbers)")
         ids = _ints(ids, n, "ids", dev)
-        uniforms = torch.as_tensor(uniforms)
-        if uniforms.shape != (n,) or not uniforms.dtype.is_floating_point:
-            raise ValueError(f"uniforms must be [{n}] numbers, got {uniforms.dtype} {tuple(uniforms.shape)}")
-        if uniforms.dtype == torch.float64:   # (the nearest number below 1 stays below it)
+        uniforms = _numbers(uniforms, n, "uniforms", dev)
+        if uniforms.dtype is torch.float64:   # (the nearest number below 1 stays below it)
             uniforms = uniforms.clamp(max=1.0 - 2.0 ** -24)
         uniforms = uniforms.to(dev, torch.float32).contiguous()
         temp, temps = _temps(temperature, n_seq, "temperature", dev)
-        draft_temp, draft_temps = _temps(draft_temperature, n_seq, "draft_temperature", dev)
-        out = torch.empty(2 * n_seq, dtype=torch.int32, device=dev)
-        accepted, next_ids = out[:n_seq], out[n_seq:]
+        draft_temp, draft_temps = temp, temps
+        if draft_temperature is not None:
+            draft_temp, draft_temps = _temps(draft_temperature, n_seq, "draft_temperature", dev)
+        accepted, next_ids = torch.empty((2, n_seq), dtype=torch.int32, device=dev).unbind(0)
         chances = torch.empty(n, dtype=torch.float32, device=dev)
         codes = _codes()
-        a = _lib.DflVerify(
-            target_logits.data_ptr(), _lib.ptr(draft_logits), target_logits.stride(0),
-            0 if draft_logits is None else draft_logits.stride(0), codes[target_logits.dtype],
-            0 if draft_logits is None else codes[draft_logits.dtype], n, vocab, n_seq, temp,
-            draft_temp, ids.data_ptr(), starts.data_ptr(), uniforms.data_ptr(), _lib.ptr(temps),
-            _lib.ptr(draft_temps), accepted.data_ptr(), next_ids.data_ptr(), chances.data_ptr(),
-            None, 0)
-        ws_bytes = L.dfl_verify_ws(ctypes.byref(a))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        a.ws, a.ws_bytes = ws.data_ptr(), ws_bytes
-        _lib.check(L.dfl_verify(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index)),
-                   "dfl_verify")
+        if draft_logits is None:
+            draft, draft_row, draft_code = None, 0, 0
+        else:
+            draft, draft_row, draft_code = (draft_logits.data_ptr(), draft_logits.stride(0),
+                                            codes[draft_logits.dtype])
+        a = _lib.DflVerify(   # (in the order of its fields: names cost 3 us)
+            target_logits.data_ptr(), draft, target_logits.stride(0), draft_row,
+            codes[target_logits.dtype], draft_code, n, vocab, n_seq, temp, draft_temp,
+            ids.data_ptr(), starts.data_ptr(), uniforms.data_ptr(), _lib.ptr(temps),
+            _lib.ptr(draft_temps), accepted.data_ptr(), next_ids.data_ptr(), chances.data_ptr())
+        at = ctypes.byref(a)
+        a.ws_bytes = L.dfl_verify_ws(at)
+        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
+        a.ws = ws.data_ptr()
+        _lib.check(L.dfl_verify(at, torch._C._cuda_getCurrentRawStream(dev.index)), "dfl_verify")
     return Verdict(accepted, next_ids, chances)

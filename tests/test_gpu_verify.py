@@ -324,3 +324,16 @@ def test_refusals():
         args.update(bad)
         with pytest.raises(ValueError):
             verify_draft(**args)
+
+
+def test_logits_that_grow_along_a_row():
+    """References that are raised again and again, over many rounds of a part and past the range
+    in which exponents are made in one step."""
+    n, vocab = 6, 30011
+    steps = torch.arange(vocab).float()
+    t = torch.stack([steps * k for k in (1e-4, 1e-2, 1.0, 50.0, -3.0, 1e34)]).clamp(max=3.4e38)
+    u = torch.rand(n, generator=torch.Generator().manual_seed(25))
+    ids = torch.tensor([5, vocab - 1, vocab - 2, vocab - 1, vocab - 1, 0], dtype=torch.int32)
+    for temp in (1.0, 300.0, 1e30):
+        check(t.cuda(), ids.cuda(), [0, 2, 4, 6], u.cuda(), temp)
+        check(t.flip(1).contiguous().cuda(), ids.cuda(), list(range(7)), u.cuda(), temp)
