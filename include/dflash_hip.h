@@ -295,6 +295,31 @@ int dfl_kv4_step(int32_t n_seq, int32_t page, int32_t width, int32_t n_pages, co
                  int32_t* positions, int32_t* scratch, int32_t* err_flags, void* stream);
 int64_t dfl_kv4_step_scratch(int32_t n_seq);
 
+/* The step of sequences that share pages, for several continuations of one text.  Sequence s keeps the
+ * first keep[s] rows of sequence parent[s] as it was before the step (NULL: of itself; keep NULL: all of
+ * them), in the same pages, and grows by grow[s].  refs [n_pages] holds for each page the number of
+ * table places that hold it; pages with 0 are free (*n_free of them after the step), and are taken
+ * lowest number first, sequence by sequence.  New rows that begin inside a page go into it if no other
+ * sequence holds it; if all that hold it write into it the first of them does; else the sequence gets
+ * a page of its own, taken before those of its new rows, and the blocks of its kept rows are
+ * copied into it, in all n_layers layers (layer l's pages at pool + l * layer_bytes, a multiple of 16).
+ * lens, table, starts, slots, positions, max_rows and err_flags as in dfl_kv4_step (table places past a
+ * sequence's pages become -1 where the step gives them up); a parent outside [0, n_seq) is a length out of
+ * range (bit 3).  A step that cannot be done changes nothing and gives no rows.  n_seq * width is less
+ * than 2^29.  scratch: dfl_kv4_fork_scratch(...) int32 (parents: whether parent is given), any
+ * content, not shared with a step that may run at the same time. */
+typedef struct dfl_kv4_fork_args {
+  int32_t n_seq, page, width, n_pages, max_rows, n_kv, n_layers;
+  const int32_t *parent, *keep, *grow;
+  int32_t *lens, *table, *refs, *n_free;
+  int32_t *starts, *slots, *positions;
+  uint8_t* pool;
+  int64_t layer_bytes;
+  int32_t *scratch, *err_flags;
+} dfl_kv4_fork_args;
+int dfl_kv4_fork(const dfl_kv4_fork_args* args, void* stream);
+int64_t dfl_kv4_fork_scratch(int32_t n_seq, int32_t width, int32_t n_pages, int32_t parents);
+
 /* Quantise rows of keys and values into their slots: row i, head h of k is at
  * k + i * k_row + h * k_head elements (strides multiples of 8, 16-byte aligned), v alike.  Slots
  * are int32; -1 skips the row, any other slot outside the pool skips it and sets bit 6.  The

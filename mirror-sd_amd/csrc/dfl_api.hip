@@ -1687,6 +1687,40 @@ int dfl_kv4_step(int32_t n_seq, int32_t page, int32_t width, int32_t n_pages, co
   return check_launch("dfl_kv4_step");
 }
 
+int64_t dfl_kv4_fork_scratch(int32_t n_seq, int32_t width, int32_t n_pages, int32_t parents) {
+  if (n_seq < 1 || n_seq > KV4_MAX_SEQS || width < 1 || n_pages < 1) return 0;
+  return kv4_fork_scratch(n_seq, width, n_pages, parents != 0);
+}
+
+int dfl_kv4_fork(const dfl_kv4_fork_args* args, void* stream) {
+  if (!args) return fail(DFL_EINVAL, "dfl_kv4_fork: null argument");
+  Kv4ForkArgs a{};
+  a.n_seq = args->n_seq;
+  a.page_shift = page_shift_of(args->page);
+  a.width = args->width;
+  a.n_pages = args->n_pages;
+  a.max_rows = args->max_rows;
+  a.n_kv = args->n_kv;
+  a.n_layers = args->n_layers;
+  a.parent = args->parent;
+  a.keep = args->keep;
+  a.grow = args->grow;
+  a.lens = args->lens;
+  a.table = args->table;
+  a.refs = args->refs;
+  a.n_free = args->n_free;
+  a.starts = args->starts;
+  a.slots = args->slots;
+  a.positions = args->positions;
+  a.pool = args->pool;
+  a.layer_bytes = args->layer_bytes;
+  a.scratch = args->scratch;
+  a.err = args->err_flags;
+  if (const char* e = check_kv4_fork(a)) return fail(DFL_EINVAL, std::string("dfl_kv4_fork: ") + e);
+  launch_kv4_fork(a, (hipStream_t)stream);
+  return check_launch("dfl_kv4_fork");
+}
+
 int dfl_kv4_append(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row,
                    int64_t v_head, int32_t dtype, int32_t rows, int32_t n_kv, int32_t page,
                    int32_t n_pages, const int32_t* slots, uint8_t* pool, int32_t* err_flags,

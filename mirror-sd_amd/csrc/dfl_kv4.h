@@ -84,6 +84,44 @@ DFL_HD bool kv4_ask(int len, int keep, int grow, int width, int page_shift, Kv4A
   return true;
 }
 
+// ---- step of sequences that share pages ----
+struct Kv4ForkArgs {
+  int n_seq, page_shift, width, n_pages, max_rows, n_kv, n_layers;
+  const int *parent, *keep, *grow;   // [n_seq], any may be null (itself, all of the parent's, nothing)
+  int *lens, *table, *refs, *n_free;
+  int *starts, *slots, *positions;
+  unsigned char* pool;               // all layers
+  long long layer_bytes;             // of a layer's pages
+  int* scratch;                      // kv4_fork_scratch(..) ints
+  int* err;
+};
+constexpr int KV4_FORK_TOTALS = 8;
+constexpr int KV4_FORK_CHUNK = 1024;   // pages whose free ones are counted together
+DFL_HD int kv4_fork_chunks(int n_pages) { return (int)(((long long)n_pages + KV4_FORK_CHUNK - 1) / KV4_FORK_CHUNK); }
+// totals; [n_seq] the copies (3), the view (9); [n_pages] writers, first writer, list of free pages; free
+// pages of the chunks; with parents the kept pages [n_seq][width]
+DFL_HD long long kv4_fork_scratch(int n_seq, int width, int n_pages, bool parents) {
+  return KV4_FORK_TOTALS + 12ll * n_seq + 3ll * n_pages + kv4_fork_chunks(n_pages) + (parents ? (long long)n_seq * width : 0);
+}
+// What one sequence asks of a step: places of tables that gain or lose a holder (counted), places that
+// are written (placed; its last kept page's apart), pages that it had (old); false if a length is out of
+// range.
+struct Kv4ForkAsk { int keep, grow, parent, old, counted, placed; };
+DFL_HD bool kv4_fork_ask(int s, int parent, int from, int len, int keep, int grow, int width, int page_shift,
+                         Kv4ForkAsk& a) {
+  const long long cap = (long long)width << page_shift;
+  const bool ok = parent >= 0 && len >= 0 && len <= cap && from >= 0 && from <= cap && keep >= 0 && keep <= from &&
+                  grow >= 0 && (long long)keep + grow <= cap;
+  a = Kv4ForkAsk{0, 0, s, 0, 0, 0};
+  if (!ok) return false;
+  const int kept = kv4_pages(keep, page_shift), now = kv4_pages(keep + grow, page_shift);
+  a = Kv4ForkAsk{keep, grow, parent, kv4_pages(len, page_shift), 0, 0};
+  const int most = now > a.old ? now : a.old;
+  a.counted = parent == s ? a.old - kept : kept + a.old;
+  a.placed = parent == s ? most - kept : most;
+  return true;
+}
+
 // ---- append / read ----
 struct Kv4RowsArgs {
   const void *k, *v;           // append: rows in; read: unused
@@ -243,6 +281,21 @@ inline const char* check_kv4_step(const Kv4StepArgs& a) {
   if (a.max_rows > 0 && (!a.slots || !a.positions)) return "null slot map";
   return nullptr;
 }
+inline const char* check_kv4_fork(const Kv4ForkArgs& a) {
+  if (const char* e = check_kv4_pool(a.n_kv, a.page_shift, a.n_pages)) return e;
+  if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
+  if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll) return "table width out of range";
+  if ((long long)a.n_seq * a.width >= (1ll << 29)) return "2^29 places in the table or more";
+  if (a.n_layers < 1 || a.n_layers > 65536) return "layers outside [1, 65536]";
+  if (a.layer_bytes < (((long long)a.n_pages * a.n_kv) << (a.page_shift - 5)) * KV4_BLOCK || (a.layer_bytes & 15))
+    return "a layer's bytes do not hold its pages, or are no multiple of 16";
+  if (a.max_rows < 0) return "negative row capacity";
+  if (!a.lens || !a.table || !a.refs || !a.n_free || !a.starts || !a.pool || !a.scratch || !a.err)
+    return "null pointer";
+  if (a.max_rows > 0 && (!a.slots || !a.positions)) return "null slot map";
+  if (reinterpret_cast<uintptr_t>(a.pool) & 15) return "the pool must be 16-byte aligned";
+  return nullptr;
+}
 inline const char* check_kv4_rows(const Kv4RowsArgs& a, bool append) {
   if (const char* e = check_kv4_pool(a.n_kv, a.page_shift, a.n_pages)) return e;
   if (a.rows < 0) return "negative row count";
@@ -277,6 +330,7 @@ inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
 }
 
 void launch_kv4_step(const Kv4StepArgs& a, hipStream_t st);
+void launch_kv4_fork(const Kv4ForkArgs& a, hipStream_t st);
 void launch_kv4_append(const Kv4RowsArgs& a, hipStream_t st);
 void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st);
 void launch_kv4_attend(const Kv4AttnArgs& a, hipStream_t st);

@@ -5,6 +5,7 @@
 #include <float.h>
 
 #include "dfl_common.h"
+#include "dfl_kv4_scan.h"
 
 namespace dfl {
 
@@ -46,27 +47,6 @@ constexpr int STEP_ONE_SEQS = 1024, STEP_ONE_ROWS = 8192;
 // one of 1000 13.9, 10.8, 9.2, 7.9.
 constexpr int STEP_N = 4, STEP_L = 16;
 
-// Sums over the workgroup's threads of three counts at once (inclusive), and their totals.
-struct Sum3 { long long a, b, c; };
-DFL_DEV Sum3 block_scan3(Sum3 v, Sum3* lds /* 16 */, Sum3& total) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, nw = blockDim.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long x = __shfl_up(v.a, o, 64), y = __shfl_up(v.b, o, 64), z = __shfl_up(v.c, o, 64);
-    if (lane >= o) { v.a += x; v.b += y; v.c += z; }
-  }
-  __syncthreads();
-  if (lane == 63) lds[wv] = v;
-  __syncthreads();
-  total = Sum3{0, 0, 0};
-  for (int w = 0; w < nw; ++w) {
-    const Sum3 x = lds[w];
-    if (w < wv) { v.a += x.a; v.b += x.b; v.c += x.c; }
-    total.a += x.a; total.b += x.b; total.c += x.c;
-  }
-  return v;
-}
-
 DFL_DEV bool step_ask(const Kv4StepArgs& a, int s, Kv4Ask& q) {
   const int len = a.lens[s];
   return kv4_ask(len, a.keep ? a.keep[s] : len, a.grow ? a.grow[s] : 0, a.width, a.page_shift, q);
@@ -80,15 +60,6 @@ DFL_DEV int step_error(const Kv4StepArgs& a, bool bad, const Sum3& all, int n_fr
   if (all.c > a.max_rows) err |= KV4_ERR_ROWS;
   return err;
 }
-// The last of the ascending n numbers at (n > 0, at[0] <= v) that is not above v, of equals the last.
-DFL_DEV int step_search(const int* at, int n, int v) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (at[mid] <= v) lo = mid; else hi = mid;
-  }
-  return lo;
-}
 // Offsets of all sequences: kept lengths, pages put back and taken before each (n_seq), new rows
 // before each (n_seq + 1).
 struct StepView { int *base, *f_at, *t_at, *starts; };
@@ -100,17 +71,6 @@ template <int N> struct StepMoves {
   int page[N];
   bool again[N];          // the step puts another page into `from`
 };
-template <int N>
-DFL_DEV void step_search(const int* at, int n_seq, int i, int n, int past, int (&s)[N]) {
-#pragma unroll
-  for (int k = 0; k < N; ++k) s[k] = 0;
-  for (int step = n_seq > 1 ? 1 << (31 - __clz(n_seq - 1)) : 0; step; step >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int mid = min(s[k] + step, n_seq - 1);
-      if (at[mid] <= min(i + k * n, past - 1)) s[k] = mid;
-    }
-}
 // Where pages that are put back come from.
 template <int N>
 DFL_DEV void step_from(const Kv4StepArgs& a, const StepView& v, int i, int n, int freed, StepMoves<N>& m) {

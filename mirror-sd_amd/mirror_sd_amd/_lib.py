@@ -45,6 +45,17 @@ class DflKv4Attn(ctypes.Structure):
     ]
 
 
+class DflKv4Fork(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", c_int32), ("page", c_int32), ("width", c_int32), ("n_pages", c_int32),
+        ("max_rows", c_int32), ("n_kv", c_int32), ("n_layers", c_int32), ("parent", c_void_p),
+        ("keep", c_void_p), ("grow", c_void_p), ("lens", c_void_p), ("table", c_void_p),
+        ("refs", c_void_p), ("n_free", c_void_p), ("starts", c_void_p), ("slots", c_void_p),
+        ("positions", c_void_p), ("pool", c_void_p), ("layer_bytes", c_int64),
+        ("scratch", c_void_p), ("err_flags", c_void_p),
+    ]
+
+
 class DflVerify(ctypes.Structure):
     _fields_ = [
         ("target", c_void_p), ("draft", c_void_p), ("target_row", c_int64),
@@ -118,6 +129,8 @@ SIGNATURES = {
                                c_void_p, c_void_p, c_void_p, c_void_p]),
     "dfl_kv4_attend": (c_int32, [ctypes.POINTER(DflKv4Attn), c_void_p]),
     "dfl_kv4_attend_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "dfl_kv4_fork": (c_int32, [ctypes.POINTER(DflKv4Fork), c_void_p]),
+    "dfl_kv4_fork_scratch": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
     "dfl_verify": (c_int32, [ctypes.POINTER(DflVerify), c_void_p]),
     "dfl_verify_ws": (c_int64, [ctypes.POINTER(DflVerify)]),
 }

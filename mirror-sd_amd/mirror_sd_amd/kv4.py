@@ -55,13 +55,16 @@ class KV4Cache:
     ``table`` [max_seqs, ceil(max_len / page)] (-1 past a sequence's pages), ``free`` [n_pages] and
     ``n_free`` [1] (a stack of free pages).  ``pool`` holds the codes.
 
+    With ``shared`` sequences may share pages: ``step`` takes ``parent``, and the state has ``refs``
+    [n_pages] (how many table places hold a page; 0: it is free) in place of ``free``.
+
     Calls enqueue work on the current stream of the cache's device; calls that use one cache's
     state from several streams are the caller's to order.  Lengths and pages that do not fit are
     found on the device: such a step changes nothing, such rows are skipped, and ``errors()``
     tells."""
 
     def __init__(self, n_kv_heads: int, n_pages: int, max_seqs: int, max_len: int, page: int = 64,
-                 n_layers: int = 1, device=None):
+                 n_layers: int = 1, device=None, shared: bool = False):
         import torch
         if page not in (32, 64, 128, 256):
             raise ValueError(f"page must be 32, 64, 128 or 256 rows, got {page}")
@@ -84,7 +87,13 @@ class KV4Cache:
                                  self.page // BLOCK_ROWS, BLOCK_BYTES), dtype=torch.uint8, device=dev)
         self.lens = torch.zeros(self.max_seqs, **ints)
         self.table = torch.full((self.max_seqs, self.width), -1, **ints)
-        self.free = torch.arange(self.n_pages - 1, -1, -1, **ints)   # page 0 is taken first
+        self.free = self.refs = None
+        if shared:
+            if self.max_seqs * self.width >= 2**29:
+                raise ValueError("2^29 places or more in a table of sequences that share pages")
+            self.refs = torch.zeros(self.n_pages, **ints)
+        else:
+            self.free = torch.arange(self.n_pages - 1, -1, -1, **ints)   # page 0 is taken first
         self.n_free = torch.full((1,), self.n_pages, **ints)
         self._err = torch.zeros(1, **ints)
         self._scratch = self._L.dfl_kv4_step_scratch(self.max_seqs)
@@ -154,15 +163,22 @@ class KV4Cache:
         return t
 
     # ------------------------------------------------------------------ the operators
-    def step(self, grow=None, keep=None, max_rows: Optional[int] = None) -> KV4Step:
+    def step(self, grow=None, keep=None, max_rows: Optional[int] = None, parent=None) -> KV4Step:
         """Bring every sequence to ``keep[s] + grow[s]`` rows: its first ``keep[s]`` (default: all
         it has) stay, pages past them are put back, pages for ``grow[s]`` new rows (default: none)
         are taken.  ``max_rows`` is the size of the slot map (default: the sum of a ``grow`` given
         on the host); rows past the last new one get slot -1, which ``append`` skips, so a
         captured graph can use one size for all its steps.  If the lengths are out of range, the
         pages do not suffice or the new rows exceed ``max_rows``, nothing changes and there are no
-        new rows (``errors()``)."""
+        new rows (``errors()``).
+
+        With ``parent`` (a cache made with ``shared``) the rows kept are the first ``keep[s]`` (default:
+        all) of sequence ``parent[s]`` as it was before the step, in the same pages: sequences that
+        go on from one text hold its rows once.  Rows that begin inside a page that others hold go
+        into a copy of it (of all layers), which the step makes; ``append`` and ``attend`` are as ever."""
         import torch
+        if parent is not None and self.refs is None:
+            raise ValueError("parent needs a cache made with shared=True")
         if max_rows is None:
             if isinstance(grow, torch.Tensor) and grow.is_cuda:
                 raise ValueError("max_rows is needed with lengths on the device")
@@ -175,6 +191,9 @@ class KV4Cache:
         with self._guard():
             grow = None if grow is None else self._ints(grow, n, "grow")
             keep = None if keep is None else self._ints(keep, n, "keep")
+            if self.refs is not None:
+                return self._shared_step(grow, keep, max_rows,
+                                         None if parent is None else self._ints(parent, n, "parent"))
             buf = torch.empty(n + 1 + 2 * max_rows + self._scratch, dtype=torch.int32,
                               device=self.device)
             starts, slots, positions, _ = buf.split_with_sizes((n + 1, max_rows, max_rows,
@@ -186,6 +205,22 @@ class KV4Cache:
                 self.n_free.data_ptr(), max_rows, at, at + 4 * (n + 1), at + 4 * (n + 1 + max_rows),
                 at + 4 * (n + 1 + 2 * max_rows), self._err.data_ptr(), self._stream()),
                 "dfl_kv4_step")
+        return KV4Step(starts, slots, positions)
+
+    def _shared_step(self, grow, keep, max_rows: int, parent) -> KV4Step:
+        import torch
+        n = self.max_seqs
+        scratch = self._L.dfl_kv4_fork_scratch(n, self.width, self.n_pages, parent is not None)
+        buf = torch.empty(n + 1 + 2 * max_rows + scratch, dtype=torch.int32, device=self.device)
+        starts, slots, positions, _ = buf.split_with_sizes((n + 1, max_rows, max_rows, scratch))
+        at = buf.data_ptr()
+        a = _lib.DflKv4Fork(   # (in the order of its fields)
+            n, self.page, self.width, self.n_pages, max_rows, self.n_kv_heads, self.n_layers,
+            _lib.ptr(parent), _lib.ptr(keep), _lib.ptr(grow), self.lens.data_ptr(),
+            self.table.data_ptr(), self.refs.data_ptr(), self.n_free.data_ptr(), at,
+            at + 4 * (n + 1), at + 4 * (n + 1 + max_rows), self.pool.data_ptr(),
+            self.pool.stride(0), at + 4 * (n + 1 + 2 * max_rows), self._err.data_ptr())
+        _lib.check(self._L.dfl_kv4_fork(ctypes.byref(a), self._stream()), "dfl_kv4_fork")
         return KV4Step(starts, slots, positions)
 
     def append(self, k, v, slots, layer: int = 0) -> None:
