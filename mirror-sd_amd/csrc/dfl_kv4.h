@@ -103,7 +103,7 @@ DFL_HD int kv4_fork_chunks(int n_pages) { return (int)(((long long)n_pages + KV4
 DFL_HD long long kv4_fork_scratch(int n_seq, int width, int n_pages, bool parents) {
   return KV4_FORK_TOTALS + 12ll * n_seq + 3ll * n_pages + kv4_fork_chunks(n_pages) + (parents ? (long long)n_seq * width : 0);
 }
-// What one sequence asks of a step: places of tables that gain or lose a holder (counted), places that
+// What one sequence asks of a step: places whose pages may gain or lose a holder (counted), places that
 // are written (placed; its last kept page's apart), pages that it had (old); false if a length is out of
 // range.
 struct Kv4ForkAsk { int keep, grow, parent, old, counted, placed; };
@@ -117,7 +117,7 @@ DFL_HD bool kv4_fork_ask(int s, int parent, int from, int len, int keep, int gro
   const int kept = kv4_pages(keep, page_shift), now = kv4_pages(keep + grow, page_shift);
   a = Kv4ForkAsk{keep, grow, parent, kv4_pages(len, page_shift), 0, 0};
   const int most = now > a.old ? now : a.old;
-  a.counted = parent == s ? a.old - kept : kept + a.old;
+  a.counted = parent == s ? a.old - kept : a.old > kept ? a.old : kept;
   a.placed = parent == s ? most - kept : most;
   return true;
 }

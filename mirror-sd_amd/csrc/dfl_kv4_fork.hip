@@ -8,15 +8,19 @@
 // it after the step, if all write into it, the first does, and the others (or, if some do not write,
 // all that do) get a page of their own with the kept rows' blocks copied.
 //
-// Phases, each over all sequences: scan (what each asks); count (a holder more or less for every place
-// that changes, pages kept from others noted, as their tables change too); mark and ask (which pages have
-// which writers; who copies, free pages counted); list (free pages by rank); place (tables, counts,
+// Phases, each over all sequences: scan (what each asks, the pages that are written into); count (a
+// holder more or less for every place that changes, pages kept from others noted, as their tables change
+// too; the writers); ask (who copies; free pages); list (free pages by rank); place (tables, counts,
 // slots); then the copies, in a launch of their own.  Nothing but the counts changes before it is known
 // that the step can be done, and they are set back if it cannot.
 //
-// Bound by latencies, as the plain step: up to FORK_ONE_SEQS and FORK_ONE_ROWS one workgroup does all
-// phases with the offsets in LDS, past that each is a launch.  Places of all sequences are numbered
-// through and found by a search in the offsets.
+// Bound by latencies, as the plain step: for few sequences, rows, pages and places (FORK_ONE_..) one
+// workgroup does all phases with the offsets in LDS, past that each is a launch.  Places of all
+// sequences are numbered through and found by a search in the offsets.  One workgroup and launches, us
+// (sequences x kept pages that all but one in 16 keep from another): 64 x 43 (half of them) 21, 36; 64 x
+// 121 29, 36; 256 x 15 28, 40; 256 x 62 43, 40; 512 x 62 72, 43; 1024 x 93 186, 50; 1024 that fork
+// nothing 29, 41.  (With an atomic for each kept page, whether it changes hands or not, the 1024 x 93
+// took 335 and 59: sequences that go on from each other share most pages already.)
 #include "dfl_kv4.h"
 
 #include "dfl_common.h"
@@ -80,14 +84,16 @@ DFL_DEV void fork_note(const Kv4ForkAsk& q, const Sum3& in, int s, const ForkVie
 }
 DFL_DEV int fork_grow(const ForkView& v, int s) { return v.starts[s + 1] - v.starts[s]; }
 
-// Place i of those that are counted: its page, and whether a holder comes or goes.
-struct ForkCount { int page, by; int* keep_at; };
+// Place i of those that are looked at: the page that the sequence gives up there and the one that it
+// holds from now on, kept from its parent (-1: none).  A sequence that goes on from one that it shares
+// pages with mostly has the same in both.
+struct ForkCount { int gives, holds; int* keep_at; };
 DFL_DEV ForkCount fork_count_at(const Kv4ForkArgs& a, const ForkScratch& x, const ForkView& v, int s, int i) {
   const int kept = kv4_pages(v.base[s], a.page_shift), j = i - v.count_at[s], par = v.par[s];
-  const long long at = (long long)s * a.width;
-  if (par == s) return ForkCount{a.table[at + kept + j], -1, nullptr};
-  if (j < kept) return ForkCount{a.table[(long long)par * a.width + j], 1, x.kept + at + j};
-  return ForkCount{a.table[at + j - kept], -1, nullptr};
+  const long long at = (long long)s * a.width + j;
+  if (par == s) return ForkCount{a.table[at + kept], -1, nullptr};
+  return ForkCount{j < v.old[s] ? a.table[at] : -1, j < kept ? a.table[(long long)par * a.width + j] : -1,
+                   j < kept ? x.kept + at : nullptr};
 }
 constexpr int FORK_N = 4;   // places of a thread under way at once
 // Counts (sign 1) or sets the counts back (-1); whether all pages are the pool's.
@@ -103,23 +109,28 @@ DFL_DEV bool fork_count(const Kv4ForkArgs& a, const ForkScratch& x, const ForkVi
       c[k] = i0 + k * nt < total ? fork_count_at(a, x, v, s[k], i0 + k * nt) : ForkCount{0, 0, nullptr};
 #pragma unroll
     for (int k = 0; k < FORK_N; ++k) {
-      if (!c[k].by) continue;
-      if (!fork_page_ok(a, c[k].page)) {
-        ok = false;
+      if (i0 + k * nt >= total) break;
+      // (a place past the sequence's old pages gives up none, one past its kept ones holds none)
+      const bool own = v.par[s[k]] == s[k], gives = own || i0 + k * nt - v.count_at[s[k]] < v.old[s[k]];
+      const bool holds = c[k].keep_at != nullptr;
+      if ((gives && !fork_page_ok(a, c[k].gives)) || (holds && !fork_page_ok(a, c[k].holds))) {
+        ok = false;   // (neither is counted: nor are they when the counts are set back)
         continue;
       }
-      atomicAdd(a.refs + c[k].page, sign * c[k].by);
-      if (c[k].keep_at) *c[k].keep_at = c[k].page;
+      if (holds) *c[k].keep_at = c[k].holds;
+      if (c[k].gives == c[k].holds) continue;
+      if (gives) atomicAdd(a.refs + c[k].gives, -sign);
+      if (holds) atomicAdd(a.refs + c[k].holds, sign);
     }
   }
   return ok;
 }
 // The page that a sequence's new rows begin inside; its marks are cleared.
-DFL_DEV bool fork_edge(const Kv4ForkArgs& a, const ForkScratch& x, const ForkView& v, int s) {
+DFL_DEV bool fork_edge(const Kv4ForkArgs& a, const ForkScratch& x, const ForkView& v, int s, const Kv4ForkAsk& q) {
   int e = -1;
   bool ok = true;
-  if (fork_grow(v, s) > 0 && (v.base[s] & ((1 << a.page_shift) - 1))) {
-    e = a.table[(long long)v.par[s] * a.width + (v.base[s] >> a.page_shift)];
+  if (q.grow > 0 && (q.keep & ((1 << a.page_shift) - 1))) {
+    e = a.table[(long long)q.parent * a.width + (q.keep >> a.page_shift)];
     ok = fork_page_ok(a, e);
     if (ok) {
       store_agent(x.writers + e, 0);
@@ -183,7 +194,7 @@ DFL_DEV void fork_row(const Kv4ForkArgs& a, const ForkScratch& x, const ForkView
   a.positions[r] = pos;
 }
 
-constexpr int FORK_ONE_SEQS = 1024, FORK_ONE_ROWS = 8192, FORK_ONE_PAGES = 65536;
+constexpr int FORK_ONE_PLACES = 16384, FORK_ONE_SEQS = 1024, FORK_ONE_ROWS = 8192, FORK_ONE_PAGES = 65536;
 
 __global__ __launch_bounds__(1024) void kv4_fork_one_kernel(Kv4ForkArgs a) {
   __shared__ Sum3 lds[16];
@@ -205,11 +216,11 @@ __global__ __launch_bounds__(1024) void kv4_fork_one_kernel(Kv4ForkArgs a) {
     if (mine) fork_note(q, in, s, v);
     if (s == 0) v.starts[a.n_seq] = rows;
     __syncthreads();
-    bool ok = !mine || fork_edge(a, x, v, s);
+    bool ok = !mine || fork_edge(a, x, v, s, q);
+    __syncthreads();
+    if (mine) fork_mark(x, v, s);
     ok = fork_count(a, x, v, counted, s, nt, 1) && ok;
     if (__syncthreads_or(!ok)) err = KV4_ERR_PAGE;
-    if (mine) fork_mark(x, v, s);
-    __syncthreads();
     // a thread's pages: some in a row
     const int per = (a.n_pages + nt - 1) / nt, p0 = min(s * per, a.n_pages), p1 = min(p0 + per, a.n_pages);
     int zeros = 0;
@@ -270,11 +281,15 @@ __global__ __launch_bounds__(1024) void kv4_fork_scan_kernel(Kv4ForkArgs a) {
     Sum3 t;
     Sum3 in = block_scan3(Sum3{q.counted, q.placed, q.grow}, lds, t);
     in.a += all.a; in.b += all.b; in.c += all.c;
-    if (s < a.n_seq) fork_note(q, in, s, x.view);
+    if (s < a.n_seq) {
+      fork_note(q, in, s, x.view);
+      if (!fork_edge(a, x, x.view, s, q)) bad |= 2;
+    }
     all.a += t.a; all.b += t.b; all.c += t.c;
   }
-  int err = __syncthreads_or(bad) ? KV4_ERR_LEN : 0;
+  int err = __syncthreads_or(bad & 1) ? KV4_ERR_LEN : 0;
   if (all.c > a.max_rows) err |= KV4_ERR_ROWS;
+  if (!err && __syncthreads_or(bad)) err = KV4_ERR_PAGE;   // (err is the same in all threads)
   if (threadIdx.x == 0) {
     x.view.starts[a.n_seq] = (int)all.c;
     *x.totals = ForkTotals{err, (int)all.a, (int)all.b, (int)all.c, 0, 0, 0, 0};
@@ -285,18 +300,11 @@ __global__ __launch_bounds__(256) void kv4_fork_count_kernel(Kv4ForkArgs a) {
   const ForkScratch x = fork_scratch(a);
   if (x.totals->err) return;
   const int t = blockIdx.x * 256 + threadIdx.x, nt = gridDim.x * 256;
-  bool ok = true;
-  for (int s = t; s < a.n_seq; s += nt) ok = fork_edge(a, x, x.view, s) && ok;
-  ok = fork_count(a, x, x.view, x.totals->counted, t, nt, 1) && ok;
-  if (!ok) {
+  for (int s = t; s < a.n_seq; s += nt) fork_mark(x, x.view, s);
+  if (!fork_count(a, x, x.view, x.totals->counted, t, nt, 1)) {
     atomicOr(&x.totals->bad, KV4_ERR_PAGE);
     atomicOr(a.err, KV4_ERR_PAGE);
   }
-}
-__global__ __launch_bounds__(256) void kv4_fork_mark_kernel(Kv4ForkArgs a) {
-  const ForkScratch x = fork_scratch(a);
-  if (x.totals->err) return;
-  for (int s = blockIdx.x * 256 + threadIdx.x; s < a.n_seq; s += gridDim.x * 256) fork_mark(x, x.view, s);
 }
 // Free pages of every KV4_FORK_CHUNK, 4 a thread.
 DFL_DEV int fork_free4(const Kv4ForkArgs& a, int chunk, bool (&free)[4]) {
@@ -393,21 +401,15 @@ __global__ __launch_bounds__(256) void kv4_fork_place_kernel(Kv4ForkArgs a) {
     for (int k = 0; k < FORK_N; ++k)
       if (i0 + k * nt < placed) fork_place(a, x, v, of[k], i0 + k * nt);
   }
-  if (!none)
-    for (int s = t; s < a.n_seq; s += nt) fork_own(a, x, v, s);
+  for (int s = t; s <= a.n_seq; s += nt) {
+    if (none) a.starts[s] = 0;
+    else if (s < a.n_seq) fork_own(a, x, v, s);
+  }
   for (long long r = t; r < a.max_rows; r += nt) {
     if (r < rows) fork_row(a, x, v, step_search(v.starts, a.n_seq, (int)r), (int)r);
     else a.slots[r] = a.positions[r] = -1;
   }
 }
-// (the row ranges are read by the launch before)
-__global__ __launch_bounds__(256) void kv4_fork_none_kernel(Kv4ForkArgs a) {
-  const ForkScratch x = fork_scratch(a);
-  if (!(x.totals->err || x.totals->bad)) return;
-  for (int s = blockIdx.x * 256 + threadIdx.x; s <= a.n_seq; s += gridDim.x * 256) a.starts[s] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) x.totals->copies = 0;
-}
-
 // The copied pages: a workgroup takes the kept rows' blocks of one layer's head, which follow on each
 // other.
 __global__ __launch_bounds__(256) void kv4_fork_copy_kernel(Kv4ForkArgs a) {
@@ -435,21 +437,21 @@ __global__ __launch_bounds__(256) void kv4_fork_copy_kernel(Kv4ForkArgs a) {
 
 void launch_kv4_fork(const Kv4ForkArgs& a, hipStream_t st) {
   const dim3 block(256);
-  if (a.n_seq <= FORK_ONE_SEQS && a.max_rows <= FORK_ONE_ROWS && a.n_pages <= FORK_ONE_PAGES) {
-    const int threads = a.n_seq <= 256 && a.max_rows <= 1024 && a.n_pages <= 4096 ? 256 : 1024;
+  // (the places that a step may look at; without parents only those that lengths give up and take)
+  const long long places = a.parent ? (long long)a.n_seq * a.width : 0;
+  if (a.n_seq <= FORK_ONE_SEQS && a.max_rows <= FORK_ONE_ROWS && a.n_pages <= FORK_ONE_PAGES && places <= FORK_ONE_PLACES) {
+    const int threads = a.n_seq <= 256 && a.max_rows <= 1024 && a.n_pages <= 4096 && places <= 2048 ? 256 : 1024;
     hipLaunchKernelGGL(kv4_fork_one_kernel, dim3(1), dim3(threads), 0, st, a);
   } else {
     // (how many places a step counts and writes is known on the device alone)
-    const dim3 wide(512), seqs(min(256, (a.n_seq + 255) / 256));
+    const dim3 wide(512);
     const dim3 pages(min(1024, max(kv4_fork_chunks(a.n_pages), (a.n_seq + 255) / 256)));
     hipLaunchKernelGGL(kv4_fork_scan_kernel, dim3(1), dim3(1024), 0, st, a);
     hipLaunchKernelGGL(kv4_fork_count_kernel, wide, block, 0, st, a);
-    hipLaunchKernelGGL(kv4_fork_mark_kernel, seqs, block, 0, st, a);
     hipLaunchKernelGGL(kv4_fork_ask_kernel, pages, block, 0, st, a);
     hipLaunchKernelGGL(kv4_fork_sum_kernel, dim3(1), dim3(1024), 0, st, a);
     hipLaunchKernelGGL(kv4_fork_list_kernel, wide, block, 0, st, a);
     hipLaunchKernelGGL(kv4_fork_place_kernel, wide, block, 0, st, a);
-    hipLaunchKernelGGL(kv4_fork_none_kernel, seqs, block, 0, st, a);
   }
   const long long most = (long long)a.n_seq * a.n_layers * a.n_kv;
   hipLaunchKernelGGL(kv4_fork_copy_kernel, dim3((unsigned)(most < 2048 ? most : 2048)), block, 0, st, a);
