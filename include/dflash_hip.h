@@ -372,6 +372,18 @@ typedef struct dfl_kv4_attn {
 int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream);
 int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq);
 
+/* The same where sequences share pages.  groups [n_groups + 1] (device, ascending, within 0 .. n_seq)
+ * names groups of sequences, group g's being groups[g] .. groups[g+1] - 1.  The pages that are the same,
+ * from the first on, in the tables of all of a group's sequences that have rows, and whose keys all
+ * those rows see (causal: that lie before each sequence's new rows), are attended once for all the
+ * group's rows; each sequence's rest follows, and the two states are joined in fp32.  Results are those
+ * of dfl_kv4_attend to the order of fp32 sums and the choice of kernel (which follows, for the shared
+ * keys, from n_groups in place of n_seq), whatever the tables hold.  Groups out of order set bit 7, and
+ * nothing is shared.  It pays where a group's rows come to read many keys less: for tokens or small
+ * blocks of several sequences behind a long text.  ws: dfl_kv4_attend_shared_ws(...) bytes. */
+int dfl_kv4_attend_shared(const dfl_kv4_attn* args, const int32_t* groups, int32_t n_groups, void* stream);
+int64_t dfl_kv4_attend_shared_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq, int32_t n_groups);
+
 /* ---- Verification of drafted blocks (the reference's caller compares argmax ids on the host,
  * generate.py:614-728; this is its form for sampled tokens, on the device) ----
  *

@@ -1772,8 +1772,7 @@ int64_t dfl_kv4_attend_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t
   return kv4_ws_bytes(c.tile_rows, c.workers);
 }
 
-int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
-  if (!args) return fail(DFL_EINVAL, "dfl_kv4_attend: null argument");
+static Kv4AttnArgs kv4_attn_args(const dfl_kv4_attn* args) {
   Kv4AttnArgs a{};
   a.q = args->q;
   a.out = args->out;
@@ -1796,6 +1795,12 @@ int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
   a.pool = args->pool;
   a.ws = static_cast<float*>(args->ws);
   a.err = args->err_flags;
+  return a;
+}
+
+int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
+  if (!args) return fail(DFL_EINVAL, "dfl_kv4_attend: null argument");
+  const Kv4AttnArgs a = kv4_attn_args(args);
   if (a.n_rows == 0) return DFL_OK;
   if (const char* e = check_kv4_attn(a)) return fail(DFL_EINVAL, std::string("dfl_kv4_attend: ") + e);
   const int64_t need = dfl_kv4_attend_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
@@ -1803,6 +1808,29 @@ int dfl_kv4_attend(const dfl_kv4_attn* args, void* stream) {
     return fail(DFL_EINVAL, "dfl_kv4_attend: workspace of " + std::to_string(need) + " bytes needed");
   launch_kv4_attend(a, (hipStream_t)stream);
   return check_launch("dfl_kv4_attend");
+}
+
+int64_t dfl_kv4_attend_shared_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, int32_t n_seq, int32_t n_groups) {
+  if (n_rows < 1 || n_heads < 1 || n_kv < 1 || n_seq < 1 || n_heads % n_kv || n_groups < 1 || n_groups > n_seq) return 0;
+  return kv4_shared_ws(n_rows, n_heads, n_kv, n_seq, n_groups).bytes;
+}
+
+int dfl_kv4_attend_shared(const dfl_kv4_attn* args, const int32_t* groups, int32_t n_groups, void* stream) {
+  if (!args) return fail(DFL_EINVAL, "dfl_kv4_attend_shared: null argument");
+  const Kv4AttnArgs a = kv4_attn_args(args);
+  if (n_groups < 1 || n_groups > a.n_seq || !groups)
+    return fail(DFL_EINVAL, "dfl_kv4_attend_shared: groups outside [1, sequences], or null");
+  if (a.n_rows == 0) return DFL_OK;
+  const char* e = check_kv4_attn(a);
+  Kv4AttnArgs b = a;   // (the shared part: groups in place of sequences)
+  b.n_seq = n_groups;
+  if (!e) e = check_kv4_attn(b);
+  if (e) return fail(DFL_EINVAL, std::string("dfl_kv4_attend_shared: ") + e);
+  const int64_t need = dfl_kv4_attend_shared_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
+  if (!a.ws || args->ws_bytes < need)
+    return fail(DFL_EINVAL, "dfl_kv4_attend_shared: workspace of " + std::to_string(need) + " bytes needed");
+  launch_kv4_attend_shared(a, groups, n_groups, (hipStream_t)stream);
+  return check_launch("dfl_kv4_attend_shared");
 }
 
 // ---- verification of drafted blocks: context-free entry points over dfl_verify.hip ----

@@ -149,6 +149,21 @@ struct Kv4AttnArgs {
   float* ws;
   int workers;                 // workgroups that share the places (Kv4Cut)
   int* err;
+  const int* ends;             // where the sequences' rows end (starts + 1)
+  // attention in two parts (KV4_SHARED, KV4_REST):
+  const int* place;            // [n_seq] the sequence whose pages a group shares; the first pages left out
+  float *state_o, *state_ml;   // [n_rows][n_heads] the first part's sums [128], (max, sum of weights)
+};
+// Parts of an attention: all keys; those that a group of sequences shares, for all of the group's rows,
+// which leave their states; the rest of each sequence, whose results join those.
+enum { KV4_WHOLE = 0, KV4_SHARED = 1, KV4_REST = 2 };
+// What the two parts go by, found from the tables of groups of sequences: groups' row ranges, shared
+// lengths and a sequence that has their pages; sequences' pages left out and lengths after them.
+struct Kv4Groups { int *q0, *q1, *len, *of, *skip, *rest; };
+struct Kv4GroupArgs {
+  const int* groups;           // [n_groups + 1] sequences of group g: groups[g] .. groups[g + 1] - 1
+  int n_groups;
+  Kv4Groups out;
 };
 
 // The work of a launch.  Sequence s contributes, for each kv head and each of its query tiles, one
@@ -224,7 +239,7 @@ DFL_HD long long kv4_piece(long long w, long long per, long long r0) {
 // sum) a row.
 DFL_HD long long kv4_piece_floats(int tile_rows) { return (long long)tile_rows * (KV4_D + 2); }
 // What a worker notes of a shared unit for the merge.
-struct Kv4Note { int w1, head, tile, q0, qlen, len, pad[2]; };
+struct Kv4Note { int w1, head, tile, q0, qlen, len, s, pad; };
 // Bytes of a launch's workspace.
 DFL_HD long long kv4_ws_bytes(int tile_rows, int workers) {
   return workers * (2 * kv4_piece_floats(tile_rows) * (long long)sizeof(float) + (long long)sizeof(Kv4Note));
@@ -260,6 +275,20 @@ inline Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
   c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
   c.workers = KV4_CUS * (c.tile_rows == 16 ? 3 : 2);
   return c;
+}
+
+// Workspace of an attention in two parts: the larger of their workspaces, the states, the groups.
+struct Kv4SharedWs { long long state_o, state_ml, groups, bytes; };   // offsets
+inline Kv4SharedWs kv4_shared_ws(int n_rows, int n_heads, int n_kv, int n_seq, int n_groups) {
+  const Kv4Cut c = kv4_cut(n_rows, n_heads, n_kv, n_groups), d = kv4_cut(n_rows, n_heads, n_kv, n_seq);
+  const long long x = kv4_ws_bytes(c.tile_rows, c.workers), y = kv4_ws_bytes(d.tile_rows, d.workers);
+  const long long rows = (long long)n_rows * n_heads;
+  Kv4SharedWs w{};
+  w.state_o = ((x > y ? x : y) + 15) / 16 * 16;
+  w.state_ml = w.state_o + rows * KV4_D * 4;
+  w.groups = w.state_ml + rows * 8;
+  w.bytes = w.groups + 4ll * (4ll * n_groups + 2ll * n_seq);
+  return w;
 }
 
 inline const char* check_kv4_pool(int n_kv, int page_shift, int n_pages) {
@@ -334,5 +363,6 @@ void launch_kv4_fork(const Kv4ForkArgs& a, hipStream_t st);
 void launch_kv4_append(const Kv4RowsArgs& a, hipStream_t st);
 void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st);
 void launch_kv4_attend(const Kv4AttnArgs& a, hipStream_t st);
+void launch_kv4_attend_shared(const Kv4AttnArgs& a, const int* groups, int n_groups, hipStream_t st);
 
 }  // namespace dfl

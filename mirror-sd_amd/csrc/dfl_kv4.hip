@@ -583,7 +583,7 @@ DFL_DEV Lanes attn_lanes(const Kv4AttnArgs& a, int tile_rows, int s0, bool repor
   const int s = s0 + lane_again();
   Lanes l{0, 0, 0, 0};
   if (s < a.n_seq) {
-    l = Lanes{a.starts[s], a.starts[s + 1], a.lens[s], 0};
+    l = Lanes{a.starts[s], a.ends[s], a.lens[s], 0};
     const Kv4Seq q = kv4_seq(l.q0, l.q1, l.len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv,
                              tile_rows, a.causal);
     if (q.bad && report) atomicOr(a.err, KV4_ERR_PAGE);
@@ -742,11 +742,33 @@ DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows, int wave) {
 DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, int wave, long long per, const Run& r) {
   if (wave || lane_again()) return;
   kv4_notes(a, tile_rows)[worker_of(a, blockIdx.x)] = Kv4Note{
-      (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, 0, 0};
+      (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, r.s, 0};
+}
+// A sequence's (or group's) places in the table.
+template <int PART>
+DFL_DEV const int* table_row(const Kv4AttnArgs& a, int s) {
+  if constexpr (PART == KV4_SHARED) return a.table + (long long)load_const(a.place + s) * a.width;
+  else if constexpr (PART == KV4_REST) return a.table + (long long)s * a.width + load_const(a.place + s);
+  else return a.table + (long long)s * a.width;
+}
+// A row's state (sums o, relative to the reference m, and l of its weights), where the keys of another
+// part may count too: 4 values of it.  Those of KV4_SHARED are kept for KV4_REST, in which sequences
+// that left out pages join them.
+DFL_DEV void keep_state(const Kv4AttnArgs& a, long long orow, int col, floatx4 o, float m, float l) {
+  *reinterpret_cast<floatx4*>(a.state_o + orow * KV4_D + col) = o;
+  if (col == 0) *reinterpret_cast<floatx2*>(a.state_ml + 2 * orow) = (floatx2){m, l};
+}
+DFL_DEV void join_state(const Kv4AttnArgs& a, long long orow, int col, floatx4& o, float& m, float& l) {
+  const floatx4 x = *reinterpret_cast<const floatx4*>(a.state_o + orow * KV4_D + col);
+  const floatx2 y = *reinterpret_cast<const floatx2*>(a.state_ml + 2 * orow);
+  const float top = fmaxf(m, y.x), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(y.x - top);
+  o = o * f + x * g;
+  l = l * f + y.y * g;
+  m = top;
 }
 // The page of block b of a run's keys; -1: there is no such page (its keys are absent).
-DFL_DEV int page_of(const Kv4AttnArgs& a, const Run& r, int b) {
-  const int page = load_const(a.table + (long long)r.s * a.width + (b >> (a.page_shift - 5)));
+DFL_DEV int page_of(const Kv4AttnArgs& a, const int* row, int b) {
+  const int page = load_const(row + (b >> (a.page_shift - 5)));
   return page >= a.n_pages || page < 0 ? -1 : page;
 }
 // Address of block b in a page (for page -1 some address in the pool).
@@ -769,7 +791,7 @@ constexpr int VROW = 288;                 // bytes of a V row in LDS: 8 banks ap
                                           // rows of a half wave's transposing read do not collide
 constexpr int VWAVE = 32 * VROW;
 
-template <typename T, int NT>
+template <typename T, int NT, int PART>
 __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnArgs a) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
@@ -822,8 +844,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
     u32x4 kc[2], vc[2];
     uint32_t sc = 0;
     int pg = 0;
+    const int* const trow = table_row<PART>(a, run.s);
     auto load_block = [&](int b) {
-      pg = page_of(a, run, b);
+      pg = page_of(a, trow, b);
       const unsigned char* p = block_in(a, run, b, pg);
       kc[0] = load_vec(p + kv4_code_at(i, g, 0));
       kc[1] = load_vec(p + kv4_code_at(16 + i, g, 0));
@@ -1019,18 +1042,26 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       } else if (r < n_row) {
         const int tok = r / ratio;
         const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + r - tok * ratio;
-        const bool none = l == 0.f;   // a row that sees no key: zeros, and the sum of none
-        T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * ge;
+        if constexpr (PART == KV4_SHARED) {
 #pragma unroll
-        for (int dd = 0; dd < 2; ++dd) {
-          typedef T v4 __attribute__((ext_vector_type(4)));
-          v4 x;
+          for (int dd = 0; dd < 2; ++dd) keep_state(a, orow, 4 * ge + 16 * (2 * wv + dd), sum[dd], m, l);
+        } else {
+          const bool joins = PART == KV4_REST && load_const(a.place + run.s) > 0;
+          T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * ge;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l);
-          *reinterpret_cast<v4*>(op + 16 * (2 * wv + dd)) = x;
+          for (int dd = 0; dd < 2; ++dd) {
+            float m_all = m, l_all = l;
+            if (joins) join_state(a, orow, 4 * ge + 16 * (2 * wv + dd), sum[dd], m_all, l_all);
+            const bool none = l_all == 0.f;   // a row that sees no key: zeros, and the sum of none
+            typedef T v4 __attribute__((ext_vector_type(4)));
+            v4 x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l_all);
+            *reinterpret_cast<v4*>(op + 16 * (2 * wv + dd)) = x;
+            if (a.lse && wv == 0 && g == 0 && dd == 0)
+              a.lse[orow] = none ? -INFINITY : (m_all - KV4_LIFT + __log2f(l_all)) * 0.69314718056f;
+          }
         }
-        if (a.lse && wv == 0 && g == 0)
-          a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
       }
     }
     __syncthreads();   // mls is written again
@@ -1187,7 +1218,7 @@ DFL_DEV const Kv4AttnArgs& args_again() {
   return *(const Kv4AttnArgs*)p;
 }
 
-template <typename T>
+template <typename T, int PART>
 __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
@@ -1260,7 +1291,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
     // Addresses of blocks, 64 at a time, a lane each (past the last block the last one again, so
     // that the count of loads under way is always the same).
     const int subs = a.page_shift - 5;
-    const int* trow = a.table + (long long)run.s * a.width;
+    const int* trow = table_row<PART>(a, run.s);
     const uint32_t per_page = (uint32_t)a.n_kv << subs, of_head = (uint32_t)run.head << subs;
     int abase = 0;                       // the first of the 64
     uint32_t mine = 0;                   // (their numbers: a register less)
@@ -1524,21 +1555,47 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
       } else if (row0 + (le & 31) < n_row) {
         const int row = row0 + (le & 31), tok = row / ratio;
         const long long orow = (long long)(sq.q0 + tok) * e.n_heads + (run.head - tok) * ratio + row;
-        const bool none = lrun == 0.f;   // a row that sees no key: zeros, and the sum of none
-        const float f = (1.f / M::kUnit) / lrun;
-        T* op = reinterpret_cast<T*>(e.out) + orow * KV4_D + 4 * (le >> 5);
+        auto of = [&](int d, int k) __attribute__((always_inline)) {   // 4 values at 32 d + 8 k + 4 (le / 32)
+          return (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+        };
+        if constexpr (PART == KV4_SHARED) {
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+          for (int d = 0; d < 4; ++d)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            typedef T v4 __attribute__((ext_vector_type(4)));
-            v4 x;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[d][4 * k + j] * f);
-            *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
+            for (int k = 0; k < 4; ++k)
+              keep_state(e, orow, 32 * d + 8 * k + 4 * (le >> 5), of(d, k) * (1.f / M::kUnit), mrun, lrun);
+        } else {
+          const bool joins = PART == KV4_REST && load_const(e.place + run.s) > 0;
+          bool none = lrun == 0.f;   // a row that sees no key: zeros, and the sum of none
+          float f = (1.f / M::kUnit) / lrun, m_all = mrun, l_all = lrun;
+          if (joins) {
+            floatx4 unused = {0.f, 0.f, 0.f, 0.f};
+            join_state(e, orow, 0, unused, m_all, l_all);
+            none = l_all == 0.f;
           }
-        if (e.lse && le < 32)
-          e.lse[orow] = none ? -INFINITY : (mrun - KV4_LIFT + __log2f(lrun)) * 0.69314718056f;
+          T* op = reinterpret_cast<T*>(e.out) + orow * KV4_D + 4 * (le >> 5);
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              typedef T v4 __attribute__((ext_vector_type(4)));
+              v4 x;
+              floatx4 y = of(d, k);
+              if (joins) {
+                float m = mrun, l = lrun;
+                y *= 1.f / M::kUnit;
+                join_state(e, orow, 32 * d + 8 * k + 4 * (le >> 5), y, m, l);
+                y = y / l;
+              } else {
+                y *= f;
+              }
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : y[j]);
+              *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
+            }
+          if (e.lse && le < 32)
+            e.lse[orow] = none ? -INFINITY : (m_all - KV4_LIFT + __log2f(l_all)) * 0.69314718056f;
+        }
       }
       more = walk_next(e, ROWS, walk, run);
       kept = Kept{walk, run};
@@ -1552,7 +1609,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
 // are kv4_tile_kernel's.  Bound by them: eight blocks leave 550 of 66 KB, 10.6 us with the launch.
 // Two partials (most of a prompt's) or eight are loaded at once: one by one two prompts' took 30 us
 // for 16.  Which they are is in notes: every workgroup finding its unit by itself took 40 us more.
-template <typename T, bool TILE>
+template <typename T, bool TILE, int PART>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
   const int lane = threadIdx.x & 63;
   const int ratio = a.n_heads / a.n_kv;
@@ -1608,6 +1665,12 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
   }
   const int tok = r / ratio;
   const long long orow = (long long)(n.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
+  if constexpr (PART == KV4_SHARED) {
+    keep_state(a, orow, col, o, m, l);
+    return;
+  }
+  if constexpr (PART == KV4_REST)
+    if (a.place[n.s] > 0) join_state(a, orow, col, o, m, l);
   const bool none = l == 0.f;
   typedef T v4 __attribute__((ext_vector_type(4)));
   v4 x;
@@ -1618,16 +1681,126 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
     a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
 }
 
-template <typename T>
-void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
+// What the sequences of a group share: the pages, from the first on, that are the same in the tables of
+// all that have rows, and whose keys all those rows see whole.  A workgroup to a group; a wave compares
+// a sequence's places with the group's first one's, 4 a lane.  Ranges or lengths that do not fit leave
+// the group nothing to share (the rest finds and reports them); boundaries out of order leave all groups
+// so.  128 sequences of 512 shared pages: 7 us.
+__global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4GroupArgs g) {
+  typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
+  __shared__ int shared_pages, first;
+  const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wv = t >> 6;
+  bool bad = false;
+  for (int i = t; i < g.n_groups; i += nt) bad |= g.groups[i] > g.groups[i + 1];
+  bad |= g.groups[0] < 0 || g.groups[g.n_groups] > a.n_seq;
+  const bool none = __syncthreads_or(bad);
+  const int i = blockIdx.x, s0 = none ? 0 : g.groups[i], s1 = none ? 0 : g.groups[i + 1];
+  if (none && i == 0 && t == 0) atomicOr(a.err, KV4_ERR_PAGE);
+  if (t == 0) {
+    shared_pages = a.width;
+    first = INT32_MAX;
+  }
+  __syncthreads();
+  // the fewest whole pages that a row sees, and the first sequence with rows
+  int most = a.width, lowest = INT32_MAX, rows = 0;
+  for (int s = s0 + t; s < s1; s += nt) {
+    const int q0 = a.starts[s], q1 = a.ends[s], len = a.lens[s];
+    const bool fits = q0 >= 0 && q1 >= q0 && q1 <= a.n_rows && len >= 0 && len <= ((long long)a.width << a.page_shift);
+    if (!fits) {
+      most = 0;
+    } else if (q1 > q0) {
+      most = min(most, max(0, a.causal ? len - (q1 - q0) : len) >> a.page_shift);
+      lowest = min(lowest, s);
+      ++rows;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    most = min(most, __shfl_xor(most, o, 64));
+    lowest = min(lowest, __shfl_xor(lowest, o, 64));
+  }
+  if (lane == 0) {
+    atomicMin(&shared_pages, most);
+    atomicMin(&first, lowest);
+  }
+  rows = __syncthreads_count(rows > 1) ? 2 : __syncthreads_count(rows > 0);   // (two or more: some share)
+  most = rows > 1 ? shared_pages : 0;
+  const int one = first;
+  __syncthreads();
+  if (rows > 1) {
+    // the first place at which some sequence differs
+    const int* p = a.table + (long long)one * a.width;
+    int same = most;
+    for (int j0 = 0; j0 < most; j0 += 256) {
+      const int j = j0 + 4 * lane, last = max(0, a.width - 4);
+      auto four = [&](const int* row) {
+        int4u v = {-1, -1, -1, -1};
+        if (a.width >= 4) {
+          v = *reinterpret_cast<const int4u*>(row + min(j, last));   // (past the last place: places before)
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) if (k < a.width) v[k] = row[k];
+        }
+        return v;
+      };
+      const int at = a.width >= 4 ? min(j, last) : 0;
+      const int4u x = four(p);
+#pragma unroll
+      for (int k = 3; k >= 0; --k)
+        if (at + k < same && (x[k] < 0 || x[k] >= a.n_pages)) same = at + k;
+#pragma unroll 4
+      for (int s = s0 + wv; s < s1; s += nt >> 6) {
+        const int4u y = four(a.table + (long long)s * a.width);
+        const bool idle = a.ends[s] <= a.starts[s];
+#pragma unroll
+        for (int k = 3; k >= 0; --k)
+          if (!idle && at + k < same && x[k] != y[k]) same = at + k;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) same = min(same, __shfl_xor(same, o, 64));
+    if (lane == 0) atomicMin(&shared_pages, same);
+    __syncthreads();
+    most = shared_pages;
+  }
+  for (int s = s0 + t; s < s1; s += nt) {
+    const int skip = a.ends[s] > a.starts[s] ? most : 0;
+    g.out.skip[s] = skip;
+    g.out.rest[s] = a.lens[s] - (skip << a.page_shift);
+  }
+  if (t == 0) {
+    g.out.q0[i] = most ? a.starts[s0] : 0;
+    g.out.q1[i] = most ? a.ends[s1 - 1] : 0;
+    g.out.len[i] = most << a.page_shift;
+    g.out.of[i] = most ? one : 0;
+  }
+  // sequences of no group
+  const int low = none ? 0 : g.groups[0], high = none ? 0 : g.groups[g.n_groups];
+  for (int s = i * nt + t; s < a.n_seq; s += nt * g.n_groups)
+    if (s < low || s >= high) {
+      g.out.skip[s] = 0;
+      g.out.rest[s] = a.lens[s];
+    }
+}
+
+template <typename T, int PART>
+void attend_part(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
   const dim3 grid(a.workers), block(256), mgrid(a.workers * (c.tile_rows / 8));
   switch (c.tile_rows) {
-    case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1>), grid, block, 0, st, a); break;
-    case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((kv4_tile_kernel<T>), grid, block, TILE_LDS, st, a);
+    case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1, PART>), grid, block, 0, st, a); break;
+    case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2, PART>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((kv4_tile_kernel<T, PART>), grid, block, TILE_LDS, st, a);
   }
-  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
-  else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);
+  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false, PART>), mgrid, block, 0, st, a, c.tile_rows);
+  else hipLaunchKernelGGL((kv4_merge_kernel<T, true, PART>), mgrid, block, 0, st, a, c.tile_rows);
+}
+template <int PART>
+void attend(const Kv4AttnArgs& a_in, hipStream_t st) {
+  Kv4AttnArgs a = a_in;
+  const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
+  a.workers = c.workers;
+  if (a.dtype == 1) attend_part<half_t, PART>(a, c, st);
+  else attend_part<bf16_t, PART>(a, c, st);
 }
 
 }  // namespace
@@ -1665,10 +1838,31 @@ void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st) {
 }
 void launch_kv4_attend(const Kv4AttnArgs& a_in, hipStream_t st) {
   Kv4AttnArgs a = a_in;
-  const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
-  a.workers = c.workers;
-  if (a.dtype == 1) attend<half_t>(a, c, st);
-  else attend<bf16_t>(a, c, st);
+  a.ends = a.starts + 1;
+  attend<KV4_WHOLE>(a, st);
+}
+void launch_kv4_attend_shared(const Kv4AttnArgs& a_in, const int* groups, int n_groups, hipStream_t st) {
+  Kv4AttnArgs a = a_in;
+  a.ends = a.starts + 1;
+  const Kv4SharedWs w = kv4_shared_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
+  char* ws = reinterpret_cast<char*>(a.ws);
+  a.state_o = reinterpret_cast<float*>(ws + w.state_o);
+  a.state_ml = reinterpret_cast<float*>(ws + w.state_ml);
+  int* p = reinterpret_cast<int*>(ws + w.groups);
+  Kv4GroupArgs g{groups, n_groups, {p, p + n_groups, p + 2ll * n_groups, p + 3ll * n_groups, p + 4ll * n_groups,
+                                    p + 4ll * n_groups + a.n_seq}};
+  hipLaunchKernelGGL(kv4_groups_kernel, dim3(n_groups), dim3(1024), 0, st, a, g);
+  Kv4AttnArgs b = a;
+  b.n_seq = n_groups;
+  b.causal = 0;
+  b.starts = g.out.q0;
+  b.ends = g.out.q1;
+  b.lens = g.out.len;
+  b.place = g.out.of;
+  attend<KV4_SHARED>(b, st);
+  a.lens = g.out.rest;
+  a.place = g.out.skip;
+  attend<KV4_REST>(a, st);
 }
 
 }  // namespace dfl

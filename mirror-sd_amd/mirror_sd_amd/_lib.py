@@ -129,6 +129,8 @@ SIGNATURES = {
                                c_void_p, c_void_p, c_void_p, c_void_p]),
     "dfl_kv4_attend": (c_int32, [ctypes.POINTER(DflKv4Attn), c_void_p]),
     "dfl_kv4_attend_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "dfl_kv4_attend_shared": (c_int32, [ctypes.POINTER(DflKv4Attn), c_void_p, c_int32, c_void_p]),
+    "dfl_kv4_attend_shared_ws": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "dfl_kv4_fork": (c_int32, [ctypes.POINTER(DflKv4Fork), c_void_p]),
     "dfl_kv4_fork_scratch": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
     "dfl_verify": (c_int32, [ctypes.POINTER(DflVerify), c_void_p]),

@@ -256,7 +256,7 @@ class KV4Cache:
         return k, v
 
     def attend(self, q, starts, layer: int = 0, causal: bool = False, scale: Optional[float] = None,
-               return_lse: bool = False, out=None):
+               return_lse: bool = False, out=None, groups=None):
         """Attention of query rows ``q`` [n, heads, 128] (fp16 or bf16; ``heads`` a multiple of
         n_kv_heads, head h reads kv head h // (heads // n_kv_heads)) over the cached rows: rows
         ``starts[s] .. starts[s + 1] - 1`` ([max_seqs + 1]) are sequence s's.  Each sees all
@@ -267,7 +267,13 @@ class KV4Cache:
         does not overlap it), with ``return_lse`` also the fp32 log of the sum of exponentials
         [n, heads], by which results over different keys can be joined.  A row that sees no key
         gives zeros and -inf.  Rows that belong to no sequence are not written (what ``out`` held,
-        else anything)."""
+        else anything).
+
+        ``groups`` [n_groups + 1] names sequences that go on from one text: those of group g are
+        ``groups[g] .. groups[g + 1] - 1``.  Pages that all of a group's sequences (those with rows) hold
+        from the first on, and whose keys all their rows see, are then read once for the group,
+        not once a sequence.  Which they are is found from the tables, so the results are those of a
+        call without groups (to the rounding of sums in another order), whatever is shared."""
         import torch
         q = self._rows(q, None, "q")
         n, heads = q.shape[0], q.shape[1]
@@ -288,7 +294,14 @@ class KV4Cache:
             if out is None:
                 out = torch.empty((n, heads, HEAD_DIM), dtype=q.dtype, device=self.device)
             lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if return_lse else None
-            ws_bytes = self._L.dfl_kv4_attend_ws(n, heads, self.n_kv_heads, self.max_seqs)
+            if groups is None:
+                ws_bytes = self._L.dfl_kv4_attend_ws(n, heads, self.n_kv_heads, self.max_seqs)
+            else:
+                groups = self._ints(groups, None, "groups")
+                n_groups = groups.shape[0] - 1
+                if not 1 <= n_groups <= self.max_seqs:
+                    raise ValueError(f"groups must hold 2 to {self.max_seqs + 1} numbers, got {n_groups + 1}")
+                ws_bytes = self._L.dfl_kv4_attend_shared_ws(n, heads, self.n_kv_heads, self.max_seqs, n_groups)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self.device)
             a = _lib.DflKv4Attn(   # (in the order of its fields: names cost 3 us)
                 q.data_ptr(), out.data_ptr(), _lib.ptr(lse), q.stride(0), q.stride(1),
@@ -296,7 +309,11 @@ class KV4Cache:
                 HEAD_DIM ** -0.5 if scale is None else float(scale), starts.data_ptr(),
                 self.lens.data_ptr(), self.table.data_ptr(), self.width, self.page, self.n_pages,
                 self._layer(layer), ws.data_ptr(), ws_bytes, self._err.data_ptr())
-            _lib.check(self._L.dfl_kv4_attend(ctypes.byref(a), self._stream()), "dfl_kv4_attend")
+            if groups is None:
+                _lib.check(self._L.dfl_kv4_attend(ctypes.byref(a), self._stream()), "dfl_kv4_attend")
+            else:
+                _lib.check(self._L.dfl_kv4_attend_shared(ctypes.byref(a), groups.data_ptr(), n_groups,
+                                                         self._stream()), "dfl_kv4_attend_shared")
         return (out, lse) if return_lse else out
 
     def errors(self) -> int:
