@@ -1821,11 +1821,7 @@ int dfl_kv4_attend_shared(const dfl_kv4_attn* args, const int32_t* groups, int32
   if (n_groups < 1 || n_groups > a.n_seq || !groups)
     return fail(DFL_EINVAL, "dfl_kv4_attend_shared: groups outside [1, sequences], or null");
   if (a.n_rows == 0) return DFL_OK;
-  const char* e = check_kv4_attn(a);
-  Kv4AttnArgs b = a;   // (the shared part: groups in place of sequences)
-  b.n_seq = n_groups;
-  if (!e) e = check_kv4_attn(b);
-  if (e) return fail(DFL_EINVAL, std::string("dfl_kv4_attend_shared: ") + e);
+  if (const char* e = check_kv4_attn(a, n_groups)) return fail(DFL_EINVAL, std::string("dfl_kv4_attend_shared: ") + e);
   const int64_t need = dfl_kv4_attend_shared_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
   if (!a.ws || args->ws_bytes < need)
     return fail(DFL_EINVAL, "dfl_kv4_attend_shared: workspace of " + std::to_string(need) + " bytes needed");

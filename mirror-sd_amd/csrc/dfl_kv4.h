@@ -150,21 +150,20 @@ struct Kv4AttnArgs {
   int workers;                 // workgroups that share the places (Kv4Cut)
   int* err;
   const int* ends;             // where the sequences' rows end (starts + 1)
-  // attention in two parts (KV4_SHARED, KV4_REST):
-  const int* place;            // [n_seq] the sequence whose pages a group shares; the first pages left out
-  float *state_o, *state_ml;   // [n_rows][n_heads] the first part's sums [128], (max, sum of weights)
-};
-// Parts of an attention: all keys; those that a group of sequences shares, for all of the group's rows,
-// which leave their states; the rest of each sequence, whose results join those.
-enum { KV4_WHOLE = 0, KV4_SHARED = 1, KV4_REST = 2 };
-// What the two parts go by, found from the tables of groups of sequences: groups' row ranges, shared
-// lengths and a sequence that has their pages; sequences' pages left out and lengths after them.
-struct Kv4Groups { int *q0, *q1, *len, *of, *skip, *rest; };
-struct Kv4GroupArgs {
-  const int* groups;           // [n_groups + 1] sequences of group g: groups[g] .. groups[g + 1] - 1
+  // attention with shared keys: the first n_groups of the n_seq sequences are groups' shared keys, not
+  // causal, the others the sequences' own rest
   int n_groups;
-  Kv4Groups out;
+  const long long* row_of;     // [n_seq] where a sequence's pages begin in the table
+  const int* skip;             // [n_seq - n_groups] pages of a sequence that its group's keys hold
+  struct Kv4Rec* recs;         // [2][n_rows][n_heads] where a row's rest and shared part lie
+  float *state_o, *state_ml;   // [2][n_rows][n_heads] states of parts that one worker has whole: sums
+                               // [128], (reference, sum of weights)
+  int* seq_of;                 // [n_rows] the sequence of a row (any value for rows of none)
+  float* shared_ws;            // partials of the shared parts
 };
+// Workers (w0 .. w1) that have partials of a row's unit and its place in them; w0 -1: in the states, -2:
+// it is written already.
+struct Kv4Rec { int w0, w1, c, pad; };
 
 // The work of a launch.  Sequence s contributes, for each kv head and each of its query tiles, one
 // unit; units are numbered sequence by sequence, head by head, tile by tile.  A unit takes up
@@ -239,7 +238,7 @@ DFL_HD long long kv4_piece(long long w, long long per, long long r0) {
 // sum) a row.
 DFL_HD long long kv4_piece_floats(int tile_rows) { return (long long)tile_rows * (KV4_D + 2); }
 // What a worker notes of a shared unit for the merge.
-struct Kv4Note { int w1, head, tile, q0, qlen, len, s, pad; };
+struct Kv4Note { int w1, head, tile, q0, qlen, len, pad[2]; };
 // Bytes of a launch's workspace.
 DFL_HD long long kv4_ws_bytes(int tile_rows, int workers) {
   return workers * (2 * kv4_piece_floats(tile_rows) * (long long)sizeof(float) + (long long)sizeof(Kv4Note));
@@ -277,17 +276,53 @@ inline Kv4Cut kv4_cut(int n_rows, int n_heads, int n_kv, int n_seq) {
   return c;
 }
 
-// Workspace of an attention in two parts: the larger of their workspaces, the states, the groups.
-struct Kv4SharedWs { long long state_o, state_ml, groups, bytes; };   // offsets
+// How an attention with shared keys is cut.  Groups and sequences are in one launch, in tiles of as
+// many rows, or the groups are in one of tiles of 128 and the sequences in one of 16.
+struct Kv4SharedCut {
+  int own, shared;     // query rows of a unit in the sequences' own parts and the shared ones; 0: not shared
+  int workers, shared_workers;
+};
+inline Kv4SharedCut kv4_shared_cut(int n_rows, int n_heads, int n_kv, int n_seq, int n_groups) {
+  // Sequences of more than 16 rows of a kv head fill their tiles: keys read once more cost them
+  // little, and the group's states are written and read on top.  Us, attended apart and together (in
+  // tiles of 128): 16 sequences of 32 rows over 1651 to 7844 shared keys 37, 49; 8 over 32000 73, 69; 16
+  // of 64 rows over 8000 79, 73.
+  const Kv4Cut own = kv4_cut(n_rows, n_heads, n_kv, n_seq);
+  if (own.tile_rows != 16) return Kv4SharedCut{0, 0, 0, 0};
+  // Rows of a kv head in a group, on average.  Us in tiles of 16, 32 and 128, 4096 and 32768 shared
+  // keys: 128 rows 34 and 69, 34 and 62, 53 and 73; 256 rows 42 and 109, 42 and 91, 60 and 85; 512
+  // rows 57 and 183 (16), 72 and 119 (128).  (64 ragged tokens in groups of 17 rows a kv head to 132: 52, 54,
+  // 67; eight tokens behind 4096 keys, 40 rows: 30, 31, 49.)
+  const long long groups = n_groups < n_rows ? n_groups : n_rows, rows = (long long)n_rows * (n_heads / n_kv);
+  if (rows >= 512 * groups) return Kv4SharedCut{16, 128, own.workers, 2 * KV4_CUS};
+  if (rows >= 128 * groups) return Kv4SharedCut{32, 32, 2 * KV4_CUS, 0};
+  return Kv4SharedCut{16, 16, own.workers, 0};
+}
+// Its workspace (offsets).
+struct Kv4SharedWs { long long own, shared, state_o, state_ml, recs, row_of, q0, q1, len, skip, seq_of, bytes; };
 inline Kv4SharedWs kv4_shared_ws(int n_rows, int n_heads, int n_kv, int n_seq, int n_groups) {
-  const Kv4Cut c = kv4_cut(n_rows, n_heads, n_kv, n_groups), d = kv4_cut(n_rows, n_heads, n_kv, n_seq);
-  const long long x = kv4_ws_bytes(c.tile_rows, c.workers), y = kv4_ws_bytes(d.tile_rows, d.workers);
-  const long long rows = (long long)n_rows * n_heads;
+  const Kv4SharedCut c = kv4_shared_cut(n_rows, n_heads, n_kv, n_seq, n_groups);
+  const long long rows = (long long)n_rows * n_heads, all = (long long)n_groups + n_seq;
   Kv4SharedWs w{};
-  w.state_o = ((x > y ? x : y) + 15) / 16 * 16;
-  w.state_ml = w.state_o + rows * KV4_D * 4;
-  w.groups = w.state_ml + rows * 8;
-  w.bytes = w.groups + 4ll * (4ll * n_groups + 2ll * n_seq);
+  if (!c.own) {   // (that of an attention without groups)
+    const Kv4Cut d = kv4_cut(n_rows, n_heads, n_kv, n_seq);
+    w.bytes = kv4_ws_bytes(d.tile_rows, d.workers);
+    return w;
+  }
+  long long at = 0;
+  auto take = [&](long long n) { const long long p = at; at += (n + 15) / 16 * 16; return p; };
+  w.own = take(kv4_ws_bytes(c.own, c.workers));
+  w.shared = c.shared_workers ? take(kv4_ws_bytes(c.shared, c.shared_workers)) : w.own;
+  w.state_o = take(2 * rows * KV4_D * 4);
+  w.state_ml = take(2 * rows * 8);
+  w.recs = take(2 * rows * (long long)sizeof(Kv4Rec));
+  w.row_of = take(8 * all);
+  w.q0 = take(4 * all);
+  w.q1 = take(4 * all);
+  w.len = take(4 * all);
+  w.skip = take(4ll * n_seq);
+  w.seq_of = take(4ll * n_rows);
+  w.bytes = at;
   return w;
 }
 
@@ -337,7 +372,8 @@ inline const char* check_kv4_rows(const Kv4RowsArgs& a, bool append) {
   if ((a.k_row | a.k_head | a.v_row | a.v_head) & 7) return "row and head strides must be multiples of 8";
   return nullptr;
 }
-inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
+// n_groups: 0, or those of a launch with shared keys.
+inline const char* check_kv4_attn(const Kv4AttnArgs& a, int n_groups = 0) {
   if (const char* e = check_kv4_pool(a.n_kv, a.page_shift, a.n_pages)) return e;
   if (a.n_rows < 0) return "negative row count";
   if (a.n_heads < 1 || a.n_heads % a.n_kv) return "query heads must be a multiple of the kv heads";
@@ -347,8 +383,11 @@ inline const char* check_kv4_attn(const Kv4AttnArgs& a) {
   if (a.n_seq < 1 || a.n_seq > KV4_MAX_SEQS) return "sequences outside [1, 65536]";
   if (a.width < 1 || ((long long)a.width << a.page_shift) > 0x7fffffffll)
     return "table width out of range";
-  if (a.n_rows > 0 && !kv4_counts_fit(a.n_rows, a.n_heads / a.n_kv, a.n_kv, a.n_seq, a.width, a.page_shift,
-                                      kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq).tile_rows))
+  if (n_groups < 0 || n_groups > a.n_seq) return "more groups than sequences";
+  // (with shared keys every row is in two sequences)
+  if (n_groups && a.n_rows > 0x3fffffff) return "too many query rows";
+  if (a.n_rows > 0 && !kv4_counts_fit(n_groups ? 2 * a.n_rows : a.n_rows, a.n_heads / a.n_kv, a.n_kv, a.n_seq + n_groups,
+                                      a.width, a.page_shift, kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq).tile_rows))
     return "too many query rows for so long a table";
   if (!(a.scale_log2 > 0.f) || a.scale_log2 > 1e30f) return "scale must be positive and finite";
   if (!a.q || !a.out || !a.starts || !a.lens || !a.table || !a.pool || !a.err) return "null pointer";

@@ -577,6 +577,8 @@ DFL_DEV long long pick_ll(long long v, int lane) {
   return (long long)((unsigned long long)hi << 32 | lo);
 }
 DFL_DEV int pick(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+// (shared keys are seen by all of a group's rows)
+DFL_DEV bool is_causal(const Kv4AttnArgs& a, int s) { return a.causal && s >= a.n_groups; }
 // Sequences one lane each, 64 at a time: sequence s0 + lane's row range and length, and its places.
 struct Lanes { int q0, q1, len; long long cost; };
 DFL_DEV Lanes attn_lanes(const Kv4AttnArgs& a, int tile_rows, int s0, bool report) {
@@ -585,7 +587,7 @@ DFL_DEV Lanes attn_lanes(const Kv4AttnArgs& a, int tile_rows, int s0, bool repor
   if (s < a.n_seq) {
     l = Lanes{a.starts[s], a.ends[s], a.lens[s], 0};
     const Kv4Seq q = kv4_seq(l.q0, l.q1, l.len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv,
-                             tile_rows, a.causal);
+                             tile_rows, is_causal(a, s));
     if (q.bad && report) atomicOr(a.err, KV4_ERR_PAGE);
     l.cost = kv4_cost(q, a.n_kv);
   }
@@ -616,8 +618,9 @@ DFL_DEV int attn_tile(const Kv4Seq& s, long long r) {
 }
 
 // Visible keys of a token of a sequence (they grow with the token).
+template <bool MIXED>
 DFL_DEV int attn_visible(const Kv4AttnArgs& a, const Kv4Seq& q, int token) {
-  return a.causal ? max(0, min(q.len, q.len - q.qlen + token + 1)) : q.len;
+  return (MIXED ? q.slope != 0 : a.causal) ? max(0, min(q.len, q.len - q.qlen + token + 1)) : q.len;
 }
 
 // A unit, and where its places are.
@@ -637,7 +640,7 @@ DFL_DEV void unit_places(Unit& u) {
 DFL_DEV void unit_of(const Kv4AttnArgs& a, int tile_rows, int s, int q0, int q1, int len, long long at,
                      long long pos, Unit& u) {
   u.s = s;
-  u.sq = kv4_seq(q0, q1, len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, tile_rows, a.causal);
+  u.sq = kv4_seq(q0, q1, len, a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, tile_rows, is_causal(a, s));
   const long long of_head = kv4_places(u.sq, u.sq.tiles);
   u.head = (int)kv4_div(pos - at, of_head);
   u.head0 = at + u.head * of_head;
@@ -722,7 +725,7 @@ DFL_DEV bool walk_next(const Kv4AttnArgs& a, int tile_rows, Walk& k, Run& r) {
       const int i = __ffsll(some) - 1;
       r.s = s0 + i;
       r.sq = kv4_seq(pick(l.q0, i), pick(l.q1, i), pick(l.len, i), a.n_rows, a.width, a.page_shift,
-                     a.n_heads / a.n_kv, tile_rows, a.causal);
+                     a.n_heads / a.n_kv, tile_rows, is_causal(a, r.s));
       r.head = r.tile = 0;
       r.head0 = k.pos;
       break;
@@ -744,27 +747,30 @@ DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, int wave, long long 
   kv4_notes(a, tile_rows)[worker_of(a, blockIdx.x)] = Kv4Note{
       (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, r.s, 0};
 }
-// A sequence's (or group's) places in the table.
-template <int PART>
+// A sequence's places in the table.
+template <bool MIXED>
 DFL_DEV const int* table_row(const Kv4AttnArgs& a, int s) {
-  if constexpr (PART == KV4_SHARED) return a.table + (long long)load_const(a.place + s) * a.width;
-  else if constexpr (PART == KV4_REST) return a.table + (long long)s * a.width + load_const(a.place + s);
+  if constexpr (MIXED)
+    return a.table + *reinterpret_cast<const __attribute__((address_space(4))) long long*>(
+                         reinterpret_cast<uintptr_t>(a.row_of + s));
   else return a.table + (long long)s * a.width;
 }
-// A row's state (sums o, relative to the reference m, and l of its weights), where the keys of another
-// part may count too: 4 values of it.  Those of KV4_SHARED are kept for KV4_REST, in which sequences
-// that left out pages join them.
-DFL_DEV void keep_state(const Kv4AttnArgs& a, long long orow, int col, floatx4 o, float m, float l) {
-  *reinterpret_cast<floatx4*>(a.state_o + orow * KV4_D + col) = o;
-  if (col == 0) *reinterpret_cast<floatx2*>(a.state_ml + 2 * orow) = (floatx2){m, l};
+// With shared keys a row has up to two parts, its group's (1) and its own rest (0).  What a part's worker
+// leaves for the join: of a unit that it begins, where its partials or its state will be.
+DFL_DEV int part_of(const Kv4AttnArgs& a, int s) { return s < a.n_groups ? 1 : 0; }
+// Whether a unit's result is the row's (if it is whole).
+DFL_DEV bool is_final(const Kv4AttnArgs& a, int s) { return s >= a.n_groups && load_const(a.skip + (s - a.n_groups)) == 0; }
+DFL_DEV void leave_rec(const Kv4AttnArgs& a, const Run& r, long long per, int row, long long orow, int c) {
+  const long long rows = (long long)a.n_rows * a.n_heads;
+  a.recs[part_of(a, r.s) * rows + orow] =
+      r.whole ? Kv4Rec{is_final(a, r.s) ? -2 : -1, -1, c, 0}
+              : Kv4Rec{worker_of(a, blockIdx.x), (int)kv4_div(r.r0 + r.nblk - 1, per), c, 0};
+  if (r.s >= a.n_groups) a.seq_of[row] = r.s - a.n_groups;
 }
-DFL_DEV void join_state(const Kv4AttnArgs& a, long long orow, int col, floatx4& o, float& m, float& l) {
-  const floatx4 x = *reinterpret_cast<const floatx4*>(a.state_o + orow * KV4_D + col);
-  const floatx2 y = *reinterpret_cast<const floatx2*>(a.state_ml + 2 * orow);
-  const float top = fmaxf(m, y.x), f = __builtin_amdgcn_exp2f(m - top), g = __builtin_amdgcn_exp2f(y.x - top);
-  o = o * f + x * g;
-  l = l * f + y.y * g;
-  m = top;
+DFL_DEV void keep_state(const Kv4AttnArgs& a, int part, long long orow, int col, floatx4 o, float m, float l) {
+  const long long at = part * (long long)a.n_rows * a.n_heads + orow;
+  *reinterpret_cast<floatx4*>(a.state_o + at * KV4_D + col) = o;
+  if (col == 0) *reinterpret_cast<floatx2*>(a.state_ml + 2 * at) = (floatx2){m, l};
 }
 // The page of block b of a run's keys; -1: there is no such page (its keys are absent).
 DFL_DEV int page_of(const Kv4AttnArgs& a, const int* row, int b) {
@@ -791,7 +797,7 @@ constexpr int VROW = 288;                 // bytes of a V row in LDS: 8 banks ap
                                           // rows of a half wave's transposing read do not collide
 constexpr int VWAVE = 32 * VROW;
 
-template <typename T, int NT, int PART>
+template <typename T, int NT, bool MIXED>
 __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnArgs a) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
@@ -810,10 +816,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
   Walk walk;
   Run run;
   bool more = walk_begin(a, ROWS, walk, run);
-  walk_no_note(a, ROWS, wv);
+  if (!MIXED) walk_no_note(a, ROWS, wv);
   for (; more; more = walk_next(a, ROWS, walk, run)) {
     if (!walk_run(walk, run)) break;   // (the worker's last places)
-    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
+    if (!MIXED && run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
     const Kv4Seq& sq = run.sq;
     // query fragments: step st covers values 32 g + 8 st ..; visible keys of this lane's rows
     v8 qf[NT][4];
@@ -827,11 +833,16 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
                     (long long)(run.head * ratio + r - tok * ratio) * a.q_head + 32 * g;
 #pragma unroll
       for (int st = 0; st < 4; ++st) qf[n][st] = *reinterpret_cast<const v8*>(qp + 8 * st);
-      vis[n] = attn_visible(a, sq, tok);
+      vis[n] = attn_visible<MIXED>(a, sq, tok);
+      if (MIXED && run.b0 == 0 && wv == 0 && g == 0 && (run.tile * NT + n) * 16 + i < n_row)
+        leave_rec(a, run, walk.per, sq.q0 + tok, (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + r - tok * ratio,
+                  16 * n + i);
     }
-    const int vmin = attn_visible(a, sq, run.tile * ROWS / ratio);
-    const int vmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
+    const int vmin = attn_visible<MIXED>(a, sq, run.tile * ROWS / ratio);
+    const int vmax = attn_visible<MIXED>(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
 
+    // (tiles of 32 rows of which a unit has 16 at most: the others' softmax and products with V are left out)
+    const bool both = n_row - run.tile * ROWS > 16;
     floatx4 o[NT][8];
     float mrun[NT], lrun[NT];
 #pragma unroll
@@ -844,7 +855,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
     u32x4 kc[2], vc[2];
     uint32_t sc = 0;
     int pg = 0;
-    const int* const trow = table_row<PART>(a, run.s);
+    const int* const trow = table_row<MIXED>(a, run.s);
     auto load_block = [&](int b) {
       pg = page_of(a, trow, b);
       const unsigned char* p = block_in(a, run, b, pg);
@@ -947,6 +958,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       v8 pf[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if (MIXED && n > 0 && !both) break;
         float v[8];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -983,6 +995,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
           pf[n][r] = p.x;
           pf[n][r + 1] = p.y;
         }
+      }
+      if (MIXED && NT > 1 && !both) {
+        static_for<0, 8>([&](auto dt) {
+          constexpr int d = dt;
+          o[0][d] = M::mfma(read_vt<T>(vread + 32 * d, vread + 16 * VROW + 32 * d), pf[0], o[0][d]);
+        });
+        continue;
       }
       static_for<0, 8>([&](auto dt) {
         constexpr int d = dt;
@@ -1042,25 +1061,23 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void kv4_attn_kernel(Kv4AttnA
       } else if (r < n_row) {
         const int tok = r / ratio;
         const long long orow = (long long)(sq.q0 + tok) * a.n_heads + run.head * ratio + r - tok * ratio;
-        if constexpr (PART == KV4_SHARED) {
+        if (MIXED && !is_final(a, run.s)) {
 #pragma unroll
-          for (int dd = 0; dd < 2; ++dd) keep_state(a, orow, 4 * ge + 16 * (2 * wv + dd), sum[dd], m, l);
+          for (int dd = 0; dd < 2; ++dd)
+            keep_state(a, part_of(a, run.s), orow, 4 * ge + 16 * (2 * wv + dd), sum[dd], m, l);
         } else {
-          const bool joins = PART == KV4_REST && load_const(a.place + run.s) > 0;
+          const bool none = l == 0.f;   // a row that sees no key: zeros, and the sum of none
           T* op = reinterpret_cast<T*>(a.out) + orow * KV4_D + 4 * ge;
 #pragma unroll
           for (int dd = 0; dd < 2; ++dd) {
-            float m_all = m, l_all = l;
-            if (joins) join_state(a, orow, 4 * ge + 16 * (2 * wv + dd), sum[dd], m_all, l_all);
-            const bool none = l_all == 0.f;   // a row that sees no key: zeros, and the sum of none
             typedef T v4 __attribute__((ext_vector_type(4)));
             v4 x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l_all);
+            for (int k = 0; k < 4; ++k) x[k] = (T)(none ? 0.f : sum[dd][k] / l);
             *reinterpret_cast<v4*>(op + 16 * (2 * wv + dd)) = x;
-            if (a.lse && wv == 0 && g == 0 && dd == 0)
-              a.lse[orow] = none ? -INFINITY : (m_all - KV4_LIFT + __log2f(l_all)) * 0.69314718056f;
           }
+          if (a.lse && wv == 0 && g == 0)
+            a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
         }
       }
     }
@@ -1218,7 +1235,7 @@ DFL_DEV const Kv4AttnArgs& args_again() {
   return *(const Kv4AttnArgs*)p;
 }
 
-template <typename T, int PART>
+template <typename T, bool MIXED>
 __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
   typedef Mat<T> M;
   typedef typename M::v8 v8;
@@ -1247,20 +1264,23 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
     more = walk_begin(args, ROWS, walk, run);
     kept = Kept{walk, run};
   }
-  walk_no_note(args, ROWS, wv);
+  if (!MIXED) walk_no_note(args, ROWS, wv);
   while (more) {
     Walk walk = scalars(kept.walk);
     Run run = scalars(kept.run);
     const Kv4AttnArgs& a = args_again();
     const int ratio = a.n_heads / a.n_kv;
     if (!walk_run(walk, run)) break;   // (the worker's last places)
-    if (run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
+    if (!MIXED && run.b0 == 0 && !run.whole) walk_note(a, ROWS, wv, walk.per, run);
     kept.run = run;
     const Kv4Seq& sq = run.sq;
     const int n_row = sq.qlen * ratio;
     const int row0 = run.tile * ROWS + 32 * wv;     // this wave's first row (may be past the last)
     int le = lane_again();   // (addresses of a run's begin and end are not kept over others)
     const int row = min(row0 + (le & 31), n_row - 1), tok = row / ratio;
+    if (MIXED && run.b0 == 0 && le < 32 && row0 + le < n_row)
+      leave_rec(a, run, walk.per, sq.q0 + tok, (long long)(sq.q0 + tok) * a.n_heads + (run.head - tok) * ratio + row,
+                32 * wv + le);
     v8 qin[2][4];   // groups h and 2 + h of the row
     const T* qp = reinterpret_cast<const T*>(a.q) + (long long)(sq.q0 + tok) * a.q_row +
                   (long long)(run.head * ratio + row - tok * ratio) * a.q_head + 32 * (le >> 5);
@@ -1273,11 +1293,11 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
       const Run r = scalars(kept.run);
       const Kv4Seq& q = r.sq;
       const int ratio = e.n_heads / e.n_kv;
-      return attn_visible(e, q, min(r.tile * ROWS + 32 * wv + (l & 31), q.qlen * ratio - 1) / ratio);
+      return attn_visible<MIXED>(e, q, min(r.tile * ROWS + 32 * wv + (l & 31), q.qlen * ratio - 1) / ratio);
     };
     // fewest and most keys that rows of the tile see
-    const int tmin = attn_visible(a, sq, run.tile * ROWS / ratio);
-    const int tmax = attn_visible(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
+    const int tmin = attn_visible<MIXED>(a, sq, run.tile * ROWS / ratio);
+    const int tmax = attn_visible<MIXED>(a, sq, (min(run.tile * ROWS + ROWS, n_row) - 1) / ratio);
     const int b_end = min(run.b1, (tmax + KV4_KEYS - 1) / KV4_KEYS);
 
     floatx16 o[4];
@@ -1291,7 +1311,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
     // Addresses of blocks, 64 at a time, a lane each (past the last block the last one again, so
     // that the count of loads under way is always the same).
     const int subs = a.page_shift - 5;
-    const int* trow = table_row<PART>(a, run.s);
+    const int* trow = table_row<MIXED>(a, run.s);
     const uint32_t per_page = (uint32_t)a.n_kv << subs, of_head = (uint32_t)run.head << subs;
     int abase = 0;                       // the first of the 64
     uint32_t mine = 0;                   // (their numbers: a register less)
@@ -1555,24 +1575,17 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
       } else if (row0 + (le & 31) < n_row) {
         const int row = row0 + (le & 31), tok = row / ratio;
         const long long orow = (long long)(sq.q0 + tok) * e.n_heads + (run.head - tok) * ratio + row;
-        auto of = [&](int d, int k) __attribute__((always_inline)) {   // 4 values at 32 d + 8 k + 4 (le / 32)
-          return (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-        };
-        if constexpr (PART == KV4_SHARED) {
+        if (MIXED && !is_final(e, run.s)) {
 #pragma unroll
           for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              keep_state(e, orow, 32 * d + 8 * k + 4 * (le >> 5), of(d, k) * (1.f / M::kUnit), mrun, lrun);
+              keep_state(e, part_of(e, run.s), orow, 32 * d + 8 * k + 4 * (le >> 5),
+                         (floatx4){o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * (1.f / M::kUnit),
+                         mrun, lrun);
         } else {
-          const bool joins = PART == KV4_REST && load_const(e.place + run.s) > 0;
-          bool none = lrun == 0.f;   // a row that sees no key: zeros, and the sum of none
-          float f = (1.f / M::kUnit) / lrun, m_all = mrun, l_all = lrun;
-          if (joins) {
-            floatx4 unused = {0.f, 0.f, 0.f, 0.f};
-            join_state(e, orow, 0, unused, m_all, l_all);
-            none = l_all == 0.f;
-          }
+          const bool none = lrun == 0.f;   // a row that sees no key: zeros, and the sum of none
+          const float f = (1.f / M::kUnit) / lrun;
           T* op = reinterpret_cast<T*>(e.out) + orow * KV4_D + 4 * (le >> 5);
 #pragma unroll
           for (int d = 0; d < 4; ++d)
@@ -1580,21 +1593,12 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
             for (int k = 0; k < 4; ++k) {
               typedef T v4 __attribute__((ext_vector_type(4)));
               v4 x;
-              floatx4 y = of(d, k);
-              if (joins) {
-                float m = mrun, l = lrun;
-                y *= 1.f / M::kUnit;
-                join_state(e, orow, 32 * d + 8 * k + 4 * (le >> 5), y, m, l);
-                y = y / l;
-              } else {
-                y *= f;
-              }
 #pragma unroll
-              for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : y[j]);
+              for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[d][4 * k + j] * f);
               *reinterpret_cast<v4*>(op + 32 * d + 8 * k) = x;
             }
           if (e.lse && le < 32)
-            e.lse[orow] = none ? -INFINITY : (m_all - KV4_LIFT + __log2f(l_all)) * 0.69314718056f;
+            e.lse[orow] = none ? -INFINITY : (mrun - KV4_LIFT + __log2f(lrun)) * 0.69314718056f;
         }
       }
       more = walk_next(e, ROWS, walk, run);
@@ -1609,7 +1613,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
 // are kv4_tile_kernel's.  Bound by them: eight blocks leave 550 of 66 KB, 10.6 us with the launch.
 // Two partials (most of a prompt's) or eight are loaded at once: one by one two prompts' took 30 us
 // for 16.  Which they are is in notes: every workgroup finding its unit by itself took 40 us more.
-template <typename T, bool TILE, int PART>
+template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
   const int lane = threadIdx.x & 63;
   const int ratio = a.n_heads / a.n_kv;
@@ -1665,12 +1669,75 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
   }
   const int tok = r / ratio;
   const long long orow = (long long)(n.q0 + tok) * a.n_heads + head * ratio + r - tok * ratio;
-  if constexpr (PART == KV4_SHARED) {
-    keep_state(a, orow, col, o, m, l);
-    return;
-  }
-  if constexpr (PART == KV4_REST)
-    if (a.place[n.s] > 0) join_state(a, orow, col, o, m, l);
+  const bool none = l == 0.f;
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  v4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[j] / l);
+  *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.out) + orow * KV4_D + col) = x;
+  if (a.lse && col == 0)
+    a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
+}
+
+// The parts of rows with shared keys joined, the group's and then its own, each from the partials of its
+// workers in the order of the keys or from its state.  A thread has 4 values of a row, 8 threads that
+// follow on each other 8 rows (of a token's heads), whose partials lie next to each other.  TILE: the
+// shared parts' partials are kv4_tile_kernel's, the own ones are kv4_attn_kernel's of 16 rows.
+template <typename T, bool TILE>
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, int own_rows) {
+  const int t = threadIdx.x, col = 4 * (t >> 3), n_own = a.n_seq - a.n_groups;
+  const long long rows = (long long)a.n_rows * a.n_heads, orow = 8ll * blockIdx.x + (t & 7);
+  if (orow >= rows) return;
+  const int row = (int)(orow / a.n_heads), s = a.seq_of[row];
+  const Kv4Rec own = a.recs[orow], shared = a.recs[rows + orow];   // (the latter perhaps nobody's)
+  if (s < 0 || s >= n_own) return;
+  const int v = a.n_groups + s, q0 = a.starts[v], q1 = a.ends[v], skip = a.skip[s];
+  const Kv4Seq sq = kv4_seq(q0, q1, a.lens[v], a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, own_rows, false);
+  if (sq.bad || row < q0 || row >= q1 || own.w0 == -2) return;   // (a row of no sequence; written already)
+  float m = -FLT_MAX, l = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 4;   // pieces under way at once
+  auto part = [&](const Kv4Rec& r, int which, auto tile, const float* ws) {
+    constexpr bool of_tile = decltype(tile)::value;
+    const int tile_rows = of_tile ? 128 : own_rows;
+    const long long pf = kv4_piece_floats(tile_rows);
+    const int c = r.c;   // (in the order of the kernels' registers)
+    const int f = of_tile ? (((c >> 5) * 4 + (col >> 5)) * 4 + ((col >> 3) & 3)) * 64 + 32 * ((col >> 2) & 1) + (c & 31)
+                       : ((c >> 4) * 8 + (col >> 4)) * 64 + 16 * ((col >> 2) & 3) + (c & 15);
+    for (int w = r.w0; w <= r.w1; w += N) {
+      floatx4 x[N];
+      floatx2 y[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int k = min(w + j, r.w1);   // (that of the first lies behind its other one)
+        const float* p = ws + (2ll * k + (k == r.w0 ? 1 : 0)) * pf;
+        const long long at = which * rows + orow;
+        x[j] = *reinterpret_cast<const floatx4*>(r.w0 < 0 ? a.state_o + at * KV4_D + col : p + 4 * f);
+        y[j] = *reinterpret_cast<const floatx2*>(r.w0 < 0 ? a.state_ml + 2 * at : p + tile_rows * KV4_D + 2 * c);
+      }
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (w + j > r.w1) {   // (0 * what lies there may be NaN)
+          x[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+          y[j] = (floatx2){-INFINITY, 0.f};
+        }
+        mn = fmaxf(mn, y[j].x);
+      }
+      const float k = __builtin_amdgcn_exp2f(m - mn);
+      o *= k;
+      l *= k;
+      m = mn;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float e = __builtin_amdgcn_exp2f(y[j].x - m);
+        l += e * y[j].y;
+        o += e * x[j];
+      }
+    }
+  };
+  if (skip > 0) part(shared, 1, std::integral_constant<bool, TILE>{}, a.shared_ws);
+  part(own, 0, std::integral_constant<bool, false>{}, a.ws);
   const bool none = l == 0.f;
   typedef T v4 __attribute__((ext_vector_type(4)));
   v4 x;
@@ -1684,25 +1751,29 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
 // What the sequences of a group share: the pages, from the first on, that are the same in the tables of
 // all that have rows, and whose keys all those rows see whole.  A workgroup to a group; a wave compares
 // a sequence's places with the group's first one's, 4 a lane.  Ranges or lengths that do not fit leave
-// the group nothing to share (the rest finds and reports them); boundaries out of order leave all groups
-// so.  128 sequences of 512 shared pages: 7 us.
+// the group nothing to share (the attention finds and reports them); boundaries out of order leave all
+// groups so.  Out: the launch's sequences, the groups first.
+struct Kv4GroupArgs {
+  const int* groups;           // [n_groups + 1] sequences of group g: groups[g] .. groups[g + 1] - 1
+  int n_groups;
+  long long* row_of;
+  int *q0, *q1, *len, *skip;
+};
 __global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4GroupArgs g) {
   typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
-  __shared__ int shared_pages, first;
-  const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wv = t >> 6;
+  __shared__ int least[2][16], with_rows[16];
+  const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wv = t >> 6, nw = nt >> 6, i = blockIdx.x;
   bool bad = false;
-  for (int i = t; i < g.n_groups; i += nt) bad |= g.groups[i] > g.groups[i + 1];
-  bad |= g.groups[0] < 0 || g.groups[g.n_groups] > a.n_seq;
-  const bool none = __syncthreads_or(bad);
-  const int i = blockIdx.x, s0 = none ? 0 : g.groups[i], s1 = none ? 0 : g.groups[i + 1];
-  if (none && i == 0 && t == 0) atomicOr(a.err, KV4_ERR_PAGE);
-  if (t == 0) {
-    shared_pages = a.width;
-    first = INT32_MAX;
+  for (int k = t; k < g.n_groups; k += nt) bad |= g.groups[k] > g.groups[k + 1];
+  const int low = g.groups[0], high = g.groups[g.n_groups];
+  int s0 = g.groups[i], s1 = g.groups[i + 1];
+  const bool none = __syncthreads_or(bad || low < 0 || high > a.n_seq);
+  if (none) {
+    s0 = s1 = 0;
+    if (i == 0 && t == 0) atomicOr(a.err, KV4_ERR_PAGE);
   }
-  __syncthreads();
-  // the fewest whole pages that a row sees, and the first sequence with rows
-  int most = a.width, lowest = INT32_MAX, rows = 0;
+  // the fewest whole pages that a row sees, the first sequence with rows, and whether there are more
+  int most = a.width, one = INT32_MAX, rows = 0;
   for (int s = s0 + t; s < s1; s += nt) {
     const int q0 = a.starts[s], q1 = a.ends[s], len = a.lens[s];
     const bool fits = q0 >= 0 && q1 >= q0 && q1 <= a.n_rows && len >= 0 && len <= ((long long)a.width << a.page_shift);
@@ -1710,46 +1781,51 @@ __global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4Grou
       most = 0;
     } else if (q1 > q0) {
       most = min(most, max(0, a.causal ? len - (q1 - q0) : len) >> a.page_shift);
-      lowest = min(lowest, s);
+      one = min(one, s);
       ++rows;
     }
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
     most = min(most, __shfl_xor(most, o, 64));
-    lowest = min(lowest, __shfl_xor(lowest, o, 64));
+    one = min(one, __shfl_xor(one, o, 64));
+    rows += __shfl_xor(rows, o, 64);
   }
   if (lane == 0) {
-    atomicMin(&shared_pages, most);
-    atomicMin(&first, lowest);
+    least[0][wv] = most;
+    least[1][wv] = one;
+    with_rows[wv] = rows;
   }
-  rows = __syncthreads_count(rows > 1) ? 2 : __syncthreads_count(rows > 0);   // (two or more: some share)
-  most = rows > 1 ? shared_pages : 0;
-  const int one = first;
   __syncthreads();
-  if (rows > 1) {
-    // the first place at which some sequence differs
+  rows = 0;
+  for (int w = 0; w < nw; ++w) {
+    most = min(most, least[0][w]);
+    one = min(one, least[1][w]);
+    rows += with_rows[w];
+  }
+  if (rows < 2) most = 0;
+  __syncthreads();
+  if (most > 0) {   // the first place at which some sequence differs
     const int* p = a.table + (long long)one * a.width;
     int same = most;
     for (int j0 = 0; j0 < most; j0 += 256) {
-      const int j = j0 + 4 * lane, last = max(0, a.width - 4);
+      const int at = max(0, min(j0 + 4 * lane, a.width - 4));   // (past the last place: places before)
       auto four = [&](const int* row) {
         int4u v = {-1, -1, -1, -1};
         if (a.width >= 4) {
-          v = *reinterpret_cast<const int4u*>(row + min(j, last));   // (past the last place: places before)
+          v = *reinterpret_cast<const int4u*>(row + at);
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) if (k < a.width) v[k] = row[k];
         }
         return v;
       };
-      const int at = a.width >= 4 ? min(j, last) : 0;
       const int4u x = four(p);
 #pragma unroll
       for (int k = 3; k >= 0; --k)
         if (at + k < same && (x[k] < 0 || x[k] >= a.n_pages)) same = at + k;
 #pragma unroll 4
-      for (int s = s0 + wv; s < s1; s += nt >> 6) {
+      for (int s = s0 + wv; s < s1; s += nw) {
         const int4u y = four(a.table + (long long)s * a.width);
         const bool idle = a.ends[s] <= a.starts[s];
 #pragma unroll
@@ -1759,48 +1835,65 @@ __global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4Grou
     }
 #pragma unroll
     for (int o = 32; o; o >>= 1) same = min(same, __shfl_xor(same, o, 64));
-    if (lane == 0) atomicMin(&shared_pages, same);
+    if (lane == 0) least[0][wv] = same;
     __syncthreads();
-    most = shared_pages;
+    for (int w = 0; w < nw; ++w) most = min(most, least[0][w]);
   }
-  for (int s = s0 + t; s < s1; s += nt) {
-    const int skip = a.ends[s] > a.starts[s] ? most : 0;
-    g.out.skip[s] = skip;
-    g.out.rest[s] = a.lens[s] - (skip << a.page_shift);
-  }
+  auto own = [&](int s, int skip) {
+    const int v = g.n_groups + s;
+    g.q0[v] = a.starts[s];
+    g.q1[v] = a.ends[s];
+    g.len[v] = a.lens[s] - (skip << a.page_shift);
+    g.row_of[v] = (long long)s * a.width + skip;
+    g.skip[s] = skip;
+  };
+  for (int s = s0 + t; s < s1; s += nt) own(s, a.ends[s] > a.starts[s] ? most : 0);
   if (t == 0) {
-    g.out.q0[i] = most ? a.starts[s0] : 0;
-    g.out.q1[i] = most ? a.ends[s1 - 1] : 0;
-    g.out.len[i] = most << a.page_shift;
-    g.out.of[i] = most ? one : 0;
+    g.q0[i] = most ? a.starts[s0] : 0;
+    g.q1[i] = most ? a.ends[s1 - 1] : 0;
+    g.len[i] = most << a.page_shift;
+    g.row_of[i] = most ? (long long)one * a.width : 0;
   }
-  // sequences of no group
-  const int low = none ? 0 : g.groups[0], high = none ? 0 : g.groups[g.n_groups];
-  for (int s = i * nt + t; s < a.n_seq; s += nt * g.n_groups)
-    if (s < low || s >= high) {
-      g.out.skip[s] = 0;
-      g.out.rest[s] = a.lens[s];
-    }
+  for (int s = i * nt + t; s < a.n_seq; s += nt * g.n_groups)   // sequences of no group
+    if (none || s < low || s >= high) own(s, 0);
 }
 
-template <typename T, int PART>
-void attend_part(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
+template <typename T>
+void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
   const dim3 grid(a.workers), block(256), mgrid(a.workers * (c.tile_rows / 8));
   switch (c.tile_rows) {
-    case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1, PART>), grid, block, 0, st, a); break;
-    case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2, PART>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((kv4_tile_kernel<T, PART>), grid, block, TILE_LDS, st, a);
+    case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1, false>), grid, block, 0, st, a); break;
+    case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2, false>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((kv4_tile_kernel<T, false>), grid, block, TILE_LDS, st, a);
   }
-  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false, PART>), mgrid, block, 0, st, a, c.tile_rows);
-  else hipLaunchKernelGGL((kv4_merge_kernel<T, true, PART>), mgrid, block, 0, st, a, c.tile_rows);
+  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
+  else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);
 }
-template <int PART>
-void attend(const Kv4AttnArgs& a_in, hipStream_t st) {
-  Kv4AttnArgs a = a_in;
-  const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
-  a.workers = c.workers;
-  if (a.dtype == 1) attend_part<half_t, PART>(a, c, st);
-  else attend_part<bf16_t, PART>(a, c, st);
+// With shared keys (a: groups and sequences in one list): in one launch, or the groups' in one of tiles.
+template <typename T>
+void attend_shared(const Kv4AttnArgs& a, const Kv4SharedCut& c, hipStream_t st) {
+  const dim3 block(256), join((unsigned)(((long long)a.n_rows * a.n_heads + 7) / 8));
+  Kv4AttnArgs own = a;
+  own.workers = c.workers;
+  if (!c.shared_workers) {
+    if (c.own == 16) hipLaunchKernelGGL((kv4_attn_kernel<T, 1, true>), dim3(c.workers), block, 0, st, own);
+    else hipLaunchKernelGGL((kv4_attn_kernel<T, 2, true>), dim3(c.workers), block, 0, st, own);
+    hipLaunchKernelGGL((kv4_join_kernel<T, false>), join, block, 0, st, a, c.own);
+    return;
+  }
+  Kv4AttnArgs groups = a;
+  groups.n_seq = a.n_groups;
+  groups.workers = c.shared_workers;
+  groups.ws = a.shared_ws;
+  hipLaunchKernelGGL((kv4_tile_kernel<T, true>), dim3(c.shared_workers), block, TILE_LDS, st, groups);
+  own.n_seq = a.n_seq - a.n_groups;
+  own.starts += a.n_groups;
+  own.ends += a.n_groups;
+  own.lens += a.n_groups;
+  own.row_of += a.n_groups;
+  own.n_groups = 0;
+  hipLaunchKernelGGL((kv4_attn_kernel<T, 1, true>), dim3(c.workers), block, 0, st, own);
+  hipLaunchKernelGGL((kv4_join_kernel<T, true>), join, block, 0, st, a, c.own);
 }
 
 }  // namespace
@@ -1838,31 +1931,41 @@ void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st) {
 }
 void launch_kv4_attend(const Kv4AttnArgs& a_in, hipStream_t st) {
   Kv4AttnArgs a = a_in;
+  const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
+  a.workers = c.workers;
   a.ends = a.starts + 1;
-  attend<KV4_WHOLE>(a, st);
+  a.n_groups = 0;
+  if (a.dtype == 1) attend<half_t>(a, c, st);
+  else attend<bf16_t>(a, c, st);
 }
 void launch_kv4_attend_shared(const Kv4AttnArgs& a_in, const int* groups, int n_groups, hipStream_t st) {
   Kv4AttnArgs a = a_in;
-  a.ends = a.starts + 1;
+  const Kv4SharedCut c = kv4_shared_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
+  if (!c.own) return launch_kv4_attend(a, st);
   const Kv4SharedWs w = kv4_shared_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
   char* ws = reinterpret_cast<char*>(a.ws);
-  a.state_o = reinterpret_cast<float*>(ws + w.state_o);
-  a.state_ml = reinterpret_cast<float*>(ws + w.state_ml);
-  int* p = reinterpret_cast<int*>(ws + w.groups);
-  Kv4GroupArgs g{groups, n_groups, {p, p + n_groups, p + 2ll * n_groups, p + 3ll * n_groups, p + 4ll * n_groups,
-                                    p + 4ll * n_groups + a.n_seq}};
-  hipLaunchKernelGGL(kv4_groups_kernel, dim3(n_groups), dim3(1024), 0, st, a, g);
-  Kv4AttnArgs b = a;
-  b.n_seq = n_groups;
-  b.causal = 0;
-  b.starts = g.out.q0;
-  b.ends = g.out.q1;
-  b.lens = g.out.len;
-  b.place = g.out.of;
-  attend<KV4_SHARED>(b, st);
-  a.lens = g.out.rest;
-  a.place = g.out.skip;
-  attend<KV4_REST>(a, st);
+  auto ints = [&](long long at) { return reinterpret_cast<int*>(ws + at); };
+  auto floats = [&](long long at) { return reinterpret_cast<float*>(ws + at); };
+  const Kv4GroupArgs g{groups, n_groups, reinterpret_cast<long long*>(ws + w.row_of), ints(w.q0), ints(w.q1),
+                       ints(w.len), ints(w.skip)};
+  a.ends = a.starts + 1;
+  const int threads = a.n_seq <= 32 * n_groups ? 256 : 1024;
+  hipLaunchKernelGGL(kv4_groups_kernel, dim3(n_groups), dim3(threads), 0, st, a, g);
+  a.n_groups = n_groups;
+  a.n_seq += n_groups;
+  a.starts = g.q0;
+  a.ends = g.q1;
+  a.lens = g.len;
+  a.row_of = g.row_of;
+  a.skip = g.skip;
+  a.recs = reinterpret_cast<Kv4Rec*>(ws + w.recs);
+  a.state_o = floats(w.state_o);
+  a.state_ml = floats(w.state_ml);
+  a.seq_of = ints(w.seq_of);
+  a.ws = floats(w.own);
+  a.shared_ws = floats(w.shared);
+  if (a.dtype == 1) attend_shared<half_t>(a, c, st);
+  else attend_shared<bf16_t>(a, c, st);
 }
 
 }  // namespace dfl
