@@ -402,7 +402,7 @@ int64_t dfl_kv4_attend_shared_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, 
  * the whole; chances [n_rows] min(1, p(x) / q(x)), 1 in a sequence's first row.
  * The sequence's new text is its accepted tokens and next_ids; its cache keeps accepted + 1 rows of
  * the block.  uniforms are of [0, 1).  Tests and draws are those of sums in 64 bits; chances are
- * off by some 2^-20 (2^-16 at most).  -infinity masks a token.  A row that holds a NaN or +infinity, or nothing
+ * off by some 2^-22 (2^-14.9 at most).  -infinity masks a token.  A row that holds a NaN or +infinity, or nothing
  * above -infinity, has no distribution: its test fails with chance 0, a draw that needs it gives -1.
  * An id outside [0, vocab) has probability 0.  Sequences without rows, or whose range does not fit,
  * get 0 accepted and -1; rows of no sequence are left as they were.  starts must ascend (else the

@@ -1686,66 +1686,67 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
 template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, int own_rows) {
   const int t = threadIdx.x, col = 4 * (t >> 3), n_own = a.n_seq - a.n_groups;
-  const long long rows = (long long)a.n_rows * a.n_heads, orow = 8ll * blockIdx.x + (t & 7);
-  if (orow >= rows) return;
-  const int row = (int)(orow / a.n_heads), s = a.seq_of[row];
-  const Kv4Rec own = a.recs[orow], shared = a.recs[rows + orow];   // (the latter perhaps nobody's)
-  if (s < 0 || s >= n_own) return;
-  const int v = a.n_groups + s, q0 = a.starts[v], q1 = a.ends[v], skip = a.skip[s];
-  const Kv4Seq sq = kv4_seq(q0, q1, a.lens[v], a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, own_rows, false);
-  if (sq.bad || row < q0 || row >= q1 || own.w0 == -2) return;   // (a row of no sequence; written already)
-  float m = -FLT_MAX, l = 0.f;
-  floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  constexpr int N = 4;   // pieces under way at once
-  auto part = [&](const Kv4Rec& r, int which, auto tile, const float* ws) {
-    constexpr bool of_tile = decltype(tile)::value;
-    const int tile_rows = of_tile ? 128 : own_rows;
-    const long long pf = kv4_piece_floats(tile_rows);
-    const int c = r.c;   // (in the order of the kernels' registers)
-    const int f = of_tile ? (((c >> 5) * 4 + (col >> 5)) * 4 + ((col >> 3) & 3)) * 64 + 32 * ((col >> 2) & 1) + (c & 31)
-                       : ((c >> 4) * 8 + (col >> 4)) * 64 + 16 * ((col >> 2) & 3) + (c & 15);
-    for (int w = r.w0; w <= r.w1; w += N) {
-      floatx4 x[N];
-      floatx2 y[N];
+  const long long rows = (long long)a.n_rows * a.n_heads;
+  for (long long orow = 8ll * blockIdx.x + (t & 7); orow < rows; orow += 8ll * gridDim.x) {
+    const int row = (int)(orow / a.n_heads), s = a.seq_of[row];
+    const Kv4Rec own = a.recs[orow], shared = a.recs[rows + orow];   // (the latter perhaps nobody's)
+    if (s < 0 || s >= n_own) continue;
+    const int v = a.n_groups + s, q0 = a.starts[v], q1 = a.ends[v], skip = a.skip[s];
+    const Kv4Seq sq = kv4_seq(q0, q1, a.lens[v], a.n_rows, a.width, a.page_shift, a.n_heads / a.n_kv, own_rows, false);
+    if (sq.bad || row < q0 || row >= q1 || own.w0 == -2) continue;   // (a row of no sequence; written already)
+    float m = -FLT_MAX, l = 0.f;
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    constexpr int N = 4;   // pieces under way at once
+    auto part = [&](const Kv4Rec& r, int which, auto tile, const float* ws) {
+      constexpr bool of_tile = decltype(tile)::value;
+      const int tile_rows = of_tile ? 128 : own_rows;
+      const long long pf = kv4_piece_floats(tile_rows);
+      const int c = r.c;   // (in the order of the kernels' registers)
+      const int f = of_tile ? (((c >> 5) * 4 + (col >> 5)) * 4 + ((col >> 3) & 3)) * 64 + 32 * ((col >> 2) & 1) + (c & 31)
+                         : ((c >> 4) * 8 + (col >> 4)) * 64 + 16 * ((col >> 2) & 3) + (c & 15);
+      for (int w = r.w0; w <= r.w1; w += N) {
+        floatx4 x[N];
+        floatx2 y[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int k = min(w + j, r.w1);   // (that of the first lies behind its other one)
-        const float* p = ws + (2ll * k + (k == r.w0 ? 1 : 0)) * pf;
-        const long long at = which * rows + orow;
-        x[j] = *reinterpret_cast<const floatx4*>(r.w0 < 0 ? a.state_o + at * KV4_D + col : p + 4 * f);
-        y[j] = *reinterpret_cast<const floatx2*>(r.w0 < 0 ? a.state_ml + 2 * at : p + tile_rows * KV4_D + 2 * c);
-      }
-      float mn = m;
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (w + j > r.w1) {   // (0 * what lies there may be NaN)
-          x[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-          y[j] = (floatx2){-INFINITY, 0.f};
+        for (int j = 0; j < N; ++j) {
+          const int k = min(w + j, r.w1);   // (that of the first lies behind its other one)
+          const float* p = ws + (2ll * k + (k == r.w0 ? 1 : 0)) * pf;
+          const long long at = which * rows + orow;
+          x[j] = *reinterpret_cast<const floatx4*>(r.w0 < 0 ? a.state_o + at * KV4_D + col : p + 4 * f);
+          y[j] = *reinterpret_cast<const floatx2*>(r.w0 < 0 ? a.state_ml + 2 * at : p + tile_rows * KV4_D + 2 * c);
         }
-        mn = fmaxf(mn, y[j].x);
-      }
-      const float k = __builtin_amdgcn_exp2f(m - mn);
-      o *= k;
-      l *= k;
-      m = mn;
+        float mn = m;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float e = __builtin_amdgcn_exp2f(y[j].x - m);
-        l += e * y[j].y;
-        o += e * x[j];
-      }
-    }
-  };
-  if (skip > 0) part(shared, 1, std::integral_constant<bool, TILE>{}, a.shared_ws);
-  part(own, 0, std::integral_constant<bool, false>{}, a.ws);
-  const bool none = l == 0.f;
-  typedef T v4 __attribute__((ext_vector_type(4)));
-  v4 x;
+        for (int j = 0; j < N; ++j) {
+          if (w + j > r.w1) {   // (0 * what lies there may be NaN)
+            x[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+            y[j] = (floatx2){-INFINITY, 0.f};
+          }
+          mn = fmaxf(mn, y[j].x);
+        }
+        const float k = __builtin_amdgcn_exp2f(m - mn);
+        o *= k;
+        l *= k;
+        m = mn;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[j] / l);
-  *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.out) + orow * KV4_D + col) = x;
-  if (a.lse && col == 0)
-    a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
+        for (int j = 0; j < N; ++j) {
+          const float e = __builtin_amdgcn_exp2f(y[j].x - m);
+          l += e * y[j].y;
+          o += e * x[j];
+        }
+      }
+    };
+    if (skip > 0) part(shared, 1, std::integral_constant<bool, TILE>{}, a.shared_ws);
+    part(own, 0, std::integral_constant<bool, false>{}, a.ws);
+    const bool none = l == 0.f;
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    v4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (T)(none ? 0.f : o[j] / l);
+    *reinterpret_cast<v4*>(reinterpret_cast<T*>(a.out) + orow * KV4_D + col) = x;
+    if (a.lse && col == 0)
+      a.lse[orow] = none ? -INFINITY : (m - KV4_LIFT + __log2f(l)) * 0.69314718056f;
+  }
 }
 
 // What the sequences of a group share: the pages, from the first on, that are the same in the tables of
@@ -1872,7 +1873,8 @@ void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
 // With shared keys (a: groups and sequences in one list): in one launch, or the groups' in one of tiles.
 template <typename T>
 void attend_shared(const Kv4AttnArgs& a, const Kv4SharedCut& c, hipStream_t st) {
-  const dim3 block(256), join((unsigned)(((long long)a.n_rows * a.n_heads + 7) / 8));
+  const long long rows8 = ((long long)a.n_rows * a.n_heads + 7) / 8;
+  const dim3 block(256), join((unsigned)(rows8 < (1 << 20) ? rows8 : 1 << 20));
   Kv4AttnArgs own = a;
   own.workers = c.workers;
   if (!c.shared_workers) {

@@ -68,15 +68,20 @@ inline VfWs vf_ws(const VerifyArgs& a) {
 // once.  1024, 2048 and 4096 parts, us: 8 blocks of 32 rows without a draft's logits 41, 45, 51; 48
 // ragged ones of a vocabulary of 32003 58, 58, 69; one block of 16 rows 41 with each.
 constexpr int VF_PARTS = 1024;
+// At most so many values of a thread and part: each of its four sums then has 128 additions.
+constexpr int VF_MOST = 512;
 inline void vf_cut(VerifyArgs& a) {
   const int t = vf_rounds(a.vocab, a.target_dtype), d = a.draft ? vf_rounds(a.vocab, a.draft_dtype) : 0;
   const long long each = (long long)a.n_rows * (t + d) / VF_PARTS;
-  auto cut = [&](int rounds, int& per, int& chunks) {
-    per = each < 1 ? 1 : each < rounds ? (int)each : rounds > 1 ? rounds : 1;
-    chunks = rounds ? (rounds + per - 1) / per : 0;
+  auto cut = [&](int rounds, int dtype, int& per, int& chunks) {
+    const int most = VF_MOST / (VF_VECS * vf_elems(dtype));
+    per = each < 1 ? 1 : each < most ? (int)each : most;
+    chunks = (rounds + per - 1) / per;
+    per = chunks ? (rounds + chunks - 1) / chunks : 1;   // (parts alike)
+    chunks = (rounds + per - 1) / per;
   };
-  cut(t, a.t_rounds, a.t_chunks);
-  cut(d, a.d_rounds, a.d_chunks);
+  cut(t, a.target_dtype, a.t_rounds, a.t_chunks);
+  cut(d, a.draft_dtype, a.d_rounds, a.d_chunks);
   a.draw_chunks = vf_draw_chunks(a.vocab);
 }
 

@@ -8,7 +8,7 @@
 // exceeds u times the whole.
 //
 // First pass (all rows): the sum of exponentials of parts of a row, in fp32; the judge joins them
-// in 64 bits and takes the sequence's first rejected row.  That sum is off by less than 2^-16: a
+// in 64 bits and takes the sequence's first rejected row.  That sum is off by 2^-15.9 at most: a
 // test that such an error could turn is made again with sums in 64 bits.  A draw has no such slack, as
 // some token's running sum almost always lies within 2^-20 of any number: it is made in 64 bits
 // throughout, over the one row of a sequence that needs it.
@@ -340,8 +340,10 @@ DFL_DEV double chance64(const void* base, int dtype, long long stride, int vocab
 
 constexpr int JUDGE = 1024, JUDGE_KEPT = 64;
 enum { ROW_YES = 0, ROW_NO = 1, ROW_CLOSE = 2 };
-// What the first pass's sums (each off by 2^-16 at most: exponents of at most 40 that matter, each
-// rounded twice, 2^-17.6, the power's 2^-22, a thread's additions 2^-18) can change in a quotient.
+// What the first pass's sums can change in a test.  Exponents down to -40 matter (smaller weights add
+// up to V 2^-40), rounded twice (three times past 2^16): 2^-24 40 ln 2 each time, 5.0e-6 in all; the
+// power is off by 2^-23, a thread's sum by 128 additions, 7.6e-6, and at most 40 rescalings, 2.4e-6,
+// the wave's by 8 more, 5e-7: 1.6e-5, 2^-15.9, of p's sum and of q's.
 constexpr double VF_CLOSE = 0x1p-14;
 
 __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const VfPart* parts, VfDraw* draws,

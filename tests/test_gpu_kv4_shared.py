@@ -567,6 +567,25 @@ def test_many_groups():
     check_rows(q, list(range(n + 1)), held, True, c.attend(q, list(range(n + 1)), causal=True, groups=wide))
 
 
+def test_thousands_of_sequences():
+    """3000 sequences, every second one going on from the one before it; a sample of them checked."""
+    n = 3000
+    c = make(n_kv_heads=1, max_seqs=n, max_len=96, n_pages=2 * n)
+    x = rows(33 * n // 2, 1, 1, torch.float16)
+    step = c.step(grow=[33, 0] * (n // 2))
+    c.append(x[:, 0], x[:, 1], step.slots)
+    y = rows(2 * n, 1, 2, torch.float16)
+    step = c.step(grow=[2] * n, keep=[33] * n, parent=[s - s % 2 for s in range(n)])
+    c.append(y[:, 0], y[:, 1], step.slots)
+    q = queries(2 * n, 4, 3, torch.float16)
+    out = c.attend(q, step.starts, causal=True, groups=list(range(0, n + 1, 2)))
+    assert c.errors() == 0
+    x, y = values(x.double().cpu().numpy()), values(y.double().cpu().numpy())
+    for s in list(range(0, n, 97)) + [n - 2, n - 1]:
+        held = np.concatenate((x[33 * (s // 2):33 * (s // 2) + 33], y[2 * s:2 * s + 2]))
+        check_rows(q[2 * s:2 * s + 2], [0, 2], [held], True, out[2 * s:2 * s + 2])
+
+
 def test_refusals_of_groups():
     c, _, _ = family(2, 32, [3], [40], [1, 1, 1], torch.float16)
     q = queries(3, 4, 1, torch.float16)

@@ -10,8 +10,10 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
-# A chance is p / q of two sums in fp32, each within 2^-16 (the kernel's bound), rounded once.
-REL = 2 * 2.0 ** -16 + 2.0 ** -23
+# A chance is p / q of two sums in fp32, rounded once.  A sum: exponents down to -40 matter, each
+# rounded three times at most, 3 * 2^-24 * 40 ln 2 = 5.0e-6; powers 2^-23; 128 additions in a thread,
+# 7.6e-6, 40 rescalings, 2.4e-6, 8 additions across a wave, 5e-7: 1.6e-5.
+REL = 2 * 1.6e-5 + 2.0 ** -23
 
 
 def call(target, ids, starts, u, temps, draft=None, draft_temps=None):
@@ -337,3 +339,24 @@ def test_logits_that_grow_along_a_row():
     for temp in (1.0, 300.0, 1e30):
         check(t.cuda(), ids.cuda(), [0, 2, 4, 6], u.cuda(), temp)
         check(t.flip(1).contiguous().cuda(), ids.cuda(), list(range(7)), u.cuda(), temp)
+
+
+@pytest.mark.parametrize("vocab,rows", [(2**20 + 3, [2, 1]), (2**24, [2]), (300007, [9] * 40)])
+def test_rows_of_many_parts(vocab, rows):
+    """Rows of more parts than a wave has lanes, of more than 256 in the draw, and of parts at their
+    longest."""
+    g = torch.Generator(device="cuda").manual_seed(26)
+    n = sum(rows)
+    t = (2 * torch.randn((n, vocab), generator=g, device="cuda")).to(torch.bfloat16)
+    d = t.roll(1, 0)
+    ids = torch.randint(vocab, (n,), generator=g, device="cuda").to(torch.int32)
+    u = torch.rand(n, generator=g, device="cuda")
+    starts = [sum(rows[:i]) for i in range(len(rows) + 1)]
+    some = range(len(rows)) if n < 10 else range(0, len(rows), 13)
+    got = call(t, ids, starts, u, 1.0, d), call(t, ids, starts, u, 0.8, None)
+    for s in some:
+        a, b = starts[s], starts[s + 1]
+        for v, temp, draft in ((got[0], 1.0, d), (got[1], 0.8, None)):
+            want = plain(t[a:b], ids[a:b], [0, b - a], u[a:b], temp, None if draft is None else draft[a:b])
+            assert v[0][s] == want[0][0] and v[1][s] == want[1][0]
+            np.testing.assert_allclose(v[2][a:b], want[2], rtol=REL, atol=2.0 ** -126)
