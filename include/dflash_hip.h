@@ -390,7 +390,7 @@ int64_t dfl_kv4_attend_shared_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, 
  * Rows starts[s] .. starts[s+1] - 1 of target [n_rows][vocab] are the target's logits behind the
  * tokens of sequence s's block: ids [n_rows] holds the block, its first row the last verified
  * token, the others drafted ones.  draft (or NULL) holds for each drafted row the logits that its
- * token was drawn from (as dfl_draft_block's out_logits; a sequence's first row is not read).
+ * token was drawn from (as dfl_draft_block's out_logits; a sequence's first row does not count).
  * dtypes: 0 fp32, 1 fp16, 2 bf16; rows target_row, draft_row elements apart, aligned to their type
  * alone.  With p the softmax of a target row divided by its sequence's temperature, q the draft's
  * (below 1e-5 all weight is on the largest logit, the first of equals; without draft logits all of

@@ -114,7 +114,7 @@ def verify_draft(target_logits, ids, starts, uniforms, temperature=1.0, draft_lo
     each row's token, ``ids`` [n] the blocks: rows ``starts[s] .. starts[s + 1] - 1`` are sequence
     s's, the first of them its last verified token, the others drafted.  ``draft_logits`` [n, vocab]
     (any of the types) are the logits that the drafted tokens were drawn from (``draft(...,
-    return_logits=True)``; a sequence's first row is not read), None for tokens that were chosen
+    return_logits=True)``; a sequence's first row does not count), None for tokens that were chosen
     otherwise (the largest logit, a lookup).  ``temperature`` is a number or a tensor [n_seq], 0
     for the largest logit alone; ``draft_temperature`` alike (default: ``temperature``).
 
