@@ -1682,7 +1682,8 @@ __global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_
 // The parts of rows with shared keys joined, the group's and then its own, each from the partials of its
 // workers in the order of the keys or from its state.  A thread has 4 values of a row, 8 threads that
 // follow on each other 8 rows (of a token's heads), whose partials lie next to each other.  TILE: the
-// shared parts' partials are kv4_tile_kernel's, the own ones are kv4_attn_kernel's of 16 rows.
+// shared parts' partials are kv4_tile_kernel's, the own ones are kv4_attn_kernel's.  Bound by latencies,
+// three reads that wait for each other: 64 tokens of 32 heads 6 us, 128 of 64 with 8 partials each 11.
 template <typename T, bool TILE>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, int own_rows) {
   const int t = threadIdx.x, col = 4 * (t >> 3), n_own = a.n_seq - a.n_groups;
@@ -1753,7 +1754,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a, int own_ro
 // all that have rows, and whose keys all those rows see whole.  A workgroup to a group; a wave compares
 // a sequence's places with the group's first one's, 4 a lane.  Ranges or lengths that do not fit leave
 // the group nothing to share (the attention finds and reports them); boundaries out of order leave all
-// groups so.  Out: the launch's sequences, the groups first.
+// groups so.  Out: the launch's sequences, the groups first.  Bound by latencies: 8 sequences of 64 pages
+// 4.4 us, 128 of 512 10.5.
 struct Kv4GroupArgs {
   const int* groups;           // [n_groups + 1] sequences of group g: groups[g] .. groups[g + 1] - 1
   int n_groups;

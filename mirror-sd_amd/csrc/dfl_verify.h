@@ -65,9 +65,11 @@ inline VfWs vf_ws(const VerifyArgs& a) {
   return w;
 }
 // How the call is cut: into parts of as many rounds as leave VF_PARTS of them, what the chip holds at
-// once.  1024, 2048 and 4096 parts, us: 8 blocks of 32 rows without a draft's logits 41, 45, 51; 48
-// ragged ones of a vocabulary of 32003 58, 58, 69; one block of 16 rows 41 with each.
-constexpr int VF_PARTS = 1024;
+// once.  768, 1024, 1536 and 4096 parts, us: 8 blocks of 32 rows without a draft's logits 32, 32, 35, 51;
+// 48 ragged ones of a vocabulary of 32003 41, 43, 43, 69; one block of 16 rows 30 with each.  (Rounds of
+// 1, 2, 3 and 4 loads with 768: the blocks 33, 32, 31, 32, the ragged ones 44, 41, 41, 43, 64 blocks of 32
+// rows 283, 259, 257, 257.)
+constexpr int VF_PARTS = 768;
 // At most so many values of a thread and part: each of its four sums then has 128 additions.
 constexpr int VF_MOST = 512;
 inline void vf_cut(VerifyArgs& a) {
