@@ -630,3 +630,46 @@ def test_candidates_are_drafted_verified_and_the_best_goes_on():
         parent = [best[s // size] for s in range(n)]
         keep = [len(held[p]) - block + accepted[p] + 1 for p in parent]
     assert c.errors() == 0
+
+
+def test_pool_past_32_bits():
+    """A pool of 5.6 GB whose last pages alone are free: copies and attention past 2^32 bytes."""
+    pages = 20000
+    if torch.cuda.mem_get_info()[0] < 9 << 30:
+        pytest.skip("needs 9 GB")
+    c = make(n_kv_heads=8, page=256, n_pages=pages, max_seqs=3, max_len=1024)
+    c.refs[:pages - 12] = 1                  # (held by tables that are not this cache's)
+    x = rows(300, 8, 1, torch.float16)
+    step = c.step(grow=[300, 0, 0])
+    assert step.slots.min().item() == 256 * (pages - 12)
+    c.append(x[:, 0], x[:, 1], step.slots)
+    y = rows(6, 8, 2, torch.float16)
+    step = c.step(grow=[1, 2, 3], keep=[300, 300, 280], parent=[0, 0, 0])
+    assert len({s // 256 for s in step.slots.tolist()}) == 3
+    c.append(y[:, 0], y[:, 1], step.slots)
+    x, y = values(x.double().cpu().numpy()), values(y.double().cpu().numpy())
+    held = [np.concatenate((x, y[:1])), np.concatenate((x, y[1:3])), np.concatenate((x[:280], y[3:]))]
+    for s in range(3):
+        got = c.read([c.table[s, r // 256].item() * 256 + r % 256 for r in range(len(held[s]))], dtype=torch.float32)
+        for i in range(2):
+            np.testing.assert_array_equal(got[i].double().cpu().numpy(), held[s][:, i])
+    q = queries(3, 16, 4, torch.float16)
+    check_rows(q, [0, 1, 2, 3], held, True, c.attend(q, [0, 1, 2, 3], causal=True, groups=[0, 3]))
+    assert c.errors() == 0
+
+
+def test_steps_that_free_everything_and_begin_again():
+    """A pool to its last page, given back in every order, by the parent, by its continuations."""
+    rng = random.Random(3)
+    c = make(max_seqs=5, n_pages=20)
+    plan = SharedPlan(5, 32, 16, 20)
+    for _ in range(8):
+        check_step(c, plan, [200, 0, 0, 0, 0], [0] * 5)
+        check_step(c, plan, [9] * 5, [200] * 5, [0] * 5)      # 7 pages and 4 copies, 2 rows into an eighth
+        order = list(range(5))
+        rng.shuffle(order)
+        for s in order:
+            keep = list(plan.lens)
+            keep[s] = 0
+            check_step(c, plan, [0] * 5, keep)
+        assert plan.refs() == [0] * 20 and c.n_free.item() == 20

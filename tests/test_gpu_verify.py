@@ -360,3 +360,58 @@ def test_rows_of_many_parts(vocab, rows):
             want = plain(t[a:b], ids[a:b], [0, b - a], u[a:b], temp, None if draft is None else draft[a:b])
             assert v[0][s] == want[0][0] and v[1][s] == want[1][0]
             np.testing.assert_allclose(v[2][a:b], want[2], rtol=REL, atol=2.0 ** -126)
+
+
+def test_logits_past_32_bits():
+    """300 rows of 2^24 tokens, 10 GB: the last sequence's rows begin past 2^32 values."""
+    n, vocab = 300, 2**24
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GB")
+    t = torch.empty((n, vocab), dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(27)
+    t.normal_(generator=g).mul_(2)
+    ids = torch.randint(vocab, (n,), generator=g, device="cuda").to(torch.int32)
+    u = torch.rand(n, generator=g, device="cuda")
+    u[299] = 0.0                       # its token passes
+    starts = list(range(0, 299, 2)) + [298, 300]
+    got = call(t, ids, starts, u, 1.0)
+    want = plain(t[298:], ids[298:], [0, 2], u[298:], 1.0)
+    assert got[0][-1] == want[0][0] == 1 and got[1][-1] == want[1][0]
+    np.testing.assert_allclose(got[2][298:], want[2], rtol=REL)
+
+
+def test_numbers_outside_of_their_range():
+    """Numbers that are not of [0, 1): some token of the vocabulary that has weight, never another."""
+    t = torch.full((6, 500), -float("inf"))
+    t[:, 100:400] = torch.randn((6, 300), generator=torch.Generator().manual_seed(28))
+    for u in (-1.0, 1.0, 7.0, float("inf"), float("nan"), -float("inf")):
+        _, next_ids, _ = call(t.cuda(), torch.zeros(6, dtype=torch.int32).cuda(), list(range(7)),
+                              torch.full((6,), u).cuda(), 1.0)
+        assert ((next_ids >= 100) & (next_ids < 400)).all(), u
+
+
+def test_two_graphs_in_one_pool():
+    """Two captured calls whose workspaces share memory, replayed in turn."""
+    from mirror_sd_amd import verify_draft
+    a = inputs([8, 3], 30011, "bf16", "bf16", 29)
+    b = inputs([2, 9, 4], 9001, "fp32", None, 30)
+    want = [call(*a[:4], 1.0, a[4]), call(*b[:4], 0.6, b[4])]
+    graphs, got = [], []
+    dev = [[x if isinstance(x, torch.Tensor) else torch.tensor(x, dtype=torch.int32).cuda() for x in c[:4]]
+           for c in (a, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c, temp, d in ((dev[0], 1.0, a[4]), (dev[1], 0.6, b[4])):
+            verify_draft(*c, temperature=temp, draft_logits=d)
+    torch.cuda.current_stream().wait_stream(side)
+    for c, temp, d in ((dev[0], 1.0, a[4]), (dev[1], 0.6, b[4])):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            got.append(verify_draft(*c, temperature=temp, draft_logits=d))
+        graphs.append(graph)
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got[i], want[i]):
+            np.testing.assert_array_equal(x.cpu().numpy(), y)
