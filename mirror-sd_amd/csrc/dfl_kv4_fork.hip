@@ -39,7 +39,7 @@ DFL_DEV void store_agent(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELA
 struct ForkView { int *base, *par, *old, *edge, *count_at, *place_at, *take_at, *copy_at, *own, *starts; };
 constexpr int FORK_ARRAYS = 9;   // (starts come on top)
 // Totals and errors, in LDS or at the scratch's start.
-struct ForkTotals { int err, counted, placed, rows, bad, need, copies, zeros; };
+struct ForkTotals { int err, counted, placed, rows, bad, need, copies, pad; };
 
 struct ForkScratch {   // in memory
   ForkTotals* totals;

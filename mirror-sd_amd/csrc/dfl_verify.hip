@@ -16,8 +16,6 @@
 // Bound by HBM: the logits are read once, the row that is drawn from two or three times more.
 #include "dfl_verify.h"
 
-#include <float.h>
-
 #include "dfl_common.h"
 
 namespace dfl {
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(JUDGE) void verify_judge_kernel(VerifyArgs a, const
       if (row - q0 < JUDGE_KEPT) q_kept[row - q0] = qr;
     }
   }
-  int stop = q0;   // the first rejected row, or the end
+  int stop = q0 + 1;   // the first rejected row, or the end (the first row has no test)
   __syncthreads();
   while (true) {
     while (stop < q1) {   // (every wave the same, 64 rows at a time)

@@ -415,3 +415,15 @@ def test_two_graphs_in_one_pool():
         torch.cuda.synchronize()
         for x, y in zip(got[i], want[i]):
             np.testing.assert_array_equal(x.cpu().numpy(), y)
+
+
+def test_ranges_that_overlap():
+    """Starts that go back: any results, but counts of the sequence's rows and tokens of the vocabulary."""
+    t, ids, _, u, d = inputs([6, 3, 8, 4], 5000, "bf16", "fp16", 31)
+    starts = [0, 6, 3, 9, 1, 21, 20]
+    for draft in (None, d):
+        accepted, next_ids, _ = call(t, ids, starts, u, 1.0, draft)
+        for s, (a, x) in enumerate(zip(accepted, next_ids)):
+            rows = starts[s + 1] - starts[s]
+            assert 0 <= a < max(rows, 1) and -1 <= x < 5000
+            assert rows > 0 or x == -1
