@@ -395,7 +395,9 @@ int64_t dfl_kv4_attend_shared_ws(int32_t n_rows, int32_t n_heads, int32_t n_kv, 
  * alone.  With p the softmax of a target row divided by its sequence's temperature, q the draft's
  * (below 1e-5 all weight is on the largest logit, the first of equals; without draft logits all of
  * q's is on the drafted token), the token x of row t is accepted if uniforms[t] * q(x) < p(x), p
- * that of row t - 1.  temps, draft_temps: [n_seq] device numbers, or NULL: temp, draft_temp for all.
+ * that of row t - 1.  temps, draft_temps: [n_seq] device numbers, or NULL: temp, draft_temp for all; a
+ * negative, infinite or NaN temp is refused, such an entry of temps leaves its sequence's rows of the
+ * target (of draft_temps: of the draft) without a distribution.
  * Out: accepted [n_seq] the drafted tokens accepted one after another; next_ids [n_seq] a token
  * drawn behind them, from max(p - q, 0) after a rejection (from p where that is zero), from p
  * after none: the first whose running sum, in the order of ids, exceeds uniforms[starts[s]] times

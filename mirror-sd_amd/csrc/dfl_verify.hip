@@ -37,9 +37,12 @@ DFL_DEV float logit_at(const void* base, int dtype, long long at) {
   if (dtype == 1) return (float)reinterpret_cast<const half_t*>(base)[at];
   return (float)reinterpret_cast<const bf16_t*>(base)[at];
 }
-// Temperature of a sequence: log2(e) / T, 0 for the largest logit alone.
+// Temperature of a sequence: log2(e) / T, 0 for the largest logit alone, -1 for a number on the device that
+// is no temperature (negative, infinite, NaN): no part of the sequence's rows is then summed, so that they
+// have no distribution.
 DFL_DEV double scale_of(const float* temps, float temp, int s) {
   const float t = temps ? temps[s] : temp;
+  if (!(t >= 0.f && t < INFINITY)) return -1.0;
   return t >= GREEDY ? LOG2E / (double)fminf(t, 1e30f) : 0.0;
 }
 // 2^x: the series of 2^f around a whole number, |f| <= 1/2, to f^12 (the next term is below 2^-52 of
@@ -175,7 +178,7 @@ DFL_DEV void soft_round(const V (&x)[VECS], SoftState& s, float c, float d, doub
       }
   }
 }
-// (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not wanted)
+// (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not wanted, or has no temperature)
 template <int DT, int VECS, typename F>
 DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stride, int row, int chunk, int rounds,
                            F scale_at, float (&lds)[2][4]) {
