@@ -98,6 +98,10 @@ def _numbers(t, n, what, device):
 def _temps(t, n_seq, what, device):
     """(one number for all, None) or (0, a device tensor [n_seq])."""
     import torch
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 0:   # (not read back)
+        if t.is_complex():
+            raise ValueError(f"{what} must be a number, got {t.dtype}")
+        t = t.to(torch.float32).expand(n_seq)
     if isinstance(t, torch.Tensor) and t.dim() == 1:
         t = _numbers(t, n_seq, what, device)
         if not t.is_cuda and not all(0.0 <= x <= 3.4e38 for x in t.tolist()):
@@ -118,10 +122,10 @@ def verify_draft(target_logits, ids, starts, uniforms, temperature=1.0, draft_lo
     s's, the first of them its last verified token, the others drafted.  ``draft_logits`` [n, vocab]
     (any of the types) are the logits that the drafted tokens were drawn from (``draft(...,
     return_logits=True)``; a sequence's first row does not count), None for tokens that were chosen
-    otherwise (the largest logit, a lookup).  ``temperature`` is a number or a tensor [n_seq], finite
-    and not negative, 0 for the largest logit alone; ``draft_temperature`` alike (default:
-    ``temperature``).  Numbers on the GPU are not read back: one that is no temperature leaves its
-    sequence's rows without a distribution (below).
+    otherwise (the largest logit, a lookup).  ``temperature`` is a number, a tensor of one (no
+    dimension) or a tensor [n_seq], finite and not negative, 0 for the largest logit alone;
+    ``draft_temperature`` alike (default: ``temperature``).  Numbers on the GPU are not read back:
+    one that is no temperature leaves its sequences' rows without a distribution (below).
 
     With p and q the softmax of the target's and the draft's rows (without draft logits all of q's
     weight is on the drafted token), row t's token x is accepted if ``uniforms[t] * q(x) < p(x)``,

@@ -67,3 +67,44 @@ def test_host_tensors_are_refused_as_numbers_are():
                 verify_draft(t, ids, starts, u, draft_logits=d, draft_temperature=temps)
     with pytest.raises(ValueError, match="finite"):   # past fp32
         verify_draft(t, ids, starts, u, temperature=torch.tensor([0.5, 1e39], dtype=torch.float64))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16, torch.int64])
+def test_a_number_on_the_gpu_is_one_for_all(dtype):
+    t, ids, starts, u, d = inputs(ROWS, 3001, "bf16", "bf16", 43)
+    for x, y in ((0, 2), (2, 0)) if dtype == torch.int64 else ((0.5, 1.25), (0.0, 0.75)):
+        want = call(t, ids, starts, u, float(x), d, float(y))
+        got = call(t, ids, starts, u, torch.tensor(x, dtype=dtype).cuda(), d, torch.tensor(y, dtype=dtype).cuda())
+        for a, b in zip(got, want):
+            np.testing.assert_array_equal(a, b)
+
+
+def test_a_number_on_the_gpu_that_is_no_temperature():
+    t, ids, starts, u, d = inputs(ROWS, 900, "bf16", "bf16", 44)
+    for x in (-0.5, NAN, INF):
+        got = call(t, ids, starts, u, torch.tensor(x).cuda(), d)
+        assert not got[0].any() and (got[1] == -1).all()
+    with pytest.raises(ValueError):
+        call(t, ids, starts, u, torch.tensor(1j).cuda(), d)
+
+
+def test_a_captured_call_takes_a_number_on_the_gpu():
+    """It is not read back: a graph can be captured with it, and follows what it holds."""
+    from mirror_sd_amd import verify_draft
+    t, ids, starts, u, d = inputs([5, 3], 5003, "fp16", "fp16", 45)
+    starts = torch.tensor(starts, dtype=torch.int32).cuda()
+    temp = torch.tensor(1.0).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        verify_draft(t, ids, starts, u, temperature=temp, draft_logits=d)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        v = verify_draft(t, ids, starts, u, temperature=temp, draft_logits=d)
+    for x in (1.0, 0.0, 0.5, 2.0, 0.5):
+        temp.fill_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(v, call(t, ids, starts, u, x, d)):
+            np.testing.assert_array_equal(a.cpu().numpy(), b)
