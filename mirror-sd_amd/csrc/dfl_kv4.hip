@@ -1608,13 +1608,25 @@ __global__ __launch_bounds__(256, 2) void kv4_tile_kernel(Kv4AttnArgs args) {
   }
 }
 
+// Whether boundaries of groups ascend within 0 .. n_seq: this thread's part of them.
+DFL_DEV bool groups_fit(const int* groups, int n_groups, int n_seq, int t, int nt) {
+  bool ok = groups[0] >= 0 && groups[n_groups] <= n_seq;
+  for (int k = t; k < n_groups; k += nt) ok &= groups[k] <= groups[k + 1];
+  return ok;
+}
+
 // Units that several workers share: their partial states joined in the order of the keys, by the
 // note of the worker that began with the unit.  A thread has 4 values of a row.  TILE: the partials
 // are kv4_tile_kernel's.  Bound by them: eight blocks leave 550 of 66 KB, 10.6 us with the launch.
 // Two partials (most of a prompt's) or eight are loaded at once: one by one two prompts' took 30 us
 // for 16.  Which they are is in notes: every workgroup finding its unit by itself took 40 us more.
-template <typename T, bool TILE>
-__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows) {
+// GROUPS: the call names groups, which are attended apart; their boundaries are looked at here (a template, as
+// a test in every call's merge costs the others up to 1 us of 48).
+template <typename T, bool TILE, bool GROUPS>
+__global__ __launch_bounds__(256) void kv4_merge_kernel(Kv4AttnArgs a, int tile_rows, const int* groups_at,
+                                                        int n_groups) {
+  if (GROUPS && blockIdx.x == 0 && !groups_fit(groups_at, n_groups, a.n_seq, threadIdx.x, 256))
+    atomicOr(a.err, KV4_ERR_PAGE);
   const int lane = threadIdx.x & 63;
   const int ratio = a.n_heads / a.n_kv;
   const int groups = tile_rows / 8;                 // workgroups of a unit
@@ -1766,11 +1778,10 @@ __global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4Grou
   typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ int least[2][16], with_rows[16];
   const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wv = t >> 6, nw = nt >> 6, i = blockIdx.x;
-  bool bad = false;
-  for (int k = t; k < g.n_groups; k += nt) bad |= g.groups[k] > g.groups[k + 1];
+  const bool bad = !groups_fit(g.groups, g.n_groups, a.n_seq, t, nt);
   const int low = g.groups[0], high = g.groups[g.n_groups];
   int s0 = g.groups[i], s1 = g.groups[i + 1];
-  const bool none = __syncthreads_or(bad || low < 0 || high > a.n_seq);
+  const bool none = __syncthreads_or(bad);
   if (none) {
     s0 = s1 = 0;
     if (i == 0 && t == 0) atomicOr(a.err, KV4_ERR_PAGE);
@@ -1862,15 +1873,16 @@ __global__ __launch_bounds__(1024) void kv4_groups_kernel(Kv4AttnArgs a, Kv4Grou
 }
 
 template <typename T>
-void attend(const Kv4AttnArgs& a, const Kv4Cut& c, hipStream_t st) {
+void attend(const Kv4AttnArgs& a, const Kv4Cut& c, const int* groups, int n_groups, hipStream_t st) {
   const dim3 grid(a.workers), block(256), mgrid(a.workers * (c.tile_rows / 8));
   switch (c.tile_rows) {
     case 16: hipLaunchKernelGGL((kv4_attn_kernel<T, 1, false>), grid, block, 0, st, a); break;
     case 32: hipLaunchKernelGGL((kv4_attn_kernel<T, 2, false>), grid, block, 0, st, a); break;
     default: hipLaunchKernelGGL((kv4_tile_kernel<T, false>), grid, block, TILE_LDS, st, a);
   }
-  if (c.tile_rows <= 32) hipLaunchKernelGGL((kv4_merge_kernel<T, false>), mgrid, block, 0, st, a, c.tile_rows);
-  else hipLaunchKernelGGL((kv4_merge_kernel<T, true>), mgrid, block, 0, st, a, c.tile_rows);
+  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, mgrid, block, 0, st, a, c.tile_rows, groups, n_groups); };
+  if (c.tile_rows <= 32) groups ? merge(kv4_merge_kernel<T, false, true>) : merge(kv4_merge_kernel<T, false, false>);
+  else groups ? merge(kv4_merge_kernel<T, true, true>) : merge(kv4_merge_kernel<T, true, false>);
 }
 // With shared keys (a: groups and sequences in one list): in one launch, or the groups' in one of tiles.
 template <typename T>
@@ -1933,19 +1945,23 @@ void launch_kv4_read(const Kv4RowsArgs& a, hipStream_t st) {
   else if (a.dtype == 1) hipLaunchKernelGGL((kv4_read_kernel<1>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((kv4_read_kernel<2>), grid, block, 0, st, a);
 }
-void launch_kv4_attend(const Kv4AttnArgs& a_in, hipStream_t st) {
+namespace {
+// Every sequence by itself; groups: null, or boundaries that are only looked at.
+void attend_apart(const Kv4AttnArgs& a_in, const int* groups, int n_groups, hipStream_t st) {
   Kv4AttnArgs a = a_in;
   const Kv4Cut c = kv4_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq);
   a.workers = c.workers;
   a.ends = a.starts + 1;
   a.n_groups = 0;
-  if (a.dtype == 1) attend<half_t>(a, c, st);
-  else attend<bf16_t>(a, c, st);
+  if (a.dtype == 1) attend<half_t>(a, c, groups, n_groups, st);
+  else attend<bf16_t>(a, c, groups, n_groups, st);
 }
+}  // namespace
+void launch_kv4_attend(const Kv4AttnArgs& a, hipStream_t st) { attend_apart(a, nullptr, 0, st); }
 void launch_kv4_attend_shared(const Kv4AttnArgs& a_in, const int* groups, int n_groups, hipStream_t st) {
   Kv4AttnArgs a = a_in;
   const Kv4SharedCut c = kv4_shared_cut(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
-  if (!c.own) return launch_kv4_attend(a, st);
+  if (!c.own) return attend_apart(a, groups, n_groups, st);
   const Kv4SharedWs w = kv4_shared_ws(a.n_rows, a.n_heads, a.n_kv, a.n_seq, n_groups);
   char* ws = reinterpret_cast<char*>(a.ws);
   auto ints = [&](long long at) { return reinterpret_cast<int*>(ws + at); };

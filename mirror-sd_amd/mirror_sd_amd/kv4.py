@@ -271,9 +271,12 @@ class KV4Cache:
 
         ``groups`` [n_groups + 1] names sequences that go on from one text: those of group g are
         ``groups[g] .. groups[g + 1] - 1``.  Pages that all of a group's sequences (those with rows) hold
-        from the first on, and whose keys all their rows see, are then read once for the group,
-        not once a sequence.  Which they are is found from the tables, so the results are those of a
-        call without groups (to the rounding of sums in another order), whatever is shared."""
+        from the first on, and whose keys all their rows see, are then attended for all of the group's
+        rows together, 16, 32 or 128 rows of a kv head at a time, in place of sequence by sequence.
+        Which pages they are is found from the tables, so the results are those of a call without
+        groups, whatever is shared, to the order of sums and the choice of kernel (above).  Calls
+        of more than 16 rows for each kv head and sequence on average are attended as without
+        groups.  Boundaries out of order, or outside 0 .. max_seqs, share nothing (``errors()``)."""
         import torch
         q = self._rows(q, None, "q")
         n, heads = q.shape[0], q.shape[1]
