@@ -107,7 +107,7 @@ DFL_DEV VfPart join(const VfPart& x, const VfPart& y, double scale) {
 }
 // ---- first pass: parts of rows
 //
-// A workgroup goes over its part of a row in rounds of VECS loads of 16 bytes a thread; the next
+// A workgroup goes over its part of a row in rounds of VF_VECS loads of 16 bytes a thread; the next
 // round's loads are on their way while this one's exponentials are made.  Bound by HBM where there is
 // enough to read (1.2 GB in bf16: 186 us, 6.6 TB/s; 65 MB 16, 4 TB/s), else by the begin and end of the
 // workgroups.  With all of a part's loads at once and two barriers' sums for each 32 KiB the 1.2 GB
@@ -119,15 +119,15 @@ template <int DT> struct Vec {
   typedef E vec __attribute__((ext_vector_type(N)));
 };
 // Vectors v, v + VF_THREADS, .. of a row's `n`; -infinity past the last.
-template <int DT, int VECS>
-DFL_DEV void load_round(const typename Vec<DT>::vec* p, int v, int n, bool inside, typename Vec<DT>::vec (&x)[VECS]) {
+template <int DT>
+DFL_DEV void load_round(const typename Vec<DT>::vec* p, int v, int n, bool inside, typename Vec<DT>::vec (&x)[VF_VECS]) {
   if (inside) {
 #pragma unroll
-    for (int j = 0; j < VECS; ++j) x[j] = __builtin_nontemporal_load(p + v + j * VF_THREADS);
+    for (int j = 0; j < VF_VECS; ++j) x[j] = __builtin_nontemporal_load(p + v + j * VF_THREADS);
     return;
   }
 #pragma unroll
-  for (int j = 0; j < VECS; ++j) {
+  for (int j = 0; j < VF_VECS; ++j) {
 #pragma unroll
     for (int i = 0; i < Vec<DT>::N; ++i) x[j][i] = (typename Vec<DT>::E)-INFINITY;
     if (v + j * VF_THREADS < n) x[j] = p[v + j * VF_THREADS];
@@ -179,11 +179,11 @@ DFL_DEV void soft_round(const V (&x)[VECS], SoftState& s, float c, float d, doub
   }
 }
 // (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not wanted, or has no temperature)
-template <int DT, int VECS, typename F>
+template <int DT, typename F>
 DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stride, int row, int chunk, int rounds,
                            F scale_at, float (&lds)[2][4]) {
   typedef Vec<DT> V;
-  constexpr int ROUND = VF_THREADS * VECS;   // vectors
+  constexpr int ROUND = VF_THREADS * VF_VECS;   // vectors
   const typename V::E* p = reinterpret_cast<const typename V::E*>(base) + row * stride;
   // whole vectors of the row, and the values before and behind them (the first part takes those)
   const int head = min(a.vocab, (int)(-(reinterpret_cast<uintptr_t>(p) / sizeof(typename V::E)) & (V::N - 1)));
@@ -195,8 +195,8 @@ DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stri
   // (threads 0 .. 7: the values before; 8 .. 15: those behind)
   const int edge = tid < V::N ? tid : tail + tid - V::N;
   const bool at_edge = chunk == 0 && (tid < V::N ? tid < head : edge < a.vocab && tid < 2 * V::N);
-  typename V::vec x[VECS], y[VECS];
-  load_round<DT, VECS>(body, begin + tid, n, inside(begin), x);
+  typename V::vec x[VF_VECS], y[VF_VECS];
+  load_round<DT>(body, begin + tid, n, inside(begin), x);
   const float extra = at_edge ? (float)p[edge] : -INFINITY;
   const double scale = scale_at();
   VfPart out{-INFINITY, 0.f, 0.0};
@@ -214,14 +214,14 @@ DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stri
     };
     if (tid < V::N) take(extra, edge);
     for (int v = begin; v < end; v += ROUND) {
-      if (v + ROUND < end) load_round<DT, VECS>(body, v + ROUND + tid, n, inside(v + ROUND), y);
+      if (v + ROUND < end) load_round<DT>(body, v + ROUND + tid, n, inside(v + ROUND), y);
 #pragma unroll
-      for (int j = 0; j < VECS; ++j)
+      for (int j = 0; j < VF_VECS; ++j)
 #pragma unroll
         for (int i = 0; i < V::N; ++i)
           take((float)x[j][i], head + (v + tid + j * VF_THREADS) * V::N + i);
 #pragma unroll
-      for (int j = 0; j < VECS; ++j) x[j] = y[j];
+      for (int j = 0; j < VF_VECS; ++j) x[j] = y[j];
     }
     if (tid >= V::N) take(extra, edge);
     const float of_wave = wave_max(top);
@@ -248,10 +248,10 @@ DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stri
     soft_round<1, 1>(one, s, c, d, scale);
   }
   for (int v = begin; v < end; v += ROUND) {
-    if (v + ROUND < end) load_round<DT, VECS>(body, v + ROUND + tid, n, inside(v + ROUND), y);
-    soft_round<VECS, V::N>(x, s, c, d, scale);
+    if (v + ROUND < end) load_round<DT>(body, v + ROUND + tid, n, inside(v + ROUND), y);
+    soft_round<VF_VECS, V::N>(x, s, c, d, scale);
 #pragma unroll
-    for (int j = 0; j < VECS; ++j) x[j] = y[j];
+    for (int j = 0; j < VF_VECS; ++j) x[j] = y[j];
   }
   const float top = wave_max(s.top), sum = wave_sum((s.sum[0] + s.sum[1]) + (s.sum[2] + s.sum[3]));
   __syncthreads();
@@ -265,7 +265,6 @@ DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stri
   return out;
 }
 
-template <int VECS>
 __global__ __launch_bounds__(VF_THREADS) void verify_parts_kernel(VerifyArgs a, VfPart* parts) {
   __shared__ float lds[2][4];
   const uint32_t t_items = (uint32_t)a.n_rows * a.t_chunks, items = t_items + (uint32_t)a.n_rows * a.d_chunks;
@@ -282,9 +281,9 @@ __global__ __launch_bounds__(VF_THREADS) void verify_parts_kernel(VerifyArgs a, 
     const long long stride = drafted ? a.draft_row : a.target_row;
     const int dt = drafted ? a.draft_dtype : a.target_dtype, rounds = drafted ? a.d_rounds : a.t_rounds;
     VfPart out;
-    if (dt == 0) out = part_of_row<0, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
-    else if (dt == 1) out = part_of_row<1, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
-    else out = part_of_row<2, VECS>(a, base, stride, row, chunk, rounds, scale, lds);
+    if (dt == 0) out = part_of_row<0>(a, base, stride, row, chunk, rounds, scale, lds);
+    else if (dt == 1) out = part_of_row<1>(a, base, stride, row, chunk, rounds, scale, lds);
+    else out = part_of_row<2>(a, base, stride, row, chunk, rounds, scale, lds);
     if (threadIdx.x == 0) parts[i] = out;
   }
 }
@@ -729,7 +728,7 @@ void launch_verify(const VerifyArgs& a_in, hipStream_t st) {
   const long long items = (long long)a.n_rows * (a.t_chunks + a.d_chunks);
   const dim3 block(VF_THREADS), grid((unsigned)(items < (1 << 20) ? items : 1 << 20));
   if (items > 0) {
-    hipLaunchKernelGGL((verify_parts_kernel<VF_VECS>), grid, block, 0, st, a, parts);
+    hipLaunchKernelGGL(verify_parts_kernel, grid, block, 0, st, a, parts);
   }
   hipLaunchKernelGGL(verify_judge_kernel, dim3(a.n_seq), dim3(JUDGE), 0, st, a, (const VfPart*)parts, draws, states);
   if (a.n_rows == 0) return;
