@@ -745,7 +745,7 @@ DFL_DEV void walk_no_note(const Kv4AttnArgs& a, int tile_rows, int wave) {
 DFL_DEV void walk_note(const Kv4AttnArgs& a, int tile_rows, int wave, long long per, const Run& r) {
   if (wave || lane_again()) return;
   kv4_notes(a, tile_rows)[worker_of(a, blockIdx.x)] = Kv4Note{
-      (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, r.s, 0};
+      (int)kv4_div(r.r0 + r.nblk - 1, per), r.head, r.tile, r.sq.q0, r.sq.qlen, r.sq.len, 0, 0};
 }
 // A sequence's places in the table.
 template <bool MIXED>
