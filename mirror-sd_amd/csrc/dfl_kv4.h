@@ -289,10 +289,18 @@ inline Kv4SharedCut kv4_shared_cut(int n_rows, int n_heads, int n_kv, int n_seq,
   // of 64 rows over 8000 79, 73.
   const Kv4Cut own = kv4_cut(n_rows, n_heads, n_kv, n_seq);
   if (own.tile_rows != 16) return Kv4SharedCut{0, 0, 0, 0};
-  // Rows of a kv head in a group, on average.  Us in tiles of 16, 32 and 128, 4096 and 32768 shared
-  // keys: 128 rows 34 and 69, 34 and 62, 53 and 73; 256 rows 42 and 109, 42 and 91, 60 and 85; 512
-  // rows 57 and 183 (16), 72 and 119 (128).  (64 ragged tokens in groups of 17 rows a kv head to 132: 52, 54,
-  // 67; eight tokens behind 4096 keys, 40 rows: 30, 31, 49.)
+  // Rows of a kv head in a group, on average.  Us in tiles of 16, 32 and 128, over 1024, 4096, 16384 and
+  // 32768 shared keys, one group, 8 kv heads in bf16:
+  //    64 rows  27 30 37 46    28 31 38 46    40 48 58 66
+  //   128       28 33 47 68    29 34 45 61    43 53 63 70
+  //   256       33 42 69 107   34 41 62 91    53 59 70 85
+  //   512       41 57 112 184  45 57 100 154  62 71 91 121
+  //  1024       50 77 184 318  52 74 160 260  64 73 116 173
+  // The borders lie where long texts turn: past 512 rows a text of 4096 keys takes 14 us more than in
+  // tiles of 32, as the host does not know its length.  The average is over all groups that the call
+  // names, also those of one sequence or with nothing in common, of which the host knows as little: 1024
+  // rows behind 32768 keys take 173 us, 242 and 309 with 4 and 8 single sequences named as groups beside
+  // them, 177 and 173 with those outside of the boundaries (without groups 520).
   const long long groups = n_groups < n_rows ? n_groups : n_rows, rows = (long long)n_rows * (n_heads / n_kv);
   if (rows >= 512 * groups) return Kv4SharedCut{16, 128, own.workers, 2 * KV4_CUS};
   if (rows >= 128 * groups) return Kv4SharedCut{32, 32, 2 * KV4_CUS, 0};

@@ -461,7 +461,13 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4RowsArgs a) {
 // head; a workgroup takes a run of key blocks of a unit (32 keys each).  Of a block:
 //   S^T = K Q^T   matrix instructions with keys on the M axis;
 //   softmax       fp32, log2 domain, the reference maximum raised only when a block exceeds it by
-//                 more than KV4_SLACK; weights rounded to the type of Q, and summed as rounded;
+//                 more than KV4_SLACK; weights rounded to the type of Q, and summed as rounded (the
+//                 16-bit matrix instructions take both operands in one type, and V fits in it;
+//                 rounding them moves results by as much as the result's own rounding: 2.6e-4 of
+//                 the norm off 64 bits for 2.1e-4 in fp16, 1.9e-3 for 1.6e-3 in bf16.  A second part
+//                 for what it leaves, with its own product with V, brings those to 2.1e-4 and 1.6e-3 in
+//                 tiles of 16 and 32, and costs them 1 to 3 us: 64 tokens behind three texts 52.4 for
+//                 51.6, 16 over 65 thousand keys 215.5 for 212; tiles of 128 are bound by products);
 //   O^T += V^T P  V converted in registers, written to LDS as rows, read back transposed
 //                 (ds_read_b64_tr_b16); P from the S^T accumulators as they lie: the rows of V that
 //                 a lane's weights stand for are those whose keys its accumulators hold.

@@ -16,11 +16,14 @@
 //
 // Bound by latencies, as the plain step: for few sequences, rows, pages and places (FORK_ONE_..) one
 // workgroup does all phases with the offsets in LDS, past that each is a launch.  Places of all
-// sequences are numbered through and found by a search in the offsets.  One workgroup and launches, us
-// (sequences x kept pages that all but one in 16 keep from another): 64 x 43 (half of them) 21, 36; 64 x
-// 121 29, 36; 256 x 15 28, 40; 256 x 62 43, 40; 512 x 62 72, 43; 1024 x 93 186, 50; 1024 that fork
-// nothing 29, 41.  (With an atomic for each kept page, whether it changes hands or not, the 1024 x 93
-// took 335 and 59: sequences that go on from each other share most pages already.)
+// sequences are numbered through and found by a search in the offsets.  One workgroup and launches, us of a
+// step in a graph (sequences x kept pages that all but the group's first keep from it): 8 x 64 7, 23; 64 x 43
+// 15, 27; 64 x 121 21, 28; 256 x 15 20, 30; 256 x 62 37, 31; 1024 x 93 195, 42.  Sequences that begin so, with
+// no pages before, take as long as those that hold the same pages already; with pages of other texts, which
+// all change hands, 256 x 62 take 45, 31 and 1024 x 31 114, 41.  (With an atomic for each kept page, whether
+// it changes hands or not, the 1024 x 93 that hold theirs already took 335 and 59.)  The host knows the
+// places that the tables have, not those that a step looks at: the 64 x 43 in tables of 512 pages each take
+// the launches, 26 where one workgroup would take 15 (17 and 10 if none forks).
 #include "dfl_kv4.h"
 
 #include "dfl_common.h"

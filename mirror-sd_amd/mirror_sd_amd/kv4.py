@@ -276,7 +276,10 @@ class KV4Cache:
         Which pages they are is found from the tables, so the results are those of a call without
         groups, whatever is shared, to the order of sums and the choice of kernel (above).  Calls
         of more than 16 rows for each kv head and sequence on average are attended as without
-        groups.  Boundaries out of order, or outside 0 .. max_seqs, share nothing (``errors()``)."""
+        groups.  Boundaries out of order, or outside 0 .. max_seqs, share nothing (``errors()``).
+        How many rows are taken at a time follows from the average over all groups that are named:
+        leave sequences that go on alone outside of the boundaries (before the first group or
+        behind the last one) where that is possible.  The workspace takes 1 KiB a row and head."""
         import torch
         q = self._rows(q, None, "q")
         n, heads = q.shape[0], q.shape[1]
