@@ -178,7 +178,8 @@ DFL_DEV void soft_round(const V (&x)[VECS], SoftState& s, float c, float d, doub
       }
   }
 }
-// (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not wanted, or has no temperature)
+// (scale_at: the row's log2(e) / T, found while the first loads are on their way; below 0: the row is not
+// wanted, or has no temperature)
 template <int DT, typename F>
 DFL_DEV VfPart part_of_row(const VerifyArgs& a, const void* base, long long stride, int row, int chunk, int rounds,
                            F scale_at, float (&lds)[2][4]) {

@@ -274,13 +274,15 @@ class KV4Cache:
         from the first on, and whose keys all their rows see, are then attended for all of the group's
         rows together, 16, 32 or 128 rows of a kv head at a time, in place of sequence by sequence.
         Which pages they are is found from the tables, so the results are those of a call without
-        groups, whatever is shared, to the order of sums and the choice of kernel (above).  It pays
-        from some 100 thousand shared rows times sequences on; below that a call takes 5 to 10 us
-        more than without groups (32 heads on 8).  Calls of more than 16 rows for each kv head and
-        sequence on average are attended as without groups.  Boundaries out of order, or outside
-        0 .. max_seqs, share nothing (``errors()``).  How many rows are taken at a time follows
-        from the average over all groups that are named: leave sequences that go on alone outside of the boundaries (before the first group or
-        behind the last one) where that is possible.  The workspace takes 1 KiB a row and head."""
+        groups, whatever is shared, to the order of sums and, with 128 rows at a time, the queries'
+        parts (as in calls of more than 32 rows for each kv head and sequence: 2^-13.9 of the
+        largest of 32).  It pays from some 100 thousand shared rows times sequences on; below that
+        a call takes 5 to 10 us more than without groups (32 heads on 8).  Calls of more than 16
+        rows for each kv head and sequence on average are attended as without groups.  Boundaries
+        out of order, or outside 0 .. max_seqs, share nothing (``errors()``).  How many rows are
+        taken at a time follows from the average over all groups that are named: leave sequences
+        that go on alone outside of the boundaries (before the first group or behind the last one)
+        where that is possible.  The workspace takes 1 KiB a row and head."""
         import torch
         q = self._rows(q, None, "q")
         n, heads = q.shape[0], q.shape[1]
